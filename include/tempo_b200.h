@@ -170,10 +170,13 @@ tempo_status tempo_block_copy(const void* source, void* destination, uint32_t ro
 #define TEMPO_GEMM_GELU 1u   /* out = GELU(round_bf16(acc + bias)) */
 #define TEMPO_GEMM_ARGMAX 2u /* no output: per-row (max, first argmax) over each N tile into the partials */
 #define TEMPO_GEMM_LN 4u     /* internal: the LayerNorm-folded mode of tempo_gemm_ln (rejected by tempo_gemm) */
+#define TEMPO_GEMM_F32 8u    /* out is FP32 and holds the accumulators; tempo_gemm only, no bias or residual */
 
 /* out[M, ldo] = epilogue(a[M, K] (row stride lda) x w_t[N, K]^T (row stride ldw)) with optional bias[N] and
  * residual[M, ldr] (added after GELU), FP32 accumulate, BF16 out; tcgen05 + TMA. K % 8 == 0; lda, ldw % 8 == 0.
- * In TEMPO_GEMM_ARGMAX mode `out` is unused and `part_val`/`part_idx` receive [M][ceil(N/256)] partials. */
+ * In TEMPO_GEMM_ARGMAX mode `out` is unused and `part_val`/`part_idx` receive [M][ceil(N/256)] partials.
+ * In TEMPO_GEMM_F32 mode (alone, without bias and residual) `out` is FP32: the logits of an LM head, whose BF16
+ * rounding would cost up to 2^-8 of their size in each log probability. */
 tempo_status tempo_gemm(const void* a, uint32_t lda, const void* w_t, uint32_t ldw, const void* bias,
                         const void* residual, uint32_t ldr, void* out, uint32_t ldo, uint32_t m, uint32_t n,
                         uint32_t k, uint32_t flags, float* part_val, int32_t* part_idx, void* stream);
@@ -265,6 +268,47 @@ tempo_status tempo_kv_store(const void* qkv, void* k_cache, void* v_cache, const
 tempo_status tempo_decode_attention(const void* qkv, const void* k_cache, const void* v_cache,
                                     const int32_t* lengths, int32_t length_offset, void* out, uint32_t seqs,
                                     uint32_t heads, uint32_t head, uint32_t capacity, void* stream);
+
+/* ---- the 4-bit key / value cache -----------------------------------------------------------------------------------
+ * uint8 [seqs][kv_heads][capacity / 16] tiles of 16 positions, capacity % 16 == 0; a tile holds one block of
+ * TEMPO_Q4_BLOCK_BYTES per group of 64 head dimensions (head 64 or 128): 16 rows of 32 bytes of key codes, 16 rows of
+ * value codes (dimension d in byte d / 2, the even one in the low half), then per position four BF16 words: key scale,
+ * key low, value scale, value low. A row of 64 stands for code * scale + low with low = its least value, scale =
+ * bf16((greatest - low) / 15) and code = (x - low) / scale rounded to the nearest integer (ties to even) in 0 .. 15, 0
+ * where the scale is 0. A row of 64 that holds a NaN or an infinity, or whose range passes FP32, reads as NaN. */
+#define TEMPO_Q4_TILE 16u
+#define TEMPO_Q4_BLOCK_BYTES 1152u
+
+/* tempo_kv_store into the 4-bit cache: the key and value columns of `rows` rows of qkv (row stride ldq elements,
+ * ldq % 8 == 0; `heads` query heads, which may be 0, then kv_heads key heads and kv_heads value heads of `head`
+ * dimensions) go to sequence seq_of[r], position pos_of[r]. Rows whose sequence or position is out of range are skipped.
+ * The places of one call must differ: one that two rows name is left holding a mixture of them. */
+tempo_status tempo_kv_store_q4(const void* qkv, uint32_t ldq, void* cache, const int32_t* seq_of,
+                               const int32_t* pos_of, uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t kv_heads,
+                               uint32_t head, uint32_t capacity, void* stream);
+
+/* The keys and values of `rows` places of the 4-bit cache as BF16 rows [2 * kv_heads * head] (row stride ldo elements,
+ * ldo % 8 == 0). Rows whose sequence or position is out of range are written as zeros. */
+tempo_status tempo_kv_load_q4(const void* cache, void* kv, uint32_t ldo, const int32_t* seq_of, const int32_t* pos_of,
+                              uint32_t rows, uint32_t seqs, uint32_t kv_heads, uint32_t head, uint32_t capacity,
+                              void* stream);
+
+/* tempo_decode_attention over the 4-bit cache: one query row per sequence (row stride ldq elements, ldq % 8 == 0; its
+ * first heads * head columns, already scaled by 1/sqrt(head)) over the first lengths[s] + length_offset positions
+ * (clamped to [0, capacity]); query head h reads key / value head h / (heads / kv_heads). A sequence of no positions is
+ * written as zeros. out: [seqs, heads * head] BF16. */
+tempo_status tempo_decode_attention_q4(const void* q, uint32_t ldq, const void* cache, const int32_t* lengths,
+                                       int32_t length_offset, void* out, uint32_t seqs, uint32_t heads,
+                                       uint32_t kv_heads, uint32_t head, uint32_t capacity, void* stream);
+
+/* Scores of `rows` rows of `vocab` logits (FP32, or BF16 with bf16 = 1; row stride ld elements, any alignment of the
+ * element): logprob[r] = log softmax(logits[r])[ids[r]] (0 where ids[r] is outside [0, vocab): a row without a token),
+ * entropy[r] = -sum p ln p, and, with 0 < top <= 32 and top <= vocab, the `top` greatest logits in descending order, ties
+ * to the lower index, as top_ids / top_logprob [rows][top]. A logit of -infinity has probability 0. A row of nothing but
+ * -infinity scores -infinity with entropy 0; a NaN or +infinity in a row makes its scores NaN, and NaN ranks first. */
+tempo_status tempo_token_logprobs(const void* logits, uint64_t ld, uint32_t bf16, const int32_t* ids, uint32_t rows,
+                                  uint32_t vocab, uint32_t top, float* logprob, float* entropy, float* top_logprob,
+                                  int32_t* top_ids, void* stream);
 
 /* Reduces argmax partials [rows][tiles] to token ids: ids[r] = first index of the row maximum (ties go to the lower
  * index, as numpy's argmax). When tokens_out is not NULL the id is also written to tokens_out[r * out_stride + c] with

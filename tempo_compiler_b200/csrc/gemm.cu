@@ -46,6 +46,7 @@ struct RowMajorParams {
   const uint16_t* bias;
   const uint16_t* residual;
   uint16_t* out;
+  float* out_f32;  // TEMPO_GEMM_F32: the output (`out` is then unused)
   float* part_val;
   int32_t* part_idx;
   uint32_t m, n, k;
@@ -340,8 +341,8 @@ __device__ __noinline__ bool ln_stats_from_stages(const uint8_t* smem, uint32_t 
 }
 
 // LN: the folded-LayerNorm variant (tempo_gemm_ln); a separate instantiation, so the statistics code adds no
-// registers to the others.
-template <int BN, int STAGES, bool STAGED, bool LN>
+// registers to the others. F32: TEMPO_GEMM_F32, the accumulators stored as they are (the LM head's logits).
+template <int BN, int STAGES, bool STAGED, bool LN, bool F32>
 __global__ void __launch_bounds__(kRowThreads, 1)
     gemm_rowmajor_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                          const __grid_constant__ CUtensorMap tmap_out, RowMajorParams p) {
@@ -555,6 +556,19 @@ __global__ void __launch_bounds__(kRowThreads, 1)
           continue;
         }
         if (!row_ok || n0 >= p.n) continue;
+        if constexpr (F32) {
+          float* orow = p.out_f32 + size_t(row) * p.ldo + n0;
+          if (n0 + kCW <= p.n) {
+#pragma unroll
+            for (uint32_t q = 0; q < kCW / 4; ++q)
+              reinterpret_cast<uint4*>(orow)[q] = make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
+          } else {
+#pragma unroll
+            for (uint32_t j = 0; j < kCW; ++j)
+              if (n0 + j < p.n) orow[j] = __uint_as_float(r[j]);
+          }
+          continue;
+        }
         if (argmax) {
 #pragma unroll
           for (uint32_t j = 0; j < kCW; ++j) {
@@ -773,7 +787,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <int BN, int STAGES, bool STAGED = false, bool LN = false>
+template <int BN, int STAGES, bool STAGED = false, bool LN = false, bool F32 = false>
 tempo_status launch_rowmajor(const void* a, uint32_t lda, const void* w_t, uint32_t ldw, const RowMajorParams& base,
                              cudaStream_t stream) {
   using L = RowMajorSmem<BN, STAGES, STAGED>;
@@ -806,7 +820,7 @@ tempo_status launch_rowmajor(const void* a, uint32_t lda, const void* w_t, uint3
   p.n_tiles = (p.n + BN - 1) / BN;
   const uint32_t tiles = p.m_tiles * p.n_tiles;
   const uint32_t grid = tiles < uint32_t(sm_count()) ? tiles : uint32_t(sm_count());
-  auto kernel = gemm_rowmajor_kernel<BN, STAGES, STAGED, LN>;
+  auto kernel = gemm_rowmajor_kernel<BN, STAGES, STAGED, LN, F32>;
   s = set_smem(reinterpret_cast<const void*>(kernel), L::kBytes);
   if (s != TEMPO_OK) return s;
   return launch(kernel, dim3(grid), dim3(kRowThreads), L::kBytes, stream, 1, "gemm_rowmajor_kernel", ta, tb, to, p);
@@ -1772,6 +1786,9 @@ static tempo_status gemm_impl(const void* a, uint32_t lda, const void* w_t, uint
   if (argmax && (flags & TEMPO_GEMM_LN)) return fail(TEMPO_ERR_VALUE, "tempo_gemm: argmax with a folded LayerNorm");
   if (argmax && (part_val == nullptr || part_idx == nullptr))
     return fail(TEMPO_ERR_VALUE, "tempo_gemm: argmax mode needs the partial buffers");
+  const bool f32 = (flags & TEMPO_GEMM_F32) != 0;
+  if (f32 && (flags != TEMPO_GEMM_F32 || bias != nullptr || residual != nullptr || row_stats != nullptr || kv.k != nullptr))
+    return fail(TEMPO_ERR_VALUE, "tempo_gemm: the FP32 output takes no bias, residual or other mode");
   if (!argmax && (out == nullptr || ldo < n || (ldo % 8) || !aligned16(out)))
     return fail(TEMPO_ERR_VALUE, "tempo_gemm: output must be 16-byte aligned with a row stride >= N, multiple of 8");
   if (residual != nullptr && (ldr < n || (ldr % 8) || !aligned16(residual)))
@@ -1781,6 +1798,7 @@ static tempo_status gemm_impl(const void* a, uint32_t lda, const void* w_t, uint
   p.bias = static_cast<const uint16_t*>(bias);
   p.residual = static_cast<const uint16_t*>(residual);
   p.out = static_cast<uint16_t*>(out);
+  p.out_f32 = static_cast<float*>(out);
   p.part_val = part_val;
   p.part_idx = part_idx;
   p.m = m;
@@ -1808,6 +1826,7 @@ static tempo_status gemm_impl(const void* a, uint32_t lda, const void* w_t, uint
     if (gemv != TEMPO_ERR_VALUE) return gemv;
   }
   if (argmax) return launch_rowmajor<256, 4>(a, lda, w_t, ldw, p, st);
+  if (f32) return launch_rowmajor<256, 4, false, false, true>(a, lda, w_t, ldw, p, st);
   // With the statistics from their producer, the folded LayerNorm runs wherever the plain projection would: narrow
   // full-K tiles for one 128-row block, else split-K.
   const bool ln_partials = ln_mode && ln.stats != nullptr;

@@ -24,6 +24,9 @@ IMAGE_BYTES = 64
 GEMM_GELU = 1
 GEMM_ARGMAX = 2
 GEMM_LN = 4
+GEMM_F32 = 8
+Q4_TILE = 16
+Q4_BLOCK_BYTES = 1152
 
 _EXCEPTIONS = {ERR_VALUE: ValueError, ERR_MEMORY: MemoryError, ERR_KEY: KeyError, ERR_RUNTIME: RuntimeError,
                ERR_TIMEOUT: TimeoutError, ERR_STATE: RuntimeError}
@@ -93,6 +96,10 @@ _SIGNATURES = {
     "tempo_attention_prefill": [_vp, _vp, _u32, _u32, _u32, _u32, _vp],
     "tempo_kv_store": [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _vp],
     "tempo_decode_attention": [_vp, _vp, _vp, _vp, _i32, _vp, _u32, _u32, _u32, _u32, _vp],
+    "tempo_kv_store_q4": [_vp, _u32, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _vp],
+    "tempo_kv_load_q4": [_vp, _vp, _u32, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _vp],
+    "tempo_decode_attention_q4": [_vp, _u32, _vp, _vp, _i32, _vp, _u32, _u32, _u32, _u32, _u32, _vp],
+    "tempo_token_logprobs": [_vp, _u64, _u32, _vp, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _vp],
     "tempo_argmax_finish": [_vp, _vp, _u32, _u32, _vp, _vp, _u32, _vp, _i32, _i32, _vp],
     "tempo_lm_head_argmax_noalloc": [_vp, _u32, _vp, _u32, _u32, _u32, _u32, _vp, _vp],
     "tempo_gemm_norm": [_vp, _u32, _vp, _vp, _f32, _vp, _u32, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _vp, _vp, _vp,

@@ -8,6 +8,7 @@ a wrong dtype or a missing library raises.
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -49,6 +50,37 @@ def _check(t: torch.Tensor, dtype: torch.dtype, name: str) -> None:
         raise ValueError(f"{name} must be contiguous")
 
 
+def _check_rows(t: torch.Tensor, dtype: torch.dtype, name: str) -> None:
+    """A matrix whose rows are contiguous, at any row stride."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor: the B200 kernels have no CPU path")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] != 1) or (t.stride(0) < t.shape[1] and t.shape[0] != 1):
+        raise ValueError(f"{name} must be a matrix of contiguous rows that do not overlap")
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Elements from row to row of a matrix that _check_rows accepts (a single row's own stride means nothing)."""
+    return t.stride(0) if t.shape[0] != 1 else (t.shape[1] + 7) // 8 * 8
+
+
+def _check_devices(first: torch.Tensor, **others: torch.Tensor | None) -> None:
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{name} is on {t.device}, the call's first operand on {first.device}")
+
+
+def _launch_at(t: torch.Tensor, name: str, *args) -> None:
+    """_launch on the current stream of `t`'s device, which need not be the current device."""
+    index = t.device.index
+    if index == torch.cuda.current_device():
+        _launch(name, *args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            _launch(name, *args, torch.cuda.current_stream().cuda_stream)
+
+
 def gemm(a: torch.Tensor, w_t: torch.Tensor, *, bias: torch.Tensor | None = None,
          residual: torch.Tensor | None = None, gelu: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
     """out[M, N] = epilogue(a[M, K] @ w_t[N, K]^T): + bias, exact-erf GELU (of the BF16-rounded sum), + residual."""
@@ -68,6 +100,26 @@ def gemm(a: torch.Tensor, w_t: torch.Tensor, *, bias: torch.Tensor | None = None
     flags = _lib.GEMM_GELU if gelu else 0
     _launch("tempo_gemm", a.data_ptr(), k, w_t.data_ptr(), k, _ptr(bias), _ptr(residual), n, out.data_ptr(), n, m, n,
               k, flags, None, None, _stream())
+    return out
+
+
+def gemm_f32(a: torch.Tensor, w_t: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
+    """out[M, N] = a[M, K] @ w_t[N, K]^T in FP32, the accumulators unrounded (an LM head's logits). `out` may have a
+    row stride of its own, a multiple of 8; without it the rows are padded to one and the view of N columns returned."""
+    _check(a, torch.bfloat16, "a")
+    _check(w_t, torch.bfloat16, "w_t")
+    m, k = a.shape
+    n = w_t.shape[0]
+    if w_t.shape[1] != k:
+        raise ValueError(f"inner dimensions differ: a {tuple(a.shape)}, w_t {tuple(w_t.shape)}")
+    if out is None:
+        out = torch.empty((m, (n + 7) // 8 * 8), dtype=torch.float32, device=a.device)[:, :n]
+    _check_rows(out, torch.float32, "out")
+    if out.shape != (m, n):
+        raise ValueError(f"out must be {(m, n)}, got {tuple(out.shape)}")
+    _check_devices(a, w_t=w_t, out=out)
+    _launch_at(a, "tempo_gemm", a.data_ptr(), k, w_t.data_ptr(), k, None, None, n, out.data_ptr(), _row_stride(out), m,
+               n, k, _lib.GEMM_F32, None, None)
     return out
 
 
@@ -285,6 +337,153 @@ def decode_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
         out = torch.empty((seqs, heads * head), dtype=torch.bfloat16, device=qkv.device)
     _launch("tempo_decode_attention", qkv.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), lengths.data_ptr(),
               length_offset, out.data_ptr(), seqs, heads, head, capacity, _stream())
+    return out
+
+
+# ---- the 4-bit key / value cache ----
+
+def kv_cache_q4(seqs: int, kv_heads: int, capacity: int, head: int = 64, *,
+                device: torch.device | str = "cuda") -> torch.Tensor:
+    """An empty 4-bit cache, [seqs, kv_heads, ceil(capacity / 16), 1152 * head / 64] uint8 (include/tempo_b200.h has
+    the layout): `capacity` positions, rounded up to whole tiles of 16, at 72 bytes per position, head and 64
+    dimensions. A slice of its sequences is a cache too."""
+    if head not in (64, 128):
+        raise ValueError(f"the 4-bit cache holds heads of 64 or 128 dimensions, got {head}")
+    if seqs <= 0 or kv_heads <= 0 or capacity <= 0:
+        raise ValueError(f"a cache needs sequences, heads and positions, got {seqs}, {kv_heads}, {capacity}")
+    tiles = (capacity + _lib.Q4_TILE - 1) // _lib.Q4_TILE
+    return torch.zeros((seqs, kv_heads, tiles, _lib.Q4_BLOCK_BYTES * head // 64), dtype=torch.uint8, device=device)
+
+
+def _q4_shape(cache: torch.Tensor) -> tuple[int, int, int, int]:
+    """(seqs, kv_heads, head, capacity) of a 4-bit cache."""
+    _check(cache, torch.uint8, "cache")
+    if cache.dim() != 4 or cache.shape[3] not in (_lib.Q4_BLOCK_BYTES, 2 * _lib.Q4_BLOCK_BYTES):
+        raise ValueError(f"cache must be [seqs, kv_heads, tiles, 1152 or 2304] as kv_cache_q4 makes it, got "
+                         f"{tuple(cache.shape)}")
+    seqs, kv_heads, tiles, size = cache.shape
+    return seqs, kv_heads, size // _lib.Q4_BLOCK_BYTES * 64, tiles * _lib.Q4_TILE
+
+
+def _check_places(rows: int, seq_of: torch.Tensor, pos_of: torch.Tensor) -> None:
+    _check(seq_of, torch.int32, "seq_of")
+    _check(pos_of, torch.int32, "pos_of")
+    if seq_of.numel() != rows or pos_of.numel() != rows:
+        raise ValueError(f"{rows} rows need as many sequences and positions, got {seq_of.numel()} and {pos_of.numel()}")
+
+
+def kv_store_q4(qkv: torch.Tensor, cache: torch.Tensor, seq_of: torch.Tensor, pos_of: torch.Tensor) -> None:
+    """kv_store into a 4-bit cache: the key and value columns of row r of qkv ([rows, (heads + 2 kv_heads) * head],
+    at any row stride that is a multiple of 8; no query columns are needed) quantised into sequence seq_of[r] at
+    position pos_of[r]. Rows outside the cache are skipped; the others must name different places."""
+    seqs, kv_heads, head, capacity = _q4_shape(cache)
+    _check_rows(qkv, torch.bfloat16, "qkv")
+    rows, width = qkv.shape
+    heads = width // head - 2 * kv_heads
+    if width % head or heads < 0:
+        raise ValueError(f"qkv rows of {width} are not query, key and value heads of {head} ({kv_heads} key heads)")
+    _check_places(rows, seq_of, pos_of)
+    _check_devices(qkv, cache=cache, seq_of=seq_of, pos_of=pos_of)
+    _launch_at(qkv, "tempo_kv_store_q4", qkv.data_ptr(), _row_stride(qkv), cache.data_ptr(), seq_of.data_ptr(),
+               pos_of.data_ptr(), rows, seqs, heads, kv_heads, head, capacity)
+
+
+def kv_load_q4(cache: torch.Tensor, seq_of: torch.Tensor, pos_of: torch.Tensor, *,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """The keys and values a 4-bit cache holds at the given places, [rows, 2 kv_heads * head] BF16 (kv_store_q4 takes
+    them back). Places outside the cache give zeros."""
+    seqs, kv_heads, head, capacity = _q4_shape(cache)
+    rows = pos_of.numel()
+    _check_places(rows, seq_of, pos_of)
+    if out is None:
+        out = torch.empty((rows, 2 * kv_heads * head), dtype=torch.bfloat16, device=cache.device)
+    _check_rows(out, torch.bfloat16, "out")
+    if out.shape != (rows, 2 * kv_heads * head):
+        raise ValueError(f"out must be {(rows, 2 * kv_heads * head)}, got {tuple(out.shape)}")
+    _check_devices(cache, seq_of=seq_of, pos_of=pos_of, out=out)
+    _launch_at(cache, "tempo_kv_load_q4", cache.data_ptr(), out.data_ptr(), _row_stride(out), seq_of.data_ptr(),
+               pos_of.data_ptr(), rows, seqs, kv_heads, head, capacity)
+    return out
+
+
+def decode_attention_q4(qkv: torch.Tensor, cache: torch.Tensor, lengths: torch.Tensor, *, length_offset: int = 0,
+                        heads: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """decode_attention over a 4-bit cache: the query columns of row s of qkv (scaled by 1/sqrt(head)) over the first
+    lengths[s] + length_offset positions of sequence s; a sequence without positions gives zeros. The row holds query,
+    key and value heads, unless `heads` says how many query heads it begins with."""
+    seqs, kv_heads, head, capacity = _q4_shape(cache)
+    _check_rows(qkv, torch.bfloat16, "qkv")
+    _check(lengths, torch.int32, "lengths")
+    width = qkv.shape[1]
+    if heads is None:
+        heads = width // head - 2 * kv_heads
+    if width % head or heads <= 0 or heads % kv_heads or heads * head > width:
+        raise ValueError(f"qkv rows of {width} do not begin with {heads} query heads of {head}, a multiple of "
+                         f"{kv_heads} key heads")
+    if qkv.shape[0] != seqs or lengths.numel() != seqs:
+        raise ValueError(f"{seqs} sequences need a query row and a length each, got {qkv.shape[0]} and "
+                         f"{lengths.numel()}")
+    if out is None:
+        out = torch.empty((seqs, heads * head), dtype=torch.bfloat16, device=qkv.device)
+    _check(out, torch.bfloat16, "out")
+    if out.shape != (seqs, heads * head):
+        raise ValueError(f"out must be {(seqs, heads * head)}, got {tuple(out.shape)}")
+    _check_devices(qkv, cache=cache, lengths=lengths, out=out)
+    _launch_at(qkv, "tempo_decode_attention_q4", qkv.data_ptr(), _row_stride(qkv), cache.data_ptr(),
+               lengths.data_ptr(), length_offset, out.data_ptr(), seqs, heads, kv_heads, head, capacity)
+    return out
+
+
+# ---- scores of logits ----
+
+class TokenScores(NamedTuple):
+    """Per row: the given token's log probability and the entropy [rows]; the alternatives' log probabilities and ids
+    [rows, top], likeliest first (absent from the tuple's values when top is 0)."""
+
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    top_logprob: torch.Tensor | None = None
+    top_ids: torch.Tensor | None = None
+
+
+def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, *, top: int = 0,
+                   out: TokenScores | None = None) -> TokenScores:
+    """Log probabilities of ids[r] under softmax(logits[r]) (FP32 or BF16 rows at any stride), the rows' entropies in
+    nats and their `top` (at most 32) likeliest tokens, ties to the lower id. A row whose id is outside the vocabulary
+    (a padded row) scores 0; include/tempo_b200.h says what infinities and NaN give."""
+    bf16 = logits.dtype == torch.bfloat16
+    _check_rows(logits, torch.bfloat16 if bf16 else torch.float32, "logits")
+    _check(ids, torch.int32, "ids")
+    rows, vocab = logits.shape
+    if ids.numel() != rows:
+        raise ValueError(f"{rows} rows need as many ids, got {ids.numel()}")
+    if not 0 <= top <= min(32, vocab):
+        raise ValueError(f"top must be in [0, {min(32, vocab)}], got {top}")
+    if out is None:
+        # one allocation: the two or three FP32 outputs and the ids
+        words = torch.empty(rows * (2 + 2 * top), dtype=torch.float32, device=logits.device)
+        logprob, entropy = words[:rows], words[rows:2 * rows]
+        top_logprob = top_ids = None
+        if top:
+            top_logprob = words[2 * rows:(2 + top) * rows].view(rows, top)
+            top_ids = words[(2 + top) * rows:].view(torch.int32).view(rows, top)
+        out = TokenScores(logprob, entropy, top_logprob, top_ids)
+    else:
+        for name, t, shape, dtype in (("logprob", out.logprob, (rows,), torch.float32),
+                                      ("entropy", out.entropy, (rows,), torch.float32),
+                                      ("top_logprob", out.top_logprob, (rows, top), torch.float32),
+                                      ("top_ids", out.top_ids, (rows, top), torch.int32)):
+            if name.startswith("top") and not top:
+                continue
+            if t is None:
+                raise ValueError(f"out.{name} is needed for {top} alternatives")
+            _check(t, dtype, f"out.{name}")
+            if t.shape != shape:
+                raise ValueError(f"out.{name} must be {shape}, got {tuple(t.shape)}")
+    _check_devices(logits, ids=ids, logprob=out.logprob, entropy=out.entropy, top_logprob=out.top_logprob,
+                   top_ids=out.top_ids)
+    _launch_at(logits, "tempo_token_logprobs", logits.data_ptr(), _row_stride(logits), int(bf16), ids.data_ptr(), rows,
+               vocab, top, out.logprob.data_ptr(), out.entropy.data_ptr(), _ptr(out.top_logprob), _ptr(out.top_ids))
     return out
 
 

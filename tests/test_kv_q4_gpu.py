@@ -1,0 +1,341 @@
+"""The 4-bit key/value cache on a B200: stored rows read back as the definition says, bit for bit; decode attention over
+the cache against the softmax average in 64 bits (tests/_q4.py derives its bound); the entry points' refusals are in
+tests/test_q4_refusals_cpu.py."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from tests import _q4
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _device():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    from tempo_compiler_b200 import lib
+    lib.load()
+    yield
+    from tempo_compiler_b200 import ops
+    torch.cuda.synchronize()
+    assert ops.watchdog() == 0
+
+
+def _i32(values) -> "torch.Tensor":
+    return torch.as_tensor(np.asarray(values, np.int32), device="cuda")
+
+
+def _rows(rng, *shape) -> "torch.Tensor":
+    x = rng.standard_normal(shape) * np.exp(0.5 * rng.standard_normal((*shape[:-1], 1)))
+    return torch.from_numpy(x.astype(np.float32)).cuda().to(torch.bfloat16)
+
+
+def _expected(qkv: "torch.Tensor", kv_heads: int, head: int) -> np.ndarray:
+    """The BF16 rows a store and a load of qkv's key and value columns give, as float32."""
+    kv = qkv[:, qkv.shape[1] - 2 * kv_heads * head:].float().cpu().numpy()
+    value = _q4.dequantise(kv.reshape(kv.shape[0], -1, 64)).reshape(kv.shape)
+    return torch.from_numpy(value).to(torch.float32).to(torch.bfloat16).float().numpy()
+
+
+def _fill(cache, rng, heads: int = 0):
+    """Random rows at every place of a cache."""
+    from tempo_compiler_b200 import ops
+    seqs, kv_heads, tiles, size = cache.shape
+    head, capacity = size // 1152 * 64, tiles * 16
+    rows = _rows(rng, seqs * capacity, 2 * kv_heads, head).reshape(seqs * capacity, -1)
+    seq = _i32(np.repeat(np.arange(seqs), capacity))
+    ops.kv_store_q4(rows, cache, seq, _i32(np.tile(np.arange(capacity), seqs)))
+    return rows
+
+
+def _check_attention(qkv, cache, lengths, heads, got) -> None:
+    head = cache.shape[3] // 1152 * 64
+    q = qkv[:, :heads * head].double().cpu().numpy().reshape(cache.shape[0], heads, head)
+    want, bound = _q4.attend(q, cache.cpu().numpy(), lengths, heads)
+    error = np.abs(got.double().cpu().numpy().reshape(want.shape) - want)
+    assert np.isfinite(error).all()
+    worst = np.max(error / np.maximum(bound, 1e-30) * (error > 0))
+    assert worst <= 1.0, f"{worst:.3f} of the bound"
+
+
+# ---- storing and reading back -----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("heads,kv_heads,head", [(12, 12, 64), (0, 1, 64), (5, 5, 128), (8, 2, 128), (3, 3, 64)])
+@pytest.mark.parametrize("seqs,tokens", [(1, 1), (3, 17), (2, 130)])
+def test_stored_rows_read_back(heads: int, kv_heads: int, head: int, seqs: int, tokens: int) -> None:
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(heads * 131 + head + tokens)
+    qkv = _rows(rng, seqs * tokens, heads + 2 * kv_heads, head).reshape(seqs * tokens, -1)
+    cache = ops.kv_cache_q4(seqs, kv_heads, tokens + 9, head)
+    seq, pos = np.repeat(np.arange(seqs), tokens), np.tile(np.arange(tokens) + 9, seqs)
+    order = rng.permutation(seqs * tokens)
+    ops.kv_store_q4(qkv[torch.from_numpy(order).cuda()].contiguous(), cache, _i32(seq[order]), _i32(pos[order]))
+    got = ops.kv_load_q4(cache, _i32(seq), _i32(pos)).float().cpu().numpy()
+    np.testing.assert_array_equal(got, _expected(qkv, kv_heads, head))
+
+
+def test_rows_with_little_or_nothing_to_tell_apart() -> None:
+    """All-equal rows (scale 0), zeros, rows of two neighbouring values, wide ranges, signed zeros and subnormals."""
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(5)
+    base = rng.standard_normal((8, 128)).astype(np.float32)
+    base[0] = 0.0
+    base[1] = -3.25
+    base[2] = np.where(np.arange(128) % 2, 1.0, 1.0078125)
+    base[3] *= 1e30
+    base[4] *= 1e-30
+    base[5, ::2] = -0.0
+    base[6] = np.arange(128) % 16          # every quotient an integer
+    base[7] = (np.arange(128) % 31) * 0.5  # ties to even
+    qkv = torch.from_numpy(base).cuda().to(torch.bfloat16)
+    cache = ops.kv_cache_q4(1, 1, 16)
+    seq, pos = _i32(np.zeros(8)), _i32(np.arange(8))
+    ops.kv_store_q4(qkv, cache, seq, pos)
+    got = ops.kv_load_q4(cache, seq, pos).float().cpu().numpy()
+    np.testing.assert_array_equal(got, _expected(qkv, 1, 64))
+
+
+def test_rows_that_are_not_finite_read_as_nan_and_leave_the_others() -> None:
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(6)
+    qkv = _rows(rng, 4, 2, 64).reshape(4, 128)
+    qkv[1, 5], qkv[2, 70], qkv[3, 0], qkv[3, 1] = float("nan"), float("inf"), 3.0e38, -3.0e38
+    cache = ops.kv_cache_q4(1, 1, 16)
+    seq, pos = _i32(np.zeros(4)), _i32(np.arange(4))
+    ops.kv_store_q4(qkv, cache, seq, pos)
+    got = ops.kv_load_q4(cache, seq, pos)
+    assert torch.isnan(got[1, :64]).all() and torch.isnan(got[2, 64:]).all() and torch.isnan(got[3, :64]).all()
+    clean = torch.ones(4, 128, dtype=torch.bool)
+    clean[1, :64] = clean[2, 64:] = clean[3, :64] = False
+    want = _expected(torch.where(clean.cuda(), qkv, torch.zeros_like(qkv)), 1, 64)
+    np.testing.assert_array_equal(got.float().cpu().numpy()[clean.numpy()], want[clean.numpy()])
+
+
+def test_places_outside_the_cache_are_skipped_and_read_as_zeros() -> None:
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(7)
+    cache = ops.kv_cache_q4(2, 3, 32)
+    _fill(cache, rng)
+    before = cache.clone()
+    qkv = _rows(rng, 6, 9, 64).reshape(6, -1)
+    seq, pos = _i32([0, -1, 2, 1, 1, 1 << 30]), _i32([-1, 3, 3, 32, 1 << 30, 0])
+    ops.kv_store_q4(qkv, cache, seq, pos)
+    assert torch.equal(cache, before)
+    assert not ops.kv_load_q4(cache, seq, pos).any()
+    # one row inside: only its own place changes
+    ops.kv_store_q4(qkv, cache, _i32([1, -1, -1, -1, -1, -1]), _i32([17, 0, 0, 0, 0, 0]))
+    changed = (cache != before).nonzero()
+    assert set(changed[:, 0].tolist()) == {1} and set(changed[:, 2].tolist()) == {1}
+    inside = changed[:, 3]
+    slot = torch.where(inside < 1024, inside % 512 // 32, (inside - 1024) // 8)
+    assert set(slot.tolist()) == {1}
+
+
+def test_rows_at_a_stride_and_offset() -> None:
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(8)
+    wide = _rows(rng, 21, 9, 64).reshape(21, -1)
+    qkv = wide[:, 64:7 * 64]  # two query heads, two key and two value heads at a row stride of nine heads
+    cache = ops.kv_cache_q4(1, 2, 32)
+    seq, pos = _i32(np.zeros(21)), _i32(np.arange(21))
+    ops.kv_store_q4(qkv, cache, seq, pos)
+    out = torch.full((21, 2 * 2 * 64 + 8), 7.0, dtype=torch.bfloat16, device="cuda")
+    ops.kv_load_q4(cache, seq, pos, out=out[:, :256])
+    np.testing.assert_array_equal(out[:, :256].float().cpu().numpy(), _expected(qkv, 2, 64))
+    assert (out[:, 256:] == 7.0).all()
+    lengths = [21]
+    got = ops.decode_attention_q4(wide[:1, 64:7 * 64], cache, _i32(lengths))
+    _check_attention(wide[:1, 64:7 * 64], cache, lengths, 2, got)
+
+
+# ---- attention --------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("heads,kv_heads,head", [(12, 12, 64), (1, 1, 64), (8, 2, 64), (9, 1, 64), (40, 2, 64),
+                                                 (4, 4, 128), (14, 2, 128), (17, 1, 128)])
+@pytest.mark.parametrize("lengths", [[1], [15, 16, 17], [0, 1, 2, 63, 64, 65, 127, 400], [513, 0, 512, 300]])
+def test_attention_matches_the_average(heads: int, kv_heads: int, head: int, lengths: list[int]) -> None:
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(heads + head + len(lengths))
+    seqs = len(lengths)
+    cache = ops.kv_cache_q4(seqs, kv_heads, max(lengths), head)
+    _fill(cache, rng)
+    qkv = (_rows(rng, seqs, heads + 2 * kv_heads, head) * (1.5 / head ** 0.5)).reshape(seqs, -1)
+    got = ops.decode_attention_q4(qkv, cache, _i32(lengths))
+    _check_attention(qkv, cache, lengths, heads, got)
+    for s, n in enumerate(lengths):
+        if n == 0:
+            assert not got[s].any()
+    # the offset counts the step's own token, and lengths past the capacity are clamped to it
+    capacity = cache.shape[2] * 16
+    shifted = [n - 1 for n in lengths]
+    assert torch.equal(ops.decode_attention_q4(qkv, cache, _i32(shifted), length_offset=1), got)
+    far = ops.decode_attention_q4(qkv, cache, _i32([2 ** 31 - 1] * seqs), length_offset=2 ** 31 - 1)
+    assert torch.equal(far, ops.decode_attention_q4(qkv, cache, _i32([capacity] * seqs)))
+    none = ops.decode_attention_q4(qkv, cache, _i32([-2 ** 31] * seqs), length_offset=-2 ** 31)
+    assert not none.any()
+
+
+@pytest.mark.parametrize("seqs,heads,kv_heads,head,length", [(1, 12, 12, 64, 5000), (1, 4, 1, 128, 20011),
+                                                             (40, 12, 12, 64, 333), (150, 2, 1, 64, 97)])
+def test_attention_over_grids_of_every_shape(seqs: int, heads: int, kv_heads: int, head: int, length: int) -> None:
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(length)
+    cache = ops.kv_cache_q4(seqs, kv_heads, length, head)
+    _fill(cache, rng)
+    lengths = rng.integers(length // 2, length + 1, seqs)
+    lengths[0] = length
+    qkv = (_rows(rng, seqs, heads, head) * (1.5 / head ** 0.5)).reshape(seqs, -1)
+    got = ops.decode_attention_q4(qkv, cache, _i32(lengths), heads=heads)
+    _check_attention(qkv, cache, lengths, heads, got)
+
+
+def test_attention_reads_nothing_past_the_length() -> None:
+    """NaN rows and a later, far greater key behind the last position change nothing."""
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(11)
+    lengths = [1, 16, 29, 70]
+    cache = ops.kv_cache_q4(4, 2, 96)
+    _fill(cache, rng)
+    qkv = (_rows(rng, 4, 4, 64) * 0.2).reshape(4, -1)
+    want = ops.decode_attention_q4(qkv, cache, _i32(lengths), heads=4)
+    bad = _rows(rng, 4, 4, 64).reshape(4, -1) * 1e4
+    bad[2] = float("nan")
+    bad[3, 100] = float("inf")
+    for ahead in (0, 1, 2, 16, 25):
+        ops.kv_store_q4(bad, cache, _i32(np.arange(4)), _i32(np.asarray(lengths) + ahead))
+    assert torch.equal(ops.decode_attention_q4(qkv, cache, _i32(lengths), heads=4), want)
+
+
+@pytest.mark.parametrize("k_size,v_size,q_size", [(1.0, 1e-6, 1.0), (1.0, 1e20, 1.0), (1e-20, 1.0, 1.0),
+                                                  (30.0, 1.0, 3.0), (1e-4, 1e-30, 1e4), (1e4, 1.0, 1e-4)])
+def test_attention_over_keys_and_values_of_any_size(k_size: float, v_size: float, q_size: float) -> None:
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(12)
+    cache = ops.kv_cache_q4(2, 2, 200)
+    rows = _rows(rng, 400, 4, 64).float()
+    rows[:, :2] *= k_size
+    rows[:, 2:] *= v_size
+    rows[7::13, 2:] = 0.0   # value rows without any range
+    rows = rows.to(torch.bfloat16).reshape(400, -1)
+    ops.kv_store_q4(rows, cache, _i32(np.repeat([0, 1], 200)), _i32(np.tile(np.arange(200), 2)))
+    qkv = (_rows(rng, 2, 2, 64).float() * 0.2 * q_size).to(torch.bfloat16).reshape(2, -1)
+    got = ops.decode_attention_q4(qkv, cache, _i32([200, 131]), heads=2)
+    _check_attention(qkv, cache, [200, 131], 2, got)
+
+
+def test_scores_that_rise_and_fall_along_the_keys() -> None:
+    """The running maximum moves at every tile, or only at the first: a weight of all but one key vanishes."""
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(13)
+    n = 300
+    cache = ops.kv_cache_q4(2, 1, n)
+    rows = _rows(rng, 2 * n, 2, 64).float()
+    slope = np.concatenate([np.arange(n), np.arange(n)[::-1]]).astype(np.float32)
+    rows[:, 0] = rows[:, 0] * 0.1 + torch.from_numpy(slope).cuda()[:, None] * 0.05
+    rows = rows.to(torch.bfloat16).reshape(2 * n, -1)
+    ops.kv_store_q4(rows, cache, _i32(np.repeat([0, 1], n)), _i32(np.tile(np.arange(n), 2)))
+    qkv = torch.full((2, 64), 0.5, dtype=torch.bfloat16, device="cuda")
+    got = ops.decode_attention_q4(qkv, cache, _i32([n, n]), heads=1)
+    _check_attention(qkv, cache, [n, n], 1, got)
+
+
+def test_a_nan_key_or_value_within_the_length_shows_in_its_own_head() -> None:
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(14)
+    cache = ops.kv_cache_q4(1, 3, 64)
+    _fill(cache, rng)
+    qkv = (_rows(rng, 1, 3, 64) * 0.2).reshape(1, -1)
+    want = ops.decode_attention_q4(qkv, cache, _i32([64]), heads=3)
+    row = _rows(rng, 1, 6, 64).reshape(1, -1)
+    ops.kv_store_q4(row, cache, _i32([0]), _i32([40]))
+    want = ops.decode_attention_q4(qkv, cache, _i32([64]), heads=3)
+    row[0, 3] = float("nan")            # key head 0
+    row[0, 5 * 64 + 1] = float("inf")   # value head 2
+    ops.kv_store_q4(row, cache, _i32([0]), _i32([40]))
+    got = ops.decode_attention_q4(qkv, cache, _i32([64]), heads=3)
+    assert torch.isnan(got[:, :64]).all() and torch.isnan(got[:, 128:]).all()
+    assert torch.equal(got[:, 64:128], want[:, 64:128])
+
+
+def test_a_slice_of_sequences_is_a_cache_and_its_neighbours_stay() -> None:
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(15)
+    cache = ops.kv_cache_q4(5, 2, 48)
+    _fill(cache, rng)
+    before = cache.clone()
+    qkv = _rows(rng, 2, 6, 64).reshape(2, -1)
+    part = cache[2:4]
+    ops.kv_store_q4(qkv, part, _i32([0, 1]), _i32([5, 47]))
+    assert torch.equal(cache[:2], before[:2]) and torch.equal(cache[4:], before[4:])
+    out = torch.full((4, 128), 3.0, dtype=torch.bfloat16, device="cuda")
+    ops.decode_attention_q4(qkv, part, _i32([6, 48]), out=out[1:3])
+    _check_attention(qkv, part, [6, 48], 2, out[1:3])
+    assert (out[0] == 3.0).all() and (out[3] == 3.0).all()
+
+
+def test_offsets_past_32_bits() -> None:
+    """The last sequence of a cache of more than 4 GiB."""
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(16)
+    seqs, capacity = 5, 1 << 20  # 5 x 12 x 65536 tiles x 1152 bytes = 4.5 GB
+    cache = ops.kv_cache_q4(seqs, 12, capacity)
+    assert cache.numel() > 1 << 32
+    qkv = _rows(rng, 3, 36, 64).reshape(3, -1)
+    seq, pos = _i32([4, 4, 4]), _i32([0, 1, capacity - 1])
+    ops.kv_store_q4(qkv, cache, seq, pos)
+    np.testing.assert_array_equal(ops.kv_load_q4(cache, seq, pos).float().cpu().numpy(), _expected(qkv, 12, 64))
+    q = (_rows(rng, seqs, 12, 64) * 0.2).reshape(seqs, -1)
+    got = ops.decode_attention_q4(q, cache, _i32([0, 0, 0, 0, 2]), heads=12)
+    assert not got[:4].any()
+    _check_attention(q[4:], cache[4:, :, :1], [2], 12, got[4:])
+
+
+def test_store_and_attention_in_one_graph_on_another_stream() -> None:
+    """A decode step's append and attention, captured once and replayed with other rows, against the eager calls."""
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(17)
+    seqs = 7
+    cache = ops.kv_cache_q4(seqs, 4, 80)
+    _fill(cache, rng)
+    qkv = (_rows(rng, seqs, 12, 64) * 0.3).reshape(seqs, -1)
+    seq, pos = _i32(np.arange(seqs)), _i32(rng.integers(0, 79, seqs))
+    out = torch.zeros((seqs, 256), dtype=torch.bfloat16, device="cuda")
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        ops.kv_store_q4(qkv, cache, seq, pos)
+        ops.decode_attention_q4(qkv, cache, pos, length_offset=1, out=out)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            ops.kv_store_q4(qkv, cache, seq, pos)
+            ops.decode_attention_q4(qkv, cache, pos, length_offset=1, out=out)
+            pos += 1
+    stream.synchronize()
+    eager_cache, eager_pos = cache.clone(), pos.clone()
+    for step in range(3):
+        qkv.copy_((_rows(rng, seqs, 12, 64) * 0.3).reshape(seqs, -1))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        stream.synchronize()
+        ops.kv_store_q4(qkv, eager_cache, seq, eager_pos)
+        want = ops.decode_attention_q4(qkv, eager_cache, eager_pos, length_offset=1)
+        eager_pos += 1
+        assert torch.equal(out, want) and torch.equal(cache, eager_cache)
+
+
+def test_the_same_inputs_give_the_same_bits() -> None:
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(18)
+    cache = ops.kv_cache_q4(3, 4, 3000)
+    _fill(cache, rng)
+    qkv = (_rows(rng, 3, 8, 64) * 0.2).reshape(3, -1)
+    lengths = _i32([3000, 1777, 5])
+    first = ops.decode_attention_q4(qkv, cache, lengths, heads=8)
+    for _ in range(5):
+        assert torch.equal(ops.decode_attention_q4(qkv, cache, lengths, heads=8), first)
