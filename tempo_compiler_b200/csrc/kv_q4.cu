@@ -2,6 +2,7 @@
 // Each row of 64 dimensions keeps its least value (exact in BF16) and a BF16 scale, so a position costs 72 bytes per
 // head and 64 dimensions for key and value together, against 256 in BF16.
 #include <cuda.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include "common.cuh"
@@ -10,6 +11,9 @@
 #include "kv_q4.cuh"
 
 namespace tempo {
+
+TEMPO_WATCHDOG_READER(watchdog_kv_q4)
+
 namespace {
 
 constexpr uint32_t kStoreThreads = 256;
@@ -99,90 +103,415 @@ __global__ void __launch_bounds__(kStoreThreads) kv_load_q4_kernel(const uint8_t
   *dst = pack8(x);
 }
 
-// One CTA per (query head, sequence), four warps; eight lanes per key, 8 dimensions of each group per lane, an online
-// softmax per lane group, merged over lane groups and warps at the end.
+// ---------------------------------------------------------------------------------------------------------------
+// Decode attention
+//
+// At 72 bytes a position the cache streams past at more than 40 codes per clock and SM, which CUDA cores cannot
+// dequantise, multiply and add in FP32 (a first kernel that did so took 4 to 150 times the read time), so both products
+// run on mma.sync with the codes as the A operand: key codes enter as the BF16 integers 128 + code and value codes as
+// the FP16 integers 64 + code, which are two logic operations per pair of codes, and scale, low and the constants are
+// applied to the products: with D = sum_d q_d (128 + code_d) and Q = sum_d q_d,
+//   q . k = scale D + (low - 128 scale) Q,
+//   sum_j p_j v_j = sum_j w_j (64 + code_j) - 64 sum_j w_j + sum_j p_j low_j,   w_j = p_j scale_j.
+// The B operand holds up to eight query heads of one key / value head (m16n8k16), so grouped heads read the cache once.
+// q is exact in BF16; w is rounded to FP16 (2^-11 of each weight; an eighth of the output's own BF16 rounding), relative
+// to a running reference that bounds w and p low alike; everything else, the sums included, is FP32.
+//
+// A CTA of four warps takes a run of tiles of one (sequence, key / value head, eight query heads); each warp streams its
+// own two-tile pieces (one bulk copy each, a ring of kRing in flight) and keeps an online softmax whose reference moves
+// only when a score passes it by 2^kSlack. Warps merge through shared memory; with `chunks` > 1 the CTAs of a cluster
+// split the positions and merge through distributed shared memory.
+// ---------------------------------------------------------------------------------------------------------------
+
+constexpr uint32_t kQ4MaxChunks = 16;
+constexpr uint32_t kQ4Queries = 8;
+constexpr uint32_t kQ4Piece = 2 * kQ4Block;  // bytes of one bulk copy: two tiles of a 64-wide head, one of a 128-wide
+constexpr uint32_t kRing = 4;
+constexpr float kSlack = 6.f;
+
 template <int G>
-__global__ void __launch_bounds__(128) decode_attention_q4_kernel(const uint16_t* __restrict__ q_rows, uint32_t ldq,
-                                                                  const uint8_t* __restrict__ cache,
-                                                                  const int32_t* __restrict__ lengths,
-                                                                  int32_t length_offset, uint16_t* __restrict__ out,
-                                                                  uint32_t heads, uint32_t kv_heads, uint32_t tiles) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const uint32_t h = blockIdx.x, s = blockIdx.y, warp = warp_id(), lane = lane_id();
-  const uint32_t g = lane >> 3, li = lane & 7u, kvh = h / (heads / kv_heads);
-  const int64_t want = int64_t(lengths[s]) + length_offset;
-  const uint32_t capacity = tiles * kQ4Tile;
-  const uint32_t len = want <= 0 ? 0u : want < int64_t(capacity) ? uint32_t(want) : capacity;
-  float q[G][8], acc[G][8], qsum[G], m = -INFINITY, l = 0.f;
+struct Q4Smem {
+  static constexpr uint32_t kWarpRing = kRing * kQ4Piece;
+  static constexpr uint32_t kPart = kQ4Queries * (64 * G + 2) * 4;  // (values, max, sum) of eight queries
+  static constexpr uint32_t kBarrierOffset = 4 * kWarpRing;
+  static constexpr uint32_t kMergeOffset = kBarrierOffset + 4 * kRing * 8;
+  static constexpr uint32_t kBytes = kMergeOffset + kPart;
+  static_assert(kPart <= kWarpRing, "a warp's partial result fits its ring");
+  static_assert(kBytes <= 48 * 1024, "fits without an opt-in");
+};
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The transpose of an 8 x 8 matrix of 16-bit words held two per lane (row lane / 4, columns 2 (lane % 4) and + 1).
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ float fast_log2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two codes, `shift` bits up in each half of w, as the BF16 integers 128 + code / the FP16 integers 64 + code.
+__device__ __forceinline__ uint32_t key_pair(uint32_t w, uint32_t shift) {
+  return ((w >> shift) & 0x000F000Fu) | 0x43004300u;
+}
+template <int NIBBLE>
+__device__ __forceinline__ uint32_t value_pair(uint32_t w) {
+  const uint32_t x = NIBBLE == 0 ? w << 4 : w >> (4 * (NIBBLE - 1));
+  return (x & 0x00F000F0u) | 0x54005400u;
+}
+
+// One warp's running state. The MMA fragments put query columns 2 t and 2 t + 1 (t = lane % 4) on a lane; with
+// g = lane / 4, acc[i][n] holds dimensions 64 i + 8 g + n ([0], [1]) and 64 i + 8 g + 4 + n ([2], [3]) of the two.
+template <int G>
+struct Q4State {
+  float acc[G][4][4];
+  float m[2], l[2];          // the reference (log2 of p times the value's size) and this lane's sum of p
+  float w[G][2], low[G][2];  // this lane's sums of w (as rounded) and of p low
+};
+
+// Folds the 16 positions of one tile in shared memory into the state; `left` positions of it exist.
+template <int G>
+__device__ __forceinline__ void q4_tile(Q4State<G>& st, const uint32_t (&qf)[G][8], const float (&qs)[G][2],
+                                        const uint8_t* tile, uint32_t left, uint32_t g, uint32_t t) {
+  // Row r of the score MMA is position pi(r) (r < 8) or 8 + pi(r - 8), pi = 0 2 1 3 6 4 7 5: the key words of eight lanes
+  // groups, and the value words of the even and of the odd rows, then fall into different banks.
+  const uint32_t pg = g & 1u ? (g >> 1) + 2 : (g < 4 ? g >> 1 : (g >> 1) + 4);
+  const uint32_t pe = t < 2 ? t : t + 4, po = t + 2;  // pi(2 t), pi(2 t + 1)
+  float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;  // scores (log2): rows g and g + 8, query columns 2 t and 2 t + 1
+  float size0 = 0x1p-100f, size1 = 0x1p-100f;
+  uint32_t vm0[G], vm1[G];
+  const bool in0 = pg < left, in1 = pg + 8 < left;
 #pragma unroll
   for (int i = 0; i < G; ++i) {
-    load8(*reinterpret_cast<const uint4*>(q_rows + size_t(s) * ldq + h * (64 * G) + i * 64 + li * 8), q[i]);
-    qsum[i] = 0.f;
-#pragma unroll
-    for (int d = 0; d < 8; ++d) {
-      q[i][d] *= kDecodeLog2e;
-      qsum[i] += q[i][d];
-      acc[i][d] = 0.f;
-    }
+    const uint8_t* block = tile + i * kQ4Block;
+    const uint2 k0 = *reinterpret_cast<const uint2*>(block + pg * 32 + t * 8);
+    const uint2 k1 = *reinterpret_cast<const uint2*>(block + (pg + 8) * 32 + t * 8);
+    uint2 meta0 = *reinterpret_cast<const uint2*>(block + 2 * kQ4Codes + pg * 8);
+    uint2 meta1 = *reinterpret_cast<const uint2*>(block + 2 * kQ4Codes + (pg + 8) * 8);
+    if (!in0) meta0 = make_uint2(0, 0);  // what lies behind the last position may be anything
+    if (!in1) meta1 = make_uint2(0, 0);
+    float d[4] = {0.f, 0.f, 0.f, 0.f};
+    mma_bf16(d, key_pair(k0.x, 0), key_pair(k1.x, 0), key_pair(k0.x, 4), key_pair(k1.x, 4), qf[i][0], qf[i][1]);
+    mma_bf16(d, key_pair(k0.x, 8), key_pair(k1.x, 8), key_pair(k0.x, 12), key_pair(k1.x, 12), qf[i][2], qf[i][3]);
+    mma_bf16(d, key_pair(k0.y, 0), key_pair(k1.y, 0), key_pair(k0.y, 4), key_pair(k1.y, 4), qf[i][4], qf[i][5]);
+    mma_bf16(d, key_pair(k0.y, 8), key_pair(k1.y, 8), key_pair(k0.y, 12), key_pair(k1.y, 12), qf[i][6], qf[i][7]);
+    const float ks0 = bf16_lo(meta0.x), ks1 = bf16_lo(meta1.x);
+    const float kl0 = fmaf(-128.f, ks0, bf16_hi(meta0.x)), kl1 = fmaf(-128.f, ks1, bf16_hi(meta1.x));
+    s0 = fmaf(ks0, d[0], fmaf(kl0, qs[i][0], s0));
+    s1 = fmaf(ks0, d[1], fmaf(kl0, qs[i][1], s1));
+    s2 = fmaf(ks1, d[2], fmaf(kl1, qs[i][0], s2));
+    s3 = fmaf(ks1, d[3], fmaf(kl1, qs[i][1], s3));
+    vm0[i] = meta0.y;
+    vm1[i] = meta1.y;
+    size0 = fmaxf(size0, fmaxf(bf16_lo(meta0.y), 0.0625f * fabsf(bf16_hi(meta0.y))));
+    size1 = fmaxf(size1, fmaxf(bf16_lo(meta1.y), 0.0625f * fabsf(bf16_hi(meta1.y))));
   }
-  for (uint32_t base = warp * 4; base < len; base += 16) {
-    const uint32_t key = base + g;
-    float score = 0.f;
-    uint32_t vw[G], vm[G];
-    if (key < len) {
+  s0 = in0 ? s0 * kDecodeLog2e : -INFINITY;
+  s1 = in0 ? s1 * kDecodeLog2e : -INFINITY;
+  s2 = in1 ? s2 * kDecodeLog2e : -INFINITY;
+  s3 = in1 ? s3 * kDecodeLog2e : -INFINITY;
+  // The reference follows log2(p size), size the value row's scale or a sixteenth of its low: w and p low stay small
+  // whatever the values' size, and a position of small values needs a larger p to move it.
+  const float g0 = fast_log2(fminf(size0, 0x1p100f)), g1 = fast_log2(fminf(size1, 0x1p100f));
+  float x0 = fmaxf(s0 + g0, s2 + g1), x1 = fmaxf(s1 + g0, s3 + g1);
+  if (__any_sync(0xFFFFFFFFu, x0 > st.m[0] + kSlack || x1 > st.m[1] + kSlack)) {
 #pragma unroll
-      for (int i = 0; i < G; ++i) {
-        const uint8_t* block = cache + q4_block(s, kvh, key, i, kv_heads, tiles, G);
-        const uint32_t slot = key % kQ4Tile;
-        const uint32_t kw = reinterpret_cast<const uint32_t*>(block + slot * 32)[li];
-        vw[i] = reinterpret_cast<const uint32_t*>(block + kQ4Codes + slot * 32)[li];
-        const uint2 meta = reinterpret_cast<const uint2*>(block + 2 * kQ4Codes)[slot];
-        vm[i] = meta.y;
-        float dot = 0.f;
+    for (int o = 4; o <= 16; o <<= 1) {
+      x0 = fmaxf(x0, __shfl_xor_sync(0xFFFFFFFFu, x0, o));
+      x1 = fmaxf(x1, __shfl_xor_sync(0xFFFFFFFFu, x1, o));
+    }
+    x0 = fmaxf(x0, st.m[0]);
+    x1 = fmaxf(x1, st.m[1]);
+    const float c0 = x0 == st.m[0] ? 1.f : fast_exp2(st.m[0] - x0), c1 = x1 == st.m[1] ? 1.f : fast_exp2(st.m[1] - x1);
+    st.m[0] = x0;
+    st.m[1] = x1;
+    st.l[0] *= c0;
+    st.l[1] *= c1;
 #pragma unroll
-        for (int d = 0; d < 8; ++d) dot = fmaf(q[i][d], float((kw >> (4 * d)) & 15u), dot);
-        score = fmaf(dot, bf16_lo(meta.x), fmaf(qsum[i], bf16_hi(meta.x), score));
+    for (int i = 0; i < G; ++i) {
+      st.w[i][0] *= c0;
+      st.w[i][1] *= c1;
+      st.low[i][0] *= c0;
+      st.low[i][1] *= c1;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        st.acc[i][n][0] *= c0;
+        st.acc[i][n][1] *= c1;
+        st.acc[i][n][2] *= c0;
+        st.acc[i][n][3] *= c1;
       }
     }
+  }
+  const float p0 = fast_exp2(s0 - st.m[0]), p1 = fast_exp2(s1 - st.m[1]);
+  const float p2 = fast_exp2(s2 - st.m[0]), p3 = fast_exp2(s3 - st.m[1]);
+  st.l[0] += p0 + p2;
+  st.l[1] += p1 + p3;
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) score += __shfl_xor_sync(0xFFFFFFFFu, score, o);
-    if (key < len) {
-      const float m_new = fmaxf(m, score), c = fast_exp2(m - m_new), p = fast_exp2(score - m_new);
-      m = m_new;
-      l = l * c + p;
+  for (int i = 0; i < G; ++i) {
+    const uint8_t* words = tile + i * kQ4Block + kQ4Codes + g * 4;
+    const uint32_t va = *reinterpret_cast<const uint32_t*>(words + pe * 32);
+    const uint32_t vb = *reinterpret_cast<const uint32_t*>(words + po * 32);
+    const uint32_t vc = *reinterpret_cast<const uint32_t*>(words + (pe + 8) * 32);
+    const uint32_t vd = *reinterpret_cast<const uint32_t*>(words + (po + 8) * 32);
+    const float vs0 = bf16_lo(vm0[i]), vs1 = bf16_lo(vm1[i]), vl0 = bf16_hi(vm0[i]), vl1 = bf16_hi(vm1[i]);
+    const __half2 h0 = __floats2half2_rn(p0 * vs0, p1 * vs0), h1 = __floats2half2_rn(p2 * vs1, p3 * vs1);
+    const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+    st.w[i][0] += f0.x + f1.x;
+    st.w[i][1] += f0.y + f1.y;
+    st.low[i][0] = fmaf(p0, vl0, fmaf(p2, vl1, st.low[i][0]));
+    st.low[i][1] = fmaf(p1, vl0, fmaf(p3, vl1, st.low[i][1]));
+    const uint32_t b0 = transpose8x8(*reinterpret_cast<const uint32_t*>(&h0));
+    const uint32_t b1 = transpose8x8(*reinterpret_cast<const uint32_t*>(&h1));
+    // The same dimension of two positions side by side: dimensions 8 g .. + 3 in e0 / e1, 8 g + 4 .. in f0 / f1.
+    const uint32_t e0 = __byte_perm(va, vb, 0x5410), o0 = __byte_perm(va, vb, 0x7632);
+    const uint32_t e1 = __byte_perm(vc, vd, 0x5410), o1 = __byte_perm(vc, vd, 0x7632);
+    mma_f16(st.acc[i][0], value_pair<0>(e0), value_pair<0>(o0), value_pair<0>(e1), value_pair<0>(o1), b0, b1);
+    mma_f16(st.acc[i][1], value_pair<1>(e0), value_pair<1>(o0), value_pair<1>(e1), value_pair<1>(o1), b0, b1);
+    mma_f16(st.acc[i][2], value_pair<2>(e0), value_pair<2>(o0), value_pair<2>(e1), value_pair<2>(o1), b0, b1);
+    mma_f16(st.acc[i][3], value_pair<3>(e0), value_pair<3>(o0), value_pair<3>(e1), value_pair<3>(o1), b0, b1);
+  }
+}
+
+__device__ __forceinline__ float ld_cluster(const float* local, uint32_t rank) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(local)), "r"(rank));
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+  return v;
+}
+
+struct Q4Attention {
+  const uint16_t* q;
+  const uint8_t* cache;
+  const int32_t* lengths;
+  uint16_t* out;
+  uint32_t ldq, heads, kv_heads, tiles;
+  int32_t length_offset;
+  uint32_t blocks;  // groups of eight query heads per key / value head
+  uint32_t early;   // the grid is resident at once: the next kernel may start at entry
+};
+
+template <int G>
+__global__ void __launch_bounds__(128) decode_attention_q4_kernel(Q4Attention p) {
+  using L = Q4Smem<G>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr uint32_t kWidth = 64 * G, kTileBytes = G * kQ4Block, kPieceTiles = kQ4Piece / kTileBytes;
+  const uint32_t warp = warp_id(), lane = lane_id(), g = lane >> 2, t = lane & 3u;
+  const uint32_t chunks = gridDim.x, chunk = blockIdx.x, s = blockIdx.z;
+  const uint32_t kvh = blockIdx.y / p.blocks, share = p.heads / p.kv_heads;
+  const uint32_t first = (blockIdx.y % p.blocks) * kQ4Queries;  // of the key / value head's query heads
+  const uint32_t queries = min(kQ4Queries, share - first);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarrierOffset) + warp * kRing;
+  uint8_t* ring = smem + warp * L::kWarpRing;
+  if (lane == 0) {
 #pragma unroll
-      for (int i = 0; i < G; ++i)
+    for (uint32_t i = 0; i < kRing; ++i) mbar_init(&full[i], 1);
+    fence_barrier_init();
+  }
+  __syncwarp();
+  if (p.early) pdl_launch_dependents();
+  pdl_wait();
+
+  const int64_t want = int64_t(p.lengths[s]) + p.length_offset;
+  const uint32_t capacity = p.tiles * kQ4Tile;
+  const uint32_t len = want <= 0 ? 0u : want < int64_t(capacity) ? uint32_t(want) : capacity;
+  // The CTA's tiles [t_begin, t_end); its warps take pieces of kPieceTiles in turn.
+  const uint32_t used = (len + kQ4Tile - 1) / kQ4Tile, per = (used + chunks - 1) / chunks;
+  const uint32_t t_begin = min(used, chunk * per), t_end = min(used, t_begin + per);
+  const uint8_t* base = p.cache + (size_t(s) * p.kv_heads + kvh) * p.tiles * kTileBytes;
+  const uint32_t pieces = (t_end - t_begin + kPieceTiles - 1) / kPieceTiles;
+  auto fetch = [&](uint32_t piece, uint32_t slot) {
+    const uint32_t tile = t_begin + piece * kPieceTiles, count = min(kPieceTiles, t_end - tile);
+    mbar_arrive_expect_tx(&full[slot], count * kTileBytes);
+    bulk_load(ring + slot * kQ4Piece, base + size_t(tile) * kTileBytes, count * kTileBytes, &full[slot]);
+  };
+  if (lane == 0) {
 #pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          const float v = fmaf(float((vw[i] >> (4 * d)) & 15u), bf16_lo(vm[i]), bf16_hi(vm[i]));
-          acc[i][d] = fmaf(p, v, acc[i][d] * c);
+    for (uint32_t i = 0; i < kRing; ++i)
+      if (warp + 4 * i < pieces) fetch(warp + 4 * i, i);
+  }
+
+  // The query fragments: lane (g, t) holds dimensions 16 t .. 16 t + 15 of each group of query g.
+  uint32_t qf[G][8];
+  float qs[G][2];
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    float sum = 0.f;
+    uint4 a = make_uint4(0, 0, 0, 0), b = a;
+    if (g < queries) {
+      const uint4* q4 = reinterpret_cast<const uint4*>(p.q + size_t(s) * p.ldq +
+                                                       size_t(kvh * share + first + g) * kWidth + i * 64 + t * 16);
+      a = q4[0];
+      b = q4[1];
+    }
+    // key_pair(word, 4 n) gives dimensions n and n + 4 of a word's eight.
+    qf[i][0] = __byte_perm(a.x, a.z, 0x5410);
+    qf[i][1] = __byte_perm(a.x, a.z, 0x7632);
+    qf[i][2] = __byte_perm(a.y, a.w, 0x5410);
+    qf[i][3] = __byte_perm(a.y, a.w, 0x7632);
+    qf[i][4] = __byte_perm(b.x, b.z, 0x5410);
+    qf[i][5] = __byte_perm(b.x, b.z, 0x7632);
+    qf[i][6] = __byte_perm(b.y, b.w, 0x5410);
+    qf[i][7] = __byte_perm(b.y, b.w, 0x7632);
+    float f[8];
+    unpack8(a, f);
+#pragma unroll
+    for (int d = 0; d < 8; ++d) sum += f[d];
+    unpack8(b, f);
+#pragma unroll
+    for (int d = 0; d < 8; ++d) sum += f[d];
+    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
+    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+    qs[i][0] = __shfl_sync(0xFFFFFFFFu, sum, 8 * t);      // the lane's own query columns, 2 t and 2 t + 1
+    qs[i][1] = __shfl_sync(0xFFFFFFFFu, sum, 8 * t + 4);
+  }
+
+  Q4State<G> st;
+  st.m[0] = st.m[1] = -INFINITY;
+  st.l[0] = st.l[1] = 0.f;
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    st.w[i][0] = st.w[i][1] = st.low[i][0] = st.low[i][1] = 0.f;
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) st.acc[i][n][c] = 0.f;
+  }
+  uint32_t slot = 0, phase = 0, limit = pieces;
+  bool ok = true;
+  for (uint32_t piece = warp; piece < limit; piece += 4) {
+    const bool landed = mbar_wait(&full[slot], phase, kWatchFull, nullptr);
+    if (ok && !__all_sync(0xFFFFFFFFu, landed)) {
+      // A copy that does not land: nothing more is issued, and the copies in flight are each waited for, bounded.
+      ok = false;
+      limit = min(limit, piece + 4 * kRing);
+    }
+    if (ok) {
+      const uint32_t tile = t_begin + piece * kPieceTiles;
+#pragma unroll
+      for (uint32_t i = 0; i < kPieceTiles; ++i)
+        if (tile + i < t_end)
+          q4_tile<G>(st, qf, qs, ring + slot * kQ4Piece + i * kTileBytes, len - (tile + i) * kQ4Tile, g, t);
+      __syncwarp();
+      if (lane == 0 && piece + 4 * kRing < pieces) fetch(piece + 4 * kRing, slot);
+    }
+    if (++slot == kRing) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+  if (!p.early) pdl_launch_dependents();
+
+  // The warp's partial result: (values at the reference, reference, sum) of each query, into its own ring.
+  __syncwarp();
+  float* part = reinterpret_cast<float*>(ring);
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+#pragma unroll
+    for (int o = 4; o <= 16; o <<= 1) st.l[c] += __shfl_xor_sync(0xFFFFFFFFu, st.l[c], o);
+    const uint32_t query = 2 * t + c;
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      float rest = fmaf(-64.f, st.w[i][c], st.low[i][c]);
+#pragma unroll
+      for (int o = 4; o <= 16; o <<= 1) rest += __shfl_xor_sync(0xFFFFFFFFu, rest, o);
+      if (query < queries) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          part[query * kWidth + i * 64 + 8 * g + n] = st.acc[i][n][c] + rest;
+          part[query * kWidth + i * 64 + 8 * g + 4 + n] = st.acc[i][n][2 + c] + rest;
         }
+      }
+    }
+    if (g == 0 && query < queries) {
+      part[kQ4Queries * kWidth + query] = st.m[c];
+      part[kQ4Queries * kWidth + kQ4Queries + query] = st.l[c];
     }
   }
-  __shared__ float sm_m[16], sm_l[16], sm_acc[16][64 * G];
-  const uint32_t part = warp * 4 + g;
-  if (li == 0) {
-    sm_m[part] = m;
-    sm_l[part] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < G; ++i)
-#pragma unroll
-    for (int d = 0; d < 8; ++d) sm_acc[part][i * 64 + li * 8 + d] = acc[i][d];
   __syncthreads();
-  if (threadIdx.x < 64 * G) {
-    float mm = -INFINITY, ll = 0.f, aa = 0.f;
-    for (int w = 0; w < 16; ++w)
-      if (sm_l[w] != 0.f) mm = fmaxf(mm, sm_m[w]);
-    for (int w = 0; w < 16; ++w) {
-      if (sm_l[w] == 0.f) continue;
-      const float f = fast_exp2(sm_m[w] - mm);
-      ll = fmaf(sm_l[w], f, ll);
-      aa = fmaf(sm_acc[w][threadIdx.x], f, aa);
+  float* merge = reinterpret_cast<float*>(smem + L::kMergeOffset);
+  uint16_t* out = p.out + (size_t(s) * p.heads + kvh * share + first) * kWidth;
+  for (uint32_t i = threadIdx.x; i < queries * kWidth; i += 128) {
+    const uint32_t query = i / kWidth;
+    float m = -INFINITY, l = 0.f, a = 0.f;
+#pragma unroll
+    for (uint32_t w = 0; w < 4; ++w)
+      m = fmaxf(m, reinterpret_cast<const float*>(smem + w * L::kWarpRing)[kQ4Queries * kWidth + query]);
+#pragma unroll
+    for (uint32_t w = 0; w < 4; ++w) {
+      const float* other = reinterpret_cast<const float*>(smem + w * L::kWarpRing);
+      const float f = fast_exp2(other[kQ4Queries * kWidth + query] - m);
+      l = fmaf(other[kQ4Queries * kWidth + kQ4Queries + query], f, l);
+      a = fmaf(other[i], f, a);
     }
-    out[size_t(s) * heads * (64 * G) + h * (64 * G) + threadIdx.x] = float_to_bf16(len == 0 ? 0.f : aa / ll);
+    if (chunks == 1) {
+      out[i] = float_to_bf16(len == 0 ? 0.f : a / l);
+    } else {
+      // (A CTA without positions has m = -inf on every warp, and must not hand on the NaN of -inf - -inf.)
+      merge[i] = t_begin == t_end ? 0.f : a;
+      if (i % kWidth == 0) {
+        merge[kQ4Queries * kWidth + query] = m;
+        merge[kQ4Queries * kWidth + kQ4Queries + query] = t_begin == t_end ? 0.f : l;
+      }
+    }
   }
+  if (chunks == 1) return;
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  // Each CTA finishes its share of the outputs, reading every CTA's partial result.
+  for (uint32_t i = chunk * 128 + threadIdx.x; i < queries * kWidth; i += chunks * 128) {
+    const uint32_t query = i / kWidth;
+    float m = -INFINITY, l = 0.f, a = 0.f;
+    for (uint32_t c = 0; c < chunks; ++c) m = fmaxf(m, ld_cluster(merge + kQ4Queries * kWidth + query, c));
+    for (uint32_t c = 0; c < chunks; ++c) {
+      const float f = fast_exp2(ld_cluster(merge + kQ4Queries * kWidth + query, c) - m);
+      l = fmaf(ld_cluster(merge + kQ4Queries * kWidth + kQ4Queries + query, c), f, l);
+      a = fmaf(ld_cluster(merge + i, c), f, a);
+    }
+    out[i] = float_to_bf16(len == 0 ? 0.f : a / l);
+  }
+  // No CTA leaves while another may still read its shared memory.
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+template <int G>
+tempo_status launch_attention(const Q4Attention& base, uint32_t seqs, cudaStream_t stream) {
+  Q4Attention p = base;
+  const uint32_t share = p.heads / p.kv_heads;
+  p.blocks = (share + kQ4Queries - 1) / kQ4Queries;
+  const uint64_t pairs = uint64_t(p.kv_heads) * p.blocks * seqs, target = 2 * uint64_t(sm_count());
+  uint32_t chunks = 1;
+  while (chunks < kQ4MaxChunks && pairs * chunks < target && p.tiles >= 8 * chunks) chunks *= 2;
+  auto kernel = decode_attention_q4_kernel<G>;
+  if (chunks > 8) {
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute(non-portable cluster size)");
+  }
+  p.early = single_wave(pairs * chunks, 4);
+  return launch(kernel, dim3(chunks, p.kv_heads * p.blocks, seqs), dim3(128), Q4Smem<G>::kBytes, stream, chunks,
+                "decode_attention_q4_kernel", p);
 }
 
 // What the three entry points check alike; `what` names the call.
@@ -246,17 +575,25 @@ extern "C" tempo_status tempo_decode_attention_q4(const void* q, uint32_t ldq, c
                                                   uint32_t capacity, void* stream) {
   tempo_status status = check_cache("tempo_decode_attention_q4", cache, seqs, kv_heads, head, capacity);
   if (status != TEMPO_OK) return status;
-  if (heads == 0 || heads % kv_heads || seqs > 65535 || kv_heads > 65535)
+  if (heads == 0 || heads % kv_heads || seqs > 65535 || heads > 65535)
     return fail(TEMPO_ERR_VALUE, "tempo_decode_attention_q4: seqs %u (up to 65535), heads %u must be a multiple of "
-                "kv_heads %u (up to 65535)", seqs, heads, kv_heads);
+                "kv_heads %u (both up to 65535)", seqs, heads, kv_heads);
   if (uint64_t(heads) * head > ldq || ldq % 8)
     return fail(TEMPO_ERR_VALUE, "tempo_decode_attention_q4: the query row stride %u must be a multiple of 8 and at "
                 "least %llu", ldq, static_cast<unsigned long long>(uint64_t(heads) * head));
   if (q == nullptr || !aligned16(q) || out == nullptr || !aligned16(out) || lengths == nullptr)
     return fail(TEMPO_ERR_VALUE, "tempo_decode_attention_q4: 16-byte aligned queries and output and the lengths are "
                 "needed");
-  auto kernel = head == 64 ? decode_attention_q4_kernel<1> : decode_attention_q4_kernel<2>;
-  return launch(kernel, dim3(heads, seqs), dim3(128), 0, static_cast<cudaStream_t>(stream), 1,
-                "decode_attention_q4_kernel", static_cast<const uint16_t*>(q), ldq, static_cast<const uint8_t*>(cache),
-                lengths, length_offset, static_cast<uint16_t*>(out), heads, kv_heads, capacity / kQ4Tile);
+  Q4Attention p{};
+  p.q = static_cast<const uint16_t*>(q);
+  p.cache = static_cast<const uint8_t*>(cache);
+  p.lengths = lengths;
+  p.out = static_cast<uint16_t*>(out);
+  p.ldq = ldq;
+  p.heads = heads;
+  p.kv_heads = kv_heads;
+  p.tiles = capacity / kQ4Tile;
+  p.length_offset = length_offset;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return head == 64 ? launch_attention<1>(p, seqs, st) : launch_attention<2>(p, seqs, st);
 }

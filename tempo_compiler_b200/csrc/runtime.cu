@@ -27,6 +27,7 @@ int watchdog_gemm();
 int watchdog_attention();
 int watchdog_prefill();
 int watchdog_decode_step();
+int watchdog_kv_q4();
 
 // ---------------------------------------------------------------------------------------------------------------
 // Errors and shared host helpers
@@ -165,9 +166,9 @@ int read_watchdogs(int* gemm, int* decode, int* prefill) {
   *gemm = watchdog_gemm();
   *decode = watchdog_attention();
   *prefill = watchdog_prefill();
-  const int step = watchdog_decode_step();
-  if (*gemm < 0 || *decode < 0 || *prefill < 0 || step < 0) return -1;
-  if (*decode == 0) *decode = step;
+  const int step = watchdog_decode_step(), q4 = watchdog_kv_q4();
+  if (*gemm < 0 || *decode < 0 || *prefill < 0 || step < 0 || q4 < 0) return -1;
+  if (*decode == 0) *decode = step != 0 ? step : q4;
   return *gemm != 0 ? *gemm : (*decode != 0 ? *decode : *prefill);
 }
 
