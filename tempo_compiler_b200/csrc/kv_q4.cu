@@ -113,21 +113,26 @@ __global__ void __launch_bounds__(kStoreThreads) kv_load_q4_kernel(const uint8_t
 // applied to the products: with D = sum_d q_d (128 + code_d) and Q = sum_d q_d,
 //   q . k = scale D + (low - 128 scale) Q,
 //   sum_j p_j v_j = sum_j w_j (64 + code_j) - 64 sum_j w_j + sum_j p_j low_j,   w_j = p_j scale_j.
-// The B operand holds up to eight query heads of one key / value head (m16n8k16), so grouped heads read the cache once.
+// The eight columns of the B operand (m16n8k16) are RP query heads of one key / value head times TP = 8 / RP tiles:
+// grouped heads read the cache once, and with few heads one softmax serves TP tiles (the first tensor-core form, one tile
+// and eight columns of queries whether they existed or not, issued 309 instructions a tile and was bound by the ALU pipe).
+// Every column holds its head's query; the scores of tile j are kept in the lanes whose columns are tile j's, and the
+// weights of the other columns are zeroed before tile j's values are multiplied.
 // q is exact in BF16; w is rounded to FP16 (2^-11 of each weight; an eighth of the output's own BF16 rounding), relative
 // to a running reference that bounds w and p low alike; everything else, the sums included, is FP32.
 //
 // A CTA of four warps takes a run of tiles of one (sequence, key / value head, eight query heads); each warp streams its
-// own two-tile pieces (one bulk copy each, a ring of kRing in flight) and keeps an online softmax whose reference moves
-// only when a score passes it by 2^kSlack. Warps merge through shared memory; with `chunks` > 1 the CTAs of a cluster
-// split the positions and merge through distributed shared memory.
+// own pieces (one bulk copy each, kRing in flight) and keeps an online softmax whose reference moves only when a score
+// passes it by 2^kSlack. Warps merge through shared memory; with `chunks` > 1 the CTAs of a cluster split the positions
+// and merge through distributed shared memory.
 // ---------------------------------------------------------------------------------------------------------------
 
 constexpr uint32_t kQ4MaxChunks = 16;
 constexpr uint32_t kQ4Queries = 8;
-constexpr uint32_t kQ4Piece = 2 * kQ4Block;  // bytes of one bulk copy: two tiles of a 64-wide head, one of a 128-wide
-constexpr uint32_t kRing = 4;
+constexpr uint32_t kQ4Piece = 4 * kQ4Block;  // bytes of one bulk copy: four tiles of a 64-wide head, two of a 128-wide
+constexpr uint32_t kRing = 2;
 constexpr float kSlack = 6.f;
+constexpr float kNoScore = -1e30f;  // the reference before any position: e^(anything - it) of an absent one is 0
 
 template <int G>
 struct Q4Smem {
@@ -153,6 +158,14 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// D = A x B: the accumulator starts at zero.
+__device__ __forceinline__ void mma_bf16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -173,18 +186,33 @@ __device__ __forceinline__ float fast_log2(float x) {
   return y;
 }
 
-// Two codes, `shift` bits up in each half of w, as the BF16 integers 128 + code / the FP16 integers 64 + code.
-__device__ __forceinline__ uint32_t key_pair(uint32_t w, uint32_t shift) {
-  return ((w >> shift) & 0x000F000Fu) | 0x43004300u;
+// (a & b) | c in one instruction; b and c are constants that the caller keeps in registers.
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
 }
-template <int NIBBLE>
-__device__ __forceinline__ uint32_t value_pair(uint32_t w) {
-  const uint32_t x = NIBBLE == 0 ? w << 4 : w >> (4 * (NIBBLE - 1));
-  return (x & 0x00F000F0u) | 0x54005400u;
+// A constant the compiler keeps in a register: as an immediate, (x & mask) | magic took two instructions, not one.
+__device__ __forceinline__ uint32_t in_register(uint32_t c) {
+  asm volatile("" : "+r"(c));
+  return c;
 }
 
-// One warp's running state. The MMA fragments put query columns 2 t and 2 t + 1 (t = lane % 4) on a lane; with
-// g = lane / 4, acc[i][n] holds dimensions 64 i + 8 g + n ([0], [1]) and 64 i + 8 g + 4 + n ([2], [3]) of the two.
+struct Q4Constants {
+  uint32_t key_mask, key_magic, value_mask, value_magic;
+};
+
+// Two codes, `shift` bits up in each half of w, as the BF16 integers 128 + code / the FP16 integers 64 + code.
+__device__ __forceinline__ uint32_t key_pair(const Q4Constants& k, uint32_t w, uint32_t shift) {
+  return and_or(w >> shift, k.key_mask, k.key_magic);
+}
+template <int NIBBLE>
+__device__ __forceinline__ uint32_t value_pair(const Q4Constants& k, uint32_t w) {
+  return and_or(NIBBLE == 0 ? w << 4 : w >> (4 * (NIBBLE - 1)), k.value_mask, k.value_magic);
+}
+
+// One warp's running state. The MMA fragments put columns 2 t and 2 t + 1 (t = lane % 4) on a lane; with g = lane / 4,
+// acc[i][n] holds dimensions 64 i + 8 g + n ([0], [1]) and 64 i + 8 g + 4 + n ([2], [3]) of the two columns.
 template <int G>
 struct Q4State {
   float acc[G][4][4];
@@ -192,42 +220,60 @@ struct Q4State {
   float w[G][2], low[G][2];  // this lane's sums of w (as rounded) and of p low
 };
 
-// Folds the 16 positions of one tile in shared memory into the state; `left` positions of it exist.
-template <int G>
-__device__ __forceinline__ void q4_tile(Q4State<G>& st, const uint32_t (&qf)[G][8], const float (&qs)[G][2],
-                                        const uint8_t* tile, uint32_t left, uint32_t g, uint32_t t) {
-  // Row r of the score MMA is position pi(r) (r < 8) or 8 + pi(r - 8), pi = 0 2 1 3 6 4 7 5: the key words of eight lanes
-  // groups, and the value words of the even and of the odd rows, then fall into different banks.
+// Folds TP = min(8 / RP, tiles of a piece) tiles in shared memory into the state. FULL: every position of them exists;
+// else `left` do.
+template <int G, int RP, bool FULL>
+__device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G][8], const float (&qs)[G][2],
+                                         const uint8_t* tiles, uint32_t left, uint32_t g, uint32_t t,
+                                         const Q4Constants& kc) {
+  constexpr uint32_t kTileBytes = G * kQ4Block, TP = 8 / RP < 4 / G ? 8 / RP : 4 / G;
+  // Row r of the score MMA is position pi(r) (r < 8) or 8 + pi(r - 8) of a tile, pi = 0 2 1 3 6 4 7 5: the key words of
+  // eight lane groups, and the value words of the even and of the odd rows, then fall into different banks.
   const uint32_t pg = g & 1u ? (g >> 1) + 2 : (g < 4 ? g >> 1 : (g >> 1) + 4);
   const uint32_t pe = t < 2 ? t : t + 4, po = t + 2;  // pi(2 t), pi(2 t + 1)
-  float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;  // scores (log2): rows g and g + 8, query columns 2 t and 2 t + 1
+  const uint32_t mine = 2 * t / RP;                   // the tile of this lane's two columns (none when >= TP)
+  float d[G][4];
+#pragma unroll
+  for (int i = 0; i < G; ++i) d[i][0] = d[i][1] = d[i][2] = d[i][3] = 0.f;
+#pragma unroll
+  for (uint32_t j = 0; j < TP; ++j) {
+    if (!FULL && j * kQ4Tile >= left) break;
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const uint8_t* block = tiles + j * kTileBytes + i * kQ4Block;
+      const uint2 k0 = *reinterpret_cast<const uint2*>(block + pg * 32 + t * 8);
+      const uint2 k1 = *reinterpret_cast<const uint2*>(block + (pg + 8) * 32 + t * 8);
+      float e[4];
+      mma_bf16_first(e, key_pair(kc, k0.x, 0), key_pair(kc, k1.x, 0), key_pair(kc, k0.x, 4), key_pair(kc, k1.x, 4), qf[i][0], qf[i][1]);
+      mma_bf16(e, key_pair(kc, k0.x, 8), key_pair(kc, k1.x, 8), key_pair(kc, k0.x, 12), key_pair(kc, k1.x, 12), qf[i][2], qf[i][3]);
+      mma_bf16(e, key_pair(kc, k0.y, 0), key_pair(kc, k1.y, 0), key_pair(kc, k0.y, 4), key_pair(kc, k1.y, 4), qf[i][4], qf[i][5]);
+      mma_bf16(e, key_pair(kc, k0.y, 8), key_pair(kc, k1.y, 8), key_pair(kc, k0.y, 12), key_pair(kc, k1.y, 12), qf[i][6], qf[i][7]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) d[i][c] = TP == 1 || mine == j ? e[c] : d[i][c];
+    }
+  }
+  const bool in0 = (TP == 4 || mine < TP) && (FULL || mine * kQ4Tile + pg < left);
+  const bool in1 = (TP == 4 || mine < TP) && (FULL || mine * kQ4Tile + pg + 8 < left);
+  const uint8_t* own = tiles + (TP == 4 || mine < TP ? mine : 0u) * kTileBytes + 2 * kQ4Codes;
+  float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;  // scores (log2): rows g and g + 8, columns 2 t and 2 t + 1
   float size0 = 0x1p-100f, size1 = 0x1p-100f;
   uint32_t vm0[G], vm1[G];
-  const bool in0 = pg < left, in1 = pg + 8 < left;
 #pragma unroll
   for (int i = 0; i < G; ++i) {
-    const uint8_t* block = tile + i * kQ4Block;
-    const uint2 k0 = *reinterpret_cast<const uint2*>(block + pg * 32 + t * 8);
-    const uint2 k1 = *reinterpret_cast<const uint2*>(block + (pg + 8) * 32 + t * 8);
-    uint2 meta0 = *reinterpret_cast<const uint2*>(block + 2 * kQ4Codes + pg * 8);
-    uint2 meta1 = *reinterpret_cast<const uint2*>(block + 2 * kQ4Codes + (pg + 8) * 8);
+    uint2 meta0 = *reinterpret_cast<const uint2*>(own + i * kQ4Block + pg * 8);
+    uint2 meta1 = *reinterpret_cast<const uint2*>(own + i * kQ4Block + (pg + 8) * 8);
     if (!in0) meta0 = make_uint2(0, 0);  // what lies behind the last position may be anything
     if (!in1) meta1 = make_uint2(0, 0);
-    float d[4] = {0.f, 0.f, 0.f, 0.f};
-    mma_bf16(d, key_pair(k0.x, 0), key_pair(k1.x, 0), key_pair(k0.x, 4), key_pair(k1.x, 4), qf[i][0], qf[i][1]);
-    mma_bf16(d, key_pair(k0.x, 8), key_pair(k1.x, 8), key_pair(k0.x, 12), key_pair(k1.x, 12), qf[i][2], qf[i][3]);
-    mma_bf16(d, key_pair(k0.y, 0), key_pair(k1.y, 0), key_pair(k0.y, 4), key_pair(k1.y, 4), qf[i][4], qf[i][5]);
-    mma_bf16(d, key_pair(k0.y, 8), key_pair(k1.y, 8), key_pair(k0.y, 12), key_pair(k1.y, 12), qf[i][6], qf[i][7]);
     const float ks0 = bf16_lo(meta0.x), ks1 = bf16_lo(meta1.x);
     const float kl0 = fmaf(-128.f, ks0, bf16_hi(meta0.x)), kl1 = fmaf(-128.f, ks1, bf16_hi(meta1.x));
-    s0 = fmaf(ks0, d[0], fmaf(kl0, qs[i][0], s0));
-    s1 = fmaf(ks0, d[1], fmaf(kl0, qs[i][1], s1));
-    s2 = fmaf(ks1, d[2], fmaf(kl1, qs[i][0], s2));
-    s3 = fmaf(ks1, d[3], fmaf(kl1, qs[i][1], s3));
+    s0 = fmaf(ks0, d[i][0], fmaf(kl0, qs[i][0], s0));
+    s1 = fmaf(ks0, d[i][1], fmaf(kl0, qs[i][1], s1));
+    s2 = fmaf(ks1, d[i][2], fmaf(kl1, qs[i][0], s2));
+    s3 = fmaf(ks1, d[i][3], fmaf(kl1, qs[i][1], s3));
     vm0[i] = meta0.y;
     vm1[i] = meta1.y;
-    size0 = fmaxf(size0, fmaxf(bf16_lo(meta0.y), 0.0625f * fabsf(bf16_hi(meta0.y))));
-    size1 = fmaxf(size1, fmaxf(bf16_lo(meta1.y), 0.0625f * fabsf(bf16_hi(meta1.y))));
+    size0 = fmax3(size0, bf16_lo(meta0.y), 0.0625f * fabsf(bf16_hi(meta0.y)));
+    size1 = fmax3(size1, bf16_lo(meta1.y), 0.0625f * fabsf(bf16_hi(meta1.y)));
   }
   s0 = in0 ? s0 * kDecodeLog2e : -INFINITY;
   s1 = in0 ? s1 * kDecodeLog2e : -INFINITY;
@@ -245,7 +291,7 @@ __device__ __forceinline__ void q4_tile(Q4State<G>& st, const uint32_t (&qf)[G][
     }
     x0 = fmaxf(x0, st.m[0]);
     x1 = fmaxf(x1, st.m[1]);
-    const float c0 = x0 == st.m[0] ? 1.f : fast_exp2(st.m[0] - x0), c1 = x1 == st.m[1] ? 1.f : fast_exp2(st.m[1] - x1);
+    const float c0 = fast_exp2(st.m[0] - x0), c1 = fast_exp2(st.m[1] - x1);
     st.m[0] = x0;
     st.m[1] = x1;
     st.l[0] *= c0;
@@ -269,13 +315,9 @@ __device__ __forceinline__ void q4_tile(Q4State<G>& st, const uint32_t (&qf)[G][
   const float p2 = fast_exp2(s2 - st.m[0]), p3 = fast_exp2(s3 - st.m[1]);
   st.l[0] += p0 + p2;
   st.l[1] += p1 + p3;
+  uint32_t b0[G], b1[G];
 #pragma unroll
   for (int i = 0; i < G; ++i) {
-    const uint8_t* words = tile + i * kQ4Block + kQ4Codes + g * 4;
-    const uint32_t va = *reinterpret_cast<const uint32_t*>(words + pe * 32);
-    const uint32_t vb = *reinterpret_cast<const uint32_t*>(words + po * 32);
-    const uint32_t vc = *reinterpret_cast<const uint32_t*>(words + (pe + 8) * 32);
-    const uint32_t vd = *reinterpret_cast<const uint32_t*>(words + (po + 8) * 32);
     const float vs0 = bf16_lo(vm0[i]), vs1 = bf16_lo(vm1[i]), vl0 = bf16_hi(vm0[i]), vl1 = bf16_hi(vm1[i]);
     const __half2 h0 = __floats2half2_rn(p0 * vs0, p1 * vs0), h1 = __floats2half2_rn(p2 * vs1, p3 * vs1);
     const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
@@ -283,15 +325,28 @@ __device__ __forceinline__ void q4_tile(Q4State<G>& st, const uint32_t (&qf)[G][
     st.w[i][1] += f0.y + f1.y;
     st.low[i][0] = fmaf(p0, vl0, fmaf(p2, vl1, st.low[i][0]));
     st.low[i][1] = fmaf(p1, vl0, fmaf(p3, vl1, st.low[i][1]));
-    const uint32_t b0 = transpose8x8(*reinterpret_cast<const uint32_t*>(&h0));
-    const uint32_t b1 = transpose8x8(*reinterpret_cast<const uint32_t*>(&h1));
-    // The same dimension of two positions side by side: dimensions 8 g .. + 3 in e0 / e1, 8 g + 4 .. in f0 / f1.
-    const uint32_t e0 = __byte_perm(va, vb, 0x5410), o0 = __byte_perm(va, vb, 0x7632);
-    const uint32_t e1 = __byte_perm(vc, vd, 0x5410), o1 = __byte_perm(vc, vd, 0x7632);
-    mma_f16(st.acc[i][0], value_pair<0>(e0), value_pair<0>(o0), value_pair<0>(e1), value_pair<0>(o1), b0, b1);
-    mma_f16(st.acc[i][1], value_pair<1>(e0), value_pair<1>(o0), value_pair<1>(e1), value_pair<1>(o1), b0, b1);
-    mma_f16(st.acc[i][2], value_pair<2>(e0), value_pair<2>(o0), value_pair<2>(e1), value_pair<2>(o1), b0, b1);
-    mma_f16(st.acc[i][3], value_pair<3>(e0), value_pair<3>(o0), value_pair<3>(e1), value_pair<3>(o1), b0, b1);
+    b0[i] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h0));
+    b1[i] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h1));
+  }
+#pragma unroll
+  for (uint32_t j = 0; j < TP; ++j) {
+    if (!FULL && j * kQ4Tile >= left) break;
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const uint8_t* words = tiles + j * kTileBytes + i * kQ4Block + kQ4Codes + g * 4;
+      const uint32_t va = *reinterpret_cast<const uint32_t*>(words + pe * 32);
+      const uint32_t vb = *reinterpret_cast<const uint32_t*>(words + po * 32);
+      const uint32_t vc = *reinterpret_cast<const uint32_t*>(words + (pe + 8) * 32);
+      const uint32_t vd = *reinterpret_cast<const uint32_t*>(words + (po + 8) * 32);
+      const uint32_t w0 = TP == 1 || g / RP == j ? b0[i] : 0u, w1 = TP == 1 || g / RP == j ? b1[i] : 0u;
+      // The same dimension of two positions side by side: dimensions 8 g .. + 3 in e0 / e1, 8 g + 4 .. in o0 / o1.
+      const uint32_t e0 = __byte_perm(va, vb, 0x5410), o0 = __byte_perm(va, vb, 0x7632);
+      const uint32_t e1 = __byte_perm(vc, vd, 0x5410), o1 = __byte_perm(vc, vd, 0x7632);
+      mma_f16(st.acc[i][0], value_pair<0>(kc, e0), value_pair<0>(kc, o0), value_pair<0>(kc, e1), value_pair<0>(kc, o1), w0, w1);
+      mma_f16(st.acc[i][1], value_pair<1>(kc, e0), value_pair<1>(kc, o0), value_pair<1>(kc, e1), value_pair<1>(kc, o1), w0, w1);
+      mma_f16(st.acc[i][2], value_pair<2>(kc, e0), value_pair<2>(kc, o0), value_pair<2>(kc, e1), value_pair<2>(kc, o1), w0, w1);
+      mma_f16(st.acc[i][3], value_pair<3>(kc, e0), value_pair<3>(kc, o0), value_pair<3>(kc, e1), value_pair<3>(kc, o1), w0, w1);
+    }
   }
 }
 
@@ -314,16 +369,17 @@ struct Q4Attention {
   uint32_t early;   // the grid is resident at once: the next kernel may start at entry
 };
 
-template <int G>
+template <int G, int RP>
 __global__ void __launch_bounds__(128) decode_attention_q4_kernel(Q4Attention p) {
   using L = Q4Smem<G>;
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr uint32_t kWidth = 64 * G, kTileBytes = G * kQ4Block, kPieceTiles = kQ4Piece / kTileBytes;
+  constexpr uint32_t TP = 8 / RP < kPieceTiles ? 8 / RP : kPieceTiles;  // tiles of one softmax
   const uint32_t warp = warp_id(), lane = lane_id(), g = lane >> 2, t = lane & 3u;
   const uint32_t chunks = gridDim.x, chunk = blockIdx.x, s = blockIdx.z;
   const uint32_t kvh = blockIdx.y / p.blocks, share = p.heads / p.kv_heads;
-  const uint32_t first = (blockIdx.y % p.blocks) * kQ4Queries;  // of the key / value head's query heads
-  const uint32_t queries = min(kQ4Queries, share - first);
+  const uint32_t first = (blockIdx.y % p.blocks) * RP;  // of the key / value head's query heads
+  const uint32_t queries = min(uint32_t(RP), share - first);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarrierOffset) + warp * kRing;
   uint8_t* ring = smem + warp * L::kWarpRing;
   if (lane == 0) {
@@ -338,36 +394,38 @@ __global__ void __launch_bounds__(128) decode_attention_q4_kernel(Q4Attention p)
   const int64_t want = int64_t(p.lengths[s]) + p.length_offset;
   const uint32_t capacity = p.tiles * kQ4Tile;
   const uint32_t len = want <= 0 ? 0u : want < int64_t(capacity) ? uint32_t(want) : capacity;
-  // The CTA's tiles [t_begin, t_end); its warps take pieces of kPieceTiles in turn.
+  // The CTA's tiles [t_begin, t_end), a run of them for each warp.
   const uint32_t used = (len + kQ4Tile - 1) / kQ4Tile, per = (used + chunks - 1) / chunks;
   const uint32_t t_begin = min(used, chunk * per), t_end = min(used, t_begin + per);
+  const uint32_t share_w = (t_end - t_begin + 3) / 4;
+  const uint32_t w_begin = min(t_end, t_begin + warp * share_w), w_end = min(t_end, w_begin + share_w);
+  const uint32_t pieces = (w_end - w_begin + kPieceTiles - 1) / kPieceTiles;
   const uint8_t* base = p.cache + (size_t(s) * p.kv_heads + kvh) * p.tiles * kTileBytes;
-  const uint32_t pieces = (t_end - t_begin + kPieceTiles - 1) / kPieceTiles;
   auto fetch = [&](uint32_t piece, uint32_t slot) {
-    const uint32_t tile = t_begin + piece * kPieceTiles, count = min(kPieceTiles, t_end - tile);
-    mbar_arrive_expect_tx(&full[slot], count * kTileBytes);
-    bulk_load(ring + slot * kQ4Piece, base + size_t(tile) * kTileBytes, count * kTileBytes, &full[slot]);
+    const uint32_t tile = w_begin + piece * kPieceTiles, bytes = min(kPieceTiles, w_end - tile) * kTileBytes;
+    mbar_arrive_expect_tx(&full[slot], bytes);
+    bulk_load(ring + slot * kQ4Piece, base + size_t(tile) * kTileBytes, bytes, &full[slot]);
   };
   if (lane == 0) {
 #pragma unroll
     for (uint32_t i = 0; i < kRing; ++i)
-      if (warp + 4 * i < pieces) fetch(warp + 4 * i, i);
+      if (i < pieces) fetch(i, i);
   }
 
-  // The query fragments: lane (g, t) holds dimensions 16 t .. 16 t + 15 of each group of query g.
+  // The query fragments: lane (g, t) holds dimensions 16 t .. 16 t + 15 of each group of its column's query.
   uint32_t qf[G][8];
   float qs[G][2];
 #pragma unroll
   for (int i = 0; i < G; ++i) {
     float sum = 0.f;
     uint4 a = make_uint4(0, 0, 0, 0), b = a;
-    if (g < queries) {
-      const uint4* q4 = reinterpret_cast<const uint4*>(p.q + size_t(s) * p.ldq +
-                                                       size_t(kvh * share + first + g) * kWidth + i * 64 + t * 16);
+    if (g % RP < queries) {
+      const uint4* q4 = reinterpret_cast<const uint4*>(
+          p.q + size_t(s) * p.ldq + size_t(kvh * share + first + g % RP) * kWidth + i * 64 + t * 16);
       a = q4[0];
       b = q4[1];
     }
-    // key_pair(word, 4 n) gives dimensions n and n + 4 of a word's eight.
+    // key_pair of a word, 4 n up, gives dimensions n and n + 4 of a word's eight.
     qf[i][0] = __byte_perm(a.x, a.z, 0x5410);
     qf[i][1] = __byte_perm(a.x, a.z, 0x7632);
     qf[i][2] = __byte_perm(a.y, a.w, 0x5410);
@@ -385,12 +443,12 @@ __global__ void __launch_bounds__(128) decode_attention_q4_kernel(Q4Attention p)
     for (int d = 0; d < 8; ++d) sum += f[d];
     sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
     sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
-    qs[i][0] = __shfl_sync(0xFFFFFFFFu, sum, 8 * t);      // the lane's own query columns, 2 t and 2 t + 1
+    qs[i][0] = __shfl_sync(0xFFFFFFFFu, sum, 8 * t);      // the lane's own columns, 2 t and 2 t + 1
     qs[i][1] = __shfl_sync(0xFFFFFFFFu, sum, 8 * t + 4);
   }
 
   Q4State<G> st;
-  st.m[0] = st.m[1] = -INFINITY;
+  st.m[0] = st.m[1] = kNoScore;
   st.l[0] = st.l[1] = 0.f;
 #pragma unroll
   for (int i = 0; i < G; ++i) {
@@ -400,23 +458,32 @@ __global__ void __launch_bounds__(128) decode_attention_q4_kernel(Q4Attention p)
 #pragma unroll
       for (int c = 0; c < 4; ++c) st.acc[i][n][c] = 0.f;
   }
+  const Q4Constants kc{in_register(0x000F000Fu), in_register(0x43004300u), in_register(0x00F000F0u),
+                       in_register(0x54005400u)};
   uint32_t slot = 0, phase = 0, limit = pieces;
   bool ok = true;
-  for (uint32_t piece = warp; piece < limit; piece += 4) {
+  for (uint32_t piece = 0; piece < limit; ++piece) {
     const bool landed = mbar_wait(&full[slot], phase, kWatchFull, nullptr);
     if (ok && !__all_sync(0xFFFFFFFFu, landed)) {
       // A copy that does not land: nothing more is issued, and the copies in flight are each waited for, bounded.
       ok = false;
-      limit = min(limit, piece + 4 * kRing);
+      limit = min(limit, piece + kRing);
     }
     if (ok) {
-      const uint32_t tile = t_begin + piece * kPieceTiles;
+      const uint32_t tile = w_begin + piece * kPieceTiles, end = min(tile + kPieceTiles, w_end);
+      const uint32_t left = min(len, end * kQ4Tile) - tile * kQ4Tile;  // positions of this piece
+      const uint8_t* data = ring + slot * kQ4Piece;
+      if (left == kPieceTiles * kQ4Tile) {
 #pragma unroll
-      for (uint32_t i = 0; i < kPieceTiles; ++i)
-        if (tile + i < t_end)
-          q4_tile<G>(st, qf, qs, ring + slot * kQ4Piece + i * kTileBytes, len - (tile + i) * kQ4Tile, g, t);
+        for (uint32_t i = 0; i < kPieceTiles; i += TP)
+          q4_tiles<G, RP, true>(st, qf, qs, data + i * kTileBytes, TP * kQ4Tile, g, t, kc);
+      } else {
+#pragma unroll 1
+        for (uint32_t i = 0; i * kQ4Tile < left; i += TP)
+          q4_tiles<G, RP, false>(st, qf, qs, data + i * kTileBytes, left - i * kQ4Tile, g, t, kc);
+      }
       __syncwarp();
-      if (lane == 0 && piece + 4 * kRing < pieces) fetch(piece + 4 * kRing, slot);
+      if (lane == 0 && piece + kRing < pieces) fetch(piece + kRing, slot);
     }
     if (++slot == kRing) {
       slot = 0;
@@ -425,30 +492,43 @@ __global__ void __launch_bounds__(128) decode_attention_q4_kernel(Q4Attention p)
   }
   if (!p.early) pdl_launch_dependents();
 
-  // The warp's partial result: (values at the reference, reference, sum) of each query, into its own ring.
+  // The warp's partial result, (values at the reference, reference, sum) of each query, into its own ring: the columns of
+  // one query (RP / 2 lanes apart) and the lanes' sums come together first.
   __syncwarp();
   float* part = reinterpret_cast<float*>(ring);
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
+    float m = st.m[c];
 #pragma unroll
-    for (int o = 4; o <= 16; o <<= 1) st.l[c] += __shfl_xor_sync(0xFFFFFFFFu, st.l[c], o);
-    const uint32_t query = 2 * t + c;
+    for (int o = RP / 2; o < 4; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    const float f = fast_exp2(st.m[c] - m);
+    float l = st.l[c] * f;
+#pragma unroll
+    for (int o = RP / 2; o < 32; o <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
+    const uint32_t query = 2 * t % RP + c;
+    const bool writes = 2 * t < RP && query < queries;
 #pragma unroll
     for (int i = 0; i < G; ++i) {
-      float rest = fmaf(-64.f, st.w[i][c], st.low[i][c]);
+      float rest = fmaf(-64.f, st.w[i][c], st.low[i][c]) * f;
 #pragma unroll
-      for (int o = 4; o <= 16; o <<= 1) rest += __shfl_xor_sync(0xFFFFFFFFu, rest, o);
-      if (query < queries) {
+      for (int o = RP / 2; o < 32; o <<= 1) rest += __shfl_xor_sync(0xFFFFFFFFu, rest, o);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          part[query * kWidth + i * 64 + 8 * g + n] = st.acc[i][n][c] + rest;
-          part[query * kWidth + i * 64 + 8 * g + 4 + n] = st.acc[i][n][2 + c] + rest;
+      for (int n = 0; n < 4; ++n) {
+        float lo = st.acc[i][n][c] * f, hi = st.acc[i][n][2 + c] * f;
+#pragma unroll
+        for (int o = RP / 2; o < 4; o <<= 1) {
+          lo += __shfl_xor_sync(0xFFFFFFFFu, lo, o);
+          hi += __shfl_xor_sync(0xFFFFFFFFu, hi, o);
+        }
+        if (writes) {
+          part[query * kWidth + i * 64 + 8 * g + n] = lo + rest;
+          part[query * kWidth + i * 64 + 8 * g + 4 + n] = hi + rest;
         }
       }
     }
-    if (g == 0 && query < queries) {
-      part[kQ4Queries * kWidth + query] = st.m[c];
-      part[kQ4Queries * kWidth + kQ4Queries + query] = st.l[c];
+    if (g == 0 && writes) {
+      part[kQ4Queries * kWidth + query] = m;
+      part[kQ4Queries * kWidth + kQ4Queries + query] = l;
     }
   }
   __syncthreads();
@@ -470,11 +550,10 @@ __global__ void __launch_bounds__(128) decode_attention_q4_kernel(Q4Attention p)
     if (chunks == 1) {
       out[i] = float_to_bf16(len == 0 ? 0.f : a / l);
     } else {
-      // (A CTA without positions has m = -inf on every warp, and must not hand on the NaN of -inf - -inf.)
-      merge[i] = t_begin == t_end ? 0.f : a;
+      merge[i] = a;
       if (i % kWidth == 0) {
         merge[kQ4Queries * kWidth + query] = m;
-        merge[kQ4Queries * kWidth + kQ4Queries + query] = t_begin == t_end ? 0.f : l;
+        merge[kQ4Queries * kWidth + kQ4Queries + query] = l;
       }
     }
   }
@@ -496,15 +575,14 @@ __global__ void __launch_bounds__(128) decode_attention_q4_kernel(Q4Attention p)
   asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
-template <int G>
+template <int G, int RP>
 tempo_status launch_attention(const Q4Attention& base, uint32_t seqs, cudaStream_t stream) {
   Q4Attention p = base;
-  const uint32_t share = p.heads / p.kv_heads;
-  p.blocks = (share + kQ4Queries - 1) / kQ4Queries;
+  p.blocks = (p.heads / p.kv_heads + RP - 1) / RP;
   const uint64_t pairs = uint64_t(p.kv_heads) * p.blocks * seqs, target = 2 * uint64_t(sm_count());
   uint32_t chunks = 1;
   while (chunks < kQ4MaxChunks && pairs * chunks < target && p.tiles >= 8 * chunks) chunks *= 2;
-  auto kernel = decode_attention_q4_kernel<G>;
+  auto kernel = decode_attention_q4_kernel<G, RP>;
   if (chunks > 8) {
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute(non-portable cluster size)");
@@ -595,5 +673,8 @@ extern "C" tempo_status tempo_decode_attention_q4(const void* q, uint32_t ldq, c
   p.tiles = capacity / kQ4Tile;
   p.length_offset = length_offset;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return head == 64 ? launch_attention<1>(p, seqs, st) : launch_attention<2>(p, seqs, st);
+  const uint32_t share = heads / kv_heads;
+  if (head == 128) return share <= 4 ? launch_attention<2, 4>(p, seqs, st) : launch_attention<2, 8>(p, seqs, st);
+  if (share <= 2) return launch_attention<1, 2>(p, seqs, st);
+  return share <= 4 ? launch_attention<1, 4>(p, seqs, st) : launch_attention<1, 8>(p, seqs, st);
 }
