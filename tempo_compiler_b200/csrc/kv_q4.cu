@@ -113,8 +113,8 @@ __global__ void __launch_bounds__(kStoreThreads) kv_load_q4_kernel(const uint8_t
 // applied to the products: with D = sum_d q_d (128 + code_d) and Q = sum_d q_d,
 //   q . k = scale D + (low - 128 scale) Q,
 //   sum_j p_j v_j = sum_j w_j (64 + code_j) - 64 sum_j w_j + sum_j p_j low_j,   w_j = p_j scale_j.
-// The eight columns of the B operand (m16n8k16) are RP query heads of one key / value head times TP = 8 / RP tiles:
-// grouped heads read the cache once, and with few heads one softmax serves TP tiles (the first tensor-core form, one tile
+// The eight columns of the B operand (m16n8k16) are query heads of one key / value head times tiles:
+// grouped heads read the cache once, and with few heads one softmax serves several tiles (the first tensor-core form, one tile
 // and eight columns of queries whether they existed or not, issued 309 instructions a tile and was bound by the ALU pipe).
 // Every column holds its head's query; the scores of tile j are kept in the lanes whose columns are tile j's, and the
 // weights of the other columns are zeroed before tile j's values are multiplied.
@@ -134,15 +134,14 @@ constexpr uint32_t kRing = 2;
 constexpr float kSlack = 6.f;
 constexpr float kNoScore = -1e30f;  // the reference before any position: e^(anything - it) of an absent one is 0
 
-template <int G>
+template <int G, int WARPS>
 struct Q4Smem {
   static constexpr uint32_t kWarpRing = kRing * kQ4Piece;
   static constexpr uint32_t kPart = kQ4Queries * (64 * G + 2) * 4;  // (values, max, sum) of eight queries
-  static constexpr uint32_t kBarrierOffset = 4 * kWarpRing;
-  static constexpr uint32_t kMergeOffset = kBarrierOffset + 4 * kRing * 8;
+  static constexpr uint32_t kBarrierOffset = WARPS * kWarpRing;
+  static constexpr uint32_t kMergeOffset = kBarrierOffset + WARPS * kRing * 8;
   static constexpr uint32_t kBytes = kMergeOffset + kPart;
   static_assert(kPart <= kWarpRing, "a warp's partial result fits its ring");
-  static_assert(kBytes <= 48 * 1024, "fits without an opt-in");
 };
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -220,18 +219,27 @@ struct Q4State {
   float w[G][2], low[G][2];  // this lane's sums of w (as rounded) and of p low
 };
 
-// Folds TP = min(8 / RP, tiles of a piece) tiles in shared memory into the state. FULL: every position of them exists;
+// Columns of a tile: the RP query heads, or two (the odd one empty) for a single head, which leaves half of each lane's
+// softmax out.
+__host__ __device__ constexpr uint32_t q4_columns(int rp) { return rp == 1 ? 2u : uint32_t(rp); }
+// Tiles of one softmax: 8 columns' worth, at most a piece.
+__host__ __device__ constexpr uint32_t q4_tiles_at_once(int g, int rp) {
+  return 8 / q4_columns(rp) < 4u / g ? 8 / q4_columns(rp) : 4u / g;
+}
+
+// Folds TP tiles in shared memory into the state. FULL: every position of them exists;
 // else `left` do.
 template <int G, int RP, bool FULL>
 __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G][8], const float (&qs)[G][2],
                                          const uint8_t* tiles, uint32_t left, uint32_t g, uint32_t t,
                                          const Q4Constants& kc) {
-  constexpr uint32_t kTileBytes = G * kQ4Block, TP = 8 / RP < 4 / G ? 8 / RP : 4 / G;
+  constexpr uint32_t kTileBytes = G * kQ4Block, CP = q4_columns(RP), TP = q4_tiles_at_once(G, RP);
+  constexpr bool kTwo = RP > 1;  // a single query takes the even columns only
   // Row r of the score MMA is position pi(r) (r < 8) or 8 + pi(r - 8) of a tile, pi = 0 2 1 3 6 4 7 5: the key words of
   // eight lane groups, and the value words of the even and of the odd rows, then fall into different banks.
   const uint32_t pg = g & 1u ? (g >> 1) + 2 : (g < 4 ? g >> 1 : (g >> 1) + 4);
   const uint32_t pe = t < 2 ? t : t + 4, po = t + 2;  // pi(2 t), pi(2 t + 1)
-  const uint32_t mine = 2 * t / RP;                   // the tile of this lane's two columns (none when >= TP)
+  const uint32_t mine = 2 * t / CP;                   // the tile of this lane's two columns (none when >= TP)
   float d[G][4];
 #pragma unroll
   for (int i = 0; i < G; ++i) d[i][0] = d[i][1] = d[i][2] = d[i][3] = 0.f;
@@ -249,7 +257,8 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
       mma_bf16(e, key_pair(kc, k0.y, 0), key_pair(kc, k1.y, 0), key_pair(kc, k0.y, 4), key_pair(kc, k1.y, 4), qf[i][4], qf[i][5]);
       mma_bf16(e, key_pair(kc, k0.y, 8), key_pair(kc, k1.y, 8), key_pair(kc, k0.y, 12), key_pair(kc, k1.y, 12), qf[i][6], qf[i][7]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) d[i][c] = TP == 1 || mine == j ? e[c] : d[i][c];
+      for (int c = 0; c < 4; ++c)
+        if (kTwo || c % 2 == 0) d[i][c] = TP == 1 || mine == j ? e[c] : d[i][c];
     }
   }
   const bool in0 = (TP == 4 || mine < TP) && (FULL || mine * kQ4Tile + pg < left);
@@ -267,9 +276,9 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
     const float ks0 = bf16_lo(meta0.x), ks1 = bf16_lo(meta1.x);
     const float kl0 = fmaf(-128.f, ks0, bf16_hi(meta0.x)), kl1 = fmaf(-128.f, ks1, bf16_hi(meta1.x));
     s0 = fmaf(ks0, d[i][0], fmaf(kl0, qs[i][0], s0));
-    s1 = fmaf(ks0, d[i][1], fmaf(kl0, qs[i][1], s1));
+    if (kTwo) s1 = fmaf(ks0, d[i][1], fmaf(kl0, qs[i][1], s1));
     s2 = fmaf(ks1, d[i][2], fmaf(kl1, qs[i][0], s2));
-    s3 = fmaf(ks1, d[i][3], fmaf(kl1, qs[i][1], s3));
+    if (kTwo) s3 = fmaf(ks1, d[i][3], fmaf(kl1, qs[i][1], s3));
     vm0[i] = meta0.y;
     vm1[i] = meta1.y;
     size0 = fmax3(size0, bf16_lo(meta0.y), 0.0625f * fabsf(bf16_hi(meta0.y)));
@@ -282,49 +291,59 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
   // The reference follows log2(p size), size the value row's scale or a sixteenth of its low: w and p low stay small
   // whatever the values' size, and a position of small values needs a larger p to move it.
   const float g0 = fast_log2(fminf(size0, 0x1p100f)), g1 = fast_log2(fminf(size1, 0x1p100f));
-  float x0 = fmaxf(s0 + g0, s2 + g1), x1 = fmaxf(s1 + g0, s3 + g1);
-  if (__any_sync(0xFFFFFFFFu, x0 > st.m[0] + kSlack || x1 > st.m[1] + kSlack)) {
+  float x0 = fmaxf(s0 + g0, s2 + g1), x1 = kTwo ? fmaxf(s1 + g0, s3 + g1) : 0.f;
+  if (__any_sync(0xFFFFFFFFu, x0 > st.m[0] + kSlack || (kTwo && x1 > st.m[1] + kSlack))) {
 #pragma unroll
     for (int o = 4; o <= 16; o <<= 1) {
       x0 = fmaxf(x0, __shfl_xor_sync(0xFFFFFFFFu, x0, o));
-      x1 = fmaxf(x1, __shfl_xor_sync(0xFFFFFFFFu, x1, o));
+      if (kTwo) x1 = fmaxf(x1, __shfl_xor_sync(0xFFFFFFFFu, x1, o));
     }
     x0 = fmaxf(x0, st.m[0]);
-    x1 = fmaxf(x1, st.m[1]);
-    const float c0 = fast_exp2(st.m[0] - x0), c1 = fast_exp2(st.m[1] - x1);
+    const float c0 = fast_exp2(st.m[0] - x0);
     st.m[0] = x0;
-    st.m[1] = x1;
     st.l[0] *= c0;
-    st.l[1] *= c1;
+    float c1 = 0.f;
+    if (kTwo) {
+      x1 = fmaxf(x1, st.m[1]);
+      c1 = fast_exp2(st.m[1] - x1);
+      st.m[1] = x1;
+      st.l[1] *= c1;
+    }
 #pragma unroll
     for (int i = 0; i < G; ++i) {
       st.w[i][0] *= c0;
-      st.w[i][1] *= c1;
       st.low[i][0] *= c0;
-      st.low[i][1] *= c1;
+      if (kTwo) {
+        st.w[i][1] *= c1;
+        st.low[i][1] *= c1;
+      }
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         st.acc[i][n][0] *= c0;
-        st.acc[i][n][1] *= c1;
         st.acc[i][n][2] *= c0;
-        st.acc[i][n][3] *= c1;
+        if (kTwo) {
+          st.acc[i][n][1] *= c1;
+          st.acc[i][n][3] *= c1;
+        }
       }
     }
   }
-  const float p0 = fast_exp2(s0 - st.m[0]), p1 = fast_exp2(s1 - st.m[1]);
-  const float p2 = fast_exp2(s2 - st.m[0]), p3 = fast_exp2(s3 - st.m[1]);
+  const float p0 = fast_exp2(s0 - st.m[0]), p2 = fast_exp2(s2 - st.m[0]);
+  const float p1 = kTwo ? fast_exp2(s1 - st.m[1]) : 0.f, p3 = kTwo ? fast_exp2(s3 - st.m[1]) : 0.f;
   st.l[0] += p0 + p2;
-  st.l[1] += p1 + p3;
+  if (kTwo) st.l[1] += p1 + p3;
   uint32_t b0[G], b1[G];
 #pragma unroll
   for (int i = 0; i < G; ++i) {
     const float vs0 = bf16_lo(vm0[i]), vs1 = bf16_lo(vm1[i]), vl0 = bf16_hi(vm0[i]), vl1 = bf16_hi(vm1[i]);
-    const __half2 h0 = __floats2half2_rn(p0 * vs0, p1 * vs0), h1 = __floats2half2_rn(p2 * vs1, p3 * vs1);
-    const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
-    st.w[i][0] += f0.x + f1.x;
-    st.w[i][1] += f0.y + f1.y;
+    const __half2 h0 = __floats2half2_rn(p0 * vs0, kTwo ? p1 * vs0 : 0.f);
+    const __half2 h1 = __floats2half2_rn(p2 * vs1, kTwo ? p3 * vs1 : 0.f);
+    st.w[i][0] += __low2float(h0) + __low2float(h1);
     st.low[i][0] = fmaf(p0, vl0, fmaf(p2, vl1, st.low[i][0]));
-    st.low[i][1] = fmaf(p1, vl0, fmaf(p3, vl1, st.low[i][1]));
+    if (kTwo) {
+      st.w[i][1] += __high2float(h0) + __high2float(h1);
+      st.low[i][1] = fmaf(p1, vl0, fmaf(p3, vl1, st.low[i][1]));
+    }
     b0[i] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h0));
     b1[i] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h1));
   }
@@ -338,7 +357,7 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
       const uint32_t vb = *reinterpret_cast<const uint32_t*>(words + po * 32);
       const uint32_t vc = *reinterpret_cast<const uint32_t*>(words + (pe + 8) * 32);
       const uint32_t vd = *reinterpret_cast<const uint32_t*>(words + (po + 8) * 32);
-      const uint32_t w0 = TP == 1 || g / RP == j ? b0[i] : 0u, w1 = TP == 1 || g / RP == j ? b1[i] : 0u;
+      const uint32_t w0 = TP == 1 || g / CP == j ? b0[i] : 0u, w1 = TP == 1 || g / CP == j ? b1[i] : 0u;
       // The same dimension of two positions side by side: dimensions 8 g .. + 3 in e0 / e1, 8 g + 4 .. in o0 / o1.
       const uint32_t e0 = __byte_perm(va, vb, 0x5410), o0 = __byte_perm(va, vb, 0x7632);
       const uint32_t e1 = __byte_perm(vc, vd, 0x5410), o1 = __byte_perm(vc, vd, 0x7632);
@@ -369,12 +388,12 @@ struct Q4Attention {
   uint32_t early;   // the grid is resident at once: the next kernel may start at entry
 };
 
-template <int G, int RP>
-__global__ void __launch_bounds__(128) decode_attention_q4_kernel(Q4Attention p) {
-  using L = Q4Smem<G>;
+template <int G, int RP, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) decode_attention_q4_kernel(Q4Attention p) {
+  using L = Q4Smem<G, WARPS>;
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr uint32_t kWidth = 64 * G, kTileBytes = G * kQ4Block, kPieceTiles = kQ4Piece / kTileBytes;
-  constexpr uint32_t TP = 8 / RP < kPieceTiles ? 8 / RP : kPieceTiles;  // tiles of one softmax
+  constexpr uint32_t CP = q4_columns(RP), TP = q4_tiles_at_once(G, RP);
   const uint32_t warp = warp_id(), lane = lane_id(), g = lane >> 2, t = lane & 3u;
   const uint32_t chunks = gridDim.x, chunk = blockIdx.x, s = blockIdx.z;
   const uint32_t kvh = blockIdx.y / p.blocks, share = p.heads / p.kv_heads;
@@ -397,7 +416,7 @@ __global__ void __launch_bounds__(128) decode_attention_q4_kernel(Q4Attention p)
   // The CTA's tiles [t_begin, t_end), a run of them for each warp.
   const uint32_t used = (len + kQ4Tile - 1) / kQ4Tile, per = (used + chunks - 1) / chunks;
   const uint32_t t_begin = min(used, chunk * per), t_end = min(used, t_begin + per);
-  const uint32_t share_w = (t_end - t_begin + 3) / 4;
+  const uint32_t share_w = (t_end - t_begin + WARPS - 1) / WARPS;
   const uint32_t w_begin = min(t_end, t_begin + warp * share_w), w_end = min(t_end, w_begin + share_w);
   const uint32_t pieces = (w_end - w_begin + kPieceTiles - 1) / kPieceTiles;
   const uint8_t* base = p.cache + (size_t(s) * p.kv_heads + kvh) * p.tiles * kTileBytes;
@@ -419,9 +438,9 @@ __global__ void __launch_bounds__(128) decode_attention_q4_kernel(Q4Attention p)
   for (int i = 0; i < G; ++i) {
     float sum = 0.f;
     uint4 a = make_uint4(0, 0, 0, 0), b = a;
-    if (g % RP < queries) {
+    if (g % CP < queries) {
       const uint4* q4 = reinterpret_cast<const uint4*>(
-          p.q + size_t(s) * p.ldq + size_t(kvh * share + first + g % RP) * kWidth + i * 64 + t * 16);
+          p.q + size_t(s) * p.ldq + size_t(kvh * share + first + g % CP) * kWidth + i * 64 + t * 16);
       a = q4[0];
       b = q4[1];
     }
@@ -493,30 +512,30 @@ __global__ void __launch_bounds__(128) decode_attention_q4_kernel(Q4Attention p)
   if (!p.early) pdl_launch_dependents();
 
   // The warp's partial result, (values at the reference, reference, sum) of each query, into its own ring: the columns of
-  // one query (RP / 2 lanes apart) and the lanes' sums come together first.
+  // one query (CP / 2 lanes apart) and the lanes' sums come together first.
   __syncwarp();
   float* part = reinterpret_cast<float*>(ring);
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
+  for (int c = 0; c < (RP > 1 ? 2 : 1); ++c) {
     float m = st.m[c];
 #pragma unroll
-    for (int o = RP / 2; o < 4; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    for (int o = CP / 2; o < 4; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
     const float f = fast_exp2(st.m[c] - m);
     float l = st.l[c] * f;
 #pragma unroll
-    for (int o = RP / 2; o < 32; o <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
-    const uint32_t query = 2 * t % RP + c;
-    const bool writes = 2 * t < RP && query < queries;
+    for (int o = CP / 2; o < 32; o <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
+    const uint32_t query = 2 * t % CP + c;
+    const bool writes = 2 * t < CP && query < queries;
 #pragma unroll
     for (int i = 0; i < G; ++i) {
       float rest = fmaf(-64.f, st.w[i][c], st.low[i][c]) * f;
 #pragma unroll
-      for (int o = RP / 2; o < 32; o <<= 1) rest += __shfl_xor_sync(0xFFFFFFFFu, rest, o);
+      for (int o = CP / 2; o < 32; o <<= 1) rest += __shfl_xor_sync(0xFFFFFFFFu, rest, o);
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         float lo = st.acc[i][n][c] * f, hi = st.acc[i][n][2 + c] * f;
 #pragma unroll
-        for (int o = RP / 2; o < 4; o <<= 1) {
+        for (int o = CP / 2; o < 4; o <<= 1) {
           lo += __shfl_xor_sync(0xFFFFFFFFu, lo, o);
           hi += __shfl_xor_sync(0xFFFFFFFFu, hi, o);
         }
@@ -534,14 +553,14 @@ __global__ void __launch_bounds__(128) decode_attention_q4_kernel(Q4Attention p)
   __syncthreads();
   float* merge = reinterpret_cast<float*>(smem + L::kMergeOffset);
   uint16_t* out = p.out + (size_t(s) * p.heads + kvh * share + first) * kWidth;
-  for (uint32_t i = threadIdx.x; i < queries * kWidth; i += 128) {
+  for (uint32_t i = threadIdx.x; i < queries * kWidth; i += 32 * WARPS) {
     const uint32_t query = i / kWidth;
     float m = -INFINITY, l = 0.f, a = 0.f;
 #pragma unroll
-    for (uint32_t w = 0; w < 4; ++w)
+    for (uint32_t w = 0; w < WARPS; ++w)
       m = fmaxf(m, reinterpret_cast<const float*>(smem + w * L::kWarpRing)[kQ4Queries * kWidth + query]);
 #pragma unroll
-    for (uint32_t w = 0; w < 4; ++w) {
+    for (uint32_t w = 0; w < WARPS; ++w) {
       const float* other = reinterpret_cast<const float*>(smem + w * L::kWarpRing);
       const float f = fast_exp2(other[kQ4Queries * kWidth + query] - m);
       l = fmaf(other[kQ4Queries * kWidth + kQ4Queries + query], f, l);
@@ -560,7 +579,7 @@ __global__ void __launch_bounds__(128) decode_attention_q4_kernel(Q4Attention p)
   if (chunks == 1) return;
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   // Each CTA finishes its share of the outputs, reading every CTA's partial result.
-  for (uint32_t i = chunk * 128 + threadIdx.x; i < queries * kWidth; i += chunks * 128) {
+  for (uint32_t i = chunk * 32 * WARPS + threadIdx.x; i < queries * kWidth; i += chunks * 32 * WARPS) {
     const uint32_t query = i / kWidth;
     float m = -INFINITY, l = 0.f, a = 0.f;
     for (uint32_t c = 0; c < chunks; ++c) m = fmaxf(m, ld_cluster(merge + kQ4Queries * kWidth + query, c));
@@ -575,21 +594,31 @@ __global__ void __launch_bounds__(128) decode_attention_q4_kernel(Q4Attention p)
   asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
-template <int G, int RP>
-tempo_status launch_attention(const Q4Attention& base, uint32_t seqs, cudaStream_t stream) {
+template <int G, int RP, int WARPS>
+tempo_status launch_attention_warps(const Q4Attention& base, uint32_t seqs, uint32_t chunks, cudaStream_t stream) {
   Q4Attention p = base;
-  p.blocks = (p.heads / p.kv_heads + RP - 1) / RP;
-  const uint64_t pairs = uint64_t(p.kv_heads) * p.blocks * seqs, target = 2 * uint64_t(sm_count());
-  uint32_t chunks = 1;
-  while (chunks < kQ4MaxChunks && pairs * chunks < target && p.tiles >= 8 * chunks) chunks *= 2;
-  auto kernel = decode_attention_q4_kernel<G, RP>;
+  auto kernel = decode_attention_q4_kernel<G, RP, WARPS>;
+  tempo_status status = set_smem(reinterpret_cast<const void*>(kernel), Q4Smem<G, WARPS>::kBytes);
+  if (status != TEMPO_OK) return status;
   if (chunks > 8) {
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute(non-portable cluster size)");
   }
-  p.early = single_wave(pairs * chunks, 4);
-  return launch(kernel, dim3(chunks, p.kv_heads * p.blocks, seqs), dim3(128), Q4Smem<G>::kBytes, stream, chunks,
-                "decode_attention_q4_kernel", p);
+  p.early = single_wave(uint64_t(p.kv_heads) * p.blocks * seqs * chunks, 16 / WARPS);
+  return launch(kernel, dim3(chunks, p.kv_heads * p.blocks, seqs), dim3(32 * WARPS), Q4Smem<G, WARPS>::kBytes, stream,
+                chunks, "decode_attention_q4_kernel", p);
+}
+
+template <int G, int RP>
+tempo_status launch_attention(const Q4Attention& base, uint32_t seqs, cudaStream_t stream) {
+  Q4Attention p = base;
+  p.blocks = (p.heads / p.kv_heads + RP - 1) / RP;
+  const uint64_t pairs = uint64_t(p.kv_heads) * p.blocks * seqs, sms = uint64_t(sm_count());
+  uint32_t chunks = 1;
+  while (chunks < kQ4MaxChunks && pairs * chunks < 2 * sms && p.tiles >= 8 * chunks) chunks *= 2;
+  if (pairs * chunks * 4 < 16 * sms && p.tiles >= 64 * chunks) return launch_attention_warps<G, RP, 8>(p, seqs, chunks, stream);
+  if (pairs >= 20 * sms) return launch_attention_warps<G, RP, 2>(p, seqs, chunks, stream);
+  return launch_attention_warps<G, RP, 4>(p, seqs, chunks, stream);
 }
 
 // What the three entry points check alike; `what` names the call.
@@ -674,7 +703,9 @@ extern "C" tempo_status tempo_decode_attention_q4(const void* q, uint32_t ldq, c
   p.length_offset = length_offset;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const uint32_t share = heads / kv_heads;
+  if (head == 128 && share == 1) return launch_attention<2, 1>(p, seqs, st);
   if (head == 128) return share <= 4 ? launch_attention<2, 4>(p, seqs, st) : launch_attention<2, 8>(p, seqs, st);
-  if (share <= 2) return launch_attention<1, 2>(p, seqs, st);
+  if (share == 1) return launch_attention<1, 1>(p, seqs, st);
+  if (share == 2) return launch_attention<1, 2>(p, seqs, st);
   return share <= 4 ? launch_attention<1, 4>(p, seqs, st) : launch_attention<1, 8>(p, seqs, st);
 }

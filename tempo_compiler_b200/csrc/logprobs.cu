@@ -2,6 +2,13 @@
 // logits: with m the row's maximum, l = sum e^(x - m) and t = sum (x - m) e^(x - m),
 //   log p(id) = x[id] - m - ln l,   entropy = ln l - t / l,
 // and the alternatives are the greatest logits, ties going to the lower index.
+//
+// One pass over the logits, which bounds the kernel (four or two bytes a logit): each thread keeps a running maximum
+// and the two sums rescaled to it, and the alternatives are found on the way. After the first chunk of a row the CTA
+// takes as threshold the top-th greatest of the lane groups' greatest keys, a lower bound on the top-th greatest
+// logit; from then on only the few logits above it go into a candidate list in shared memory, which is thinned by the
+// same device when it fills up and sorted by counting at the end. (A key joins a logit with its index, so keys have no
+// ties, and a later logit equal to the threshold's is below it.) Few rows are split over the CTAs of a cluster, whose sums and sorted candidates the first one merges.
 #include <cfloat>
 
 #include <cuda_runtime.h>
@@ -13,14 +20,24 @@ namespace tempo {
 namespace {
 
 constexpr uint32_t kThreads = 256;
+constexpr uint32_t kWarps = kThreads / 32;
+constexpr uint32_t kLogits = 16;                    // of one thread and chunk
+constexpr uint32_t kChunkLogits = kThreads * kLogits;
+constexpr uint32_t kLanes = 4;                      // of a group whose greatest keys give a threshold
+constexpr uint32_t kGroups = kThreads / kLanes;
 constexpr uint32_t kMaxTop = 32;
+constexpr uint32_t kThin = 512;                     // more candidates are thinned before the next chunk
+constexpr uint32_t kCapacity = kThin + kChunkLogits + 8;  // a full chunk on top of them, and the logits behind the words
+constexpr uint32_t kMaxChunks = 8;                  // CTAs of a cluster sharing one row
 constexpr float kLog2e = 1.4426950408889634f;
+static_assert(kGroups >= 2 * kMaxTop, "thinning drops at least half of the groups");
+static_assert(kMaxChunks * kMaxTop <= kThreads, "a thread for each candidate of a cluster");
 
 struct LogprobParams {
   const void* logits;
   uint64_t ld;
   const int32_t* ids;
-  uint32_t vocab, top;
+  uint32_t vocab, top, chunks;
   float* logprob;
   float* entropy;
   float* top_logprob;
@@ -28,14 +45,35 @@ struct LogprobParams {
 };
 
 template <typename T>
-__device__ __forceinline__ float logit(const T* row, uint32_t i);
+struct Vector;  // the logits of one 16-byte word
 template <>
-__device__ __forceinline__ float logit(const float* row, uint32_t i) { return row[i]; }
+struct Vector<float> {
+  static constexpr uint32_t kCount = 4;
+  static __device__ __forceinline__ void unpack(const uint4& w, float (&x)[4]) {
+    x[0] = __uint_as_float(w.x);
+    x[1] = __uint_as_float(w.y);
+    x[2] = __uint_as_float(w.z);
+    x[3] = __uint_as_float(w.w);
+  }
+  static __device__ __forceinline__ float one(const float* p) { return *p; }
+};
 template <>
-__device__ __forceinline__ float logit(const uint16_t* row, uint32_t i) { return bf16_to_float(row[i]); }
+struct Vector<uint16_t> {
+  static constexpr uint32_t kCount = 8;
+  static __device__ __forceinline__ void unpack(const uint4& w, float (&x)[8]) { unpack8(w, x); }
+  static __device__ __forceinline__ float one(const uint16_t* p) { return bf16_to_float(*p); }
+};
+
+__device__ __forceinline__ uint4 ld_once(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
 
 // A logit and its index as one unsigned key: greater logits first (NaN before all, -0 equal to +0), then the lower
-// index. Keys of a row differ, so an order by key has no ties.
+// index. Keys of a row differ, so an order by key has no ties. 0 is below every key.
 __device__ __forceinline__ uint64_t order_key(float x, uint32_t index) {
   const uint32_t bits = __float_as_uint(x + 0.f);
   uint32_t rank = bits & 0x80000000u ? ~bits : bits | 0x80000000u;
@@ -47,71 +85,334 @@ __device__ __forceinline__ float key_logit(uint64_t key) {
   return __uint_as_float(rank & 0x80000000u ? rank & 0x7FFFFFFFu : ~rank);
 }
 
-__device__ __forceinline__ float block_sum(float v, float* scratch) {
-  v = warp_sum(v);
-  if (lane_id() == 0) scratch[warp_id()] = v;
+struct Candidates {
+  uint64_t keys[kCapacity];
+  uint64_t group[kGroups];
+  uint64_t threshold;
+  uint32_t count;
+};
+
+// Sets the threshold to the top-th greatest of the groups' greatest keys (0 when fewer groups hold a key). `best` is
+// this thread's greatest key. Ends with every thread seeing the threshold.
+__device__ __forceinline__ void set_threshold(Candidates& c, uint64_t best, uint32_t top) {
+#pragma unroll
+  for (uint32_t o = 1; o < kLanes; o <<= 1) {
+    const uint64_t other = __shfl_xor_sync(0xFFFFFFFFu, best, o);
+    best = other > best ? other : best;
+  }
+  if (threadIdx.x % kLanes == 0) c.group[threadIdx.x / kLanes] = best;
+  if (threadIdx.x == 0) c.threshold = 0;
   __syncthreads();
-  float sum = 0.f;
-  for (uint32_t w = 0; w < kThreads / 32; ++w) sum += scratch[w];
+  if (threadIdx.x < kGroups) {
+    const uint64_t own = c.group[threadIdx.x];
+    uint32_t above = 0;
+#pragma unroll 8
+    for (uint32_t i = 0; i < kGroups; ++i) above += c.group[i] > own ? 1u : 0u;
+    if (above == top - 1 && own != 0) c.threshold = own;  // keys differ: one thread at most
+  }
   __syncthreads();
-  return sum;
 }
 
-// One CTA per row: the maximum, the sums, then the alternatives one by one, each the greatest key below the last.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogprobParams p) {
-  __shared__ float scratch[kThreads / 32];
-  __shared__ uint64_t keys[kThreads / 32];
-  pdl_wait();
-  pdl_launch_dependents();
-  const uint32_t r = blockIdx.x;
-  const T* row = static_cast<const T*>(p.logits) + size_t(r) * p.ld;
-  float m = -INFINITY;
-  for (uint32_t i = threadIdx.x; i < p.vocab; i += kThreads) m = fmaxf(m, logit(row, i));
+// Drops candidates that cannot be among the `top` greatest: at least the kGroups - top groups whose greatest key is below
+// the threshold, half of a list that fills the groups evenly. Called by the whole CTA, with the list settled.
+__device__ __noinline__ void thin(Candidates& c, uint32_t top) {
+  constexpr uint32_t kPer = (kCapacity + kThreads - 1) / kThreads;
+  const uint32_t count = c.count;
+  uint64_t own[kPer], best = 0;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-  if (lane_id() == 0) scratch[warp_id()] = m;
-  __syncthreads();
-  for (uint32_t w = 0; w < kThreads / 32; ++w) m = fmaxf(m, scratch[w]);
-  __syncthreads();
-  const float base = fmaxf(m, -FLT_MAX);
-  float l = 0.f, t = 0.f;
-  for (uint32_t i = threadIdx.x; i < p.vocab; i += kThreads) {
-    const float d = logit(row, i) - base, e = fast_exp2(d * kLog2e);
-    l += e;
-    t = fmaf(fmaxf(d, -1000.f), e, t);
+  for (uint32_t i = 0; i < kPer; ++i) {
+    const uint32_t at = i * kThreads + threadIdx.x;
+    own[i] = at < count ? c.keys[at] : 0;
+    best = own[i] > best ? own[i] : best;
   }
-  l = block_sum(l, scratch);
-  t = block_sum(t, scratch);
-  const float log_l = logf(l);
-  const bool empty = l == 0.f;
-  if (threadIdx.x == 0) {
-    const uint32_t id = uint32_t(p.ids[r]);
-    p.logprob[r] = id >= p.vocab ? 0.f : empty ? -INFINITY : logit(row, id) - base - log_l;
-    p.entropy[r] = empty ? 0.f : log_l - t / l;
+  set_threshold(c, best, top);
+  if (threadIdx.x == 0) c.count = 0;
+  __syncthreads();
+  const uint64_t threshold = c.threshold;
+#pragma unroll
+  for (uint32_t i = 0; i < kPer; ++i)
+    if (own[i] != 0 && own[i] >= threshold) c.keys[atomicAdd(&c.count, 1u)] = own[i];
+  __syncthreads();
+}
+
+// (m, l, t) of a part of the row: l and t are sums over e^(x - m).
+struct Sums {
+  float m, l, t;
+};
+
+// The sums of both at the greater maximum: with x - m' = (x - m) + (m - m').
+__device__ __forceinline__ Sums merge(const Sums& a, const Sums& b) {
+  Sums r;
+  r.m = fmaxf(a.m, b.m);
+  const float da = a.m - r.m, db = b.m - r.m;
+  const float fa = fast_exp2(da * kLog2e), fb = fast_exp2(db * kLog2e);
+  r.l = a.l * fa + b.l * fb;
+  // (a part that is nothing beside the other may lie infinitely below it)
+  r.t = fmaf(fmaxf(da, -1000.f), a.l, a.t) * fa + fmaf(fmaxf(db, -1000.f), b.l, b.t) * fb;
+  return r;
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t in_rank(const void* local, uint32_t rank) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(local)), "r"(rank));
+  return remote;
+}
+__device__ __forceinline__ float ld_rank(const float* local, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(in_rank(local, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint64_t ld_rank(const uint64_t* local, uint32_t rank) {
+  uint64_t v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(in_rank(local, rank)) : "memory");
+  return v;
+}
+
+// The running sums over `n` more logits. A masked logit is infinitely far down: its weight is 0, and so is its product.
+template <uint32_t N>
+__device__ __forceinline__ float add(Sums& s, const float (&x)[N]) {
+  float m = x[0];
+#pragma unroll
+  for (uint32_t j = 1; j + 1 < N; j += 2) m = fmax3(m, x[j], x[j + 1]);
+  if (N % 2 == 0) m = fmaxf(m, x[N - 1]);
+  if (m > s.m) {
+    const float d = s.m - m, f = fast_exp2(d * kLog2e);
+    s.t = fmaf(fmaxf(d, -1000.f), s.l, s.t) * f;
+    s.l *= f;
+    s.m = m;
   }
-  uint64_t last = ~0ull;
-  for (uint32_t k = 0; k < p.top; ++k) {
-    uint64_t best = 0;
-    for (uint32_t i = threadIdx.x; i < p.vocab; i += kThreads) {
-      const uint64_t key = order_key(logit(row, i), i);
-      if (key < last && key > best) best = key;
+  const uint64_t base = f2_splat(-s.m), scale = f2_splat(kLog2e);
+  uint64_t l = f2_splat(0.f), t = f2_splat(0.f);
+#pragma unroll
+  for (uint32_t j = 0; j + 1 < N; j += 2) {
+    const uint64_t d = f2_add(f2_pack(x[j], x[j + 1]), base);
+    float e0, e1, d0, d1;
+    f2_unpack(f2_mul(d, scale), e0, e1);
+    f2_unpack(d, d0, d1);
+    const uint64_t e = f2_pack(fast_exp2(e0), fast_exp2(e1));
+    l = f2_add(l, e);
+    t = f2_fma(f2_pack(fmaxf(d0, -1000.f), fmaxf(d1, -1000.f)), e, t);
+  }
+  float l0, l1, t0, t1;
+  f2_unpack(l, l0, l1);
+  f2_unpack(t, t0, t1);
+  if (N % 2 == 1) {
+    const float d = x[N - 1] - s.m, e = fast_exp2(d * kLog2e);
+    l0 += e;
+    t0 = fmaf(fmaxf(d, -1000.f), e, t0);
+  }
+  s.l += l0 + l1;
+  s.t += t0 + t1;
+  return m;
+}
+
+// A cluster of `chunks` CTAs per row, each taking a contiguous share of its 16-byte words. TOP: alternatives wanted.
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogprobParams p) {
+  using V = Vector<T>;
+  constexpr uint32_t kN = V::kCount, kVectors = kLogits / kN, kChunk = kThreads * kVectors;  // a chunk in words
+  extern __shared__ __align__(16) uint8_t raw[];
+  Candidates& c = *reinterpret_cast<Candidates*>(raw);
+  __shared__ Sums warp_sums[kWarps];
+  __shared__ Sums cta_sums;
+  __shared__ uint64_t sorted[kMaxTop];
+  const uint32_t chunks = p.chunks, chunk = chunks > 1 ? cluster_rank() : 0u, r = blockIdx.x / chunks;
+  if (TOP && threadIdx.x == 0) c.count = 0;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  // The row: up to kN - 1 logits before its first 16-byte word, the words, up to kN - 1 logits behind them.
+  const T* row = static_cast<const T*>(p.logits) + size_t(r) * p.ld;
+  const uint32_t lead = uint32_t((16 - (reinterpret_cast<uintptr_t>(row) & 15u)) & 15u) / sizeof(T);
+  const uint32_t head = lead < p.vocab ? lead : p.vocab;
+  const uint32_t words = (p.vocab - head) / kN, tail = p.vocab - head - words * kN;
+  const uint4* body = reinterpret_cast<const uint4*>(row + head);
+  const uint32_t per = (words + chunks - 1) / chunks;
+  const uint32_t begin = min(words, chunk * per), end = min(words, begin + per);
+
+  Sums s{-FLT_MAX, 0.f, 0.f};
+  uint4 next[kVectors];
+  auto load = [&](uint32_t base) {
+#pragma unroll
+    for (uint32_t v = 0; v < kVectors; ++v) {
+      const uint32_t w = base + v * kThreads + threadIdx.x;
+      next[v] = make_uint4(0, 0, 0, 0);
+      if (w < end) next[v] = ld_once(body + w);
     }
+  };
+  load(begin);
+  // The first CTA takes the logits before the first word, one to a thread.
+  uint64_t best = 0;  // the thread's greatest key so far
+  if (chunk == 0 && threadIdx.x < head) {
+    const float x[1] = {V::one(row + threadIdx.x)};
+    add(s, x);
+    if (TOP) best = order_key(x[0], threadIdx.x);
+  }
+  bool opened = false;
+  float bar = 0.f;  // the threshold's logit, once the first chunk has opened the list
+  for (uint32_t base = begin; base < end || (TOP && !opened); base += kChunk) {
+    float x[kLogits];
+    uint32_t have = 0;  // this thread's words of the chunk
+#pragma unroll
+    for (uint32_t v = 0; v < kVectors; ++v) {
+      float y[kN];
+      V::unpack(next[v], y);
+      const bool in = base + v * kThreads + threadIdx.x < end;
+      have += in ? 1u : 0u;
+#pragma unroll
+      for (uint32_t j = 0; j < kN; ++j) x[v * kN + j] = in ? y[j] : -INFINITY;
+    }
+    load(base + kChunk);
+    const float greatest = add(s, x);
+    if (TOP) {
+      auto key_of = [&](uint32_t i) {
+        return order_key(x[i], head + (base + i / kN * kThreads + threadIdx.x) * kN + i % kN);
+      };
+      if (!opened) {
+        // The first chunk (and the logits before the words) set the threshold, then offer their own.
+        const uint64_t edge = best;
+#pragma unroll
+        for (uint32_t i = 0; i < kLogits; ++i) {
+          const uint64_t key = i / kN < have ? key_of(i) : 0;
+          best = key > best ? key : best;
+        }
+        set_threshold(c, best, p.top);
+        const uint64_t threshold = c.threshold;
+        if (best != 0 && best >= threshold) {
+          if (edge != 0 && edge >= threshold) c.keys[atomicAdd(&c.count, 1u)] = edge;
+#pragma unroll
+          for (uint32_t i = 0; i < kLogits; ++i) {
+            const uint64_t key = i / kN < have ? key_of(i) : 0;
+            if (key != 0 && key >= threshold) c.keys[atomicAdd(&c.count, 1u)] = key;
+          }
+        }
+        opened = true;
+        bar = key_logit(threshold);  // (a chunk that cannot set it is not full, so no other follows)
+      } else if (have > 0 && !(greatest <= bar && s.l == s.l)) {
+        // fmax3 passes over a NaN, which the sum does not.
+#pragma unroll
+        for (uint32_t i = 0; i < kLogits; ++i)
+          if (!(x[i] <= bar) && i / kN < have) c.keys[atomicAdd(&c.count, 1u)] = key_of(i);
+      }
+      __syncthreads();
+      if (base + kChunk < end) {
+        bool thinned = false;
+        while (c.count > kThin) {
+          thin(c, p.top);
+          thinned = true;
+        }
+        if (thinned) bar = key_logit(c.threshold);
+        // (No thread may add to the list while another still reads its length.)
+        __syncthreads();
+      }
+    }
+  }
+  // The last CTA takes the logits behind the last word.
+  if (chunk == chunks - 1 && threadIdx.x < tail) {
+    const uint32_t i = head + words * kN + threadIdx.x;
+    const float x[1] = {V::one(row + i)};
+    add(s, x);
+    if (TOP) c.keys[atomicAdd(&c.count, 1u)] = order_key(x[0], i);
+  }
+
+  // The CTA's sums.
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Sums other;
+    other.m = __shfl_xor_sync(0xFFFFFFFFu, s.m, o);
+    other.l = __shfl_xor_sync(0xFFFFFFFFu, s.l, o);
+    other.t = __shfl_xor_sync(0xFFFFFFFFu, s.t, o);
+    s = merge(s, other);
+  }
+  if (lane_id() == 0) warp_sums[warp_id()] = s;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    s = threadIdx.x < kWarps ? warp_sums[threadIdx.x] : Sums{-FLT_MAX, 0.f, 0.f};
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-      const uint64_t other = __shfl_xor_sync(0xFFFFFFFFu, best, o);
-      best = other > best ? other : best;
+      Sums other;
+      other.m = __shfl_xor_sync(0xFFFFFFFFu, s.m, o);
+      other.l = __shfl_xor_sync(0xFFFFFFFFu, s.l, o);
+      other.t = __shfl_xor_sync(0xFFFFFFFFu, s.t, o);
+      s = merge(s, other);
     }
-    if (lane_id() == 0) keys[warp_id()] = best;
-    __syncthreads();
-    for (uint32_t w = 0; w < kThreads / 32; ++w) best = keys[w] > best ? keys[w] : best;
-    __syncthreads();
-    last = best;
-    if (threadIdx.x == 0) {
-      p.top_ids[size_t(r) * p.top + k] = int32_t(0xFFFFFFFFu - uint32_t(best));
-      p.top_logprob[size_t(r) * p.top + k] = empty ? -INFINITY : key_logit(best) - base - log_l;
-    }
+    if (threadIdx.x == 0) cta_sums = s;
   }
+  __syncthreads();
+  // Its greatest keys in order: a short list, in which each candidate counts those above it.
+  auto sort = [&]() {
+    while (c.count > 4 * kMaxTop) thin(c, p.top);
+    const uint32_t count = c.count;
+    if (threadIdx.x < kMaxTop) sorted[threadIdx.x] = 0;
+    __syncthreads();
+    if (threadIdx.x < count) {
+      const uint64_t own = c.keys[threadIdx.x];
+      uint32_t above = 0;
+#pragma unroll 4
+      for (uint32_t k = 0; k < count; ++k) above += c.keys[k] > own ? 1u : 0u;
+      if (above < p.top) sorted[above] = own;
+    }
+    __syncthreads();
+  };
+  if (TOP) sort();
+
+  if (chunks > 1) {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (chunk == 0) {
+      s = Sums{ld_rank(&cta_sums.m, 0), ld_rank(&cta_sums.l, 0), ld_rank(&cta_sums.t, 0)};
+      for (uint32_t k = 1; k < chunks; ++k)
+        s = merge(s, Sums{ld_rank(&cta_sums.m, k), ld_rank(&cta_sums.l, k), ld_rank(&cta_sums.t, k)});
+      if (TOP) {
+        uint64_t key = 0;
+        if (threadIdx.x < chunks * kMaxTop) key = ld_rank(&sorted[threadIdx.x % kMaxTop], threadIdx.x / kMaxTop);
+        if (threadIdx.x == 0) c.count = 0;
+        __syncthreads();
+        if (key != 0) c.keys[atomicAdd(&c.count, 1u)] = key;
+        __syncthreads();
+      }
+    }
+    // No CTA leaves while the first may still read its shared memory.
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (chunk != 0) return;
+    if (TOP) sort();
+  } else {
+    s = cta_sums;
+  }
+
+  const float log_l = logf(s.l);
+  const bool empty = s.l == 0.f;
+  if (threadIdx.x == 0) {
+    const uint32_t id = uint32_t(p.ids[r]);
+    p.logprob[r] = id >= p.vocab ? 0.f : empty ? -INFINITY : V::one(row + id) - s.m - log_l;
+    p.entropy[r] = empty ? 0.f : log_l - s.t / s.l;
+  }
+  if (TOP && threadIdx.x < p.top) {
+    const uint64_t key = sorted[threadIdx.x];
+    p.top_ids[size_t(r) * p.top + threadIdx.x] = int32_t(0xFFFFFFFFu - uint32_t(key));
+    p.top_logprob[size_t(r) * p.top + threadIdx.x] = empty ? -INFINITY : key_logit(key) - s.m - log_l;
+  }
+}
+
+template <typename T, bool TOP>
+tempo_status launch_logprobs(const LogprobParams& base, uint32_t rows, cudaStream_t stream) {
+  LogprobParams p = base;
+  constexpr uint32_t kBytes = TOP ? sizeof(Candidates) : 0;
+  auto kernel = token_logprobs_kernel<T, TOP>;
+  tempo_status status = set_smem(reinterpret_cast<const void*>(kernel), kBytes);
+  if (status != TEMPO_OK) return status;
+  // Fewer rows than SMs: a cluster for each, every CTA with at least a quarter of a chunk.
+  p.chunks = 1;
+  while (p.chunks < kMaxChunks && uint64_t(rows) * p.chunks < uint64_t(sm_count()) &&
+         p.vocab >= 2 * p.chunks * (kChunkLogits / 4))
+    p.chunks *= 2;
+  if (uint64_t(rows) * p.chunks > 0x7FFFFFFFull)
+    return fail(TEMPO_ERR_VALUE, "tempo_token_logprobs: %u rows are too many for one call", rows);
+  return launch(kernel, dim3(rows * p.chunks), dim3(kThreads), kBytes, stream, p.chunks, "token_logprobs_kernel", p);
 }
 
 }  // namespace
@@ -131,7 +432,8 @@ extern "C" tempo_status tempo_token_logprobs(const void* logits, uint64_t ld, ui
   if (logits == nullptr || (reinterpret_cast<uintptr_t>(logits) & (bf16 ? 1u : 3u)) || ids == nullptr ||
       logprob == nullptr || entropy == nullptr || (top > 0 && (top_logprob == nullptr || top_ids == nullptr)))
     return fail(TEMPO_ERR_VALUE, "tempo_token_logprobs: aligned logits, ids and every output are needed");
-  const LogprobParams p{logits, ld, ids, vocab, top, logprob, entropy, top_logprob, top_ids};
-  auto kernel = bf16 ? token_logprobs_kernel<uint16_t> : token_logprobs_kernel<float>;
-  return launch(kernel, dim3(rows), dim3(kThreads), 0, static_cast<cudaStream_t>(stream), 1, "token_logprobs_kernel", p);
+  const LogprobParams p{logits, ld, ids, vocab, top, 1, logprob, entropy, top_logprob, top_ids};
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (bf16) return top > 0 ? launch_logprobs<uint16_t, true>(p, rows, st) : launch_logprobs<uint16_t, false>(p, rows, st);
+  return top > 0 ? launch_logprobs<float, true>(p, rows, st) : launch_logprobs<float, false>(p, rows, st);
 }
