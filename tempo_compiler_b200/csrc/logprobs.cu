@@ -6,9 +6,11 @@
 // One pass over the logits, which bounds the kernel (four or two bytes a logit): each thread keeps a running maximum
 // and the two sums rescaled to it, and the alternatives are found on the way. After the first chunk of a row the CTA
 // takes as threshold the top-th greatest of the lane groups' greatest keys, a lower bound on the top-th greatest
-// logit; from then on only the few logits above it go into a candidate list in shared memory, which is thinned by the
-// same device when it fills up and sorted by counting at the end. (A key joins a logit with its index, so keys have no
-// ties, and a later logit equal to the threshold's is below it.) Few rows are split over the CTAs of a cluster, whose sums and sorted candidates the first one merges.
+// logit; from then on only the few logits above it go into a candidate list in shared memory, without a barrier, and
+// the list is thinned by the same device and sorted by counting at the end. (A key joins a logit with its index, so keys
+// have no ties, and a later logit equal to the threshold's is below it.) A row that overflows the list, such as one in
+// rising order, is gone over once more with the threshold raised on the way. Few rows are split over the CTAs of a
+// cluster, whose sums and sorted candidates the first one merges.
 #include <cfloat>
 
 #include <cuda_runtime.h>
@@ -26,8 +28,8 @@ constexpr uint32_t kChunkLogits = kThreads * kLogits;
 constexpr uint32_t kLanes = 4;                      // of a group whose greatest keys give a threshold
 constexpr uint32_t kGroups = kThreads / kLanes;
 constexpr uint32_t kMaxTop = 32;
-constexpr uint32_t kThin = 512;                     // more candidates are thinned before the next chunk
-constexpr uint32_t kCapacity = kThin + kChunkLogits + 8;  // a full chunk on top of them, and the logits behind the words
+constexpr uint32_t kCapacity = 1024;                // candidates
+constexpr uint32_t kThin = kCapacity - kThreads;    // the second look thins above this
 constexpr uint32_t kMaxChunks = 8;                  // CTAs of a cluster sharing one row
 constexpr float kLog2e = 1.4426950408889634f;
 static_assert(kGroups >= 2 * kMaxTop, "thinning drops at least half of the groups");
@@ -92,31 +94,38 @@ struct Candidates {
   uint32_t count;
 };
 
+__device__ __forceinline__ void offer(Candidates& c, uint64_t key) {
+  const uint32_t at = atomicAdd(&c.count, 1u);
+  if (at < kCapacity) c.keys[at] = key;
+}
+
 // Sets the threshold to the top-th greatest of the groups' greatest keys (0 when fewer groups hold a key). `best` is
-// this thread's greatest key. Ends with every thread seeing the threshold.
+// this thread's greatest key. Ends with every thread seeing the threshold. A handful of alternatives is served by
+// half as many groups.
 __device__ __forceinline__ void set_threshold(Candidates& c, uint64_t best, uint32_t top) {
-#pragma unroll
-  for (uint32_t o = 1; o < kLanes; o <<= 1) {
+  const uint32_t lanes = top <= 8 ? 2 * kLanes : kLanes, groups = kThreads / lanes;
+  for (uint32_t o = 1; o < lanes; o <<= 1) {
     const uint64_t other = __shfl_xor_sync(0xFFFFFFFFu, best, o);
     best = other > best ? other : best;
   }
-  if (threadIdx.x % kLanes == 0) c.group[threadIdx.x / kLanes] = best;
+  if (threadIdx.x % lanes == 0) c.group[threadIdx.x / lanes] = best;
   if (threadIdx.x == 0) c.threshold = 0;
   __syncthreads();
-  if (threadIdx.x < kGroups) {
+  if (threadIdx.x < groups) {
     const uint64_t own = c.group[threadIdx.x];
     uint32_t above = 0;
 #pragma unroll 8
-    for (uint32_t i = 0; i < kGroups; ++i) above += c.group[i] > own ? 1u : 0u;
+    for (uint32_t i = 0; i < groups; ++i) above += c.group[i] > own ? 1u : 0u;
     if (above == top - 1 && own != 0) c.threshold = own;  // keys differ: one thread at most
   }
   __syncthreads();
 }
 
-// Drops candidates that cannot be among the `top` greatest: at least the kGroups - top groups whose greatest key is below
-// the threshold, half of a list that fills the groups evenly. Called by the whole CTA, with the list settled.
+// Drops candidates that cannot be among the `top` greatest: at most `top` groups hold a key at or above the threshold,
+// so n keys leave at most top * lanes * ceil(n / kThreads), which is less while n > 4 kMaxTop. Called by the whole CTA,
+// with the list settled and not overflown.
 __device__ __noinline__ void thin(Candidates& c, uint32_t top) {
-  constexpr uint32_t kPer = (kCapacity + kThreads - 1) / kThreads;
+  constexpr uint32_t kPer = kCapacity / kThreads;
   const uint32_t count = c.count;
   uint64_t own[kPer], best = 0;
 #pragma unroll
@@ -150,6 +159,15 @@ __device__ __forceinline__ Sums merge(const Sums& a, const Sums& b) {
   // (a part that is nothing beside the other may lie infinitely below it)
   r.t = fmaf(fmaxf(da, -1000.f), a.l, a.t) * fa + fmaf(fmaxf(db, -1000.f), b.l, b.t) * fb;
   return r;
+}
+
+// The warp's sums: one rescaling to its maximum, then plain additions.
+__device__ __forceinline__ Sums warp_merge(Sums s) {
+  float m = s.m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  const float d = s.m - m, f = fast_exp2(d * kLog2e);
+  return Sums{m, warp_sum(s.l * f), warp_sum(fmaf(fmaxf(d, -1000.f), s.l, s.t) * f)};
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -213,7 +231,7 @@ __device__ __forceinline__ float add(Sums& s, const float (&x)[N]) {
 
 // A cluster of `chunks` CTAs per row, each taking a contiguous share of its 16-byte words. TOP: alternatives wanted.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogprobParams p) {
+__global__ void __launch_bounds__(kThreads, TOP ? 4 : 6) token_logprobs_kernel(LogprobParams p) {
   using V = Vector<T>;
   constexpr uint32_t kN = V::kCount, kVectors = kLogits / kN, kChunk = kThreads * kVectors;  // a chunk in words
   extern __shared__ __align__(16) uint8_t raw[];
@@ -255,61 +273,68 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogprobParams 
   }
   bool opened = false;
   float bar = 0.f;  // the threshold's logit, once the first chunk has opened the list
-  for (uint32_t base = begin; base < end || (TOP && !opened); base += kChunk) {
+  auto index_of = [&](uint32_t base, uint32_t i) {
+    return head + (base + i / kN * kThreads + threadIdx.x) * kN + i % kN;
+  };
+  auto take = [&](uint32_t base, uint32_t have) {  // the chunk in `next`, of which this thread has `have` words
     float x[kLogits];
-    uint32_t have = 0;  // this thread's words of the chunk
 #pragma unroll
     for (uint32_t v = 0; v < kVectors; ++v) {
       float y[kN];
       V::unpack(next[v], y);
-      const bool in = base + v * kThreads + threadIdx.x < end;
-      have += in ? 1u : 0u;
 #pragma unroll
-      for (uint32_t j = 0; j < kN; ++j) x[v * kN + j] = in ? y[j] : -INFINITY;
+      for (uint32_t j = 0; j < kN; ++j) x[v * kN + j] = v < have ? y[j] : -INFINITY;
     }
     load(base + kChunk);
     const float greatest = add(s, x);
-    if (TOP) {
-      auto key_of = [&](uint32_t i) {
-        return order_key(x[i], head + (base + i / kN * kThreads + threadIdx.x) * kN + i % kN);
-      };
-      if (!opened) {
-        // The first chunk (and the logits before the words) set the threshold, then offer their own.
-        const uint64_t edge = best;
-#pragma unroll
-        for (uint32_t i = 0; i < kLogits; ++i) {
-          const uint64_t key = i / kN < have ? key_of(i) : 0;
-          best = key > best ? key : best;
-        }
-        set_threshold(c, best, p.top);
-        const uint64_t threshold = c.threshold;
-        if (best != 0 && best >= threshold) {
-          if (edge != 0 && edge >= threshold) c.keys[atomicAdd(&c.count, 1u)] = edge;
-#pragma unroll
-          for (uint32_t i = 0; i < kLogits; ++i) {
-            const uint64_t key = i / kN < have ? key_of(i) : 0;
-            if (key != 0 && key >= threshold) c.keys[atomicAdd(&c.count, 1u)] = key;
-          }
-        }
-        opened = true;
-        bar = key_logit(threshold);  // (a chunk that cannot set it is not full, so no other follows)
-      } else if (have > 0 && !(greatest <= bar && s.l == s.l)) {
-        // fmax3 passes over a NaN, which the sum does not.
+    if (!TOP) return;
+    if (opened) {
+      // (The maximum passes over a NaN, which the sum does not.)
+      if (!(greatest <= bar && s.l == s.l)) {
 #pragma unroll
         for (uint32_t i = 0; i < kLogits; ++i)
-          if (!(x[i] <= bar) && i / kN < have) c.keys[atomicAdd(&c.count, 1u)] = key_of(i);
+          if (!(x[i] <= bar) && i / kN < have) offer(c, order_key(x[i], index_of(base, i)));
       }
-      __syncthreads();
-      if (base + kChunk < end) {
-        bool thinned = false;
-        while (c.count > kThin) {
-          thin(c, p.top);
-          thinned = true;
+      return;
+    }
+    // The first chunk (and the logits before the words) set the threshold, then offer their own.
+    const uint64_t edge = best;
+    if (s.l == s.l) {
+      uint32_t at = 0;
+#pragma unroll
+      for (int i = kLogits - 1; i >= 0; --i)
+        if (x[i] == greatest) at = i;  // the lowest index of the greatest
+      const uint64_t key = have > 0 ? order_key(greatest, index_of(base, at)) : 0;
+      best = key > best ? key : best;
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < kLogits; ++i) {
+        const uint64_t key = i / kN < have ? order_key(x[i], index_of(base, i)) : 0;
+        best = key > best ? key : best;
+      }
+    }
+    set_threshold(c, best, p.top);
+    const uint64_t threshold = c.threshold;
+    bar = key_logit(threshold);  // (a chunk that cannot set it is not full, so no other follows)
+    if (best != 0 && best >= threshold) {
+      if (edge != 0 && edge >= threshold) offer(c, edge);
+#pragma unroll
+      for (uint32_t i = 0; i < kLogits; ++i)
+        if (!(x[i] < bar) && i / kN < have) {
+          const uint64_t key = order_key(x[i], index_of(base, i));
+          if (key >= threshold) offer(c, key);
         }
-        if (thinned) bar = key_logit(c.threshold);
-        // (No thread may add to the list while another still reads its length.)
-        __syncthreads();
-      }
+    }
+    opened = true;
+  };
+  for (uint32_t base = begin; base < end || (TOP && !opened); base += kChunk) {
+    if (base + kChunk <= end) {
+      take(base, kVectors);
+    } else {
+      uint32_t have = 0;
+#pragma unroll
+      for (uint32_t v = 0; v < kVectors; ++v) have += base + v * kThreads + threadIdx.x < end ? 1u : 0u;
+      take(base, have);
     }
   }
   // The last CTA takes the logits behind the last word.
@@ -317,31 +342,36 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogprobParams 
     const uint32_t i = head + words * kN + threadIdx.x;
     const float x[1] = {V::one(row + i)};
     add(s, x);
-    if (TOP) c.keys[atomicAdd(&c.count, 1u)] = order_key(x[0], i);
+    if (TOP) offer(c, order_key(x[0], i));
   }
 
   // The CTA's sums.
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Sums other;
-    other.m = __shfl_xor_sync(0xFFFFFFFFu, s.m, o);
-    other.l = __shfl_xor_sync(0xFFFFFFFFu, s.l, o);
-    other.t = __shfl_xor_sync(0xFFFFFFFFu, s.t, o);
-    s = merge(s, other);
-  }
+  s = warp_merge(s);
   if (lane_id() == 0) warp_sums[warp_id()] = s;
   __syncthreads();
   if (threadIdx.x < 32) {
-    s = threadIdx.x < kWarps ? warp_sums[threadIdx.x] : Sums{-FLT_MAX, 0.f, 0.f};
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      Sums other;
-      other.m = __shfl_xor_sync(0xFFFFFFFFu, s.m, o);
-      other.l = __shfl_xor_sync(0xFFFFFFFFu, s.l, o);
-      other.t = __shfl_xor_sync(0xFFFFFFFFu, s.t, o);
-      s = merge(s, other);
-    }
+    s = warp_merge(threadIdx.x < kWarps ? warp_sums[threadIdx.x] : Sums{-FLT_MAX, 0.f, 0.f});
     if (threadIdx.x == 0) cta_sums = s;
+  }
+  if (TOP && c.count > kCapacity) {
+    // More candidates than the list holds: the CTA's logits once more, a logit of each thread at a time, with the list
+    // thinned and the threshold raised whenever it fills up.
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      c.count = 0;
+      c.threshold = 0;
+    }
+    __syncthreads();
+    const uint32_t from = chunk == 0 ? 0 : head + begin * kN;
+    const uint32_t to = chunk == chunks - 1 ? p.vocab : head + end * kN;
+    for (uint32_t i0 = from; i0 < to; i0 += kThreads) {
+      const uint32_t i = i0 + threadIdx.x;
+      const uint64_t key = i < to ? order_key(V::one(row + i), i) : 0;
+      if (key > c.threshold) offer(c, key);
+      __syncthreads();
+      while (c.count > kThin) thin(c, p.top);
+      __syncthreads();
+    }
   }
   __syncthreads();
   // Its greatest keys in order: a short list, in which each candidate counts those above it.
