@@ -3,14 +3,14 @@
 //   log p(id) = x[id] - m - ln l,   entropy = ln l - t / l,
 // and the alternatives are the greatest logits, ties going to the lower index.
 //
-// One pass over the logits, which bounds the kernel (four or two bytes a logit): each thread keeps a running maximum
-// and the two sums rescaled to it, and the alternatives are found on the way. After the first chunk of a row the CTA
-// takes as threshold the top-th greatest of the lane groups' greatest keys, a lower bound on the top-th greatest
-// logit; from then on only the few logits above it go into a candidate list in shared memory, without a barrier, and
-// the list is thinned by the same device and sorted by counting at the end. (A key joins a logit with its index, so keys
-// have no ties, and a later logit equal to the threshold's is below it.) A row that overflows the list, such as one in
-// rising order, is gone over once more with the threshold raised on the way. Few rows are split over the CTAs of a
-// cluster, whose sums and sorted candidates the first one merges.
+// One pass over the logits bounds the kernel (four or two bytes a logit): each thread keeps a running maximum and the
+// two sums rescaled to it. The alternatives cost that pass nothing more. From the threads' maxima, the CTA takes the
+// top-th greatest of its lane groups' as a bar, a lower bound on the top-th greatest logit that only about as many
+// logits pass; they lie in the columns of the few threads whose maximum does, which the CTA reads again (from L2) to
+// gather them, as keys that join a logit with its index and so have no ties, and sorts them by counting. A row with more
+// ties at the bar than the list holds, or with a NaN, is searched exactly, at a slower pace. Few rows are split over the
+// CTAs of a cluster, whose sums and sorted candidates the first one merges. (Collecting candidates on the way, against
+// a threshold that rose with the row, took 230 us for 8192 BF16 rows of 50257 instead of 160.)
 #include <cfloat>
 
 #include <cuda_runtime.h>
@@ -23,8 +23,8 @@ namespace {
 
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kWarps = kThreads / 32;
-constexpr uint32_t kLogits = 16;                    // of one thread and chunk
-constexpr uint32_t kChunkLogits = kThreads * kLogits;
+constexpr uint32_t kVectors = 4;                    // 16-byte words of one thread and chunk
+constexpr uint32_t kChunk = kThreads * kVectors;    // a chunk, in 16-byte words
 constexpr uint32_t kLanes = 4;                      // of a group whose greatest keys give a threshold
 constexpr uint32_t kGroups = kThreads / kLanes;
 constexpr uint32_t kMaxTop = 32;
@@ -46,24 +46,58 @@ struct LogprobParams {
   int32_t* top_ids;
 };
 
+// The least of three floats (PTX min.f32 with three inputs); a NaN operand is ignored, as by fminf.
+__device__ __forceinline__ float fmin3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// The logits of 32-bit words: how many, the pairs of them as floats, and the greatest and least of several words.
 template <typename T>
-struct Vector;  // the logits of one 16-byte word
+struct Logits;
 template <>
-struct Vector<float> {
-  static constexpr uint32_t kCount = 4;
-  static __device__ __forceinline__ void unpack(const uint4& w, float (&x)[4]) {
-    x[0] = __uint_as_float(w.x);
-    x[1] = __uint_as_float(w.y);
-    x[2] = __uint_as_float(w.z);
-    x[3] = __uint_as_float(w.w);
-  }
+struct Logits<float> {
+  static constexpr uint32_t kPerWord = 1;                 // logits of a 32-bit word
+  static constexpr uint32_t kMasked = 0xFF800000u;        // a word of -infinity
   static __device__ __forceinline__ float one(const float* p) { return *p; }
+  template <uint32_t N>
+  static __device__ __forceinline__ void pair(const uint32_t (&w)[N], uint32_t i, float& a, float& b) {
+    a = __uint_as_float(w[2 * i]);
+    b = __uint_as_float(w[2 * i + 1]);
+  }
+  template <uint32_t N>
+  static __device__ __forceinline__ void range(const uint32_t (&w)[N], float& most, float& least) {
+    most = least = __uint_as_float(w[0]);
+#pragma unroll
+    for (uint32_t i = 1; i < N; i += 2) {
+      const float a = __uint_as_float(w[i]), b = __uint_as_float(w[i + 1 < N ? i + 1 : i]);
+      most = fmax3(most, a, b);
+      least = fmin3(least, a, b);
+    }
+  }
 };
 template <>
-struct Vector<uint16_t> {
-  static constexpr uint32_t kCount = 8;
-  static __device__ __forceinline__ void unpack(const uint4& w, float (&x)[8]) { unpack8(w, x); }
+struct Logits<uint16_t> {
+  static constexpr uint32_t kPerWord = 2;
+  static constexpr uint32_t kMasked = 0xFF80FF80u;
   static __device__ __forceinline__ float one(const uint16_t* p) { return bf16_to_float(*p); }
+  template <uint32_t N>
+  static __device__ __forceinline__ void pair(const uint32_t (&w)[N], uint32_t i, float& a, float& b) {
+    a = bf16_lo(w[i]);
+    b = bf16_hi(w[i]);
+  }
+  template <uint32_t N>
+  static __device__ __forceinline__ void range(const uint32_t (&w)[N], float& most, float& least) {
+    uint32_t high = w[0], low = w[0];
+#pragma unroll
+    for (uint32_t i = 1; i < N; ++i) {
+      asm("max.bf16x2 %0, %0, %1;" : "+r"(high) : "r"(w[i]));
+      asm("min.bf16x2 %0, %0, %1;" : "+r"(low) : "r"(w[i]));
+    }
+    most = fmaxf(bf16_lo(high), bf16_hi(high));
+    least = fminf(bf16_lo(low), bf16_hi(low));
+  }
 };
 
 __device__ __forceinline__ uint4 ld_once(const uint4* p) {
@@ -92,6 +126,9 @@ struct Candidates {
   uint64_t group[kGroups];
   uint64_t threshold;
   uint32_t count;
+  uint32_t columns;            // threads whose greatest logit reaches the bar
+  uint32_t column[kThreads];
+  float bar;
 };
 
 __device__ __forceinline__ void offer(Candidates& c, uint64_t key) {
@@ -111,18 +148,38 @@ __device__ __forceinline__ void set_threshold(Candidates& c, uint64_t best, uint
   if (threadIdx.x % lanes == 0) c.group[threadIdx.x / lanes] = best;
   if (threadIdx.x == 0) c.threshold = 0;
   __syncthreads();
-  if (threadIdx.x < groups) {
-    const uint64_t own = c.group[threadIdx.x];
-    uint32_t above = 0;
-#pragma unroll 8
-    for (uint32_t i = 0; i < groups; ++i) above += c.group[i] > own ? 1u : 0u;
-    if (above == top - 1 && own != 0) c.threshold = own;  // keys differ: one thread at most
+  const uint64_t own = c.group[threadIdx.x / lanes];
+  uint32_t above = 0;  // the lanes of a group share the counting
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x % lanes; i < groups; i += lanes) above += c.group[i] > own ? 1u : 0u;
+  for (uint32_t o = 1; o < lanes; o <<= 1) above += __shfl_xor_sync(0xFFFFFFFFu, above, o);
+  if (above == top - 1 && own != 0) c.threshold = own;  // keys differ: one group at most
+  __syncthreads();
+}
+
+// The top-th greatest of the groups' greatest logits: a lower bound on the top-th greatest of them all.
+__device__ __forceinline__ void set_bar(Candidates& c, float greatest, uint32_t top) {
+  const uint32_t lanes = top <= 8 ? 2 * kLanes : kLanes, groups = kThreads / lanes;
+  float* group = reinterpret_cast<float*>(c.group);
+  for (uint32_t o = 1; o < lanes; o <<= 1) greatest = fmaxf(greatest, __shfl_xor_sync(0xFFFFFFFFu, greatest, o));
+  if (threadIdx.x % lanes == 0) group[threadIdx.x / lanes] = greatest;
+  __syncthreads();
+  uint32_t above = 0, from = 0;  // groups above this one's, and at or above it
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x % lanes; i < groups; i += lanes) {
+    above += group[i] > greatest ? 1u : 0u;
+    from += group[i] >= greatest ? 1u : 0u;
   }
+  for (uint32_t o = 1; o < lanes; o <<= 1) {
+    above += __shfl_xor_sync(0xFFFFFFFFu, above, o);
+    from += __shfl_xor_sync(0xFFFFFFFFu, from, o);
+  }
+  if (above < top && from >= top) c.bar = greatest;  // (groups that write it write the same)
   __syncthreads();
 }
 
 // Drops candidates that cannot be among the `top` greatest: at most `top` groups hold a key at or above the threshold,
-// so n keys leave at most top * lanes * ceil(n / kThreads), which is less while n > 4 kMaxTop. Called by the whole CTA,
+// so n keys leave at most top * lanes * ceil(n / kThreads), which is less while n > kThreads. Called by the whole CTA,
 // with the list settled and not overflown.
 __device__ __noinline__ void thin(Candidates& c, uint32_t top) {
   constexpr uint32_t kPer = kCapacity / kThreads;
@@ -191,56 +248,72 @@ __device__ __forceinline__ uint64_t ld_rank(const uint64_t* local, uint32_t rank
   return v;
 }
 
-// The running sums over `n` more logits. A masked logit is infinitely far down: its weight is 0, and so is its product.
-template <uint32_t N>
-__device__ __forceinline__ float add(Sums& s, const float (&x)[N]) {
-  float m = x[0];
-#pragma unroll
-  for (uint32_t j = 1; j + 1 < N; j += 2) m = fmax3(m, x[j], x[j + 1]);
-  if (N % 2 == 0) m = fmaxf(m, x[N - 1]);
+__device__ __forceinline__ void raise(Sums& s, float m) {
   if (m > s.m) {
     const float d = s.m - m, f = fast_exp2(d * kLog2e);
     s.t = fmaf(fmaxf(d, -1000.f), s.l, s.t) * f;
     s.l *= f;
     s.m = m;
   }
+}
+
+// One more logit. A masked one is infinitely far down: its weight is 0, and so is its product.
+__device__ __forceinline__ void add_one(Sums& s, float x) {
+  raise(s, x);
+  const float d = x - s.m, e = fast_exp2(d * kLog2e);
+  s.l += e;
+  s.t = fmaf(fmaxf(d, -1000.f), e, s.t);
+}
+
+// 2 M more logits at the current maximum, in pairs. MASKED: some may be infinitely far down.
+template <typename T, uint32_t M, bool MASKED, uint32_t N>
+__device__ __forceinline__ void add_pairs(Sums& s, const uint32_t (&w)[N]) {
   const uint64_t base = f2_splat(-s.m), scale = f2_splat(kLog2e);
   uint64_t l = f2_splat(0.f), t = f2_splat(0.f);
 #pragma unroll
-  for (uint32_t j = 0; j + 1 < N; j += 2) {
-    const uint64_t d = f2_add(f2_pack(x[j], x[j + 1]), base);
-    float e0, e1, d0, d1;
+  for (uint32_t j = 0; j < M; ++j) {
+    float a, b, e0, e1;
+    Logits<T>::pair(w, j, a, b);
+    uint64_t d = f2_add(f2_pack(a, b), base);
     f2_unpack(f2_mul(d, scale), e0, e1);
-    f2_unpack(d, d0, d1);
     const uint64_t e = f2_pack(fast_exp2(e0), fast_exp2(e1));
+    if (MASKED) {
+      f2_unpack(d, a, b);
+      d = f2_pack(fmaxf(a, -1000.f), fmaxf(b, -1000.f));
+    }
     l = f2_add(l, e);
-    t = f2_fma(f2_pack(fmaxf(d0, -1000.f), fmaxf(d1, -1000.f)), e, t);
+    t = f2_fma(d, e, t);
   }
   float l0, l1, t0, t1;
   f2_unpack(l, l0, l1);
   f2_unpack(t, t0, t1);
-  if (N % 2 == 1) {
-    const float d = x[N - 1] - s.m, e = fast_exp2(d * kLog2e);
-    l0 += e;
-    t0 = fmaf(fmaxf(d, -1000.f), e, t0);
-  }
   s.l += l0 + l1;
   s.t += t0 + t1;
-  return m;
+}
+
+// The running sums over the logits of N words; returns the greatest of them.
+template <typename T, uint32_t N>
+__device__ __forceinline__ float add(Sums& s, const uint32_t (&w)[N]) {
+  float most, least;
+  Logits<T>::range(w, most, least);
+  raise(s, most);
+  if (least - s.m >= -1000.f) add_pairs<T, N * Logits<T>::kPerWord / 2, false>(s, w);
+  else add_pairs<T, N * Logits<T>::kPerWord / 2, true>(s, w);
+  return most;
 }
 
 // A cluster of `chunks` CTAs per row, each taking a contiguous share of its 16-byte words. TOP: alternatives wanted.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads, TOP ? 4 : 6) token_logprobs_kernel(LogprobParams p) {
-  using V = Vector<T>;
-  constexpr uint32_t kN = V::kCount, kVectors = kLogits / kN, kChunk = kThreads * kVectors;  // a chunk in words
+__global__ void __launch_bounds__(kThreads, TOP ? (sizeof(T) == 2 ? 4 : 4) : 5) token_logprobs_kernel(LogprobParams p) {
+  using V = Logits<T>;
+  constexpr uint32_t kN = 4 * V::kPerWord;  // logits of a 16-byte word
   extern __shared__ __align__(16) uint8_t raw[];
   Candidates& c = *reinterpret_cast<Candidates*>(raw);
   __shared__ Sums warp_sums[kWarps];
   __shared__ Sums cta_sums;
   __shared__ uint64_t sorted[kMaxTop];
   const uint32_t chunks = p.chunks, chunk = chunks > 1 ? cluster_rank() : 0u, r = blockIdx.x / chunks;
-  if (TOP && threadIdx.x == 0) c.count = 0;
+  if (TOP && threadIdx.x == 0) c.count = c.columns = 0;
   pdl_launch_dependents();
   pdl_wait();
 
@@ -264,85 +337,27 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 6) token_logprobs_kernel(L
     }
   };
   load(begin);
-  // The first CTA takes the logits before the first word, one to a thread.
-  uint64_t best = 0;  // the thread's greatest key so far
-  if (chunk == 0 && threadIdx.x < head) {
-    const float x[1] = {V::one(row + threadIdx.x)};
-    add(s, x);
-    if (TOP) best = order_key(x[0], threadIdx.x);
+  // The first CTA takes the logits before the first word and the last one those behind the last, one to a thread.
+  const bool edge = (chunk == 0 && threadIdx.x < head) || (chunk == chunks - 1 && threadIdx.x - kN < tail);
+  const uint32_t edge_index = threadIdx.x < kN ? threadIdx.x : head + words * kN + threadIdx.x - kN;
+  float edge_logit = -INFINITY;
+  if (edge) {
+    edge_logit = V::one(row + edge_index);
+    add_one(s, edge_logit);
   }
-  bool opened = false;
-  float bar = 0.f;  // the threshold's logit, once the first chunk has opened the list
-  auto index_of = [&](uint32_t base, uint32_t i) {
-    return head + (base + i / kN * kThreads + threadIdx.x) * kN + i % kN;
-  };
-  auto take = [&](uint32_t base, uint32_t have) {  // the chunk in `next`, of which this thread has `have` words
-    float x[kLogits];
+  float highest = edge_logit;  // the greatest of this thread's logits
+  for (uint32_t base = begin; base < end; base += kChunk) {
+    uint32_t w[4 * kVectors];
 #pragma unroll
     for (uint32_t v = 0; v < kVectors; ++v) {
-      float y[kN];
-      V::unpack(next[v], y);
-#pragma unroll
-      for (uint32_t j = 0; j < kN; ++j) x[v * kN + j] = v < have ? y[j] : -INFINITY;
+      const bool in = base + v * kThreads + threadIdx.x < end;
+      w[4 * v] = in ? next[v].x : V::kMasked;
+      w[4 * v + 1] = in ? next[v].y : V::kMasked;
+      w[4 * v + 2] = in ? next[v].z : V::kMasked;
+      w[4 * v + 3] = in ? next[v].w : V::kMasked;
     }
     load(base + kChunk);
-    const float greatest = add(s, x);
-    if (!TOP) return;
-    if (opened) {
-      // (The maximum passes over a NaN, which the sum does not.)
-      if (!(greatest <= bar && s.l == s.l)) {
-#pragma unroll
-        for (uint32_t i = 0; i < kLogits; ++i)
-          if (!(x[i] <= bar) && i / kN < have) offer(c, order_key(x[i], index_of(base, i)));
-      }
-      return;
-    }
-    // The first chunk (and the logits before the words) set the threshold, then offer their own.
-    const uint64_t edge = best;
-    if (s.l == s.l) {
-      uint32_t at = 0;
-#pragma unroll
-      for (int i = kLogits - 1; i >= 0; --i)
-        if (x[i] == greatest) at = i;  // the lowest index of the greatest
-      const uint64_t key = have > 0 ? order_key(greatest, index_of(base, at)) : 0;
-      best = key > best ? key : best;
-    } else {
-#pragma unroll
-      for (uint32_t i = 0; i < kLogits; ++i) {
-        const uint64_t key = i / kN < have ? order_key(x[i], index_of(base, i)) : 0;
-        best = key > best ? key : best;
-      }
-    }
-    set_threshold(c, best, p.top);
-    const uint64_t threshold = c.threshold;
-    bar = key_logit(threshold);  // (a chunk that cannot set it is not full, so no other follows)
-    if (best != 0 && best >= threshold) {
-      if (edge != 0 && edge >= threshold) offer(c, edge);
-#pragma unroll
-      for (uint32_t i = 0; i < kLogits; ++i)
-        if (!(x[i] < bar) && i / kN < have) {
-          const uint64_t key = order_key(x[i], index_of(base, i));
-          if (key >= threshold) offer(c, key);
-        }
-    }
-    opened = true;
-  };
-  for (uint32_t base = begin; base < end || (TOP && !opened); base += kChunk) {
-    if (base + kChunk <= end) {
-      take(base, kVectors);
-    } else {
-      uint32_t have = 0;
-#pragma unroll
-      for (uint32_t v = 0; v < kVectors; ++v) have += base + v * kThreads + threadIdx.x < end ? 1u : 0u;
-      take(base, have);
-    }
-  }
-  // The last CTA takes the logits behind the last word.
-  if (chunk == chunks - 1 && threadIdx.x < tail) {
-    const uint32_t i = head + words * kN + threadIdx.x;
-    const float x[1] = {V::one(row + i)};
-    add(s, x);
-    if (TOP) offer(c, order_key(x[0], i));
+    highest = fmaxf(highest, add<T>(s, w));
   }
 
   // The CTA's sums.
@@ -353,40 +368,81 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 6) token_logprobs_kernel(L
     s = warp_merge(threadIdx.x < kWarps ? warp_sums[threadIdx.x] : Sums{-FLT_MAX, 0.f, 0.f});
     if (threadIdx.x == 0) cta_sums = s;
   }
-  if (TOP && c.count > kCapacity) {
-    // More candidates than the list holds: the CTA's logits once more, a logit of each thread at a time, with the list
-    // thinned and the threshold raised whenever it fills up.
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      c.count = 0;
-      c.threshold = 0;
+  if (TOP) {
+    set_bar(c, highest, p.top);
+    const float bar = c.bar;
+    const bool regular = cta_sums.l == cta_sums.l;  // no NaN and no infinity
+    if (regular) {
+      if (highest >= bar) c.column[atomicAdd(&c.columns, 1u)] = threadIdx.x;
+      if (edge && edge_logit >= bar) offer(c, order_key(edge_logit, edge_index));
+      __syncthreads();
+      const uint32_t steps = (end - begin + kThreads - 1) / kThreads, items = c.columns * steps;
+      for (uint32_t k = threadIdx.x; k < items; k += kThreads) {
+        const uint32_t at = begin + k % steps * kThreads + c.column[k / steps];
+        if (at >= end) continue;
+        if (*reinterpret_cast<volatile uint32_t*>(&c.count) > kCapacity) break;
+        const uint4 word = ld_once(body + at);
+        const uint32_t w[4] = {word.x, word.y, word.z, word.w};
+#pragma unroll
+        for (uint32_t i = 0; i < kN; i += 2) {
+          float a, b;
+          V::pair(w, i / 2, a, b);
+          if (a >= bar) offer(c, order_key(a, head + at * kN + i));
+          if (b >= bar) offer(c, order_key(b, head + at * kN + i + 1));
+        }
+      }
     }
     __syncthreads();
-    const uint32_t from = chunk == 0 ? 0 : head + begin * kN;
-    const uint32_t to = chunk == chunks - 1 ? p.vocab : head + end * kN;
-    for (uint32_t i0 = from; i0 < to; i0 += kThreads) {
-      const uint32_t i = i0 + threadIdx.x;
-      const uint64_t key = i < to ? order_key(V::one(row + i), i) : 0;
-      if (key > c.threshold) offer(c, key);
+    if (!regular || c.count > kCapacity) {
+      // Rounds of eight logits a thread: most add nothing once the threshold stands; the others go in one by one, with
+      // the list thinned and the threshold raised whenever it fills up.
       __syncthreads();
-      while (c.count > kThin) thin(c, p.top);
+      if (threadIdx.x == 0) {
+        c.count = 0;
+        c.threshold = 0;
+      }
       __syncthreads();
+      const uint32_t from = chunk == 0 ? 0 : head + begin * kN;
+      const uint32_t to = chunk == chunks - 1 ? p.vocab : head + end * kN;
+      for (uint32_t i0 = from; i0 < to; i0 += 8 * kThreads) {
+        uint64_t key[8];
+        bool any = false;
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) {
+          const uint32_t i = i0 + j * kThreads + threadIdx.x;
+          key[j] = i < to ? order_key(V::one(row + i), i) : 0;
+          any = any || key[j] > c.threshold;
+        }
+        if (!__syncthreads_or(any)) continue;
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) {
+          if (key[j] > c.threshold) c.keys[atomicAdd(&c.count, 1u)] = key[j];
+          __syncthreads();
+          while (c.count > kThin) thin(c, p.top);
+          __syncthreads();
+        }
+      }
     }
+    __syncthreads();
   }
-  __syncthreads();
   // Its greatest keys in order: a short list, in which each candidate counts those above it.
   auto sort = [&]() {
-    while (c.count > 4 * kMaxTop) thin(c, p.top);
+    if (c.count > kThreads / 4) thin(c, p.top);
+    while (c.count > kThreads) thin(c, p.top);
     const uint32_t count = c.count;
     if (threadIdx.x < kMaxTop) sorted[threadIdx.x] = 0;
     __syncthreads();
-    if (threadIdx.x < count) {
-      const uint64_t own = c.keys[threadIdx.x];
-      uint32_t above = 0;
+    // A short list leaves several lanes to each candidate, which share the counting.
+    const uint32_t lanes = count <= kThreads / 8 ? 8 : count <= kThreads / 4 ? 4 : count <= kThreads / 2 ? 2 : 1;
+    const uint32_t at = threadIdx.x / lanes;
+    const uint64_t own = at < count ? c.keys[at] : 0;
+    uint32_t above = 0;
+    if (at < count) {
 #pragma unroll 4
-      for (uint32_t k = 0; k < count; ++k) above += c.keys[k] > own ? 1u : 0u;
-      if (above < p.top) sorted[above] = own;
+      for (uint32_t k = threadIdx.x % lanes; k < count; k += lanes) above += c.keys[k] > own ? 1u : 0u;
     }
+    for (uint32_t o = 1; o < lanes; o <<= 1) above += __shfl_xor_sync(0xFFFFFFFFu, above, o);
+    if (at < count && above < p.top) sorted[above] = own;
     __syncthreads();
   };
   if (TOP) sort();
@@ -435,10 +491,10 @@ tempo_status launch_logprobs(const LogprobParams& base, uint32_t rows, cudaStrea
   auto kernel = token_logprobs_kernel<T, TOP>;
   tempo_status status = set_smem(reinterpret_cast<const void*>(kernel), kBytes);
   if (status != TEMPO_OK) return status;
-  // Fewer rows than SMs: a cluster for each, every CTA with at least a quarter of a chunk.
+  // At most a row for two SMs: a cluster for each, every CTA with at least 1024 logits.
   p.chunks = 1;
-  while (p.chunks < kMaxChunks && uint64_t(rows) * p.chunks < uint64_t(sm_count()) &&
-         p.vocab >= 2 * p.chunks * (kChunkLogits / 4))
+  while (p.chunks < kMaxChunks && uint64_t(rows) * p.chunks * 2 <= uint64_t(sm_count()) &&
+         p.vocab >= 2 * p.chunks * 1024)
     p.chunks *= 2;
   if (uint64_t(rows) * p.chunks > 0x7FFFFFFFull)
     return fail(TEMPO_ERR_VALUE, "tempo_token_logprobs: %u rows are too many for one call", rows);
