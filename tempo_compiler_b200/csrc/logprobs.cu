@@ -4,11 +4,12 @@
 // and the alternatives are the greatest logits, ties going to the lower index.
 //
 // One pass over the logits bounds the kernel (four or two bytes a logit): each thread keeps a running maximum and the
-// two sums rescaled to it. The alternatives cost that pass nothing more. From the threads' maxima, the CTA takes the
-// top-th greatest of its lane groups' as a bar, a lower bound on the top-th greatest logit that only about as many
-// logits pass; they lie in the columns of the few threads whose maximum does, which the CTA reads again (from L2) to
-// gather them, as keys that join a logit with its index and so have no ties, and sorts them by counting. A row with more
-// ties at the bar than the list holds, or with a NaN, is searched exactly, at a slower pace. Few rows are split over the
+// two sums rescaled to it, and notes the maximum of every cell (its share of a few chunks) in shared memory. The
+// alternatives cost that pass nothing more. From the threads' maxima, the CTA takes the top-th greatest of its lane
+// groups' as a bar, a lower bound on the top-th greatest logit that only about as many logits pass; the CTA reads again
+// the few cells whose maximum does, gathers the logits at or above the bar as keys (which join a logit with its index,
+// and so have no ties) and sorts them by counting. A row with more
+// ties at the bar than the lists hold, or with a NaN, is searched exactly, at a slower pace. Few rows are split over the
 // CTAs of a cluster, whose sums and sorted candidates the first one merges. (Collecting candidates on the way, against
 // a threshold that rose with the row, took 230 us for 8192 BF16 rows of 50257 instead of 160.)
 #include <cfloat>
@@ -30,10 +31,11 @@ constexpr uint32_t kGroups = kThreads / kLanes;
 constexpr uint32_t kMaxTop = 32;
 constexpr uint32_t kCapacity = 1024;                // candidates
 constexpr uint32_t kThin = kCapacity - kThreads;    // the second look thins above this
+constexpr uint32_t kCells = 32;                     // of a thread
+constexpr uint32_t kListed = 512;                   // cells read again
 constexpr uint32_t kMaxChunks = 8;                  // CTAs of a cluster sharing one row
 constexpr float kLog2e = 1.4426950408889634f;
 static_assert(kGroups >= 2 * kMaxTop, "thinning drops at least half of the groups");
-static_assert(kMaxChunks * kMaxTop <= kThreads, "a thread for each candidate of a cluster");
 
 struct LogprobParams {
   const void* logits;
@@ -126,9 +128,10 @@ struct Candidates {
   uint64_t group[kGroups];
   uint64_t threshold;
   uint32_t count;
-  uint32_t columns;            // threads whose greatest logit reaches the bar
-  uint32_t column[kThreads];
   float bar;
+  uint32_t cells;                       // cells whose greatest logit reaches the bar
+  uint32_t cell[kListed];               // thread | number << 16
+  float most[kCells][kThreads];         // the greatest logit of each cell
 };
 
 __device__ __forceinline__ void offer(Candidates& c, uint64_t key) {
@@ -304,7 +307,7 @@ __device__ __forceinline__ float add(Sums& s, const uint32_t (&w)[N]) {
 
 // A cluster of `chunks` CTAs per row, each taking a contiguous share of its 16-byte words. TOP: alternatives wanted.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads, TOP ? (sizeof(T) == 2 ? 4 : 4) : 5) token_logprobs_kernel(LogprobParams p) {
+__global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_logprobs_kernel(LogprobParams p) {
   using V = Logits<T>;
   constexpr uint32_t kN = 4 * V::kPerWord;  // logits of a 16-byte word
   extern __shared__ __align__(16) uint8_t raw[];
@@ -313,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? (sizeof(T) == 2 ? 4 : 4) : 5) 
   __shared__ Sums cta_sums;
   __shared__ uint64_t sorted[kMaxTop];
   const uint32_t chunks = p.chunks, chunk = chunks > 1 ? cluster_rank() : 0u, r = blockIdx.x / chunks;
-  if (TOP && threadIdx.x == 0) c.count = c.columns = 0;
+  if (TOP && threadIdx.x == 0) c.count = c.cells = 0;
   pdl_launch_dependents();
   pdl_wait();
 
@@ -346,6 +349,9 @@ __global__ void __launch_bounds__(kThreads, TOP ? (sizeof(T) == 2 ? 4 : 4) : 5) 
     add_one(s, edge_logit);
   }
   float highest = edge_logit;  // the greatest of this thread's logits
+  const uint32_t stride = (end - begin + kChunk * kCells - 1) / (kChunk * kCells);  // chunks of a cell
+  uint32_t cell = 0, in_cell = 0;
+  float most = -INFINITY;
   for (uint32_t base = begin; base < end; base += kChunk) {
     uint32_t w[4 * kVectors];
 #pragma unroll
@@ -357,7 +363,17 @@ __global__ void __launch_bounds__(kThreads, TOP ? (sizeof(T) == 2 ? 4 : 4) : 5) 
       w[4 * v + 3] = in ? next[v].w : V::kMasked;
     }
     load(base + kChunk);
-    highest = fmaxf(highest, add<T>(s, w));
+    most = fmaxf(most, add<T>(s, w));
+    if (TOP && ++in_cell == stride) {
+      c.most[cell++][threadIdx.x] = most;
+      highest = fmaxf(highest, most);
+      most = -INFINITY;
+      in_cell = 0;
+    }
+  }
+  if (TOP && in_cell > 0) {
+    c.most[cell++][threadIdx.x] = most;
+    highest = fmaxf(highest, most);
   }
 
   // The CTA's sums.
@@ -373,12 +389,19 @@ __global__ void __launch_bounds__(kThreads, TOP ? (sizeof(T) == 2 ? 4 : 4) : 5) 
     const float bar = c.bar;
     const bool regular = cta_sums.l == cta_sums.l;  // no NaN and no infinity
     if (regular) {
-      if (highest >= bar) c.column[atomicAdd(&c.columns, 1u)] = threadIdx.x;
+      if (highest >= bar) {
+        for (uint32_t j = 0; j < cell; ++j)
+          if (c.most[j][threadIdx.x] >= bar) {
+            const uint32_t at = atomicAdd(&c.cells, 1u);
+            if (at < kListed) c.cell[at] = threadIdx.x | j << 16;
+          }
+      }
       if (edge && edge_logit >= bar) offer(c, order_key(edge_logit, edge_index));
       __syncthreads();
-      const uint32_t steps = (end - begin + kThreads - 1) / kThreads, items = c.columns * steps;
+      const uint32_t steps = stride * kVectors, items = min(c.cells, kListed) * steps;
       for (uint32_t k = threadIdx.x; k < items; k += kThreads) {
-        const uint32_t at = begin + k % steps * kThreads + c.column[k / steps];
+        const uint32_t which = c.cell[k / steps];
+        const uint32_t at = begin + ((which >> 16) * steps + k % steps) * kThreads + (which & 0xFFFFu);
         if (at >= end) continue;
         if (*reinterpret_cast<volatile uint32_t*>(&c.count) > kCapacity) break;
         const uint4 word = ld_once(body + at);
@@ -393,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? (sizeof(T) == 2 ? 4 : 4) : 5) 
       }
     }
     __syncthreads();
-    if (!regular || c.count > kCapacity) {
+    if (!regular || c.count > kCapacity || c.cells > kListed) {
       // Rounds of eight logits a thread: most add nothing once the threshold stands; the others go in one by one, with
       // the list thinned and the threshold raised whenever it fills up.
       __syncthreads();
@@ -427,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? (sizeof(T) == 2 ? 4 : 4) : 5) 
   }
   // Its greatest keys in order: a short list, in which each candidate counts those above it.
   auto sort = [&]() {
-    if (c.count > kThreads / 4) thin(c, p.top);
+    if (c.count > 2 * kMaxTop) thin(c, p.top);
     while (c.count > kThreads) thin(c, p.top);
     const uint32_t count = c.count;
     if (threadIdx.x < kMaxTop) sorted[threadIdx.x] = 0;
@@ -454,11 +477,12 @@ __global__ void __launch_bounds__(kThreads, TOP ? (sizeof(T) == 2 ? 4 : 4) : 5) 
       for (uint32_t k = 1; k < chunks; ++k)
         s = merge(s, Sums{ld_rank(&cta_sums.m, k), ld_rank(&cta_sums.l, k), ld_rank(&cta_sums.t, k)});
       if (TOP) {
-        uint64_t key = 0;
-        if (threadIdx.x < chunks * kMaxTop) key = ld_rank(&sorted[threadIdx.x % kMaxTop], threadIdx.x / kMaxTop);
         if (threadIdx.x == 0) c.count = 0;
         __syncthreads();
-        if (key != 0) c.keys[atomicAdd(&c.count, 1u)] = key;
+        for (uint32_t k = threadIdx.x; k < chunks * kMaxTop; k += kThreads) {
+          const uint64_t key = ld_rank(&sorted[k % kMaxTop], k / kMaxTop);
+          if (key != 0) c.keys[atomicAdd(&c.count, 1u)] = key;
+        }
         __syncthreads();
       }
     }
