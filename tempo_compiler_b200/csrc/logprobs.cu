@@ -160,13 +160,21 @@ __device__ __forceinline__ void set_threshold(Candidates& c, uint64_t best, uint
   __syncthreads();
 }
 
-// The top-th greatest of the groups' greatest logits: a lower bound on the top-th greatest of them all.
-__device__ __forceinline__ void set_bar(Candidates& c, float greatest, uint32_t top) {
-  const uint32_t lanes = top <= 8 ? 2 * kLanes : kLanes, groups = kThreads / lanes;
-  float* group = reinterpret_cast<float*>(c.group);
+// The lanes whose greatest logits make one group, from which the bar is taken.
+__device__ __forceinline__ uint32_t group_lanes(uint32_t top) { return top <= 8 ? 2 * kLanes : kLanes; }
+
+// Publishes the greatest logit of each group.
+__device__ __forceinline__ float group_greatest(Candidates& c, float greatest, uint32_t top) {
+  const uint32_t lanes = group_lanes(top);
   for (uint32_t o = 1; o < lanes; o <<= 1) greatest = fmaxf(greatest, __shfl_xor_sync(0xFFFFFFFFu, greatest, o));
-  if (threadIdx.x % lanes == 0) group[threadIdx.x / lanes] = greatest;
-  __syncthreads();
+  if (threadIdx.x % lanes == 0) reinterpret_cast<float*>(c.group)[threadIdx.x / lanes] = greatest;
+  return greatest;
+}
+
+// Sets the bar to the top-th greatest of the groups' greatest logits, a lower bound on the top-th greatest of them all.
+__device__ __forceinline__ void set_bar(Candidates& c, float greatest, uint32_t top) {
+  const uint32_t lanes = group_lanes(top), groups = kThreads / lanes;
+  const float* group = reinterpret_cast<const float*>(c.group);
   uint32_t above = 0, from = 0;  // groups above this one's, and at or above it
 #pragma unroll 4
   for (uint32_t i = threadIdx.x % lanes; i < groups; i += lanes) {
@@ -178,7 +186,6 @@ __device__ __forceinline__ void set_bar(Candidates& c, float greatest, uint32_t 
     from += __shfl_xor_sync(0xFFFFFFFFu, from, o);
   }
   if (above < top && from >= top) c.bar = greatest;  // (groups that write it write the same)
-  __syncthreads();
 }
 
 // Drops candidates that cannot be among the `top` greatest: at most `top` groups hold a key at or above the threshold,
@@ -317,6 +324,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_logprobs_kernel(L
   __shared__ uint64_t sorted[kMaxTop];
   const uint32_t chunks = p.chunks, chunk = chunks > 1 ? cluster_rank() : 0u, r = blockIdx.x / chunks;
   if (TOP && threadIdx.x == 0) c.count = c.cells = 0;
+  if (TOP && threadIdx.x < kMaxTop) sorted[threadIdx.x] = 0;
   pdl_launch_dependents();
   pdl_wait();
 
@@ -330,16 +338,17 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_logprobs_kernel(L
   const uint32_t begin = min(words, chunk * per), end = min(words, begin + per);
 
   Sums s{-FLT_MAX, 0.f, 0.f};
+  const uint32_t full = (end - begin) / kChunk;  // whole chunks; fewer than kChunk words follow them
   uint4 next[kVectors];
-  auto load = [&](uint32_t base) {
+  auto load = [&](uint32_t i) {
+    const uint4* at = body + begin + i * kChunk + threadIdx.x;
 #pragma unroll
-    for (uint32_t v = 0; v < kVectors; ++v) {
-      const uint32_t w = base + v * kThreads + threadIdx.x;
-      next[v] = make_uint4(0, 0, 0, 0);
-      if (w < end) next[v] = ld_once(body + w);
-    }
+    for (uint32_t v = 0; v < kVectors; ++v)
+      if (i < full || begin + i * kChunk + v * kThreads + threadIdx.x < end) next[v] = ld_once(at + v * kThreads);
   };
-  load(begin);
+  load(0);
+  const bool reports = chunk == 0 && threadIdx.x == 0;
+  const uint32_t id = reports ? uint32_t(p.ids[r]) : 0xFFFFFFFFu;
   // The first CTA takes the logits before the first word and the last one those behind the last, one to a thread.
   const bool edge = (chunk == 0 && threadIdx.x < head) || (chunk == chunks - 1 && threadIdx.x - kN < tail);
   const uint32_t edge_index = threadIdx.x < kN ? threadIdx.x : head + words * kN + threadIdx.x - kN;
@@ -352,43 +361,56 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_logprobs_kernel(L
   const uint32_t stride = (end - begin + kChunk * kCells - 1) / (kChunk * kCells);  // chunks of a cell
   uint32_t cell = 0, in_cell = 0;
   float most = -INFINITY;
-  for (uint32_t base = begin; base < end; base += kChunk) {
+  auto close = [&]() {  // the cell is complete
+    c.most[cell++][threadIdx.x] = most;
+    highest = fmaxf(highest, most);
+    most = -INFINITY;
+    in_cell = 0;
+  };
+  for (uint32_t i = 0; i < full; ++i) {
     uint32_t w[4 * kVectors];
 #pragma unroll
     for (uint32_t v = 0; v < kVectors; ++v) {
-      const bool in = base + v * kThreads + threadIdx.x < end;
-      w[4 * v] = in ? next[v].x : V::kMasked;
-      w[4 * v + 1] = in ? next[v].y : V::kMasked;
-      w[4 * v + 2] = in ? next[v].z : V::kMasked;
-      w[4 * v + 3] = in ? next[v].w : V::kMasked;
+      w[4 * v] = next[v].x;
+      w[4 * v + 1] = next[v].y;
+      w[4 * v + 2] = next[v].z;
+      w[4 * v + 3] = next[v].w;
     }
-    load(base + kChunk);
+    load(i + 1);
     most = fmaxf(most, add<T>(s, w));
-    if (TOP && ++in_cell == stride) {
-      c.most[cell++][threadIdx.x] = most;
-      highest = fmaxf(highest, most);
-      most = -INFINITY;
-      in_cell = 0;
-    }
+    if (TOP && ++in_cell == stride) close();
   }
-  if (TOP && in_cell > 0) {
-    c.most[cell++][threadIdx.x] = most;
-    highest = fmaxf(highest, most);
+  // The words behind the whole chunks, a quarter chunk at a time, as far as the warp has any.
+#pragma unroll
+  for (uint32_t v = 0; v < kVectors; ++v) {
+    const uint32_t at = begin + full * kChunk + v * kThreads + threadIdx.x;
+    if (at - lane_id() >= end) break;
+    const bool in = at < end;
+    const uint32_t w[4] = {in ? next[v].x : V::kMasked, in ? next[v].y : V::kMasked, in ? next[v].z : V::kMasked,
+                           in ? next[v].w : V::kMasked};
+    most = fmaxf(most, add<T>(s, w));
   }
+  if (TOP && (in_cell > 0 || begin + full * kChunk < end)) close();
 
-  // The CTA's sums.
+  const float given = id < p.vocab ? V::one(row + id) : 0.f;  // the given token's logit, on its way meanwhile
   s = warp_merge(s);
   if (lane_id() == 0) warp_sums[warp_id()] = s;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    s = warp_merge(threadIdx.x < kWarps ? warp_sums[threadIdx.x] : Sums{-FLT_MAX, 0.f, 0.f});
-    if (threadIdx.x == 0) cta_sums = s;
-  }
+  float group = 0.f;
+  if (TOP) group = group_greatest(c, highest, p.top);
+  const bool regular = !__syncthreads_or(s.l != s.l);  // no NaN and no infinity
+  // The last warp sums up while the others look for the alternatives.
+  auto finish_sums = [&]() {
+    if (threadIdx.x >= kThreads - 32) {
+      s = warp_merge(lane_id() < kWarps ? warp_sums[lane_id()] : Sums{-FLT_MAX, 0.f, 0.f});
+      if (lane_id() == 0) cta_sums = s;
+    }
+  };
+  if (!TOP) finish_sums();
   if (TOP) {
-    set_bar(c, highest, p.top);
-    const float bar = c.bar;
-    const bool regular = cta_sums.l == cta_sums.l;  // no NaN and no infinity
     if (regular) {
+      set_bar(c, group, p.top);
+      __syncthreads();
+      const float bar = c.bar;
       if (highest >= bar) {
         for (uint32_t j = 0; j < cell; ++j)
           if (c.most[j][threadIdx.x] >= bar) {
@@ -397,6 +419,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_logprobs_kernel(L
           }
       }
       if (edge && edge_logit >= bar) offer(c, order_key(edge_logit, edge_index));
+      finish_sums();
       __syncthreads();
       const uint32_t steps = stride * kVectors, items = min(c.cells, kListed) * steps;
       for (uint32_t k = threadIdx.x; k < items; k += kThreads) {
@@ -415,6 +438,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_logprobs_kernel(L
         }
       }
     }
+    if (!regular) finish_sums();
     __syncthreads();
     if (!regular || c.count > kCapacity || c.cells > kListed) {
       // Rounds of eight logits a thread: most add nothing once the threshold stands; the others go in one by one, with
@@ -446,15 +470,12 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_logprobs_kernel(L
         }
       }
     }
-    __syncthreads();
   }
-  // Its greatest keys in order: a short list, in which each candidate counts those above it.
+  // Its greatest keys in order: a short list, in which each candidate counts those above it. (`sorted` is empty before.)
   auto sort = [&]() {
-    if (c.count > 2 * kMaxTop) thin(c, p.top);
+    if (c.count > kThreads / 4) thin(c, p.top);
     while (c.count > kThreads) thin(c, p.top);
     const uint32_t count = c.count;
-    if (threadIdx.x < kMaxTop) sorted[threadIdx.x] = 0;
-    __syncthreads();
     // A short list leaves several lanes to each candidate, which share the counting.
     const uint32_t lanes = count <= kThreads / 8 ? 8 : count <= kThreads / 4 ? 4 : count <= kThreads / 2 ? 2 : 1;
     const uint32_t at = threadIdx.x / lanes;
@@ -469,6 +490,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_logprobs_kernel(L
     __syncthreads();
   };
   if (TOP) sort();
+  else __syncthreads();
 
   if (chunks > 1) {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -496,9 +518,8 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_logprobs_kernel(L
 
   const float log_l = logf(s.l);
   const bool empty = s.l == 0.f;
-  if (threadIdx.x == 0) {
-    const uint32_t id = uint32_t(p.ids[r]);
-    p.logprob[r] = id >= p.vocab ? 0.f : empty ? -INFINITY : V::one(row + id) - s.m - log_l;
+  if (reports) {
+    p.logprob[r] = id >= p.vocab ? 0.f : empty ? -INFINITY : given - s.m - log_l;
     p.entropy[r] = empty ? 0.f : log_l - s.t / s.l;
   }
   if (TOP && threadIdx.x < p.top) {
