@@ -305,7 +305,8 @@ tempo_status tempo_decode_attention_q4(const void* q, uint32_t ldq, const void* 
  * element): logprob[r] = log softmax(logits[r])[ids[r]] (0 where ids[r] is outside [0, vocab): a row without a token),
  * entropy[r] = -sum p ln p, and, with 0 < top <= 32 and top <= vocab, the `top` greatest logits in descending order, ties
  * to the lower index, as top_ids / top_logprob [rows][top]. A logit of -infinity has probability 0. A row of nothing but
- * -infinity scores -infinity with entropy 0; a NaN or +infinity in a row makes its scores NaN, and NaN ranks first. */
+ * -infinity scores -infinity with entropy 0; a NaN, or a logit above 2e38, makes its row's scores NaN, and NaN ranks
+ * first. */
 tempo_status tempo_token_logprobs(const void* logits, uint64_t ld, uint32_t bf16, const int32_t* ids, uint32_t rows,
                                   uint32_t vocab, uint32_t top, float* logprob, float* entropy, float* top_logprob,
                                   int32_t* top_ids, void* stream);

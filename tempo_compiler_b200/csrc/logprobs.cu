@@ -12,7 +12,6 @@
 // ties at the bar than the lists hold, or with a NaN, is searched exactly, at a slower pace. Few rows are split over the
 // CTAs of a cluster, whose sums and sorted candidates the first one merges. (Collecting candidates on the way, against
 // a threshold that rose with the row, took 230 us for 8192 BF16 rows of 50257 instead of 160.)
-#include <cfloat>
 
 #include <cuda_runtime.h>
 
@@ -34,7 +33,7 @@ constexpr uint32_t kThin = kCapacity - kThreads;    // the second look thins abo
 constexpr uint32_t kCells = 32;                     // of a thread
 constexpr uint32_t kListed = 512;                   // cells read again
 constexpr uint32_t kMaxChunks = 8;                  // CTAs of a cluster sharing one row
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 static_assert(kGroups >= 2 * kMaxTop, "thinning drops at least half of the groups");
 
 struct LogprobParams {
@@ -211,20 +210,23 @@ __device__ __noinline__ void thin(Candidates& c, uint32_t top) {
   __syncthreads();
 }
 
-// (m, l, t) of a part of the row: l and t are sums over e^(x - m).
+// A part of the row: l = sum 2^(y - m) and t = sum (y - m) 2^(y - m) over its logits in bits, y = x log2 e. One fused
+// multiply-add gives y - m, rounded once; m is whatever reference the products were taken against, so its own rounding
+// cancels. Logits at or below kDeep (masks of -infinity or of the type's lowest value) weigh nothing beside others; a
+// row of nothing else has l = 0 and is summed on its own.
+constexpr float kDeep = -1e30f;
 struct Sums {
   float m, l, t;
 };
+__device__ __forceinline__ Sums no_sums() { return Sums{2.f * kDeep, 0.f, 0.f}; }
 
-// The sums of both at the greater maximum: with x - m' = (x - m) + (m - m').
+// The sums of both at the greater reference: with y - m' = (y - m) + (m - m').
 __device__ __forceinline__ Sums merge(const Sums& a, const Sums& b) {
   Sums r;
   r.m = fmaxf(a.m, b.m);
-  const float da = a.m - r.m, db = b.m - r.m;
-  const float fa = fast_exp2(da * kLog2e), fb = fast_exp2(db * kLog2e);
+  const float da = a.m - r.m, db = b.m - r.m, fa = fast_exp2(da), fb = fast_exp2(db);
   r.l = a.l * fa + b.l * fb;
-  // (a part that is nothing beside the other may lie infinitely below it)
-  r.t = fmaf(fmaxf(da, -1000.f), a.l, a.t) * fa + fmaf(fmaxf(db, -1000.f), b.l, b.t) * fb;
+  r.t = fmaf(da, a.l, a.t) * fa + fmaf(db, b.l, b.t) * fb;
   return r;
 }
 
@@ -233,8 +235,8 @@ __device__ __forceinline__ Sums warp_merge(Sums s) {
   float m = s.m;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-  const float d = s.m - m, f = fast_exp2(d * kLog2e);
-  return Sums{m, warp_sum(s.l * f), warp_sum(fmaf(fmaxf(d, -1000.f), s.l, s.t) * f)};
+  const float d = s.m - m, f = fast_exp2(d);
+  return Sums{m, warp_sum(s.l * f), warp_sum(fmaf(d, s.l, s.t) * f)};
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -258,58 +260,92 @@ __device__ __forceinline__ uint64_t ld_rank(const uint64_t* local, uint32_t rank
   return v;
 }
 
-__device__ __forceinline__ void raise(Sums& s, float m) {
+// Moves the reference up to the logit `most`.
+__device__ __forceinline__ void raise(Sums& s, float most) {
+  const float m = most * kLog2e;
   if (m > s.m) {
-    const float d = s.m - m, f = fast_exp2(d * kLog2e);
-    s.t = fmaf(fmaxf(d, -1000.f), s.l, s.t) * f;
+    const float d = s.m - m, f = fast_exp2(d);
+    s.t = fmaf(d, s.l, s.t) * f;
     s.l *= f;
     s.m = m;
   }
 }
 
-// One more logit. A masked one is infinitely far down: its weight is 0, and so is its product.
 __device__ __forceinline__ void add_one(Sums& s, float x) {
+  if (x <= kDeep) return;
   raise(s, x);
-  const float d = x - s.m, e = fast_exp2(d * kLog2e);
+  const float y = fmaf(x, kLog2e, -s.m), e = fast_exp2(y);
   s.l += e;
-  s.t = fmaf(fmaxf(d, -1000.f), e, s.t);
-}
-
-// 2 M more logits at the current maximum, in pairs. MASKED: some may be infinitely far down.
-template <typename T, uint32_t M, bool MASKED, uint32_t N>
-__device__ __forceinline__ void add_pairs(Sums& s, const uint32_t (&w)[N]) {
-  const uint64_t base = f2_splat(-s.m), scale = f2_splat(kLog2e);
-  uint64_t l = f2_splat(0.f), t = f2_splat(0.f);
-#pragma unroll
-  for (uint32_t j = 0; j < M; ++j) {
-    float a, b, e0, e1;
-    Logits<T>::pair(w, j, a, b);
-    uint64_t d = f2_add(f2_pack(a, b), base);
-    f2_unpack(f2_mul(d, scale), e0, e1);
-    const uint64_t e = f2_pack(fast_exp2(e0), fast_exp2(e1));
-    if (MASKED) {
-      f2_unpack(d, a, b);
-      d = f2_pack(fmaxf(a, -1000.f), fmaxf(b, -1000.f));
-    }
-    l = f2_add(l, e);
-    t = f2_fma(d, e, t);
-  }
-  float l0, l1, t0, t1;
-  f2_unpack(l, l0, l1);
-  f2_unpack(t, t0, t1);
-  s.l += l0 + l1;
-  s.t += t0 + t1;
+  s.t = fmaf(y, e, s.t);
 }
 
 // The running sums over the logits of N words; returns the greatest of them.
 template <typename T, uint32_t N>
 __device__ __forceinline__ float add(Sums& s, const uint32_t (&w)[N]) {
+  constexpr uint32_t kPairs = N * Logits<T>::kPerWord / 2;
   float most, least;
   Logits<T>::range(w, most, least);
-  raise(s, most);
-  if (least - s.m >= -1000.f) add_pairs<T, N * Logits<T>::kPerWord / 2, false>(s, w);
-  else add_pairs<T, N * Logits<T>::kPerWord / 2, true>(s, w);
+  raise(s, most);  // (a reference below every logit that counts stays)
+  if (least > kDeep) {
+    const uint64_t base = f2_splat(-s.m), scale = f2_splat(kLog2e);
+    uint64_t l = f2_splat(0.f), t = f2_splat(0.f);
+#pragma unroll
+    for (uint32_t j = 0; j < kPairs; ++j) {
+      float a, b;
+      Logits<T>::pair(w, j, a, b);
+      const uint64_t y = f2_fma(f2_pack(a, b), scale, base);
+      f2_unpack(y, a, b);
+      const uint64_t e = f2_pack(fast_exp2(a), fast_exp2(b));
+      l = f2_add(l, e);
+      t = f2_fma(y, e, t);
+    }
+    float l0, l1, t0, t1;
+    f2_unpack(l, l0, l1);
+    f2_unpack(t, t0, t1);
+    s.l += l0 + l1;
+    s.t += t0 + t1;
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < 2 * kPairs; ++j) {
+      float a, b;
+      Logits<T>::pair(w, j / 2, a, b);
+      const float x = j % 2 ? b : a, y = fmaf(x <= kDeep ? kDeep : x, kLog2e, -s.m);
+      const float e = x <= kDeep ? 0.f : fast_exp2(y);
+      s.l += e;
+      s.t = fmaf(y, e, s.t);
+    }
+  }
   return most;
+}
+
+// A row of logits at or below kDeep by one CTA, in the plain units of the logits: d = x - greatest. Sums of e^d and d e^d.
+template <typename T>
+__device__ __noinline__ Sums deep_sums(const T* row, uint32_t vocab, Sums* scratch) {
+  Sums s{-INFINITY, 0.f, 0.f};
+  for (uint32_t i = threadIdx.x; i < vocab; i += kThreads) s.m = fmaxf(s.m, Logits<T>::one(row + i));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s.m = fmaxf(s.m, __shfl_xor_sync(0xFFFFFFFFu, s.m, o));
+  __syncthreads();
+  if (lane_id() == 0) scratch[warp_id()].m = s.m;
+  __syncthreads();
+  for (uint32_t w = 0; w < kWarps; ++w) s.m = fmaxf(s.m, scratch[w].m);
+  if (s.m == -INFINITY) return s;
+  for (uint32_t i = threadIdx.x; i < vocab; i += kThreads) {
+    const float d = fmaxf(Logits<T>::one(row + i) - s.m, -1000.f), e = fast_exp2(d * kLog2e);
+    s.l += e;
+    s.t = fmaf(d, e, s.t);
+  }
+  s.l = warp_sum(s.l);
+  s.t = warp_sum(s.t);
+  __syncthreads();
+  if (lane_id() == 0) scratch[warp_id()] = s;
+  __syncthreads();
+  s.l = s.t = 0.f;
+  for (uint32_t w = 0; w < kWarps; ++w) {
+    s.l += scratch[w].l;
+    s.t += scratch[w].t;
+  }
+  return s;
 }
 
 // A cluster of `chunks` CTAs per row, each taking a contiguous share of its 16-byte words. TOP: alternatives wanted.
@@ -337,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_logprobs_kernel(L
   const uint32_t per = (words + chunks - 1) / chunks;
   const uint32_t begin = min(words, chunk * per), end = min(words, begin + per);
 
-  Sums s{-FLT_MAX, 0.f, 0.f};
+  Sums s = no_sums();
   const uint32_t full = (end - begin) / kChunk;  // whole chunks; fewer than kChunk words follow them
   uint4 next[kVectors];
   auto load = [&](uint32_t i) {
@@ -401,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_logprobs_kernel(L
   // The last warp sums up while the others look for the alternatives.
   auto finish_sums = [&]() {
     if (threadIdx.x >= kThreads - 32) {
-      s = warp_merge(lane_id() < kWarps ? warp_sums[lane_id()] : Sums{-FLT_MAX, 0.f, 0.f});
+      s = warp_merge(lane_id() < kWarps ? warp_sums[lane_id()] : no_sums());
       if (lane_id() == 0) cta_sums = s;
     }
   };
@@ -516,16 +552,24 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_logprobs_kernel(L
     s = cta_sums;
   }
 
-  const float log_l = logf(s.l);
-  const bool empty = s.l == 0.f;
+  const bool deep = s.l == 0.f;
+  if (deep) s = deep_sums<T>(row, p.vocab, warp_sums);  // (uniform: every thread has the row's sums)
+  const bool empty = deep && s.l == 0.f;
+  const float log_l = logf(s.l), unit = deep ? 1.f : kLn2;
+  auto log_probability = [&](float x) {
+    if (empty) return -INFINITY;
+    if (deep) return x - s.m - log_l;
+    // (a masked logit in bits would overflow)
+    return x <= kDeep ? x - fmaf(s.m, kLn2, log_l) : fmaf(fmaf(x, kLog2e, -s.m), kLn2, -log_l);
+  };
   if (reports) {
-    p.logprob[r] = id >= p.vocab ? 0.f : empty ? -INFINITY : given - s.m - log_l;
-    p.entropy[r] = empty ? 0.f : log_l - s.t / s.l;
+    p.logprob[r] = id >= p.vocab ? 0.f : log_probability(given);
+    p.entropy[r] = empty ? 0.f : log_l - unit * (s.t / s.l);
   }
   if (TOP && threadIdx.x < p.top) {
     const uint64_t key = sorted[threadIdx.x];
     p.top_ids[size_t(r) * p.top + threadIdx.x] = int32_t(0xFFFFFFFFu - uint32_t(key));
-    p.top_logprob[size_t(r) * p.top + threadIdx.x] = empty ? -INFINITY : key_logit(key) - s.m - log_l;
+    p.top_logprob[size_t(r) * p.top + threadIdx.x] = log_probability(key_logit(key));
   }
 }
 
