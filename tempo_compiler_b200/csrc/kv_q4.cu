@@ -17,90 +17,182 @@ TEMPO_WATCHDOG_READER(watchdog_kv_q4)
 namespace {
 
 constexpr uint32_t kStoreThreads = 256;
+constexpr uint32_t kUnitLanes = 4;  // lanes that share one row of 64 dimensions, 16 each
 
-// Eight lanes take one row of 64 dimensions (a key or value of one position, head and group), 8 dimensions each: the
-// least and greatest value by shuffles, scale = bf16((greatest - least) / 15), code = rne((x - least) / scale). The
-// subtraction, the two divisions and the roundings are the IEEE ones, so the codes are a function of the row alone.
-// A row whose scale rounds to zero (all values equal) has codes 0; one with a NaN or an infinity has a scale that is
-// not finite, and reads back as NaN.
-__global__ void __launch_bounds__(kStoreThreads) kv_store_q4_kernel(const uint16_t* __restrict__ rows_kv, uint32_t ld,
-                                                                    uint8_t* __restrict__ cache,
-                                                                    const int32_t* __restrict__ seq_of,
-                                                                    const int32_t* __restrict__ pos_of, uint64_t units,
-                                                                    uint32_t seqs, uint32_t kv_heads, uint32_t groups,
-                                                                    uint32_t tiles) {
+// Division by a number known at launch: n / d = (mulhi(n, mul) + n) >> shift for n < 2^31.
+struct Divisor {
+  uint32_t mul, shift;
+};
+Divisor divisor(uint32_t d) {
+  uint32_t shift = 0;
+  while ((uint64_t(1) << shift) < d) ++shift;
+  return Divisor{uint32_t(((uint64_t(1) << 32) * ((uint64_t(1) << shift) - d)) / d + 1), shift};
+}
+__device__ __forceinline__ uint32_t divide(uint32_t n, Divisor d) { return (__umulhi(n, d.mul) + n) >> d.shift; }
+
+// Rows of keys and values (bf16, `ld` elements apart) and their places in a cache.
+struct Q4Rows {
+  uint16_t* rows;
+  uint8_t* cache;
+  const int32_t* seq_of;
+  const int32_t* pos_of;
+  uint32_t ld, units, seqs, kv_heads, tiles;
+  Divisor per_row;      // units of a row: 2 * kv_heads * groups
+  uint32_t units_a_row;
+};
+
+// The unit of this thread: a row's 64 dimensions (columns 64 `column` on of row `row`) and where they are kept.
+template <int G>
+struct Q4Unit {
+  uint32_t row, column, value, slot;
+  uint8_t* block;  // null: the place is outside the cache
+  __device__ __forceinline__ Q4Unit(const Q4Rows& p, uint32_t unit) {
+    row = divide(unit, p.per_row);
+    column = unit - row * p.units_a_row;
+    const uint32_t seq = uint32_t(p.seq_of[row]), pos = uint32_t(p.pos_of[row]);
+    const uint32_t keys = p.kv_heads * G;
+    value = column >= keys ? 1u : 0u;
+    const uint32_t of = column - value * keys;
+    slot = pos % kQ4Tile;
+    block = seq < p.seqs && pos < p.tiles * kQ4Tile
+                ? p.cache + q4_block(seq, of / G, pos, of % G, p.kv_heads, p.tiles, G)
+                : nullptr;
+  }
+  __device__ __forceinline__ uint2* codes(uint32_t li) const {
+    return reinterpret_cast<uint2*>(block + value * kQ4Codes + slot * 32) + li;
+  }
+  __device__ __forceinline__ uint32_t* meta() const {
+    return reinterpret_cast<uint32_t*>(block + 2 * kQ4Codes) + slot * 2 + value;
+  }
+};
+
+__device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t min_nan_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+// Four codes (integers 0 .. 15 as floats) as a 16-bit field: c0 + 16 c1 + 256 c2 + 4096 c3 is exact in FP32, and adding
+// 2^23 leaves it in the low bits.
+__device__ __forceinline__ uint32_t pack_codes(float c0, float c1, float c2, float c3) {
+  return __float_as_uint(fmaf(4096.f, c3, fmaf(256.f, c2, fmaf(16.f, c1, c0))) + 8388608.f);
+}
+
+// Storing is bound by the bytes it moves as long as the arithmetic stays near ten instructions a value. The least and
+// greatest value come from packed BF16 comparisons (a NaN stays); scale = bf16((greatest - least) / 15); and the
+// code is the quotient (x - least) / scale, correctly rounded to FP32, rounded to the nearest integer, ties to even. With
+// r = 1 / scale correctly rounded, q = d r and q + (d - q scale) r is the correctly rounded quotient (Markstein's
+// theorem) while nothing underflows; scales outside [2^-90, 2^100] take the division itself. Adding 1.5 2^23 rounds.
+// A row of values that are all equal has scale 0 and codes 0; one with a NaN, an infinity or a range that
+// passes FP32 has a scale that is not finite, and reads back as NaN. (A first form, eight lanes to a row with a 64-bit
+// index division, FP32 divisions and conversions, took 304 us for storing and reading 65536 rows of 12 heads.)
+template <int G>
+__global__ void __launch_bounds__(kStoreThreads) kv_store_q4_kernel(Q4Rows p) {
   pdl_wait();
   pdl_launch_dependents();
-  const uint64_t unit = (uint64_t(blockIdx.x) * kStoreThreads + threadIdx.x) >> 3;
-  const uint32_t li = threadIdx.x & 7u;
-  if (unit >= units) return;  // whole groups of eight lanes leave together
-  const uint32_t mask = 0xFFu << (threadIdx.x & 24u);
-  const uint32_t per_row = 2 * kv_heads * groups;
-  const uint32_t row = uint32_t(unit / per_row), column = uint32_t(unit % per_row);
-  const uint32_t seq = uint32_t(seq_of[row]), pos = uint32_t(pos_of[row]);
-  if (seq >= seqs || pos >= tiles * kQ4Tile) return;
-  const uint32_t value = column / (kv_heads * groups), head = column / groups % kv_heads, group = column % groups;
-  float x[8];
-  unpack8(*reinterpret_cast<const uint4*>(rows_kv + size_t(row) * ld + column * kQ4Group + li * 8), x);
-  float low = x[0], high = x[0];
-  bool finite = true;
+  const uint32_t at = blockIdx.x * kStoreThreads + threadIdx.x, li = at % kUnitLanes;
+  if (at / kUnitLanes >= p.units) return;  // whole units leave together
+  const uint32_t mask = 0xFu << (threadIdx.x & 28u);
+  const Q4Unit<G> unit(p, at / kUnitLanes);
+  if (unit.block == nullptr) return;
+  const uint4* src = reinterpret_cast<const uint4*>(p.rows + size_t(unit.row) * p.ld + unit.column * kQ4Group) + 2 * li;
+  const uint4 a = src[0], b = src[1];
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  uint32_t most = w[0], least = w[0];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    low = fminf(low, x[j]);
-    high = fmaxf(high, x[j]);
-    finite = finite && fabsf(x[j]) < INFINITY;  // false for NaN too
+  for (int i = 1; i < 8; ++i) {
+    most = max_nan_bf16x2(most, w[i]);
+    least = min_nan_bf16x2(least, w[i]);
   }
 #pragma unroll
-  for (int o = 4; o > 0; o >>= 1) {
-    low = fminf(low, __shfl_xor_sync(mask, low, o));
-    high = fmaxf(high, __shfl_xor_sync(mask, high, o));
+  for (int o = 1; o <= 2; o <<= 1) {
+    most = max_nan_bf16x2(most, __shfl_xor_sync(mask, most, o));
+    least = min_nan_bf16x2(least, __shfl_xor_sync(mask, least, o));
   }
-  finite = (__ballot_sync(mask, finite) & mask) == mask;
+  // both halves of each word
+  most = max_nan_bf16x2(most, __byte_perm(most, 0, 0x1032));
+  least = min_nan_bf16x2(least, __byte_perm(least, 0, 0x1032));
+  const float high = bf16_lo(most), low = bf16_lo(least);
+  const bool finite = fabsf(high) < INFINITY && fabsf(low) < INFINITY;  // false for a NaN too
   const float scale = finite ? round_bf16(__fdiv_rn(high - low, 15.f)) : __int_as_float(0x7FC00000);
-  uint32_t word = 0;
-  if (scale > 0.f) {
+  float c[16];
+  if (scale >= 0x1p-90f && scale <= 0x1p100f) {
+    const float r = __frcp_rn(scale);
+    const uint64_t r2 = f2_splat(r), s2 = f2_splat(-scale), low2 = f2_splat(-low), round2 = f2_splat(12582912.f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float code = fminf(fmaxf(rintf(__fdiv_rn(x[j] - low, scale)), 0.f), 15.f);
-      word |= uint32_t(code) << (4 * j);
+    for (int i = 0; i < 8; ++i) {
+      const uint64_t d = f2_add(f2_pack(bf16_lo(w[i]), bf16_hi(w[i])), low2);
+      const uint64_t q = f2_mul(d, r2);
+      const uint64_t exact = f2_fma(f2_fma(q, s2, d), r2, q);
+      // in 0 .. 15: the scale's rounding moves a quotient by at most 15 / 256
+      f2_unpack(f2_add(f2_add(exact, round2), f2_splat(-12582912.f)), c[2 * i], c[2 * i + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float x = i % 2 ? bf16_hi(w[i / 2]) : bf16_lo(w[i / 2]);
+      c[i] = scale > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(x - low, scale)), 0.f), 15.f) : 0.f;
     }
   }
-  uint8_t* block = cache + q4_block(seq, head, pos, group, kv_heads, tiles, groups);
-  const uint32_t slot = pos % kQ4Tile;
-  reinterpret_cast<uint32_t*>(block + value * kQ4Codes + slot * 32)[li] = word;
-  if (li == 0)
-    reinterpret_cast<uint32_t*>(block + 2 * kQ4Codes)[slot * 2 + value] = pack_bf16x2(scale, finite ? low : 0.f);
+  uint2 word;
+  word.x = __byte_perm(pack_codes(c[0], c[1], c[2], c[3]), pack_codes(c[4], c[5], c[6], c[7]), 0x5410);
+  word.y = __byte_perm(pack_codes(c[8], c[9], c[10], c[11]), pack_codes(c[12], c[13], c[14], c[15]), 0x5410);
+  *unit.codes(li) = word;
+  if (li == 0) *unit.meta() = pack_bf16x2(scale, finite ? low : 0.f);
 }
 
 // The rows' keys and values back as BF16: code x scale + low in FP32, rounded once.
-__global__ void __launch_bounds__(kStoreThreads) kv_load_q4_kernel(const uint8_t* __restrict__ cache,
-                                                                   uint16_t* __restrict__ out, uint32_t ldo,
-                                                                   const int32_t* __restrict__ seq_of,
-                                                                   const int32_t* __restrict__ pos_of, uint64_t units,
-                                                                   uint32_t seqs, uint32_t kv_heads, uint32_t groups,
-                                                                   uint32_t tiles) {
+template <int G>
+__global__ void __launch_bounds__(kStoreThreads) kv_load_q4_kernel(Q4Rows p) {
   pdl_wait();
   pdl_launch_dependents();
-  const uint64_t unit = (uint64_t(blockIdx.x) * kStoreThreads + threadIdx.x) >> 3;
-  const uint32_t li = threadIdx.x & 7u;
-  if (unit >= units) return;
-  const uint32_t per_row = 2 * kv_heads * groups;
-  const uint32_t row = uint32_t(unit / per_row), column = uint32_t(unit % per_row);
-  const uint32_t seq = uint32_t(seq_of[row]), pos = uint32_t(pos_of[row]);
-  uint4* dst = reinterpret_cast<uint4*>(out + size_t(row) * ldo + column * kQ4Group + li * 8);
-  if (seq >= seqs || pos >= tiles * kQ4Tile) {
-    *dst = make_uint4(0, 0, 0, 0);
+  const uint32_t at = blockIdx.x * kStoreThreads + threadIdx.x, li = at % kUnitLanes;
+  if (at / kUnitLanes >= p.units) return;
+  const Q4Unit<G> unit(p, at / kUnitLanes);
+  uint4* dst = reinterpret_cast<uint4*>(p.rows + size_t(unit.row) * p.ld + unit.column * kQ4Group) + 2 * li;
+  if (unit.block == nullptr) {
+    dst[0] = dst[1] = make_uint4(0, 0, 0, 0);
     return;
   }
-  const uint32_t value = column / (kv_heads * groups), head = column / groups % kv_heads, group = column % groups;
-  const uint8_t* block = cache + q4_block(seq, head, pos, group, kv_heads, tiles, groups);
-  const uint32_t slot = pos % kQ4Tile;
-  const uint32_t word = reinterpret_cast<const uint32_t*>(block + value * kQ4Codes + slot * 32)[li];
-  const uint32_t meta = reinterpret_cast<const uint32_t*>(block + 2 * kQ4Codes)[slot * 2 + value];
-  float x[8];
+  const uint2 codes = *unit.codes(li);
+  const uint32_t meta = *unit.meta();
+  const float s = bf16_lo(meta), l = bf16_hi(meta);
+  uint32_t out[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] = fmaf(float((word >> (4 * j)) & 15u), bf16_lo(meta), bf16_hi(meta));
-  *dst = pack8(x);
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t word = (i < 4 ? codes.x : codes.y) >> (8 * (i % 4));
+    // a code under the exponent of 2^23 is the float 2^23 + code
+    const float c0 = __uint_as_float((word & 15u) | 0x4B000000u) - 8388608.f;
+    const float c1 = __uint_as_float(((word >> 4) & 15u) | 0x4B000000u) - 8388608.f;
+    out[i] = pack_bf16x2(fmaf(c0, s, l), fmaf(c1, s, l));
+  }
+  dst[0] = make_uint4(out[0], out[1], out[2], out[3]);
+  dst[1] = make_uint4(out[4], out[5], out[6], out[7]);
+}
+
+// Launches `kernel` over `rows` rows, in as many calls as 31-bit thread numbers need.
+tempo_status launch_rows(void (*kernel)(Q4Rows), Q4Rows p, uint32_t rows, uint32_t groups, cudaStream_t stream,
+                         const char* name) {
+  p.units_a_row = 2 * p.kv_heads * groups;
+  p.per_row = divisor(p.units_a_row);
+  const uint32_t most = 0x7FFFFF00u / (kUnitLanes * p.units_a_row);
+  for (uint32_t done = 0; done < rows;) {
+    const uint32_t count = rows - done < most ? rows - done : most;
+    p.units = count * p.units_a_row;
+    const tempo_status status = launch(kernel, dim3((p.units * kUnitLanes + kStoreThreads - 1) / kStoreThreads),
+                                       dim3(kStoreThreads), 0, stream, 1, name, p);
+    if (status != TEMPO_OK) return status;
+    p.rows += size_t(count) * p.ld;
+    p.seq_of += count;
+    p.pos_of += count;
+    done += count;
+  }
+  return TEMPO_OK;
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -624,9 +716,10 @@ tempo_status launch_attention(const Q4Attention& base, uint32_t seqs, cudaStream
 // What the three entry points check alike; `what` names the call.
 tempo_status check_cache(const char* what, const void* cache, uint32_t seqs, uint32_t kv_heads, uint32_t head,
                          uint32_t capacity) {
-  if (seqs == 0 || kv_heads == 0 || capacity == 0 || capacity % kQ4Tile || (head != 64 && head != 128))
-    return fail(TEMPO_ERR_VALUE, "%s: seqs %u kv_heads %u head %u (64 or 128) capacity %u (a multiple of 16)", what,
-                seqs, kv_heads, head, capacity);
+  if (seqs == 0 || kv_heads == 0 || kv_heads > 65535 || capacity == 0 || capacity % kQ4Tile ||
+      (head != 64 && head != 128))
+    return fail(TEMPO_ERR_VALUE, "%s: seqs %u kv_heads %u (up to 65535) head %u (64 or 128) capacity %u (a multiple of "
+                "16)", what, seqs, kv_heads, head, capacity);
   if (cache == nullptr || !aligned16(cache)) return fail(TEMPO_ERR_VALUE, "%s: the cache must be 16-byte aligned", what);
   return TEMPO_OK;
 }
@@ -642,18 +735,22 @@ extern "C" tempo_status tempo_kv_store_q4(const void* qkv, uint32_t ldq, void* c
   tempo_status status = check_cache("tempo_kv_store_q4", cache, seqs, kv_heads, head, capacity);
   if (status != TEMPO_OK) return status;
   const uint64_t width = (uint64_t(heads) + 2ull * kv_heads) * head;
-  if (rows == 0 || width > ldq || ldq % 8)
+  if (rows == 0 || rows > 0x7FFFFFFFu || width > ldq || ldq % 8)
     return fail(TEMPO_ERR_VALUE, "tempo_kv_store_q4: rows %u, row stride %u (a multiple of 8, at least %llu)", rows, ldq,
                 static_cast<unsigned long long>(width));
   if (qkv == nullptr || !aligned16(qkv) || seq_of == nullptr || pos_of == nullptr)
     return fail(TEMPO_ERR_VALUE, "tempo_kv_store_q4: 16-byte aligned rows, a sequence and a position of each are needed");
-  const uint64_t units = uint64_t(rows) * 2 * kv_heads * (head / kQ4Group);
-  const uint64_t blocks = (units * 8 + kStoreThreads - 1) / kStoreThreads;
-  if (blocks > 0x7FFFFFFFull) return fail(TEMPO_ERR_VALUE, "tempo_kv_store_q4: %u rows are too many for one call", rows);
-  return launch(kv_store_q4_kernel, dim3(uint32_t(blocks)), dim3(kStoreThreads), 0, static_cast<cudaStream_t>(stream),
-                1, "kv_store_q4_kernel", static_cast<const uint16_t*>(qkv) + size_t(heads) * head, ldq,
-                static_cast<uint8_t*>(cache), seq_of, pos_of, units, seqs, kv_heads, head / kQ4Group,
-                capacity / kQ4Tile);
+  Q4Rows p{};
+  p.rows = const_cast<uint16_t*>(static_cast<const uint16_t*>(qkv)) + size_t(heads) * head;
+  p.cache = static_cast<uint8_t*>(cache);
+  p.seq_of = seq_of;
+  p.pos_of = pos_of;
+  p.ld = ldq;
+  p.seqs = seqs;
+  p.kv_heads = kv_heads;
+  p.tiles = capacity / kQ4Tile;
+  return launch_rows(head == 64 ? kv_store_q4_kernel<1> : kv_store_q4_kernel<2>, p, rows, head / kQ4Group,
+                     static_cast<cudaStream_t>(stream), "kv_store_q4_kernel");
 }
 
 extern "C" tempo_status tempo_kv_load_q4(const void* cache, void* kv, uint32_t ldo, const int32_t* seq_of,
@@ -662,18 +759,23 @@ extern "C" tempo_status tempo_kv_load_q4(const void* cache, void* kv, uint32_t l
   tempo_status status = check_cache("tempo_kv_load_q4", cache, seqs, kv_heads, head, capacity);
   if (status != TEMPO_OK) return status;
   const uint64_t width = 2ull * kv_heads * head;
-  if (rows == 0 || width > ldo || ldo % 8)
+  if (rows == 0 || rows > 0x7FFFFFFFu || width > ldo || ldo % 8)
     return fail(TEMPO_ERR_VALUE, "tempo_kv_load_q4: rows %u, row stride %u (a multiple of 8, at least %llu)", rows, ldo,
                 static_cast<unsigned long long>(width));
   if (kv == nullptr || !aligned16(kv) || seq_of == nullptr || pos_of == nullptr)
     return fail(TEMPO_ERR_VALUE, "tempo_kv_load_q4: a 16-byte aligned output, a sequence and a position of each row are "
                 "needed");
-  const uint64_t units = uint64_t(rows) * 2 * kv_heads * (head / kQ4Group);
-  const uint64_t blocks = (units * 8 + kStoreThreads - 1) / kStoreThreads;
-  if (blocks > 0x7FFFFFFFull) return fail(TEMPO_ERR_VALUE, "tempo_kv_load_q4: %u rows are too many for one call", rows);
-  return launch(kv_load_q4_kernel, dim3(uint32_t(blocks)), dim3(kStoreThreads), 0, static_cast<cudaStream_t>(stream), 1,
-                "kv_load_q4_kernel", static_cast<const uint8_t*>(cache), static_cast<uint16_t*>(kv), ldo, seq_of, pos_of,
-                units, seqs, kv_heads, head / kQ4Group, capacity / kQ4Tile);
+  Q4Rows p{};
+  p.rows = static_cast<uint16_t*>(kv);
+  p.cache = const_cast<uint8_t*>(static_cast<const uint8_t*>(cache));
+  p.seq_of = seq_of;
+  p.pos_of = pos_of;
+  p.ld = ldo;
+  p.seqs = seqs;
+  p.kv_heads = kv_heads;
+  p.tiles = capacity / kQ4Tile;
+  return launch_rows(head == 64 ? kv_load_q4_kernel<1> : kv_load_q4_kernel<2>, p, rows, head / kQ4Group,
+                     static_cast<cudaStream_t>(stream), "kv_load_q4_kernel");
 }
 
 extern "C" tempo_status tempo_decode_attention_q4(const void* q, uint32_t ldq, const void* cache,
