@@ -36,33 +36,38 @@ struct Q4Rows {
   uint8_t* cache;
   const int32_t* seq_of;
   const int32_t* pos_of;
-  uint32_t ld, units, seqs, kv_heads, tiles;
+  uint32_t ld, count, seqs, kv_heads, tiles;
   Divisor per_row;      // units of a row: 2 * kv_heads * groups
   uint32_t units_a_row;
 };
 
-// The unit of this thread: a row's 64 dimensions (columns 64 `column` on of row `row`) and where they are kept.
+// A unit: a row's 64 dimensions (columns 64 `column` on of row `row`) and where they are kept. Eight consecutive units, a
+// warp's, are the same column of eight rows: of a prompt, 256 bytes of codes side by side.
 template <int G>
 struct Q4Unit {
-  uint32_t row, column, value, slot;
-  uint8_t* block;  // null: the place is outside the cache
+  uint32_t row, column, seq, pos, value;
   __device__ __forceinline__ Q4Unit(const Q4Rows& p, uint32_t unit) {
-    row = divide(unit, p.per_row);
-    column = unit - row * p.units_a_row;
-    const uint32_t seq = uint32_t(p.seq_of[row]), pos = uint32_t(p.pos_of[row]);
-    const uint32_t keys = p.kv_heads * G;
-    value = column >= keys ? 1u : 0u;
-    const uint32_t of = column - value * keys;
-    slot = pos % kQ4Tile;
-    block = seq < p.seqs && pos < p.tiles * kQ4Tile
-                ? p.cache + q4_block(seq, of / G, pos, of % G, p.kv_heads, p.tiles, G)
-                : nullptr;
+    const uint32_t eight = divide(unit >> 3, p.per_row);
+    column = (unit >> 3) - eight * p.units_a_row;
+    row = eight * 8 + (unit & 7u);
+    seq = pos = 0;
+    if (row < p.count) {
+      seq = uint32_t(p.seq_of[row]);
+      pos = uint32_t(p.pos_of[row]);
+    }
+    value = column >= p.kv_heads * G ? 1u : 0u;
   }
-  __device__ __forceinline__ uint2* codes(uint32_t li) const {
-    return reinterpret_cast<uint2*>(block + value * kQ4Codes + slot * 32) + li;
+  // The unit's block, or null when the place is outside the cache.
+  __device__ __forceinline__ uint8_t* place(const Q4Rows& p) const {
+    const uint32_t of = column - value * p.kv_heads * G;
+    if (seq >= p.seqs || pos >= p.tiles * kQ4Tile) return nullptr;
+    return p.cache + q4_block(seq, of / G, pos, of % G, p.kv_heads, p.tiles, G);
   }
-  __device__ __forceinline__ uint32_t* meta() const {
-    return reinterpret_cast<uint32_t*>(block + 2 * kQ4Codes) + slot * 2 + value;
+  __device__ __forceinline__ uint2* codes(uint8_t* block) const {
+    return reinterpret_cast<uint2*>(block + value * kQ4Codes + pos % kQ4Tile * 32);
+  }
+  __device__ __forceinline__ uint32_t* meta(uint8_t* block) const {
+    return reinterpret_cast<uint32_t*>(block + 2 * kQ4Codes) + pos % kQ4Tile * 2 + value;
   }
 };
 
@@ -91,17 +96,8 @@ __device__ __forceinline__ uint32_t pack_codes(float c0, float c1, float c2, flo
 // A row of values that are all equal has scale 0 and codes 0; one with a NaN, an infinity or a range that
 // passes FP32 has a scale that is not finite, and reads back as NaN. (A first form, eight lanes to a row with a 64-bit
 // index division, FP32 divisions and conversions, took 304 us for storing and reading 65536 rows of 12 heads.)
-template <int G>
-__global__ void __launch_bounds__(kStoreThreads) kv_store_q4_kernel(Q4Rows p) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const uint32_t at = blockIdx.x * kStoreThreads + threadIdx.x, li = at % kUnitLanes;
-  if (at / kUnitLanes >= p.units) return;  // whole units leave together
-  const uint32_t mask = 0xFu << (threadIdx.x & 28u);
-  const Q4Unit<G> unit(p, at / kUnitLanes);
-  if (unit.block == nullptr) return;
-  const uint4* src = reinterpret_cast<const uint4*>(p.rows + size_t(unit.row) * p.ld + unit.column * kQ4Group) + 2 * li;
-  const uint4 a = src[0], b = src[1];
+__device__ __forceinline__ void store_unit(const uint4& a, const uint4& b, uint32_t mask, uint32_t li, uint2* codes,
+                                           uint32_t* meta) {
   const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
   uint32_t most = w[0], least = w[0];
 #pragma unroll
@@ -139,11 +135,26 @@ __global__ void __launch_bounds__(kStoreThreads) kv_store_q4_kernel(Q4Rows p) {
       c[i] = scale > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(x - low, scale)), 0.f), 15.f) : 0.f;
     }
   }
+  if (codes == nullptr) return;
   uint2 word;
   word.x = __byte_perm(pack_codes(c[0], c[1], c[2], c[3]), pack_codes(c[4], c[5], c[6], c[7]), 0x5410);
   word.y = __byte_perm(pack_codes(c[8], c[9], c[10], c[11]), pack_codes(c[12], c[13], c[14], c[15]), 0x5410);
-  *unit.codes(li) = word;
-  if (li == 0) *unit.meta() = pack_bf16x2(scale, finite ? low : 0.f);
+  codes[li] = word;
+  if (li == 0) *meta = pack_bf16x2(scale, finite ? low : 0.f);
+}
+
+template <int G>
+__global__ void __launch_bounds__(kStoreThreads) kv_store_q4_kernel(Q4Rows p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const uint32_t li = threadIdx.x % kUnitLanes, mask = 0xFu << (threadIdx.x & 28u);
+  const Q4Unit<G> unit(p, (blockIdx.x * kStoreThreads + threadIdx.x) / kUnitLanes);
+  if (unit.row >= p.count) return;  // whole units leave together
+  // The row is on its way before its place is known; a place outside the cache only keeps it from being stored.
+  const uint4* src = reinterpret_cast<const uint4*>(p.rows + size_t(unit.row) * p.ld + unit.column * kQ4Group) + 2 * li;
+  const uint4 a = src[0], b = src[1];
+  uint8_t* block = unit.place(p);
+  store_unit(a, b, mask, li, block == nullptr ? nullptr : unit.codes(block), unit.meta(block));
 }
 
 // The rows' keys and values back as BF16: code x scale + low in FP32, rounded once.
@@ -151,16 +162,16 @@ template <int G>
 __global__ void __launch_bounds__(kStoreThreads) kv_load_q4_kernel(Q4Rows p) {
   pdl_wait();
   pdl_launch_dependents();
-  const uint32_t at = blockIdx.x * kStoreThreads + threadIdx.x, li = at % kUnitLanes;
-  if (at / kUnitLanes >= p.units) return;
-  const Q4Unit<G> unit(p, at / kUnitLanes);
-  uint4* dst = reinterpret_cast<uint4*>(p.rows + size_t(unit.row) * p.ld + unit.column * kQ4Group) + 2 * li;
-  if (unit.block == nullptr) {
-    dst[0] = dst[1] = make_uint4(0, 0, 0, 0);
-    return;
+  const uint32_t li = threadIdx.x % kUnitLanes;
+  const Q4Unit<G> unit(p, (blockIdx.x * kStoreThreads + threadIdx.x) / kUnitLanes);
+  if (unit.row >= p.count) return;
+  uint8_t* block = unit.place(p);
+  uint2 codes = make_uint2(0, 0);
+  uint32_t meta = 0;  // a place outside the cache: zeros
+  if (block != nullptr) {
+    codes = unit.codes(block)[li];
+    meta = *unit.meta(block);
   }
-  const uint2 codes = *unit.codes(li);
-  const uint32_t meta = *unit.meta();
   const float s = bf16_lo(meta), l = bf16_hi(meta);
   uint32_t out[8];
 #pragma unroll
@@ -171,6 +182,7 @@ __global__ void __launch_bounds__(kStoreThreads) kv_load_q4_kernel(Q4Rows p) {
     const float c1 = __uint_as_float(((word >> 4) & 15u) | 0x4B000000u) - 8388608.f;
     out[i] = pack_bf16x2(fmaf(c0, s, l), fmaf(c1, s, l));
   }
+  uint4* dst = reinterpret_cast<uint4*>(p.rows + size_t(unit.row) * p.ld + unit.column * kQ4Group) + 2 * li;
   dst[0] = make_uint4(out[0], out[1], out[2], out[3]);
   dst[1] = make_uint4(out[4], out[5], out[6], out[7]);
 }
@@ -180,12 +192,13 @@ tempo_status launch_rows(void (*kernel)(Q4Rows), Q4Rows p, uint32_t rows, uint32
                          const char* name) {
   p.units_a_row = 2 * p.kv_heads * groups;
   p.per_row = divisor(p.units_a_row);
-  const uint32_t most = 0x7FFFFF00u / (kUnitLanes * p.units_a_row);
+  const uint32_t most = 0x7FFFFF00u / (8 * kUnitLanes * p.units_a_row) * 8;
   for (uint32_t done = 0; done < rows;) {
     const uint32_t count = rows - done < most ? rows - done : most;
-    p.units = count * p.units_a_row;
-    const tempo_status status = launch(kernel, dim3((p.units * kUnitLanes + kStoreThreads - 1) / kStoreThreads),
-                                       dim3(kStoreThreads), 0, stream, 1, name, p);
+    p.count = count;
+    const uint32_t threads = (count + 7) / 8 * 8 * p.units_a_row * kUnitLanes;
+    const tempo_status status = launch(kernel, dim3((threads - 1) / kStoreThreads + 1), dim3(kStoreThreads), 0, stream, 1,
+                                       name, p);
     if (status != TEMPO_OK) return status;
     p.rows += size_t(count) * p.ld;
     p.seq_of += count;
