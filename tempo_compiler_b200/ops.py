@@ -19,7 +19,8 @@ _LAUNCHES = [0]
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The current device's current stream, as the library takes it (a Stream object costs 3 us more to make)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _launch(name: str, *args) -> None:
@@ -56,8 +57,12 @@ def _check_rows(t: torch.Tensor, dtype: torch.dtype, name: str) -> None:
         raise ValueError(f"{name} must be a CUDA tensor: the B200 kernels have no CPU path")
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] != 1) or (t.stride(0) < t.shape[1] and t.shape[0] != 1):
-        raise ValueError(f"{name} must be a matrix of contiguous rows that do not overlap")
+    if t.dim() == 2:
+        rows, width = t.shape
+        step, unit = t.stride()
+        if (unit == 1 or width == 1) and (step >= width or rows == 1):
+            return
+    raise ValueError(f"{name} must be a matrix of contiguous rows that do not overlap")
 
 
 def _row_stride(t: torch.Tensor) -> int:
@@ -66,19 +71,29 @@ def _row_stride(t: torch.Tensor) -> int:
 
 
 def _check_devices(first: torch.Tensor, **others: torch.Tensor | None) -> None:
+    device = first.get_device()
     for name, t in others.items():
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != device:
             raise ValueError(f"{name} is on {t.device}, the call's first operand on {first.device}")
+
+
+_ENTRIES: dict[str, object] = {}
 
 
 def _launch_at(t: torch.Tensor, name: str, *args) -> None:
     """_launch on the current stream of `t`'s device, which need not be the current device."""
-    index = t.device.index
-    if index == torch.cuda.current_device():
-        _launch(name, *args, torch.cuda.current_stream().cuda_stream)
+    entry = _ENTRIES.get(name)
+    if entry is None:
+        entry = _ENTRIES[name] = getattr(_lib.load(), name)
+    device = t.get_device()
+    if device == torch._C._cuda_getDevice():
+        status = entry(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
-        with torch.cuda.device(index):
-            _launch(name, *args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(device):
+            status = entry(*args, torch._C._cuda_getCurrentRawStream(device))
+    _LAUNCHES[0] += 1
+    if status:
+        _lib.check(status)
 
 
 def gemm(a: torch.Tensor, w_t: torch.Tensor, *, bias: torch.Tensor | None = None,
@@ -113,7 +128,7 @@ def gemm_f32(a: torch.Tensor, w_t: torch.Tensor, *, out: torch.Tensor | None = N
     if w_t.shape[1] != k:
         raise ValueError(f"inner dimensions differ: a {tuple(a.shape)}, w_t {tuple(w_t.shape)}")
     if out is None:
-        out = torch.empty((m, (n + 7) // 8 * 8), dtype=torch.float32, device=a.device)[:, :n]
+        out = a.new_empty((m, (n + 7) // 8 * 8), dtype=torch.float32)[:, :n]
     _check_rows(out, torch.float32, "out")
     if out.shape != (m, n):
         raise ValueError(f"out must be {(m, n)}, got {tuple(out.shape)}")
@@ -358,11 +373,12 @@ def kv_cache_q4(seqs: int, kv_heads: int, capacity: int, head: int = 64, *,
 def _q4_shape(cache: torch.Tensor) -> tuple[int, int, int, int]:
     """(seqs, kv_heads, head, capacity) of a 4-bit cache."""
     _check(cache, torch.uint8, "cache")
-    if cache.dim() != 4 or cache.shape[3] not in (_lib.Q4_BLOCK_BYTES, 2 * _lib.Q4_BLOCK_BYTES):
-        raise ValueError(f"cache must be [seqs, kv_heads, tiles, 1152 or 2304] as kv_cache_q4 makes it, got "
-                         f"{tuple(cache.shape)}")
-    seqs, kv_heads, tiles, size = cache.shape
-    return seqs, kv_heads, size // _lib.Q4_BLOCK_BYTES * 64, tiles * _lib.Q4_TILE
+    if cache.dim() == 4:
+        seqs, kv_heads, tiles, size = cache.shape
+        if size == _lib.Q4_BLOCK_BYTES or size == 2 * _lib.Q4_BLOCK_BYTES:
+            return seqs, kv_heads, 64 if size == _lib.Q4_BLOCK_BYTES else 128, tiles * _lib.Q4_TILE
+    raise ValueError(f"cache must be [seqs, kv_heads, tiles, 1152 or 2304] as kv_cache_q4 makes it, got "
+                     f"{tuple(cache.shape)}")
 
 
 def _check_places(rows: int, seq_of: torch.Tensor, pos_of: torch.Tensor) -> None:
@@ -396,10 +412,11 @@ def kv_load_q4(cache: torch.Tensor, seq_of: torch.Tensor, pos_of: torch.Tensor, 
     rows = pos_of.numel()
     _check_places(rows, seq_of, pos_of)
     if out is None:
-        out = torch.empty((rows, 2 * kv_heads * head), dtype=torch.bfloat16, device=cache.device)
-    _check_rows(out, torch.bfloat16, "out")
-    if out.shape != (rows, 2 * kv_heads * head):
-        raise ValueError(f"out must be {(rows, 2 * kv_heads * head)}, got {tuple(out.shape)}")
+        out = cache.new_empty((rows, 2 * kv_heads * head), dtype=torch.bfloat16)
+    else:
+        _check_rows(out, torch.bfloat16, "out")
+        if out.shape != (rows, 2 * kv_heads * head):
+            raise ValueError(f"out must be {(rows, 2 * kv_heads * head)}, got {tuple(out.shape)}")
     _check_devices(cache, seq_of=seq_of, pos_of=pos_of, out=out)
     _launch_at(cache, "tempo_kv_load_q4", cache.data_ptr(), out.data_ptr(), _row_stride(out), seq_of.data_ptr(),
                pos_of.data_ptr(), rows, seqs, kv_heads, head, capacity)
@@ -424,10 +441,11 @@ def decode_attention_q4(qkv: torch.Tensor, cache: torch.Tensor, lengths: torch.T
         raise ValueError(f"{seqs} sequences need a query row and a length each, got {qkv.shape[0]} and "
                          f"{lengths.numel()}")
     if out is None:
-        out = torch.empty((seqs, heads * head), dtype=torch.bfloat16, device=qkv.device)
-    _check(out, torch.bfloat16, "out")
-    if out.shape != (seqs, heads * head):
-        raise ValueError(f"out must be {(seqs, heads * head)}, got {tuple(out.shape)}")
+        out = qkv.new_empty((seqs, heads * head))
+    else:
+        _check(out, torch.bfloat16, "out")
+        if out.shape != (seqs, heads * head):
+            raise ValueError(f"out must be {(seqs, heads * head)}, got {tuple(out.shape)}")
     _check_devices(qkv, cache=cache, lengths=lengths, out=out)
     _launch_at(qkv, "tempo_decode_attention_q4", qkv.data_ptr(), _row_stride(qkv), cache.data_ptr(),
                lengths.data_ptr(), length_offset, out.data_ptr(), seqs, heads, kv_heads, head, capacity)
@@ -460,13 +478,14 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, *, top: int = 0,
     if not 0 <= top <= min(32, vocab):
         raise ValueError(f"top must be in [0, {min(32, vocab)}], got {top}")
     if out is None:
-        # one allocation: the two or three FP32 outputs and the ids
-        words = torch.empty(rows * (2 + 2 * top), dtype=torch.float32, device=logits.device)
-        logprob, entropy = words[:rows], words[rows:2 * rows]
-        top_logprob = top_ids = None
+        # one allocation, split
         if top:
-            top_logprob = words[2 * rows:(2 + top) * rows].view(rows, top)
-            top_ids = words[(2 + top) * rows:].view(torch.int32).view(rows, top)
+            words = logits.new_empty(2 * rows * (1 + top), dtype=torch.float32)
+            logprob, entropy, best, order = words.split((rows, rows, rows * top, rows * top))
+            top_logprob, top_ids = best.view(rows, top), order.view(torch.int32).view(rows, top)
+        else:
+            logprob, entropy = logits.new_empty((2, rows), dtype=torch.float32).unbind()
+            top_logprob = top_ids = None
         out = TokenScores(logprob, entropy, top_logprob, top_ids)
     else:
         for name, t, shape, dtype in (("logprob", out.logprob, (rows,), torch.float32),
@@ -480,8 +499,9 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, *, top: int = 0,
             _check(t, dtype, f"out.{name}")
             if t.shape != shape:
                 raise ValueError(f"out.{name} must be {shape}, got {tuple(t.shape)}")
-    _check_devices(logits, ids=ids, logprob=out.logprob, entropy=out.entropy, top_logprob=out.top_logprob,
-                   top_ids=out.top_ids)
+        _check_devices(logits, logprob=out.logprob, entropy=out.entropy, top_logprob=out.top_logprob,
+                       top_ids=out.top_ids)
+    _check_devices(logits, ids=ids)
     _launch_at(logits, "tempo_token_logprobs", logits.data_ptr(), _row_stride(logits), int(bf16), ids.data_ptr(), rows,
                vocab, top, out.logprob.data_ptr(), out.entropy.data_ptr(), _ptr(out.top_logprob), _ptr(out.top_ids))
     return out
