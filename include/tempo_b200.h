@@ -306,10 +306,13 @@ tempo_status tempo_decode_attention_q4(const void* q, uint32_t ldq, const void* 
  * entropy[r] = -sum p ln p, and, with 0 < top <= 32 and top <= vocab, the `top` greatest logits in descending order, ties
  * to the lower index, as top_ids / top_logprob [rows][top]. A logit of -infinity has probability 0. A row of nothing but
  * -infinity scores -infinity with entropy 0; a NaN, or a logit above 2e38, makes its row's scores NaN, and NaN ranks
- * first. */
+ * first. With slot_of (NULL for none), the outputs hold `slots` blocks of `rows` rows and row r's results go to block
+ * slot_of[r] + slot_offset, or nowhere when there is no such block: a captured decode step writes each step's results
+ * behind the last's. */
 tempo_status tempo_token_logprobs(const void* logits, uint64_t ld, uint32_t bf16, const int32_t* ids, uint32_t rows,
                                   uint32_t vocab, uint32_t top, float* logprob, float* entropy, float* top_logprob,
-                                  int32_t* top_ids, void* stream);
+                                  int32_t* top_ids, const int32_t* slot_of, int32_t slot_offset, uint32_t slots,
+                                  void* stream);
 
 /* Reduces argmax partials [rows][tiles] to token ids: ids[r] = first index of the row maximum (ties go to the lower
  * index, as numpy's argmax). When tokens_out is not NULL the id is also written to tokens_out[r * out_stride + c] with

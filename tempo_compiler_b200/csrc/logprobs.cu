@@ -40,11 +40,16 @@ struct LogprobParams {
   const void* logits;
   uint64_t ld;
   const int32_t* ids;
-  uint32_t vocab, top, chunks;
+  uint32_t rows, vocab, top, chunks;
   float* logprob;
   float* entropy;
   float* top_logprob;
   int32_t* top_ids;
+  // With slot_of, row r's results go to row slot * rows + r of the outputs, slot = slot_of[r] + slot_offset, and nowhere
+  // unless 0 <= slot < slots.
+  const int32_t* slot_of;
+  int32_t slot_offset;
+  uint32_t slots;
 };
 
 // The least of three floats (PTX min.f32 with three inputs); a NaN operand is ignored, as by fminf.
@@ -562,20 +567,27 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_logprobs_kernel(L
     // (a masked logit in bits would overflow)
     return x <= kDeep ? x - fmaf(s.m, kLn2, log_l) : fmaf(fmaf(x, kLog2e, -s.m), kLn2, -log_l);
   };
+  uint64_t to = r;
+  if (p.slot_of != nullptr) {
+    const int64_t slot = int64_t(p.slot_of[r]) + p.slot_offset;
+    if (slot < 0 || slot >= int64_t(p.slots)) return;
+    to = uint64_t(slot) * p.rows + r;
+  }
   if (reports) {
-    p.logprob[r] = id >= p.vocab ? 0.f : log_probability(given);
-    p.entropy[r] = empty ? 0.f : log_l - unit * (s.t / s.l);
+    p.logprob[to] = id >= p.vocab ? 0.f : log_probability(given);
+    p.entropy[to] = empty ? 0.f : log_l - unit * (s.t / s.l);
   }
   if (TOP && threadIdx.x < p.top) {
     const uint64_t key = sorted[threadIdx.x];
-    p.top_ids[size_t(r) * p.top + threadIdx.x] = int32_t(0xFFFFFFFFu - uint32_t(key));
-    p.top_logprob[size_t(r) * p.top + threadIdx.x] = log_probability(key_logit(key));
+    p.top_ids[to * p.top + threadIdx.x] = int32_t(0xFFFFFFFFu - uint32_t(key));
+    p.top_logprob[to * p.top + threadIdx.x] = log_probability(key_logit(key));
   }
 }
 
 template <typename T, bool TOP>
-tempo_status launch_logprobs(const LogprobParams& base, uint32_t rows, cudaStream_t stream) {
+tempo_status launch_logprobs(const LogprobParams& base, cudaStream_t stream) {
   LogprobParams p = base;
+  const uint32_t rows = p.rows;
   constexpr uint32_t kBytes = TOP ? sizeof(Candidates) : 0;
   auto kernel = token_logprobs_kernel<T, TOP>;
   tempo_status status = set_smem(reinterpret_cast<const void*>(kernel), kBytes);
@@ -597,7 +609,9 @@ using namespace tempo;
 
 extern "C" tempo_status tempo_token_logprobs(const void* logits, uint64_t ld, uint32_t bf16, const int32_t* ids,
                                              uint32_t rows, uint32_t vocab, uint32_t top, float* logprob,
-                                             float* entropy, float* top_logprob, int32_t* top_ids, void* stream) {
+                                             float* entropy, float* top_logprob, int32_t* top_ids,
+                                             const int32_t* slot_of, int32_t slot_offset, uint32_t slots,
+                                             void* stream) {
   if (rows == 0 || vocab == 0 || vocab > 0x7FFFFFFFu || rows > 0x7FFFFFFFu || ld < vocab)
     return fail(TEMPO_ERR_VALUE, "tempo_token_logprobs: rows %u vocab %u, row stride %llu (at least the vocabulary)", rows,
                 vocab, static_cast<unsigned long long>(ld));
@@ -607,8 +621,10 @@ extern "C" tempo_status tempo_token_logprobs(const void* logits, uint64_t ld, ui
   if (logits == nullptr || (reinterpret_cast<uintptr_t>(logits) & (bf16 ? 1u : 3u)) || ids == nullptr ||
       logprob == nullptr || entropy == nullptr || (top > 0 && (top_logprob == nullptr || top_ids == nullptr)))
     return fail(TEMPO_ERR_VALUE, "tempo_token_logprobs: aligned logits, ids and every output are needed");
-  const LogprobParams p{logits, ld, ids, vocab, top, 1, logprob, entropy, top_logprob, top_ids};
+  if (slot_of != nullptr && slots == 0) return fail(TEMPO_ERR_VALUE, "tempo_token_logprobs: no slots to write to");
+  const LogprobParams p{logits, ld, ids, rows, vocab, top, 1, logprob, entropy, top_logprob, top_ids, slot_of, slot_offset,
+                        slots};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (bf16) return top > 0 ? launch_logprobs<uint16_t, true>(p, rows, st) : launch_logprobs<uint16_t, false>(p, rows, st);
-  return top > 0 ? launch_logprobs<float, true>(p, rows, st) : launch_logprobs<float, false>(p, rows, st);
+  if (bf16) return top > 0 ? launch_logprobs<uint16_t, true>(p, st) : launch_logprobs<uint16_t, false>(p, st);
+  return top > 0 ? launch_logprobs<float, true>(p, st) : launch_logprobs<float, false>(p, st);
 }

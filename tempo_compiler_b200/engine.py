@@ -18,6 +18,11 @@ is the B200 layout of the same math:
 * the decode step (embedding, 12 layers, LM head, argmax, position advance) is captured once as a CUDA graph and
   replayed, its varying state (ids, positions) living in device buffers.
 
+Two options change what the decode step reads and reports: ``kv_bits=4`` keeps the cache in 4 bits (72 bytes per position
+and head instead of 256, ``ops.kv_store_q4`` and ``ops.decode_attention_q4``), and ``alternatives`` reports each generated
+token's log probability, the entropy and the likeliest other tokens from the LM head's FP32 logits (``ops.gemm_f32``,
+``ops.token_logprobs``). ``Engine.score`` rates given tokens the same way.
+
 Every kernel is libtempo_b200.so's (through ``tempo_compiler_b200.ops``); torch only provides memory and streams.
 Sequences in one batch share one prompt length.
 """
@@ -27,6 +32,7 @@ from __future__ import annotations
 import dataclasses
 import math
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -35,6 +41,7 @@ from tempo_compiler_b200 import ops
 from tempo_compiler_b200.weights import GPT2_SMALL, GPT2Shape
 
 LN_EPSILON = 1e-5
+SCORE_ROWS = 2048  # rows of logits that score() holds at a time (412 MB at GPT-2's vocabulary)
 
 
 def _bf16(array: np.ndarray, device) -> torch.Tensor:
@@ -74,6 +81,16 @@ class LayerWeights:
     fc_folded: tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None = None
 
 
+class Scores(NamedTuple):
+    """What token_logprobs reports, on the host: per sequence and token the log probability of the token and the entropy
+    of its distribution (nats), and the `alternatives` likeliest tokens with their log probabilities, likeliest first."""
+
+    logprob: np.ndarray      # [batch, tokens] float32
+    entropy: np.ndarray      # [batch, tokens] float32
+    top_logprob: np.ndarray  # [batch, tokens, alternatives] float32
+    top_ids: np.ndarray      # [batch, tokens, alternatives] int32
+
+
 class Engine:
     """Batched GPT-2 greedy generation on one GPU.
 
@@ -103,12 +120,19 @@ class Engine:
             step takes 293 / 341 / 706 us persistent against 279 / 308 / 690 us kernel-per-op at 1 / 2 / 8
             sequences. A grid barrier costs 1.36 us, about what a dependent launch's boundary costs, and the step
             has 61 dependent phases either way.
+        kv_bits: 16 (the cache holds BF16) or 4 (``ops.kv_cache_q4``). With 4, decode attention reads 28 % of the
+            bytes and the prompts' own attention still uses their BF16 keys and values; the tokens are those of a model
+            whose cached keys and values are rounded to 16 levels per row. Excludes persistent_decode.
+        alternatives: with 0 or more, each generated token's scores are kept for ``scores()``, with that many (at most
+            32) of the likeliest tokens; None (the default) keeps none. Needs one decode group and excludes
+            persistent_decode. The tokens are the same with and without.
     """
 
     def __init__(self, layers: list[dict], shared: dict, *, batch: int, prompt: int, capacity: int,
                  shape: GPT2Shape = GPT2_SMALL, device: str | torch.device = "cuda",
                  decode_groups: int | None = None, fold_layernorms: bool | None = None,
-                 fuse_small_norms: bool | None = None, persistent_decode: bool | None = None) -> None:
+                 fuse_small_norms: bool | None = None, persistent_decode: bool | None = None, kv_bits: int = 16,
+                 alternatives: int | None = None) -> None:
         if not torch.cuda.is_available():
             raise RuntimeError("the B200 engine needs a CUDA device; there is no CPU path")
         self.device = torch.device(device)
@@ -120,6 +144,15 @@ class Engine:
         if not 0 < prompt <= capacity <= shape.positions:
             raise ValueError(f"prompt {prompt} and capacity {capacity} must satisfy 0 < prompt <= capacity <= "
                              f"{shape.positions}, the model's learned positions")
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 16 or 4, got {kv_bits}")
+        if alternatives is not None and not 0 <= alternatives <= min(32, shape.vocab):
+            raise ValueError(f"alternatives must be in [0, {min(32, shape.vocab)}], got {alternatives}")
+        if persistent_decode and (kv_bits != 16 or alternatives is not None):
+            raise ValueError("the persistent decode step has a BF16 cache and reports no scores")
+        if alternatives is not None and decode_groups not in (None, 1):
+            raise ValueError("scores of generated tokens need one decode group")
+        self.kv_bits, self.alternatives = kv_bits, alternatives
         width, heads = shape.width, shape.heads
         scale = np.ones(3 * width, dtype=np.float32)
         scale[:width] = 1.0 / math.sqrt(width // heads)
@@ -145,9 +178,15 @@ class Engine:
                 lw.qkv_folded = fold_layernorm(lw.ln1_g, lw.ln1_b, lw.w_qkv, lw.b_qkv)
                 lw.fc_folded = fold_layernorm(lw.ln2_g, lw.ln2_b, lw.w_fc, lw.b_fc)
         n_layers = len(layers)
-        cache_shape = (batch, heads, capacity, shape.head)
-        self.k_cache = [torch.empty(cache_shape, dtype=torch.bfloat16, device=self.device) for _ in range(n_layers)]
-        self.v_cache = [torch.empty(cache_shape, dtype=torch.bfloat16, device=self.device) for _ in range(n_layers)]
+        if kv_bits == 4:
+            self.kv_cache = [ops.kv_cache_q4(batch, heads, capacity, shape.head, device=self.device)
+                             for _ in range(n_layers)]
+        else:
+            cache_shape = (batch, heads, capacity, shape.head)
+            self.k_cache = [torch.empty(cache_shape, dtype=torch.bfloat16, device=self.device)
+                            for _ in range(n_layers)]
+            self.v_cache = [torch.empty(cache_shape, dtype=torch.bfloat16, device=self.device)
+                            for _ in range(n_layers)]
         rows = batch * prompt
         bf = dict(dtype=torch.bfloat16, device=self.device)
         i32 = dict(dtype=torch.int32, device=self.device)
@@ -177,6 +216,10 @@ class Engine:
         self.part_val = torch.empty((batch, self.tiles), dtype=torch.float32, device=self.device)
         self.part_idx = torch.empty((batch, self.tiles), **i32)
         self.tokens: torch.Tensor | None = None
+        # FP32 logits of one step's sequences (which captured graphs write into) and of a block of score()'s rows
+        self._step_logits = None if alternatives is None else self._logits_rows(batch)
+        self._block_logits: torch.Tensor | None = None
+        self._scores: ops.TokenScores | None = None
         self._graph: torch.cuda.CUDAGraph | None = None
         self._prefill_graph: torch.cuda.CUDAGraph | None = None
         # generate()'s pinned host staging for the prompts and the tokens, kept between calls
@@ -208,30 +251,48 @@ class Engine:
             self._normalising_decode_layer(lw, index, x, qkv, attn, h, seqs)
             return
         ops.layernorm(x, lw.ln1_g, lw.ln1_b, epsilon=LN_EPSILON, out=ln)
-        # the projection's epilogue also writes this step's keys and values into the layer's cache
-        k_cache, v_cache = self.k_cache[index][seqs], self.v_cache[index][seqs]
-        if decode:
-            positions = self.positions[seqs]
-            ops.gemm_qkv(ln, lw.w_qkv, lw.b_qkv, qkv, k_cache, v_cache, positions=positions)
-            ops.decode_attention(qkv, k_cache, v_cache, positions, length_offset=1, out=attn)
+        if self.kv_bits == 4:
+            ops.gemm(ln, lw.w_qkv, bias=lw.b_qkv, out=qkv)
+            if decode:
+                self._attend_q4(index, qkv, attn, seqs)
+            else:
+                ops.kv_store_q4(qkv, self.kv_cache[index], self.prompt_seq, self.prompt_pos)
+                ops.attention_prefill(qkv, self.batch, self.prompt, self.shape.heads, out=attn)
         else:
-            ops.gemm_qkv(ln, lw.w_qkv, lw.b_qkv, qkv, k_cache, v_cache, tokens_per_seq=self.prompt)
-            ops.attention_prefill(qkv, self.batch, self.prompt, self.shape.heads, out=attn)
+            # the projection's epilogue also writes this step's keys and values into the layer's cache
+            k_cache, v_cache = self.k_cache[index][seqs], self.v_cache[index][seqs]
+            if decode:
+                positions = self.positions[seqs]
+                ops.gemm_qkv(ln, lw.w_qkv, lw.b_qkv, qkv, k_cache, v_cache, positions=positions)
+                ops.decode_attention(qkv, k_cache, v_cache, positions, length_offset=1, out=attn)
+            else:
+                ops.gemm_qkv(ln, lw.w_qkv, lw.b_qkv, qkv, k_cache, v_cache, tokens_per_seq=self.prompt)
+                ops.attention_prefill(qkv, self.batch, self.prompt, self.shape.heads, out=attn)
         ops.gemm(attn, lw.w_proj, bias=lw.b_proj, residual=x, out=x)
         ops.layernorm(x, lw.ln2_g, lw.ln2_b, epsilon=LN_EPSILON, out=ln)
         ops.gemm(ln, lw.w_fc, bias=lw.b_fc, gelu=True, out=h)
         ops.gemm(h, lw.w_out, bias=lw.b_out, residual=x, out=x)
+
+    def _attend_q4(self, index: int, qkv, attn, seqs: slice) -> None:
+        """One decode step's new keys and values into the layer's 4-bit cache, then the attention over it."""
+        cache, positions = self.kv_cache[index][seqs], self.positions[seqs]
+        ops.kv_store_q4(qkv, cache, self.seq_index[:cache.shape[0]], positions)
+        ops.decode_attention_q4(qkv, cache, positions, length_offset=1, out=attn)
 
     def _fused_norms(self, x) -> bool:
         return self.fuse_small_norms and x.shape[0] <= 8
 
     def _normalising_decode_layer(self, lw: LayerWeights, index: int, x, qkv, attn, h, seqs: slice) -> None:
         """One decode block of at most 8 sequences, each LayerNorm computed inside the projection after it."""
-        k_cache, v_cache = self.k_cache[index][seqs], self.v_cache[index][seqs]
-        positions = self.positions[seqs]
-        ops.gemm_norm(x, lw.ln1_g, lw.ln1_b, lw.w_qkv, epsilon=LN_EPSILON, bias=lw.b_qkv, out=qkv, k_cache=k_cache,
-                      v_cache=v_cache, positions=positions)
-        ops.decode_attention(qkv, k_cache, v_cache, positions, length_offset=1, out=attn)
+        if self.kv_bits == 4:
+            ops.gemm_norm(x, lw.ln1_g, lw.ln1_b, lw.w_qkv, epsilon=LN_EPSILON, bias=lw.b_qkv, out=qkv)
+            self._attend_q4(index, qkv, attn, seqs)
+        else:
+            k_cache, v_cache = self.k_cache[index][seqs], self.v_cache[index][seqs]
+            positions = self.positions[seqs]
+            ops.gemm_norm(x, lw.ln1_g, lw.ln1_b, lw.w_qkv, epsilon=LN_EPSILON, bias=lw.b_qkv, out=qkv, k_cache=k_cache,
+                          v_cache=v_cache, positions=positions)
+            ops.decode_attention(qkv, k_cache, v_cache, positions, length_offset=1, out=attn)
         ops.gemm(attn, lw.w_proj, bias=lw.b_proj, residual=x, out=x)
         ops.gemm_norm(x, lw.ln2_g, lw.ln2_b, lw.w_fc, epsilon=LN_EPSILON, bias=lw.b_fc, gelu=True, out=h)
         ops.gemm(h, lw.w_out, bias=lw.b_out, residual=x, out=x)
@@ -239,13 +300,17 @@ class Engine:
     def _folded_decode_layer(self, lw: LayerWeights, index: int, x, qkv, attn, h, seqs: slice) -> None:
         """One decode block with both LayerNorms folded into the projections after them: each residual projection
         also writes the statistics partials of the rows it stores, and the next projection combines them."""
-        k_cache, v_cache = self.k_cache[index][seqs], self.v_cache[index][seqs]
-        positions = self.positions[seqs]
         stats1, stats2 = self.dstats1[seqs], self.dstats2[seqs]
         w, cs, bf = lw.qkv_folded
-        ops.gemm_ln_rowstats(x, w, cs, bf, stats1, epsilon=LN_EPSILON, out=qkv, k_cache=k_cache, v_cache=v_cache,
-                             positions=positions)
-        ops.decode_attention(qkv, k_cache, v_cache, positions, length_offset=1, out=attn)
+        if self.kv_bits == 4:
+            ops.gemm_ln_rowstats(x, w, cs, bf, stats1, epsilon=LN_EPSILON, out=qkv)
+            self._attend_q4(index, qkv, attn, seqs)
+        else:
+            k_cache, v_cache = self.k_cache[index][seqs], self.v_cache[index][seqs]
+            positions = self.positions[seqs]
+            ops.gemm_ln_rowstats(x, w, cs, bf, stats1, epsilon=LN_EPSILON, out=qkv, k_cache=k_cache, v_cache=v_cache,
+                                 positions=positions)
+            ops.decode_attention(qkv, k_cache, v_cache, positions, length_offset=1, out=attn)
         ops.gemm_rowstats(attn, lw.w_proj, stats2, bias=lw.b_proj, residual=x, out=x)
         w, cs, bf = lw.fc_folded
         ops.gemm_ln_rowstats(x, w, cs, bf, stats2, epsilon=LN_EPSILON, gelu=True, out=h)
@@ -279,21 +344,39 @@ class Engine:
             self._prefill_body()
         self._prefill_graph = graph
 
-    def _prefill_body(self) -> None:
+    def _prefill_layers(self) -> None:
         ops.embed(self.prompt_ids, self.prompt_pos, self.wte, self.wpe, out=self.x)
         for index, lw in enumerate(self.layers):
             self._layer(lw, index, self.x, self.ln, self.qkv, self.attn, self.h, decode=False)
+
+    def _prefill_body(self) -> None:
+        self._prefill_layers()
         # final LayerNorm on each sequence's last token only, then the LM head with its argmax fused
         last = self.x[self.prompt - 1:]
         ops.layernorm(last, self.lnf_g, self.lnf_b, epsilon=LN_EPSILON, out=self.dln, rows=self.batch,
                       row_stride=self.prompt * self.shape.width)
         self.positions.fill_(self.prompt)
         self._head(index_offset=-self.prompt, advance=0)
+        self._keep_scores()
 
     def _head(self, *, index_offset: int, advance: int, seqs: slice = slice(None)) -> None:
         ops.gemm_argmax(self.dln[seqs], self.wte, self.part_val[seqs], self.part_idx[seqs])
         ops.argmax_finish(self.part_val[seqs], self.part_idx[seqs], self.ids[seqs], tokens_out=self.tokens[seqs],
                           positions=self.positions[seqs], index_offset=index_offset, advance=advance)
+
+    def _logits_rows(self, rows: int) -> torch.Tensor:
+        """Room for `rows` rows of FP32 logits, their stride padded to eight columns."""
+        width = (self.shape.vocab + 7) // 8 * 8
+        return torch.empty((rows, width), dtype=torch.float32, device=self.device)[:, :self.shape.vocab]
+
+    def _keep_scores(self) -> None:
+        """The scores of the tokens just picked (self.ids, from the normalised rows in self.dln), into the slot of their
+        step: the token picked at position p is generated token p - prompt."""
+        if self.alternatives is None:
+            return
+        logits = ops.gemm_f32(self.dln, self.wte, out=self._step_logits)
+        ops.token_logprobs(logits, self.ids, top=self.alternatives, out=self._scores, slots=self.positions,
+                           slot_offset=-self.prompt)
 
     # ---- decode ----------------------------------------------------------------------------------------------
 
@@ -336,9 +419,13 @@ class Engine:
                           part_idx=self.part_idx[seqs])
             ops.argmax_finish(self.part_val[seqs], self.part_idx[seqs], self.ids[seqs], tokens_out=self.tokens[seqs],
                               positions=self.positions[seqs], index_offset=1 - self.prompt, advance=1)
+            if self.alternatives is not None:
+                ops.layernorm(dx, self.lnf_g, self.lnf_b, epsilon=LN_EPSILON, out=dln)
+                self._keep_scores()
             return
         ops.layernorm(dx, self.lnf_g, self.lnf_b, epsilon=LN_EPSILON, out=dln)
         self._head(index_offset=1 - self.prompt, advance=1, seqs=seqs)
+        self._keep_scores()
 
     def _decode_step(self) -> None:
         main = torch.cuda.current_stream(self.device)
@@ -398,6 +485,12 @@ class Engine:
             self.tokens = torch.zeros((self.batch, steps + 1), dtype=torch.int32, device=self.device)
             self._graph = None
             self._prefill_graph = None  # both graphs write into the token buffer
+            if self.alternatives is not None:
+                shape, k = (steps + 1, self.batch), self.alternatives
+                f32 = dict(dtype=torch.float32, device=self.device)
+                self._scores = ops.TokenScores(
+                    torch.zeros(shape, **f32), torch.zeros(shape, **f32), torch.zeros((*shape, k), **f32),
+                    torch.zeros((*shape, k), dtype=torch.int32, device=self.device))
         self._prefill_loaded(graph)
         self.decode(steps, graph=graph)
         return self.tokens
@@ -419,3 +512,43 @@ class Engine:
         self._pinned_tokens.copy_(tokens, non_blocking=True)
         torch.cuda.current_stream(self.device).synchronize()
         return self._pinned_tokens.numpy().copy()
+
+    def scores(self) -> Scores:
+        """The scores of the tokens the last run or generate call picked, [batch, steps + 1] on the host."""
+        if self._scores is None:
+            raise RuntimeError("no scores: the engine needs alternatives=0 or more, and a run before")
+        return self._scores_on_host(self._scores)
+
+    @staticmethod
+    def _scores_on_host(scores: ops.TokenScores) -> Scores:
+        return Scores(*(t.transpose(0, 1).cpu().numpy() for t in scores))
+
+    def score(self, token_ids: np.ndarray, *, alternatives: int = 0) -> Scores:
+        """Rates given tokens: token t + 1 of each sequence under what the model predicts after its first t + 1
+        ([batch, prompt] host ids in, [batch, prompt - 1] scores out, with the likeliest `alternatives` at each place).
+        An id outside the vocabulary (padding) scores 0. The prompts go through prefill, so the caches hold them
+        afterwards, and any generation under way is lost."""
+        ids = np.asarray(token_ids)
+        if ids.shape != (self.batch, self.prompt) or self.prompt < 2:
+            raise ValueError(f"expected prompts of shape {(self.batch, self.prompt)} and 2 tokens or more, got "
+                             f"{tuple(ids.shape)}")
+        if not 0 <= alternatives <= min(32, self.shape.vocab):
+            raise ValueError(f"alternatives must be in [0, {min(32, self.shape.vocab)}], got {alternatives}")
+        host = torch.from_numpy(np.ascontiguousarray(ids, dtype=np.int32))
+        self.prompt_ids.view(self.batch, self.prompt).copy_(host)
+        targets = torch.full((self.batch, self.prompt), -1, dtype=torch.int32, device=self.device)
+        targets[:, :-1] = self.prompt_ids.view(self.batch, self.prompt)[:, 1:]
+        targets = targets.view(-1)
+        self._prefill_layers()
+        ops.layernorm(self.x, self.lnf_g, self.lnf_b, epsilon=LN_EPSILON, out=self.ln)
+        rows, block, f32 = self.batch * self.prompt, SCORE_ROWS, dict(dtype=torch.float32, device=self.device)
+        out = ops.TokenScores(torch.empty(rows, **f32), torch.empty(rows, **f32), torch.empty((rows, alternatives), **f32),
+                              torch.empty((rows, alternatives), dtype=torch.int32, device=self.device))
+        if self._block_logits is None:
+            self._block_logits = self._logits_rows(min(rows, block))
+        for r in range(0, rows, block):
+            part = slice(r, min(rows, r + block))
+            logits = ops.gemm_f32(self.ln[part], self.wte, out=self._block_logits[:part.stop - r])
+            ops.token_logprobs(logits, targets[part], top=alternatives, out=ops.TokenScores(*(t[part] for t in out)))
+        shape = (self.batch, self.prompt)
+        return Scores(*(t.view(*shape, *t.shape[1:])[:, :-1].cpu().numpy() for t in out))

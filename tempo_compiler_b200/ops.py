@@ -464,11 +464,13 @@ class TokenScores(NamedTuple):
     top_ids: torch.Tensor | None = None
 
 
-def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, *, top: int = 0,
-                   out: TokenScores | None = None) -> TokenScores:
+def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, *, top: int = 0, out: TokenScores | None = None,
+                   slots: torch.Tensor | None = None, slot_offset: int = 0) -> TokenScores:
     """Log probabilities of ids[r] under softmax(logits[r]) (FP32 or BF16 rows at any stride), the rows' entropies in
     nats and their `top` (at most 32) likeliest tokens, ties to the lower id. A row whose id is outside the vocabulary
-    (a padded row) scores 0; include/tempo_b200.h says what infinities and NaN give."""
+    (a padded row) scores 0; include/tempo_b200.h says what infinities and NaN give. With `slots` (int32, one a row)
+    the tensors of `out` have a leading dimension, and row r's results go to its index slots[r] + slot_offset, or
+    nowhere when that is outside: one captured call serves every step."""
     bf16 = logits.dtype == torch.bfloat16
     _check_rows(logits, torch.bfloat16 if bf16 else torch.float32, "logits")
     _check(ids, torch.int32, "ids")
@@ -477,7 +479,10 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, *, top: int = 0,
         raise ValueError(f"{rows} rows need as many ids, got {ids.numel()}")
     if not 0 <= top <= min(32, vocab):
         raise ValueError(f"top must be in [0, {min(32, vocab)}], got {top}")
+    blocks = 0
     if out is None:
+        if slots is not None:
+            raise ValueError("slots need the outputs they index")
         # one allocation, split
         if top:
             words = logits.new_empty(2 * rows * (1 + top), dtype=torch.float32)
@@ -488,10 +493,17 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, *, top: int = 0,
             top_logprob = top_ids = None
         out = TokenScores(logprob, entropy, top_logprob, top_ids)
     else:
-        for name, t, shape, dtype in (("logprob", out.logprob, (rows,), torch.float32),
-                                      ("entropy", out.entropy, (rows,), torch.float32),
-                                      ("top_logprob", out.top_logprob, (rows, top), torch.float32),
-                                      ("top_ids", out.top_ids, (rows, top), torch.int32)):
+        lead = ()
+        if slots is not None:
+            _check(slots, torch.int32, "slots")
+            if slots.numel() != rows:
+                raise ValueError(f"{rows} rows need as many slots, got {slots.numel()}")
+            blocks = out.logprob.shape[0]
+            lead = (blocks,)
+        for name, t, shape, dtype in (("logprob", out.logprob, (*lead, rows), torch.float32),
+                                      ("entropy", out.entropy, (*lead, rows), torch.float32),
+                                      ("top_logprob", out.top_logprob, (*lead, rows, top), torch.float32),
+                                      ("top_ids", out.top_ids, (*lead, rows, top), torch.int32)):
             if name.startswith("top") and not top:
                 continue
             if t is None:
@@ -500,10 +512,11 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, *, top: int = 0,
             if t.shape != shape:
                 raise ValueError(f"out.{name} must be {shape}, got {tuple(t.shape)}")
         _check_devices(logits, logprob=out.logprob, entropy=out.entropy, top_logprob=out.top_logprob,
-                       top_ids=out.top_ids)
+                       top_ids=out.top_ids, slots=slots)
     _check_devices(logits, ids=ids)
     _launch_at(logits, "tempo_token_logprobs", logits.data_ptr(), _row_stride(logits), int(bf16), ids.data_ptr(), rows,
-               vocab, top, out.logprob.data_ptr(), out.entropy.data_ptr(), _ptr(out.top_logprob), _ptr(out.top_ids))
+               vocab, top, out.logprob.data_ptr(), out.entropy.data_ptr(), _ptr(out.top_logprob), _ptr(out.top_ids),
+               _ptr(slots), slot_offset, blocks)
     return out
 
 

@@ -215,6 +215,26 @@ def test_outputs_of_the_caller_and_a_replayed_graph() -> None:
         assert b[0] == 9.0 and b[-1] == 9.0
 
 
+def test_slots_take_the_results() -> None:
+    """Each row's results in the block its slot names, and nothing elsewhere, over one row to many."""
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(10)
+    for rows in (1, 5, 200):
+        vocab, top, blocks = 9001, 3, 4
+        logits = _logits(rng, rows, vocab, torch.float32)
+        ids = _i32(rng.integers(0, vocab, rows))
+        want = ops.token_logprobs(logits, ids, top=top)
+        out = ops.TokenScores(torch.full((blocks, rows), 7.0, device="cuda"), torch.full((blocks, rows), 7.0, device="cuda"),
+                              torch.full((blocks, rows, top), 7.0, device="cuda"),
+                              torch.full((blocks, rows, top), 7, dtype=torch.int32, device="cuda"))
+        slots = rng.integers(8, 14, rows)  # less 10: blocks -2 .. 3
+        ops.token_logprobs(logits, ids, top=top, out=out, slots=_i32(slots), slot_offset=-10)
+        for r, slot in enumerate(slots - 10):
+            for got, value in zip(out, want):
+                for b in range(blocks):
+                    assert torch.equal(got[b, r], value[r]) if b == slot else (got[b, r] == 7).all()
+
+
 def test_offsets_past_32_bits() -> None:
     """Rows 2^31 elements into a matrix, and a row stride that makes byte offsets pass 2^32."""
     from tempo_compiler_b200 import ops

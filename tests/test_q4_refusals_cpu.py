@@ -77,7 +77,7 @@ def test_scores_refuse(change: dict) -> None:
     a = {**dict(ld=100, bf16=0, rows=2, vocab=100, top=5), **change}
     p = _buffer()
     assert _status("tempo_token_logprobs", p, a["ld"], a["bf16"], p, a["rows"], a["vocab"], a["top"], p, p, p, p,
-                   None) == lib.ERR_VALUE
+                   None, 0, 0, None) == lib.ERR_VALUE
 
 
 @pytest.mark.parametrize("which,bad", [(0, None), (0, 2), (1, None), (2, None), (3, None), (4, None), (5, None)])
@@ -85,7 +85,14 @@ def test_scores_refuse_pointers(which: int, bad) -> None:
     from tempo_compiler_b200 import lib
     p = [_buffer()] * 6
     p[which] = None if bad is None else p[which] + bad
-    assert _status("tempo_token_logprobs", p[0], 100, 0, p[1], 2, 100, 5, p[2], p[3], p[4], p[5], None) == lib.ERR_VALUE
+    assert _status("tempo_token_logprobs", p[0], 100, 0, p[1], 2, 100, 5, p[2], p[3], p[4], p[5], None, 0, 0,
+                   None) == lib.ERR_VALUE
+
+
+def test_scores_refuse_slots_without_any() -> None:
+    from tempo_compiler_b200 import lib
+    p = _buffer()
+    assert _status("tempo_token_logprobs", p, 100, 0, p, 2, 100, 0, p, p, None, None, p, 0, 0, None) == lib.ERR_VALUE
 
 
 def test_fp32_product_refuses_other_modes() -> None:
