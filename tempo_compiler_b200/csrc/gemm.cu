@@ -45,8 +45,7 @@ constexpr int kBK = 64;        // 64 BF16 = 128 bytes: one 128B-swizzle atom row
 struct RowMajorParams {
   const uint16_t* bias;
   const uint16_t* residual;
-  uint16_t* out;
-  float* out_f32;  // TEMPO_GEMM_F32: the output (`out` is then unused)
+  uint16_t* out;  // (FP32 in TEMPO_GEMM_F32 mode)
   float* part_val;
   int32_t* part_idx;
   uint32_t m, n, k;
@@ -71,14 +70,15 @@ struct RowMajorParams {
   KvStore kv;  // QKV projection: key and value columns also stored into the caches
 };
 
-template <int BN, int STAGES, bool STAGED = false>
+template <int BN, int STAGES, bool STAGED = false, bool F32 = false>
 struct RowMajorSmem {
   static constexpr uint32_t kABytes = 128 * kBK * 2;
   static constexpr uint32_t kBBytes = BN * kBK * 2;
   static constexpr uint32_t kStageBytes = kABytes + kBBytes;
-  // STAGED: one 32 x 32 BF16 staging tile (2 KB) per epilogue warp for TMA stores of the output.
+  // STAGED: one 32 x 32 staging tile (2 KB of BF16, 4 KB of FP32) per epilogue warp for TMA stores of the output.
   static constexpr uint32_t kStagingOffset = STAGES * kStageBytes;
-  static constexpr uint32_t kStagingBytes = STAGED ? 16u * 2048u : 0u;
+  static constexpr uint32_t kStagingTile = F32 ? 4096u : 2048u;
+  static constexpr uint32_t kStagingBytes = STAGED ? 16u * kStagingTile : 0u;
   static constexpr uint32_t kBarrierOffset = kStagingOffset + kStagingBytes;
   // full[S], empty[S], acc_full[2], acc_empty[2], final, epilogue-wide (row statistics)
   static constexpr uint32_t kBarriers = 2 * STAGES + 6;
@@ -104,6 +104,26 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
                ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(src)), "r"(c0), "r"(c1)
                : "memory");
+}
+
+// One thread's 32 accumulators of its row into the warp's FP32 staging tile, as they are: row `lane` at 128 bytes, its
+// 16-byte words swizzled by the row (the TMA 128-byte swizzle, which spreads the warp's writes over all banks).
+__device__ __forceinline__ void stage_f32(const uint32_t (&r)[32], uint8_t* staging, uint32_t lane) {
+  uint4* row = reinterpret_cast<uint4*>(staging + lane * 128);
+#pragma unroll
+  for (uint32_t q = 0; q < 8; ++q)
+    row[q ^ (lane & 7u)] = make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
+}
+
+// The FP32 columns n0 .. n - 1 of one row, fewer than a staging tile's 32, by plain stores: a TMA store clips at 16-byte
+// steps and would overwrite up to three columns behind the row, which may be the caller's.
+__device__ __forceinline__ void store_f32_tail(const RowMajorParams& p, const uint32_t (&r)[32], uint32_t row,
+                                               uint32_t n0) {
+  if (row >= p.m) return;
+  float* out = reinterpret_cast<float*>(p.out) + size_t(row) * p.ldo + n0;
+#pragma unroll
+  for (uint32_t j = 0; j < 32; ++j)
+    if (n0 + j < p.n) out[j] = __uint_as_float(r[j]);
 }
 
 // One thread's kCW accumulator columns n0 .. n0 + kCW - 1 of output row `row`: the folded LayerNorm (mean / rstd of the
@@ -346,7 +366,8 @@ template <int BN, int STAGES, bool STAGED, bool LN, bool F32>
 __global__ void __launch_bounds__(kRowThreads, 1)
     gemm_rowmajor_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                          const __grid_constant__ CUtensorMap tmap_out, RowMajorParams p) {
-  using L = RowMajorSmem<BN, STAGES, STAGED>;
+  using L = RowMajorSmem<BN, STAGES, STAGED, F32>;
+  static_assert(STAGED || !F32, "FP32 outputs are staged");
   static_assert(!STAGED || BN >= 128, "staged stores need 32-column chunks");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -542,11 +563,21 @@ __global__ void __launch_bounds__(kRowThreads, 1)
           // clipped by the copy). Never in argmax mode.
           const uint32_t row0 = m_blk * 128 + lane_base;
           if (row0 >= p.m || n0 >= p.n) continue;  // warp-uniform
-          uint8_t* staging = smem + L::kStagingOffset + (warp - 2) * 2048;
+          uint8_t* staging = smem + L::kStagingOffset + (warp - 2) * L::kStagingTile;
+          if constexpr (F32) {
+            if (n0 + kCW > p.n) {  // warp-uniform
+              store_f32_tail(p, r, row, n0);
+              continue;
+            }
+          }
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
           __syncwarp();
-          const float mu = ln ? ln_mean[row_in_tile] : 0.f, rs = ln ? ln_rstd[row_in_tile] : 0.f;
-          epilogue_chunk<kCW, true>(p, r, row, n0, gelu, ln, mu, rs, staging + lane * 64, (lane >> 1) & 3u);
+          if constexpr (F32) {
+            stage_f32(r, staging, lane);
+          } else {
+            const float mu = ln ? ln_mean[row_in_tile] : 0.f, rs = ln ? ln_rstd[row_in_tile] : 0.f;
+            epilogue_chunk<kCW, true>(p, r, row, n0, gelu, ln, mu, rs, staging + lane * 64, (lane >> 1) & 3u);
+          }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) {
@@ -556,19 +587,6 @@ __global__ void __launch_bounds__(kRowThreads, 1)
           continue;
         }
         if (!row_ok || n0 >= p.n) continue;
-        if constexpr (F32) {
-          float* orow = p.out_f32 + size_t(row) * p.ldo + n0;
-          if (n0 + kCW <= p.n) {
-#pragma unroll
-            for (uint32_t q = 0; q < kCW / 4; ++q)
-              reinterpret_cast<uint4*>(orow)[q] = make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
-          } else {
-#pragma unroll
-            for (uint32_t j = 0; j < kCW; ++j)
-              if (n0 + j < p.n) orow[j] = __uint_as_float(r[j]);
-          }
-          continue;
-        }
         if (argmax) {
 #pragma unroll
           for (uint32_t j = 0; j < kCW; ++j) {
@@ -790,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <int BN, int STAGES, bool STAGED = false, bool LN = false, bool F32 = false>
 tempo_status launch_rowmajor(const void* a, uint32_t lda, const void* w_t, uint32_t ldw, const RowMajorParams& base,
                              cudaStream_t stream) {
-  using L = RowMajorSmem<BN, STAGES, STAGED>;
+  using L = RowMajorSmem<BN, STAGES, STAGED, F32>;
   CUtensorMap ta, tb;
   const uint64_t a_dims[2] = {base.k, base.m};
   const uint64_t a_strides[1] = {uint64_t(lda) * 2};
@@ -808,10 +826,10 @@ tempo_status launch_rowmajor(const void* a, uint32_t lda, const void* w_t, uint3
   CUtensorMap to = ta;  // unused unless STAGED
   if (STAGED) {
     const uint64_t o_dims[2] = {base.n, base.m};
-    const uint64_t o_strides[1] = {uint64_t(base.ldo) * 2};
+    const uint64_t o_strides[1] = {uint64_t(base.ldo) * (F32 ? 4 : 2)};
     const uint32_t o_box[2] = {32, 32};
-    s = encode_tmap(&to, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base.out, o_dims, o_strides, o_box,
-                    CU_TENSOR_MAP_SWIZZLE_64B);
+    s = encode_tmap(&to, F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base.out, o_dims,
+                    o_strides, o_box, F32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
     if (s != TEMPO_OK) return s;
   }
   RowMajorParams p = base;
@@ -1244,14 +1262,15 @@ tempo_status launch_splitk(const void* a, uint32_t lda, const void* w_t, uint32_
 
 constexpr uint32_t kPairBN = 256;
 
-template <int STAGES>
+template <int STAGES, bool F32 = false>
 struct PairSmem {
   static constexpr uint32_t kABytes = 128 * kBK * 2;
   static constexpr uint32_t kBBytes = 128 * kBK * 2;
   static constexpr uint32_t kStageBytes = kABytes + kBBytes;
-  // One 32 x 32 BF16 staging tile (2 KB) per epilogue warp for the output's TMA stores.
+  // One 32 x 32 staging tile (2 KB of BF16, 4 KB of FP32) per epilogue warp for the output's TMA stores.
   static constexpr uint32_t kStagingOffset = STAGES * kStageBytes;
-  static constexpr uint32_t kStagingBytes = (kRowEpiThreads / 32) * 2048;
+  static constexpr uint32_t kStagingTile = F32 ? 4096u : 2048u;
+  static constexpr uint32_t kStagingBytes = (kRowEpiThreads / 32) * kStagingTile;
   static constexpr uint32_t kBarrierOffset = kStagingOffset + kStagingBytes;
   // full[S] (the leader's), empty[S], acc_full[2], acc_empty[2] (the leader's), final
   static constexpr uint32_t kBarriers = 2 * STAGES + 5;
@@ -1302,11 +1321,13 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
 }
 
-template <int STAGES>
+// F32: TEMPO_GEMM_F32, the accumulators stored as they are. Its tiles go down the rows first: the LM head's weights are
+// then read once, by the pairs that share them, and not once per 256 rows behind 50257 columns of output.
+template <int STAGES, bool F32>
 __global__ void __launch_bounds__(kRowThreads, 1)
     gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                      const __grid_constant__ CUtensorMap tmap_out, RowMajorParams p) {
-  using L = PairSmem<STAGES>;
+  using L = PairSmem<STAGES, F32>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarrierOffset);
@@ -1326,6 +1347,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   const uint32_t pairs = gridDim.x / 2, pair = blockIdx.x / 2;
   const uint32_t tiles = p.m_tiles * p.n_tiles;  // 256 x 256 tiles
   const uint32_t kblocks = (p.k + kBK - 1) / kBK;
+  auto m_tile = [&](uint32_t t) { return F32 ? t % p.m_tiles : t / p.n_tiles; };
+  auto n_tile = [&](uint32_t t) { return F32 ? t / p.m_tiles : t % p.n_tiles; };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -1365,8 +1388,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       bool ok = true;
       pdl_wait();
       for (uint32_t t = pair; t < tiles && ok; t += pairs) {
-        const int32_t m0 = int32_t((t / p.n_tiles) * 256 + rank * 128);
-        const int32_t n0 = int32_t((t % p.n_tiles) * kPairBN + rank * 128);
+        const int32_t m0 = int32_t(m_tile(t) * 256 + rank * 128);
+        const int32_t n0 = int32_t(n_tile(t) * kPairBN + rank * 128);
         for (uint32_t kb = 0; kb < kblocks; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1u, kWatchEmpty, abort_flag)) { ok = false; break; }
           uint8_t* a_dst = smem + stage * L::kStageBytes;
@@ -1430,7 +1453,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     const bool gelu = (p.flags & TEMPO_GEMM_GELU) != 0;
     // This warp's 32 x 32 staging tile: row `lane` at 64 bytes, its four 16-byte words swizzled by (lane / 2) % 4
     // (the TMA 64-byte swizzle, which also spreads the warp's writes over all banks).
-    uint8_t* staging = smem + L::kStagingOffset + (warp - 2) * 2048;
+    uint8_t* staging = smem + L::kStagingOffset + (warp - 2) * L::kStagingTile;
     uint8_t* stage_row = staging + lane * 64;
     const uint32_t swizzle = (lane >> 1) & 3u;
     uint32_t acc = 0, acc_phase = 0;
@@ -1438,9 +1461,9 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     for (uint32_t t = pair; t < tiles; t += pairs) {
       if (!mbar_wait(&acc_full[acc], acc_phase, kWatchAccFull, abort_flag)) break;
       tc_fence_after();
-      const uint32_t row0 = (t / p.n_tiles) * 256 + rank * 128 + lane_base;  // this warp's first row
+      const uint32_t row0 = m_tile(t) * 256 + rank * 128 + lane_base;  // this warp's first row
       const uint32_t row = row0 + lane;
-      const uint32_t n_base = (t % p.n_tiles) * kPairBN;
+      const uint32_t n_base = n_tile(t) * kPairBN;
 #pragma unroll 1
       for (uint32_t c = group * kGroupCols; c < (group + 1) * kGroupCols; c += kCW) {
         uint32_t r[kCW];
@@ -1448,10 +1471,17 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         tmem_wait_ld();
         const uint32_t n0 = n_base + c;
         if (row0 >= p.m || n0 >= p.n) continue;  // warp-uniform: the whole 32 x 32 block lies outside
+        if constexpr (F32) {
+          if (n0 + kCW > p.n) {
+            store_f32_tail(p, r, row, n0);
+            continue;
+          }
+        }
         // The staging tile is free once the previous store from it has been read.
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         __syncwarp();
-        epilogue_chunk<kCW, true>(p, r, row, n0, gelu, false, 0.f, 0.f, stage_row, swizzle);
+        if constexpr (F32) stage_f32(r, staging, lane);
+        else epilogue_chunk<kCW, true>(p, r, row, n0, gelu, false, 0.f, 0.f, stage_row, swizzle);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         // Rows past M and columns past N are clipped by the copy.
@@ -1479,10 +1509,10 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   }
 }
 
-template <int STAGES>
+template <int STAGES, bool F32 = false>
 tempo_status launch_pair(const void* a, uint32_t lda, const void* w_t, uint32_t ldw, const RowMajorParams& base,
                          cudaStream_t stream) {
-  using L = PairSmem<STAGES>;
+  using L = PairSmem<STAGES, F32>;
   CUtensorMap ta, tb;
   const uint64_t a_dims[2] = {base.k, base.m};
   const uint64_t a_strides[1] = {uint64_t(lda) * 2};
@@ -1497,16 +1527,16 @@ tempo_status launch_pair(const void* a, uint32_t lda, const void* w_t, uint32_t 
   if (s != TEMPO_OK) return s;
   CUtensorMap to;
   const uint64_t o_dims[2] = {base.n, base.m};
-  const uint64_t o_strides[1] = {uint64_t(base.ldo) * 2};
+  const uint64_t o_strides[1] = {uint64_t(base.ldo) * (F32 ? 4 : 2)};
   const uint32_t o_box[2] = {32, 32};
-  s = encode_tmap(&to, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base.out, o_dims, o_strides, o_box,
-                  CU_TENSOR_MAP_SWIZZLE_64B);
+  s = encode_tmap(&to, F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base.out, o_dims,
+                  o_strides, o_box, F32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
   if (s != TEMPO_OK) return s;
   RowMajorParams p = base;
   p.m_tiles = (p.m + 255) / 256;
   p.n_tiles = (p.n + kPairBN - 1) / kPairBN;
   const uint32_t tiles = p.m_tiles * p.n_tiles;
-  auto kernel = gemm_pair_kernel<STAGES>;
+  auto kernel = gemm_pair_kernel<STAGES, F32>;
   s = set_smem(reinterpret_cast<const void*>(kernel), L::kBytes);
   if (s != TEMPO_OK) return s;
   // The tiles are dealt out statically, so every pair must be resident at once: as many pairs as the GPCs can hold.
@@ -1798,7 +1828,6 @@ static tempo_status gemm_impl(const void* a, uint32_t lda, const void* w_t, uint
   p.bias = static_cast<const uint16_t*>(bias);
   p.residual = static_cast<const uint16_t*>(residual);
   p.out = static_cast<uint16_t*>(out);
-  p.out_f32 = static_cast<float*>(out);
   p.part_val = part_val;
   p.part_idx = part_idx;
   p.m = m;
@@ -1820,13 +1849,20 @@ static tempo_status gemm_impl(const void* a, uint32_t lda, const void* w_t, uint
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // A handful of rows (decode of a few sequences): stream the weights on the CUDA cores instead (no statistics).
-  if (m <= 8 && !ln_mode && row_stats == nullptr) {
+  if (m <= 8 && !ln_mode && !f32 && row_stats == nullptr) {
     const tempo_status gemv = gemv_dispatch(a, lda, w_t, ldw, bias, residual, ldr, out, ldo, m, n, k, flags, part_val,
                                             part_idx, kv, st);
     if (gemv != TEMPO_ERR_VALUE) return gemv;
   }
   if (argmax) return launch_rowmajor<256, 4>(a, lda, w_t, ldw, p, st);
-  if (f32) return launch_rowmajor<256, 4, false, false, true>(a, lda, w_t, ldw, p, st);
+  if (f32) {
+    // An LM head has far more columns than tiles need: 256 x 256 tiles on CTA pairs from four to a pair, as for any
+    // product (512 rows of 50257 x 768: 50 us against 80 with direct stores), else 128-column tiles, whose 393 over 148 SMs leave less idle
+    // than 197 of 256 columns (64 rows: 16.8 us against 19.3).
+    if (uint64_t((m + 255) / 256) * ((n + 255) / 256) >= 4ull * (uint64_t(sm_count()) / 2))
+      return launch_pair<4, true>(a, lda, w_t, ldw, p, st);
+    return launch_rowmajor<128, 4, true, false, true>(a, lda, w_t, ldw, p, st);
+  }
   // With the statistics from their producer, the folded LayerNorm runs wherever the plain projection would: narrow
   // full-K tiles for one 128-row block, else split-K.
   const bool ln_partials = ln_mode && ln.stats != nullptr;

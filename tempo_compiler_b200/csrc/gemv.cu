@@ -99,10 +99,6 @@ __global__ void __launch_bounds__(kWarps * 32) gemv_kernel(GemvParams p) {
         if (lane != uint32_t(c * M + r) || r >= int(p.m) || n0 + c >= p.n) continue;
         const uint32_t col = n0 + c;
         float v = acc[c][r];
-        if (p.flags & TEMPO_GEMM_F32) {
-          reinterpret_cast<float*>(p.out)[size_t(r) * p.ldo + col] = v;
-          continue;
-        }
         if (p.bias != nullptr) v += bf16_to_float(p.bias[col]);
         if (gelu) v = gelu_erf(round_bf16(v));
         if (p.residual != nullptr) v += bf16_to_float(p.residual[size_t(r) * p.ldr + col]);
