@@ -296,10 +296,15 @@ tempo_status tempo_kv_load_q4(const void* cache, void* kv, uint32_t ldo, const i
 /* tempo_decode_attention over the 4-bit cache: one query row per sequence (row stride ldq elements, ldq % 8 == 0; its
  * first heads * head columns, already scaled by 1/sqrt(head)) over the first lengths[s] + length_offset positions
  * (clamped to [0, capacity]); query head h reads key / value head h / (heads / kv_heads). A sequence of no positions is
- * written as zeros. out: [seqs, heads * head] BF16. */
+ * written as zeros. out: [seqs, heads * head] BF16. Few sequences of a long capacity are split over more CTAs than a
+ * cluster holds; their partial results then go through `workspace` (tempo_decode_attention_q4_workspace bytes, 16-byte
+ * aligned, of any content; NULL when that is 0), which no other call may use until this one has finished. */
+tempo_status tempo_decode_attention_q4_workspace(uint32_t seqs, uint32_t heads, uint32_t kv_heads, uint32_t head,
+                                                 uint32_t capacity, uint64_t* bytes);
 tempo_status tempo_decode_attention_q4(const void* q, uint32_t ldq, const void* cache, const int32_t* lengths,
                                        int32_t length_offset, void* out, uint32_t seqs, uint32_t heads,
-                                       uint32_t kv_heads, uint32_t head, uint32_t capacity, void* stream);
+                                       uint32_t kv_heads, uint32_t head, uint32_t capacity, void* workspace,
+                                       uint64_t workspace_bytes, void* stream);
 
 /* Scores of `rows` rows of `vocab` logits (FP32, or BF16 with bf16 = 1; row stride ld elements, any alignment of the
  * element): logprob[r] = log softmax(logits[r])[ids[r]] (0 where ids[r] is outside [0, vocab): a row without a token),

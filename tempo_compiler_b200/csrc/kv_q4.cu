@@ -1,6 +1,8 @@
 // The 4-bit key/value cache: storing rows of a QKV projection into it, reading rows back, and decode attention over it.
 // Each row of 64 dimensions keeps its least value (exact in BF16) and a BF16 scale, so a position costs 72 bytes per
 // head and 64 dimensions for key and value together, against 256 in BF16.
+#include <algorithm>
+
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -229,10 +231,11 @@ tempo_status launch_rows(void (*kernel)(Q4Rows), Q4Rows p, uint32_t rows, uint32
 // A CTA of four warps takes a run of tiles of one (sequence, key / value head, eight query heads); each warp streams its
 // own pieces (one bulk copy each, kRing in flight) and keeps an online softmax whose reference moves only when a score
 // passes it by 2^kSlack. Warps merge through shared memory; with `chunks` > 1 the CTAs of a cluster split the positions
-// and merge through distributed shared memory.
+// and merge through distributed shared memory, or, when a pair needs more of them, through a workspace and a second kernel.
 // ---------------------------------------------------------------------------------------------------------------
 
-constexpr uint32_t kQ4MaxChunks = 16;
+constexpr uint32_t kQ4MaxChunks = 16;    // CTAs of a cluster
+constexpr uint32_t kQ4MaxSplits = 160;   // CTAs that share a pair through the workspace
 constexpr uint32_t kQ4Queries = 8;
 constexpr uint32_t kQ4Piece = 4 * kQ4Block;  // bytes of one bulk copy: four tiles of a 64-wide head, two of a 128-wide
 constexpr uint32_t kRing = 2;
@@ -242,11 +245,15 @@ constexpr float kNoScore = -1e30f;  // the reference before any position: e^(any
 template <int G, int WARPS>
 struct Q4Smem {
   static constexpr uint32_t kWarpRing = kRing * kQ4Piece;
-  static constexpr uint32_t kPart = kQ4Queries * (64 * G + 2) * 4;  // (values, max, sum) of eight queries
+  // A partial result of eight queries: 64 G values each (dimension 64 i + 8 g + n at 64 i + 8 n + g, eight words more to
+  // the next query: the lanes of a fragment store into different banks), then the references, then the sums.
+  static constexpr uint32_t kStride = 64 * G + 8;
+  static constexpr uint32_t kReferences = kQ4Queries * kStride, kSums = kReferences + kQ4Queries;
+  static constexpr uint32_t kPart = (kSums + kQ4Queries) * 4;
   static constexpr uint32_t kBarrierOffset = WARPS * kWarpRing;
   static constexpr uint32_t kMergeOffset = kBarrierOffset + WARPS * kRing * 8;
   static constexpr uint32_t kBytes = kMergeOffset + kPart;
-  static_assert(kPart <= kWarpRing, "a warp's partial result fits its ring");
+  static_assert(kPart <= kWarpRing && kPart % 16 == 0, "a warp's partial result fits its ring");
 };
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -482,6 +489,9 @@ __device__ __forceinline__ float ld_cluster(const float* local, uint32_t rank) {
   return v;
 }
 
+// The dimension of word `at` of a query's values in a partial result.
+__device__ __forceinline__ uint32_t q4_dimension(uint32_t at) { return (at & ~63u) | (at & 7u) << 3 | (at >> 3 & 7u); }
+
 struct Q4Attention {
   const uint16_t* q;
   const uint8_t* cache;
@@ -489,7 +499,8 @@ struct Q4Attention {
   uint16_t* out;
   uint32_t ldq, heads, kv_heads, tiles;
   int32_t length_offset;
-  uint32_t blocks;  // groups of eight query heads per key / value head
+  uint32_t blocks;  // groups of query heads per key / value head
+  float* parts;     // split over more CTAs than a cluster holds: each leaves its partial result here
   uint32_t early;   // the grid is resident at once: the next kernel may start at entry
 };
 
@@ -645,58 +656,132 @@ __global__ void __launch_bounds__(32 * WARPS) decode_attention_q4_kernel(Q4Atten
           hi += __shfl_xor_sync(0xFFFFFFFFu, hi, o);
         }
         if (writes) {
-          part[query * kWidth + i * 64 + 8 * g + n] = lo + rest;
-          part[query * kWidth + i * 64 + 8 * g + 4 + n] = hi + rest;
+          part[query * L::kStride + i * 64 + 8 * n + g] = lo + rest;
+          part[query * L::kStride + i * 64 + 8 * (4 + n) + g] = hi + rest;
         }
       }
     }
     if (g == 0 && writes) {
-      part[kQ4Queries * kWidth + query] = m;
-      part[kQ4Queries * kWidth + kQ4Queries + query] = l;
+      part[L::kReferences + query] = m;
+      part[L::kSums + query] = l;
     }
   }
   __syncthreads();
-  float* merge = reinterpret_cast<float*>(smem + L::kMergeOffset);
+  // The warps' results together: output, or the CTA's own partial result, in its shared memory or in the workspace.
+  const bool whole = chunks == 1 && p.parts == nullptr;
+  float* merge = p.parts != nullptr
+                     ? p.parts + (size_t(s * gridDim.y + blockIdx.y) * chunks + chunk) * (L::kPart / 4)
+                     : reinterpret_cast<float*>(smem + L::kMergeOffset);
   uint16_t* out = p.out + (size_t(s) * p.heads + kvh * share + first) * kWidth;
   for (uint32_t i = threadIdx.x; i < queries * kWidth; i += 32 * WARPS) {
-    const uint32_t query = i / kWidth;
-    float m = -INFINITY, l = 0.f, a = 0.f;
+    const uint32_t query = i / kWidth, at = query * L::kStride + i % kWidth;
+    float m = kNoScore, l = 0.f, a = 0.f;
 #pragma unroll
     for (uint32_t w = 0; w < WARPS; ++w)
-      m = fmaxf(m, reinterpret_cast<const float*>(smem + w * L::kWarpRing)[kQ4Queries * kWidth + query]);
+      m = fmaxf(m, reinterpret_cast<const float*>(smem + w * L::kWarpRing)[L::kReferences + query]);
 #pragma unroll
     for (uint32_t w = 0; w < WARPS; ++w) {
       const float* other = reinterpret_cast<const float*>(smem + w * L::kWarpRing);
-      const float f = fast_exp2(other[kQ4Queries * kWidth + query] - m);
-      l = fmaf(other[kQ4Queries * kWidth + kQ4Queries + query], f, l);
-      a = fmaf(other[i], f, a);
+      const float f = fast_exp2(other[L::kReferences + query] - m);
+      l = fmaf(other[L::kSums + query], f, l);
+      a = fmaf(other[at], f, a);
     }
-    if (chunks == 1) {
-      out[i] = float_to_bf16(len == 0 ? 0.f : a / l);
+    if (whole) {
+      out[query * kWidth + q4_dimension(i % kWidth)] = float_to_bf16(len == 0 ? 0.f : a / l);
     } else {
-      merge[i] = a;
+      merge[at] = a;
       if (i % kWidth == 0) {
-        merge[kQ4Queries * kWidth + query] = m;
-        merge[kQ4Queries * kWidth + kQ4Queries + query] = l;
+        merge[L::kReferences + query] = m;
+        merge[L::kSums + query] = l;
       }
     }
   }
-  if (chunks == 1) return;
+  if (whole || p.parts != nullptr) return;
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   // Each CTA finishes its share of the outputs, reading every CTA's partial result.
   for (uint32_t i = chunk * 32 * WARPS + threadIdx.x; i < queries * kWidth; i += chunks * 32 * WARPS) {
-    const uint32_t query = i / kWidth;
-    float m = -INFINITY, l = 0.f, a = 0.f;
-    for (uint32_t c = 0; c < chunks; ++c) m = fmaxf(m, ld_cluster(merge + kQ4Queries * kWidth + query, c));
+    const uint32_t query = i / kWidth, at = query * L::kStride + i % kWidth;
+    float m = kNoScore, l = 0.f, a = 0.f;
+    for (uint32_t c = 0; c < chunks; ++c) m = fmaxf(m, ld_cluster(merge + L::kReferences + query, c));
     for (uint32_t c = 0; c < chunks; ++c) {
-      const float f = fast_exp2(ld_cluster(merge + kQ4Queries * kWidth + query, c) - m);
-      l = fmaf(ld_cluster(merge + kQ4Queries * kWidth + kQ4Queries + query, c), f, l);
-      a = fmaf(ld_cluster(merge + i, c), f, a);
+      const float f = fast_exp2(ld_cluster(merge + L::kReferences + query, c) - m);
+      l = fmaf(ld_cluster(merge + L::kSums + query, c), f, l);
+      a = fmaf(ld_cluster(merge + at, c), f, a);
     }
-    out[i] = float_to_bf16(len == 0 ? 0.f : a / l);
+    out[query * kWidth + q4_dimension(i % kWidth)] = float_to_bf16(len == 0 ? 0.f : a / l);
   }
   // No CTA leaves while another may still read its shared memory.
   asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// One CTA per (sequence, query head): the partial results of `chunks` CTAs, summed in a fixed order. kMergeThreads / 64 G
+// threads share a dimension, so a long row of partials is a few loads deep.
+constexpr uint32_t kMergeThreads = 512;
+static_assert(kQ4MaxSplits <= kMergeThreads, "a thread for each partial result");
+
+template <int G>
+__global__ void __launch_bounds__(kMergeThreads) decode_merge_q4_kernel(Q4Attention p, uint32_t chunks, uint32_t rp) {
+  using L = Q4Smem<G, 4>;
+  constexpr uint32_t kWidth = 64 * G, kShares = kMergeThreads / kWidth, kPart = L::kPart / 4;
+  __shared__ float factor[kQ4MaxSplits];
+  __shared__ float warp_m[kMergeThreads / 32], warp_l[kMergeThreads / 32];
+  __shared__ float sums[kShares][kWidth];
+  pdl_wait();
+  pdl_launch_dependents();
+  const uint32_t share = p.heads / p.kv_heads, h = blockIdx.x, s = blockIdx.y;
+  const uint32_t kvh = h / share, block = h % share / rp, query = h % share % rp;
+  const float* parts = p.parts + size_t((s * p.kv_heads + kvh) * p.blocks + block) * chunks * kPart;
+  const bool has = threadIdx.x < chunks;
+  const float m = has ? parts[threadIdx.x * kPart + L::kReferences + query] : kNoScore;
+  const float part_l = has ? parts[threadIdx.x * kPart + L::kSums + query] : 0.f;
+  float most = m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
+  if (lane_id() == 0) warp_m[warp_id()] = most;
+  __syncthreads();
+#pragma unroll
+  for (uint32_t w = 0; w < kMergeThreads / 32; ++w) most = fmaxf(most, warp_m[w]);
+  const float f = fast_exp2(m - most), l_warp = warp_sum(part_l * f);
+  if (has) factor[threadIdx.x] = f;
+  if (lane_id() == 0) warp_l[warp_id()] = l_warp;
+  __syncthreads();
+  const uint32_t at = threadIdx.x % kWidth, part = threadIdx.x / kWidth;
+  const float* values = parts + query * L::kStride + at;
+  float a = 0.f;
+#pragma unroll 8
+  for (uint32_t c = part; c < chunks; c += kShares) a = fmaf(values[c * kPart], factor[c], a);
+  sums[part][at] = a;
+  __syncthreads();
+  if (threadIdx.x >= kWidth) return;
+  float l = 0.f;
+#pragma unroll
+  for (uint32_t w = 0; w < kMergeThreads / 32; ++w) l += warp_l[w];
+  a = 0.f;
+#pragma unroll
+  for (uint32_t i = 0; i < kShares; ++i) a += sums[i][at];
+  const bool empty = int64_t(p.lengths[s]) + p.length_offset <= 0;
+  p.out[(size_t(s) * p.heads + h) * kWidth + q4_dimension(at)] = float_to_bf16(empty ? 0.f : a / l);
+}
+
+// How the positions of a pair (a sequence's key / value head and block of query heads) are shared out: CTAs of `warps`
+// warps, `chunks` of them to a pair, merged through a cluster's shared memory or, with `parts`, through the workspace.
+//
+// The kernel wants about 20 warps an SM, each with four tiles or more. Measured on a B200 (us; w warps, c CTAs, p through
+// the workspace): 12 pairs of 72 tiles w4c4 4.8, w8c1 5.7; 192 pairs of 72 w4c1 7.6, w4c4 8.6; 768 of 72 w4c1 17.4, w8c1 18.8,
+// w4c2 20.0; 96 of 256 w4c8 11.5, w4c4 12.9; 16 of 4096 (128-wide) w4c48p 43.0, w8c16 50.0, w4c16 60.5. From 20 pairs an SM
+// on a CTA's fixed cost (a few microseconds of latency) weighs more than its width: 6144 of 72 w2c1 91, w4c1 97, w4c2 128.
+struct Q4Split {
+  uint32_t warps, chunks;
+  bool parts;
+};
+Q4Split q4_split(uint64_t pairs, uint32_t tiles) {
+  const uint64_t sms = uint64_t(sm_count()), wanted = std::min<uint64_t>(20 * sms / pairs, tiles / 4);  // warps of a pair
+  if (wanted > 8 * kQ4MaxChunks) return Q4Split{4, uint32_t(std::min<uint64_t>(wanted / 4, kQ4MaxSplits)), true};
+  uint32_t warps = 4;  // the nearest power of two
+  while (2ull * warps * warps <= wanted * wanted) warps *= 2;
+  if (warps == 4) return Q4Split{pairs >= 20 * sms ? 2u : 4u, 1, false};
+  if (warps == 8) return Q4Split{8, 1, false};
+  return warps / 4 <= kQ4MaxChunks ? Q4Split{4, warps / 4, false} : Q4Split{8, kQ4MaxChunks, false};
 }
 
 template <int G, int RP, int WARPS>
@@ -705,25 +790,46 @@ tempo_status launch_attention_warps(const Q4Attention& base, uint32_t seqs, uint
   auto kernel = decode_attention_q4_kernel<G, RP, WARPS>;
   tempo_status status = set_smem(reinterpret_cast<const void*>(kernel), Q4Smem<G, WARPS>::kBytes);
   if (status != TEMPO_OK) return status;
-  if (chunks > 8) {
+  const bool cluster = chunks > 1 && p.parts == nullptr;
+  if (cluster && chunks > 8) {
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute(non-portable cluster size)");
   }
   p.early = single_wave(uint64_t(p.kv_heads) * p.blocks * seqs * chunks, 16 / WARPS);
   return launch(kernel, dim3(chunks, p.kv_heads * p.blocks, seqs), dim3(32 * WARPS), Q4Smem<G, WARPS>::kBytes, stream,
-                chunks, "decode_attention_q4_kernel", p);
+                cluster ? chunks : 1, "decode_attention_q4_kernel", p);
 }
 
 template <int G, int RP>
-tempo_status launch_attention(const Q4Attention& base, uint32_t seqs, cudaStream_t stream) {
+tempo_status launch_attention(const Q4Attention& base, uint32_t seqs, const Q4Split& split, float* workspace,
+                              cudaStream_t stream) {
   Q4Attention p = base;
-  p.blocks = (p.heads / p.kv_heads + RP - 1) / RP;
-  const uint64_t pairs = uint64_t(p.kv_heads) * p.blocks * seqs, sms = uint64_t(sm_count());
-  uint32_t chunks = 1;
-  while (chunks < kQ4MaxChunks && pairs * chunks < 2 * sms && p.tiles >= 8 * chunks) chunks *= 2;
-  if (pairs * chunks * 4 < 16 * sms && p.tiles >= 64 * chunks) return launch_attention_warps<G, RP, 8>(p, seqs, chunks, stream);
-  if (pairs >= 20 * sms) return launch_attention_warps<G, RP, 2>(p, seqs, chunks, stream);
-  return launch_attention_warps<G, RP, 4>(p, seqs, chunks, stream);
+  p.parts = split.parts ? workspace : nullptr;
+  if (split.warps == 2) return launch_attention_warps<G, RP, 2>(p, seqs, split.chunks, stream);
+  if (split.warps == 8) return launch_attention_warps<G, RP, 8>(p, seqs, split.chunks, stream);
+  tempo_status status = launch_attention_warps<G, RP, 4>(p, seqs, split.chunks, stream);
+  if (status != TEMPO_OK || !split.parts) return status;
+  return launch(decode_merge_q4_kernel<G>, dim3(p.heads, seqs), dim3(kMergeThreads), 0, stream, 1, "decode_merge_q4_kernel", p,
+                split.chunks, uint32_t(RP));
+}
+
+// Query heads of one CTA: all that share a key / value head, up to eight.
+uint32_t q4_queries(uint32_t head, uint32_t share) {
+  return share == 1 ? 1 : share == 2 && head == 64 ? 2 : share <= 4 ? 4 : 8;
+}
+
+uint64_t q4_workspace(uint32_t seqs, uint32_t heads, uint32_t kv_heads, uint32_t head, uint32_t capacity) {
+  const uint32_t share = heads / kv_heads, rp = q4_queries(head, share);
+  const uint64_t pairs = uint64_t(seqs) * kv_heads * ((share + rp - 1) / rp);
+  const Q4Split split = q4_split(pairs, capacity / kQ4Tile);
+  return split.parts ? pairs * split.chunks * (head == 64 ? Q4Smem<1, 4>::kPart : Q4Smem<2, 4>::kPart) : 0;
+}
+
+tempo_status check_attention(const char* what, uint32_t seqs, uint32_t heads, uint32_t kv_heads) {
+  if (heads == 0 || heads % kv_heads || seqs > 65535 || heads > 65535)
+    return fail(TEMPO_ERR_VALUE, "%s: seqs %u (up to 65535), heads %u must be a multiple of kv_heads %u (both up to "
+                "65535)", what, seqs, heads, kv_heads);
+  return TEMPO_OK;
 }
 
 // What the three entry points check alike; `what` names the call.
@@ -791,21 +897,38 @@ extern "C" tempo_status tempo_kv_load_q4(const void* cache, void* kv, uint32_t l
                      static_cast<cudaStream_t>(stream), "kv_load_q4_kernel");
 }
 
+extern "C" tempo_status tempo_decode_attention_q4_workspace(uint32_t seqs, uint32_t heads, uint32_t kv_heads,
+                                                            uint32_t head, uint32_t capacity, uint64_t* bytes) {
+  alignas(16) static const char placeholder[16] = {};
+  tempo_status status = check_cache("tempo_decode_attention_q4_workspace", placeholder, seqs, kv_heads, head, capacity);
+  if (status != TEMPO_OK) return status;
+  status = check_attention("tempo_decode_attention_q4_workspace", seqs, heads, kv_heads);
+  if (status != TEMPO_OK) return status;
+  if (bytes == nullptr) return fail(TEMPO_ERR_VALUE, "tempo_decode_attention_q4_workspace: nowhere to put the size");
+  *bytes = q4_workspace(seqs, heads, kv_heads, head, capacity);
+  return TEMPO_OK;
+}
+
 extern "C" tempo_status tempo_decode_attention_q4(const void* q, uint32_t ldq, const void* cache,
                                                   const int32_t* lengths, int32_t length_offset, void* out,
                                                   uint32_t seqs, uint32_t heads, uint32_t kv_heads, uint32_t head,
-                                                  uint32_t capacity, void* stream) {
+                                                  uint32_t capacity, void* workspace, uint64_t workspace_bytes,
+                                                  void* stream) {
   tempo_status status = check_cache("tempo_decode_attention_q4", cache, seqs, kv_heads, head, capacity);
   if (status != TEMPO_OK) return status;
-  if (heads == 0 || heads % kv_heads || seqs > 65535 || heads > 65535)
-    return fail(TEMPO_ERR_VALUE, "tempo_decode_attention_q4: seqs %u (up to 65535), heads %u must be a multiple of "
-                "kv_heads %u (both up to 65535)", seqs, heads, kv_heads);
+  status = check_attention("tempo_decode_attention_q4", seqs, heads, kv_heads);
+  if (status != TEMPO_OK) return status;
   if (uint64_t(heads) * head > ldq || ldq % 8)
     return fail(TEMPO_ERR_VALUE, "tempo_decode_attention_q4: the query row stride %u must be a multiple of 8 and at "
                 "least %llu", ldq, static_cast<unsigned long long>(uint64_t(heads) * head));
   if (q == nullptr || !aligned16(q) || out == nullptr || !aligned16(out) || lengths == nullptr)
     return fail(TEMPO_ERR_VALUE, "tempo_decode_attention_q4: 16-byte aligned queries and output and the lengths are "
                 "needed");
+  const uint64_t needed = q4_workspace(seqs, heads, kv_heads, head, capacity);
+  if (needed > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < needed))
+    return fail(TEMPO_ERR_VALUE, "tempo_decode_attention_q4: a 16-byte aligned workspace of %llu bytes is needed, got "
+                "%llu", static_cast<unsigned long long>(needed), static_cast<unsigned long long>(workspace_bytes));
+  const uint32_t share = heads / kv_heads, rp = q4_queries(head, share);
   Q4Attention p{};
   p.q = static_cast<const uint16_t*>(q);
   p.cache = static_cast<const uint8_t*>(cache);
@@ -816,11 +939,15 @@ extern "C" tempo_status tempo_decode_attention_q4(const void* q, uint32_t ldq, c
   p.kv_heads = kv_heads;
   p.tiles = capacity / kQ4Tile;
   p.length_offset = length_offset;
+  p.blocks = (share + rp - 1) / rp;
+  const Q4Split split = q4_split(uint64_t(seqs) * kv_heads * p.blocks, p.tiles);
+  float* parts = static_cast<float*>(workspace);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const uint32_t share = heads / kv_heads;
-  if (head == 128 && share == 1) return launch_attention<2, 1>(p, seqs, st);
-  if (head == 128) return share <= 4 ? launch_attention<2, 4>(p, seqs, st) : launch_attention<2, 8>(p, seqs, st);
-  if (share == 1) return launch_attention<1, 1>(p, seqs, st);
-  if (share == 2) return launch_attention<1, 2>(p, seqs, st);
-  return share <= 4 ? launch_attention<1, 4>(p, seqs, st) : launch_attention<1, 8>(p, seqs, st);
+  if (head == 128) {
+    if (rp == 1) return launch_attention<2, 1>(p, seqs, split, parts, st);
+    return rp == 4 ? launch_attention<2, 4>(p, seqs, split, parts, st) : launch_attention<2, 8>(p, seqs, split, parts, st);
+  }
+  if (rp == 1) return launch_attention<1, 1>(p, seqs, split, parts, st);
+  if (rp == 2) return launch_attention<1, 2>(p, seqs, split, parts, st);
+  return rp == 4 ? launch_attention<1, 4>(p, seqs, split, parts, st) : launch_attention<1, 8>(p, seqs, split, parts, st);
 }

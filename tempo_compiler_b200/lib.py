@@ -98,7 +98,8 @@ _SIGNATURES = {
     "tempo_decode_attention": [_vp, _vp, _vp, _vp, _i32, _vp, _u32, _u32, _u32, _u32, _vp],
     "tempo_kv_store_q4": [_vp, _u32, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _vp],
     "tempo_kv_load_q4": [_vp, _vp, _u32, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _vp],
-    "tempo_decode_attention_q4": [_vp, _u32, _vp, _vp, _i32, _vp, _u32, _u32, _u32, _u32, _u32, _vp],
+    "tempo_decode_attention_q4_workspace": [_u32, _u32, _u32, _u32, _u32, ctypes.POINTER(_u64)],
+    "tempo_decode_attention_q4": [_vp, _u32, _vp, _vp, _i32, _vp, _u32, _u32, _u32, _u32, _u32, _vp, _u64, _vp],
     "tempo_token_logprobs": [_vp, _u64, _u32, _vp, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _vp, _i32, _u32, _vp],
     "tempo_argmax_finish": [_vp, _vp, _u32, _u32, _vp, _vp, _u32, _vp, _i32, _i32, _vp],
     "tempo_lm_head_argmax_noalloc": [_vp, _u32, _vp, _u32, _u32, _u32, _u32, _vp, _vp],

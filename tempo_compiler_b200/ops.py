@@ -8,6 +8,7 @@ a wrong dtype or a missing library raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple
 
 import torch
@@ -423,6 +424,14 @@ def kv_load_q4(cache: torch.Tensor, seq_of: torch.Tensor, pos_of: torch.Tensor, 
     return out
 
 
+@functools.lru_cache(maxsize=1024)
+def decode_attention_q4_workspace_bytes(seqs: int, heads: int, kv_heads: int, head: int, capacity: int) -> int:
+    """Bytes of workspace a decode_attention_q4 call of these sizes needs (0 for most)."""
+    size = ctypes.c_uint64()
+    _lib.call("tempo_decode_attention_q4_workspace", seqs, heads, kv_heads, head, capacity, ctypes.byref(size))
+    return int(size.value)
+
+
 def decode_attention_q4(qkv: torch.Tensor, cache: torch.Tensor, lengths: torch.Tensor, *, length_offset: int = 0,
                         heads: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """decode_attention over a 4-bit cache: the query columns of row s of qkv (scaled by 1/sqrt(head)) over the first
@@ -447,8 +456,11 @@ def decode_attention_q4(qkv: torch.Tensor, cache: torch.Tensor, lengths: torch.T
         if out.shape != (seqs, heads * head):
             raise ValueError(f"out must be {(seqs, heads * head)}, got {tuple(out.shape)}")
     _check_devices(qkv, cache=cache, lengths=lengths, out=out)
+    size = decode_attention_q4_workspace_bytes(seqs, heads, kv_heads, head, capacity)
+    workspace = qkv.new_empty(size, dtype=torch.uint8) if size else None
     _launch_at(qkv, "tempo_decode_attention_q4", qkv.data_ptr(), _row_stride(qkv), cache.data_ptr(),
-               lengths.data_ptr(), length_offset, out.data_ptr(), seqs, heads, kv_heads, head, capacity)
+               lengths.data_ptr(), length_offset, out.data_ptr(), seqs, heads, kv_heads, head, capacity,
+               _ptr(workspace), size)
     return out
 
 

@@ -59,7 +59,10 @@ def test_attention_refuses(change: dict) -> None:
     a = {**dict(ldq=768, seqs=2, heads=12, kv_heads=12, head=64, capacity=32), **change}
     p = _buffer()
     assert _status("tempo_decode_attention_q4", p, a["ldq"], p, p, 0, p, a["seqs"], a["heads"], a["kv_heads"], a["head"],
-                   a["capacity"], None) == lib.ERR_VALUE
+                   a["capacity"], None, 0, None) == lib.ERR_VALUE
+    if "ldq" not in change:
+        assert _status("tempo_decode_attention_q4_workspace", a["seqs"], a["heads"], a["kv_heads"], a["head"],
+                       a["capacity"], ctypes.byref(ctypes.c_uint64())) == lib.ERR_VALUE
 
 
 @pytest.mark.parametrize("which,bad", [(0, None), (0, 8), (1, None), (1, 8), (2, None), (3, None), (3, 8)])
@@ -67,7 +70,23 @@ def test_attention_refuses_pointers(which: int, bad) -> None:
     from tempo_compiler_b200 import lib
     p = [_buffer()] * 4
     p[which] = None if bad is None else p[which] + bad
-    assert _status("tempo_decode_attention_q4", p[0], 768, p[1], p[2], 0, p[3], 2, 12, 12, 64, 32, None) == lib.ERR_VALUE
+    assert _status("tempo_decode_attention_q4", p[0], 768, p[1], p[2], 0, p[3], 2, 12, 12, 64, 32, None, 0,
+                   None) == lib.ERR_VALUE
+
+
+def test_attention_refuses_a_workspace_that_is_missing_small_or_misaligned() -> None:
+    """One sequence of one key head and a long capacity needs one; short or many sequences do not."""
+    from tempo_compiler_b200 import lib
+    size, p = ctypes.c_uint64(), _buffer()
+    assert _status("tempo_decode_attention_q4_workspace", 1, 4, 1, 128, 65536, ctypes.byref(size)) == lib.OK
+    assert size.value > 0
+    for pointer, given in ((None, size.value), (p, size.value - 1), (p + 8, size.value)):
+        assert _status("tempo_decode_attention_q4", p, 512, p, p, 0, p, 1, 4, 1, 128, 65536, pointer, given,
+                       None) == lib.ERR_VALUE
+    assert _status("tempo_decode_attention_q4_workspace", 1, 4, 1, 128, 65536, None) == lib.ERR_VALUE
+    for seqs, capacity in ((1, 256), (512, 65536)):
+        assert _status("tempo_decode_attention_q4_workspace", seqs, 12, 12, 64, capacity, ctypes.byref(size)) == lib.OK
+        assert size.value == 0
 
 
 @pytest.mark.parametrize("change", [dict(rows=0), dict(vocab=0), dict(ld=99), dict(top=33), dict(vocab=8, top=9),
