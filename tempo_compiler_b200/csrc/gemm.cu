@@ -77,7 +77,7 @@ struct RowMajorSmem {
   static constexpr uint32_t kStageBytes = kABytes + kBBytes;
   // STAGED: one 32 x 32 staging tile (2 KB of BF16, 4 KB of FP32) per epilogue warp for TMA stores of the output.
   static constexpr uint32_t kStagingOffset = STAGES * kStageBytes;
-  static constexpr uint32_t kStagingTile = F32 ? 4096u : 2048u;
+  static constexpr uint32_t kStagingTile = 2048u;
   static constexpr uint32_t kStagingBytes = STAGED ? 16u * kStagingTile : 0u;
   static constexpr uint32_t kBarrierOffset = kStagingOffset + kStagingBytes;
   // full[S], empty[S], acc_full[2], acc_empty[2], final, epilogue-wide (row statistics)
@@ -106,13 +106,32 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
                : "memory");
 }
 
-// One thread's 32 accumulators of its row into the warp's FP32 staging tile, as they are: row `lane` at 128 bytes, its
-// 16-byte words swizzled by the row (the TMA 128-byte swizzle, which spreads the warp's writes over all banks).
-__device__ __forceinline__ void stage_f32(const uint32_t (&r)[32], uint8_t* staging, uint32_t lane) {
-  uint4* row = reinterpret_cast<uint4*>(staging + lane * 128);
+// Sixteen of one thread's accumulators into the warp's FP32 staging tile (32 rows x 16 columns), as they are: row `lane` at
+// 64 bytes, its 16-byte words swizzled as the TMA 64-byte swizzle has them.
+__device__ __forceinline__ void stage_f32(const uint32_t (&r)[32], uint32_t half, uint8_t* staging, uint32_t lane) {
+  uint4* row = reinterpret_cast<uint4*>(staging + lane * 64);
 #pragma unroll
-  for (uint32_t q = 0; q < 8; ++q)
-    row[q ^ (lane & 7u)] = make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
+  for (uint32_t q = 0; q < 4; ++q) {
+    const uint32_t j = 16 * half + 4 * q;
+    row[q ^ ((lane >> 1) & 3u)] = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+  }
+}
+
+// The warp's 32 x 32 FP32 block by two TMA stores through its staging tile.
+__device__ __forceinline__ void store_f32(const CUtensorMap* map, const uint32_t (&r)[32], uint8_t* staging, uint32_t lane,
+                                          uint32_t n0, uint32_t row0) {
+#pragma unroll
+  for (uint32_t half = 0; half < 2; ++half) {
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
+    stage_f32(r, half, staging, lane);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_2d(map, staging, int32_t(n0 + 16 * half), int32_t(row0));
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+  }
 }
 
 // The FP32 columns n0 .. n - 1 of one row, fewer than a staging tile's 32, by plain stores: a TMA store clips at 16-byte
@@ -565,19 +584,14 @@ __global__ void __launch_bounds__(kRowThreads, 1)
           if (row0 >= p.m || n0 >= p.n) continue;  // warp-uniform
           uint8_t* staging = smem + L::kStagingOffset + (warp - 2) * L::kStagingTile;
           if constexpr (F32) {
-            if (n0 + kCW > p.n) {  // warp-uniform
-              store_f32_tail(p, r, row, n0);
-              continue;
-            }
+            if (n0 + kCW > p.n) store_f32_tail(p, r, row, n0);  // warp-uniform
+            else store_f32(&tmap_out, r, staging, lane, n0, row0);
+            continue;
           }
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
           __syncwarp();
-          if constexpr (F32) {
-            stage_f32(r, staging, lane);
-          } else {
-            const float mu = ln ? ln_mean[row_in_tile] : 0.f, rs = ln ? ln_rstd[row_in_tile] : 0.f;
-            epilogue_chunk<kCW, true>(p, r, row, n0, gelu, ln, mu, rs, staging + lane * 64, (lane >> 1) & 3u);
-          }
+          const float mu = ln ? ln_mean[row_in_tile] : 0.f, rs = ln ? ln_rstd[row_in_tile] : 0.f;
+          epilogue_chunk<kCW, true>(p, r, row, n0, gelu, ln, mu, rs, staging + lane * 64, (lane >> 1) & 3u);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) {
@@ -813,7 +827,9 @@ tempo_status launch_rowmajor(const void* a, uint32_t lda, const void* w_t, uint3
   const uint64_t a_dims[2] = {base.k, base.m};
   const uint64_t a_strides[1] = {uint64_t(lda) * 2};
   // At most 64 rows: a 64-row box, so the copy fills no out-of-range rows (the MMA's upper 64 rows are discarded).
-  const uint32_t a_rows = base.m <= 64 ? 64 : 128;
+  // (FP32 outputs: no row more than whole swizzle atoms of eight; rows that the copy fills slow it down, 4 rows of an LM
+  // head 20.2 us with a 64-row box, 12.2 with 8.)
+  const uint32_t a_rows = F32 ? (base.m < 128 ? (base.m + 7) / 8 * 8 : 128) : base.m <= 64 ? 64 : 128;
   const uint32_t a_box[2] = {kBK, a_rows};
   tempo_status s = encode_tmap(&ta, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a, a_dims, a_strides, a_box,
                                CU_TENSOR_MAP_SWIZZLE_128B);
@@ -827,9 +843,9 @@ tempo_status launch_rowmajor(const void* a, uint32_t lda, const void* w_t, uint3
   if (STAGED) {
     const uint64_t o_dims[2] = {base.n, base.m};
     const uint64_t o_strides[1] = {uint64_t(base.ldo) * (F32 ? 4 : 2)};
-    const uint32_t o_box[2] = {32, 32};
+    const uint32_t o_box[2] = {F32 ? 16 : 32, 32};
     s = encode_tmap(&to, F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base.out, o_dims,
-                    o_strides, o_box, F32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+                    o_strides, o_box, CU_TENSOR_MAP_SWIZZLE_64B);
     if (s != TEMPO_OK) return s;
   }
   RowMajorParams p = base;
@@ -1269,7 +1285,7 @@ struct PairSmem {
   static constexpr uint32_t kStageBytes = kABytes + kBBytes;
   // One 32 x 32 staging tile (2 KB of BF16, 4 KB of FP32) per epilogue warp for the output's TMA stores.
   static constexpr uint32_t kStagingOffset = STAGES * kStageBytes;
-  static constexpr uint32_t kStagingTile = F32 ? 4096u : 2048u;
+  static constexpr uint32_t kStagingTile = 2048u;
   static constexpr uint32_t kStagingBytes = (kRowEpiThreads / 32) * kStagingTile;
   static constexpr uint32_t kBarrierOffset = kStagingOffset + kStagingBytes;
   // full[S] (the leader's), empty[S], acc_full[2], acc_empty[2] (the leader's), final
@@ -1472,16 +1488,14 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         const uint32_t n0 = n_base + c;
         if (row0 >= p.m || n0 >= p.n) continue;  // warp-uniform: the whole 32 x 32 block lies outside
         if constexpr (F32) {
-          if (n0 + kCW > p.n) {
-            store_f32_tail(p, r, row, n0);
-            continue;
-          }
+          if (n0 + kCW > p.n) store_f32_tail(p, r, row, n0);
+          else store_f32(&tmap_out, r, staging, lane, n0, row0);
+          continue;
         }
         // The staging tile is free once the previous store from it has been read.
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         __syncwarp();
-        if constexpr (F32) stage_f32(r, staging, lane);
-        else epilogue_chunk<kCW, true>(p, r, row, n0, gelu, false, 0.f, 0.f, stage_row, swizzle);
+        epilogue_chunk<kCW, true>(p, r, row, n0, gelu, false, 0.f, 0.f, stage_row, swizzle);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         // Rows past M and columns past N are clipped by the copy.
@@ -1528,9 +1542,9 @@ tempo_status launch_pair(const void* a, uint32_t lda, const void* w_t, uint32_t 
   CUtensorMap to;
   const uint64_t o_dims[2] = {base.n, base.m};
   const uint64_t o_strides[1] = {uint64_t(base.ldo) * (F32 ? 4 : 2)};
-  const uint32_t o_box[2] = {32, 32};
+  const uint32_t o_box[2] = {F32 ? 16 : 32, 32};
   s = encode_tmap(&to, F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base.out, o_dims,
-                  o_strides, o_box, F32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+                  o_strides, o_box, CU_TENSOR_MAP_SWIZZLE_64B);
   if (s != TEMPO_OK) return s;
   RowMajorParams p = base;
   p.m_tiles = (p.m + 255) / 256;
@@ -1857,11 +1871,11 @@ static tempo_status gemm_impl(const void* a, uint32_t lda, const void* w_t, uint
   if (argmax) return launch_rowmajor<256, 4>(a, lda, w_t, ldw, p, st);
   if (f32) {
     // An LM head has far more columns than tiles need: 256 x 256 tiles on CTA pairs from four to a pair, as for any
-    // product (512 rows of 50257 x 768: 50 us against 80 with direct stores), else 128-column tiles, whose 393 over 148 SMs leave less idle
-    // than 197 of 256 columns (64 rows: 16.8 us against 19.3).
+    // product (512 rows of 50257 x 768: 44 us against 80 with direct stores), else 128-column tiles, whose 393 over 148 SMs leave less idle
+    // than 197 of 256 columns (64 rows: 14.6 us against 16.7).
     if (uint64_t((m + 255) / 256) * ((n + 255) / 256) >= 4ull * (uint64_t(sm_count()) / 2))
-      return launch_pair<4, true>(a, lda, w_t, ldw, p, st);
-    return launch_rowmajor<128, 4, true, false, true>(a, lda, w_t, ldw, p, st);
+      return launch_pair<5, true>(a, lda, w_t, ldw, p, st);
+    return launch_rowmajor<128, 5, true, false, true>(a, lda, w_t, ldw, p, st);
   }
   // With the statistics from their producer, the folded LayerNorm runs wherever the plain projection would: narrow
   // full-K tiles for one 128-row block, else split-K.
