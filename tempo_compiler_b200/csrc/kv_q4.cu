@@ -215,18 +215,21 @@ tempo_status launch_rows(void (*kernel)(Q4Rows), Q4Rows p, uint32_t rows, uint32
 //
 // At 72 bytes a position the cache streams past at more than 40 codes per clock and SM, which CUDA cores cannot
 // dequantise, multiply and add in FP32 (a first kernel that did so took 4 to 150 times the read time), so both products
-// run on mma.sync with the codes as the A operand: key codes enter as the BF16 integers 128 + code and value codes as
-// the FP16 integers 64 + code, which are two logic operations per pair of codes, and scale, low and the constants are
-// applied to the products: with D = sum_d q_d (128 + code_d) and Q = sum_d q_d,
-//   q . k = scale D + (low - 128 scale) Q,
+// run on mma.sync with the codes as the A operand: pairs of codes become the FP16 integers 64 + code by a logic operation,
+// and scale, low and the constants are applied to the products: with D = sum_d q_d (64 + code_d) and Q = sum_d q_d,
+//   q . k = scale D + (low - 64 scale) Q,
 //   sum_j p_j v_j = sum_j w_j (64 + code_j) - 64 sum_j w_j + sum_j p_j low_j,   w_j = p_j scale_j.
+// What bounds the kernel is the logic pipe: a code pair costs one logic operation to mask and one to move, of which those
+// to the left are multiplications by 16 and run beside them (shifts for all of them, the keys as BF16 integers 128 +
+// code, took 91 us for 512 sequences of 12 heads and 1152 positions instead of 89.6).
 // The eight columns of the B operand (m16n8k16) are query heads of one key / value head times tiles:
 // grouped heads read the cache once, and with few heads one softmax serves several tiles (the first tensor-core form, one tile
 // and eight columns of queries whether they existed or not, issued 309 instructions a tile and was bound by the ALU pipe).
 // Every column holds its head's query; the scores of tile j are kept in the lanes whose columns are tile j's, and the
 // weights of the other columns are zeroed before tile j's values are multiplied.
-// q is exact in BF16; w is rounded to FP16 (2^-11 of each weight; an eighth of the output's own BF16 rounding), relative
-// to a running reference that bounds w and p low alike; everything else, the sums included, is FP32.
+// A query row is scaled by a power of two to at most 2, where FP16 holds its BF16 values but for what lies 2^-14 below its
+// greatest, and there to 2^-25; w is rounded to FP16 (2^-11 of each weight; an eighth of the output's own BF16 rounding),
+// relative to a running reference that bounds w and p low alike; everything else, the sums included, is FP32.
 //
 // A CTA of four warps takes a run of tiles of one (sequence, key / value head, eight query heads); each warp streams its
 // own pieces (one bulk copy each, kRing in flight) and keeps an online softmax whose reference moves only when a score
@@ -252,7 +255,8 @@ struct Q4Smem {
   static constexpr uint32_t kPart = (kSums + kQ4Queries) * 4;
   static constexpr uint32_t kBarrierOffset = WARPS * kWarpRing;
   static constexpr uint32_t kMergeOffset = kBarrierOffset + WARPS * kRing * 8;
-  static constexpr uint32_t kBytes = kMergeOffset + kPart;
+  // The CTA's own partial result, which only a cluster needs: without it six CTAs of four warps fit an SM, not five.
+  static constexpr uint32_t bytes(bool cluster) { return kMergeOffset + (cluster ? kPart : 0); }
   static_assert(kPart <= kWarpRing && kPart % 16 == 0, "a warp's partial result fits its ring");
 };
 
@@ -262,21 +266,15 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 // D = A x B: the accumulator starts at zero.
-__device__ __forceinline__ void mma_bf16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                               uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%10, %10, %10, %10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
+// D += A x B.
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -310,17 +308,15 @@ __device__ __forceinline__ uint32_t in_register(uint32_t c) {
 }
 
 struct Q4Constants {
-  uint32_t key_mask, key_magic, value_mask, value_magic;
+  uint32_t mask, magic, sixteen;
 };
 
-// Two codes, `shift` bits up in each half of w, as the BF16 integers 128 + code / the FP16 integers 64 + code.
-__device__ __forceinline__ uint32_t key_pair(const Q4Constants& k, uint32_t w, uint32_t shift) {
-  return and_or(w >> shift, k.key_mask, k.key_magic);
-}
-template <int NIBBLE>
-__device__ __forceinline__ uint32_t value_pair(const Q4Constants& k, uint32_t w) {
-  return and_or(NIBBLE == 0 ? w << 4 : w >> (4 * (NIBBLE - 1)), k.value_mask, k.value_magic);
-}
+// Two codes as the FP16 integers 64 + code: code 0 or 1 of each half of w (bits 0 .. 3 or 4 .. 7). The multiplier is not
+// known to be 16 when the kernel is compiled, so the product stays one, beside the logic pipe.
+__device__ __forceinline__ uint32_t pair0(const Q4Constants& k, uint32_t w) { return and_or(w * k.sixteen, k.mask, k.magic); }
+__device__ __forceinline__ uint32_t pair1(const Q4Constants& k, uint32_t w) { return and_or(w, k.mask, k.magic); }
+// The bytes of each half swapped: codes 2 and 3 where 0 and 1 were.
+__device__ __forceinline__ uint32_t swap_bytes(uint32_t w) { return __byte_perm(w, 0, 0x2301); }
 
 // One warp's running state. The MMA fragments put columns 2 t and 2 t + 1 (t = lane % 4) on a lane; with g = lane / 4,
 // acc[i][n] holds dimensions 64 i + 8 g + n ([0], [1]) and 64 i + 8 g + 4 + n ([2], [3]) of the two columns.
@@ -343,6 +339,7 @@ __host__ __device__ constexpr uint32_t q4_tiles_at_once(int g, int rp) {
 // else `left` do.
 template <int G, int RP, bool FULL>
 __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G][8], const float (&qs)[G][2],
+                                         const float (&unit)[2],
                                          const uint8_t* tiles, uint32_t left, uint32_t g, uint32_t t,
                                          const Q4Constants& kc) {
   constexpr uint32_t kTileBytes = G * kQ4Block, CP = q4_columns(RP), TP = q4_tiles_at_once(G, RP);
@@ -364,10 +361,11 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
       const uint2 k0 = *reinterpret_cast<const uint2*>(block + pg * 32 + t * 8);
       const uint2 k1 = *reinterpret_cast<const uint2*>(block + (pg + 8) * 32 + t * 8);
       float e[4];
-      mma_bf16_first(e, key_pair(kc, k0.x, 0), key_pair(kc, k1.x, 0), key_pair(kc, k0.x, 4), key_pair(kc, k1.x, 4), qf[i][0], qf[i][1]);
-      mma_bf16(e, key_pair(kc, k0.x, 8), key_pair(kc, k1.x, 8), key_pair(kc, k0.x, 12), key_pair(kc, k1.x, 12), qf[i][2], qf[i][3]);
-      mma_bf16(e, key_pair(kc, k0.y, 0), key_pair(kc, k1.y, 0), key_pair(kc, k0.y, 4), key_pair(kc, k1.y, 4), qf[i][4], qf[i][5]);
-      mma_bf16(e, key_pair(kc, k0.y, 8), key_pair(kc, k1.y, 8), key_pair(kc, k0.y, 12), key_pair(kc, k1.y, 12), qf[i][6], qf[i][7]);
+      const uint32_t x0 = swap_bytes(k0.x), x1 = swap_bytes(k1.x), y0 = swap_bytes(k0.y), y1 = swap_bytes(k1.y);
+      mma_f16_first(e, pair0(kc, k0.x), pair0(kc, k1.x), pair1(kc, k0.x), pair1(kc, k1.x), qf[i][0], qf[i][1]);
+      mma_f16(e, pair0(kc, x0), pair0(kc, x1), pair1(kc, x0), pair1(kc, x1), qf[i][2], qf[i][3]);
+      mma_f16(e, pair0(kc, k0.y), pair0(kc, k1.y), pair1(kc, k0.y), pair1(kc, k1.y), qf[i][4], qf[i][5]);
+      mma_f16(e, pair0(kc, y0), pair0(kc, y1), pair1(kc, y0), pair1(kc, y1), qf[i][6], qf[i][7]);
 #pragma unroll
       for (int c = 0; c < 4; ++c)
         if (kTwo || c % 2 == 0) d[i][c] = TP == 1 || mine == j ? e[c] : d[i][c];
@@ -386,7 +384,7 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
     if (!in0) meta0 = make_uint2(0, 0);  // what lies behind the last position may be anything
     if (!in1) meta1 = make_uint2(0, 0);
     const float ks0 = bf16_lo(meta0.x), ks1 = bf16_lo(meta1.x);
-    const float kl0 = fmaf(-128.f, ks0, bf16_hi(meta0.x)), kl1 = fmaf(-128.f, ks1, bf16_hi(meta1.x));
+    const float kl0 = fmaf(-64.f, ks0, bf16_hi(meta0.x)), kl1 = fmaf(-64.f, ks1, bf16_hi(meta1.x));
     s0 = fmaf(ks0, d[i][0], fmaf(kl0, qs[i][0], s0));
     if (kTwo) s1 = fmaf(ks0, d[i][1], fmaf(kl0, qs[i][1], s1));
     s2 = fmaf(ks1, d[i][2], fmaf(kl1, qs[i][0], s2));
@@ -396,10 +394,10 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
     size0 = fmax3(size0, bf16_lo(meta0.y), 0.0625f * fabsf(bf16_hi(meta0.y)));
     size1 = fmax3(size1, bf16_lo(meta1.y), 0.0625f * fabsf(bf16_hi(meta1.y)));
   }
-  s0 = in0 ? s0 * kDecodeLog2e : -INFINITY;
-  s1 = in0 ? s1 * kDecodeLog2e : -INFINITY;
-  s2 = in1 ? s2 * kDecodeLog2e : -INFINITY;
-  s3 = in1 ? s3 * kDecodeLog2e : -INFINITY;
+  s0 = in0 ? s0 * unit[0] : -INFINITY;
+  s1 = in0 ? s1 * unit[1] : -INFINITY;
+  s2 = in1 ? s2 * unit[0] : -INFINITY;
+  s3 = in1 ? s3 * unit[1] : -INFINITY;
   // The reference follows log2(p size), size the value row's scale or a sixteenth of its low: w and p low stay small
   // whatever the values' size, and a position of small values needs a larger p to move it.
   const float g0 = fast_log2(fminf(size0, 0x1p100f)), g1 = fast_log2(fminf(size1, 0x1p100f));
@@ -470,13 +468,15 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
       const uint32_t vc = *reinterpret_cast<const uint32_t*>(words + (pe + 8) * 32);
       const uint32_t vd = *reinterpret_cast<const uint32_t*>(words + (po + 8) * 32);
       const uint32_t w0 = TP == 1 || g / CP == j ? b0[i] : 0u, w1 = TP == 1 || g / CP == j ? b1[i] : 0u;
-      // The same dimension of two positions side by side: dimensions 8 g .. + 3 in e0 / e1, 8 g + 4 .. in o0 / o1.
-      const uint32_t e0 = __byte_perm(va, vb, 0x5410), o0 = __byte_perm(va, vb, 0x7632);
-      const uint32_t e1 = __byte_perm(vc, vd, 0x5410), o1 = __byte_perm(vc, vd, 0x7632);
-      mma_f16(st.acc[i][0], value_pair<0>(kc, e0), value_pair<0>(kc, o0), value_pair<0>(kc, e1), value_pair<0>(kc, o1), w0, w1);
-      mma_f16(st.acc[i][1], value_pair<1>(kc, e0), value_pair<1>(kc, o0), value_pair<1>(kc, e1), value_pair<1>(kc, o1), w0, w1);
-      mma_f16(st.acc[i][2], value_pair<2>(kc, e0), value_pair<2>(kc, o0), value_pair<2>(kc, e1), value_pair<2>(kc, o1), w0, w1);
-      mma_f16(st.acc[i][3], value_pair<3>(kc, e0), value_pair<3>(kc, o0), value_pair<3>(kc, e1), value_pair<3>(kc, o1), w0, w1);
+      // The same dimension of two positions side by side: dimensions 8 g + 0, 1 in e, + 2, 3 in f, + 4, 5 in o, + 6, 7 in r.
+      const uint32_t e0 = __byte_perm(va, vb, 0x5410), f0 = __byte_perm(va, vb, 0x4501);
+      const uint32_t o0 = __byte_perm(va, vb, 0x7632), r0 = __byte_perm(va, vb, 0x6723);
+      const uint32_t e1 = __byte_perm(vc, vd, 0x5410), f1 = __byte_perm(vc, vd, 0x4501);
+      const uint32_t o1 = __byte_perm(vc, vd, 0x7632), r1 = __byte_perm(vc, vd, 0x6723);
+      mma_f16(st.acc[i][0], pair0(kc, e0), pair0(kc, o0), pair0(kc, e1), pair0(kc, o1), w0, w1);
+      mma_f16(st.acc[i][1], pair1(kc, e0), pair1(kc, o0), pair1(kc, e1), pair1(kc, o1), w0, w1);
+      mma_f16(st.acc[i][2], pair0(kc, f0), pair0(kc, r0), pair0(kc, f1), pair0(kc, r1), w0, w1);
+      mma_f16(st.acc[i][3], pair1(kc, f0), pair1(kc, r0), pair1(kc, f1), pair1(kc, r1), w0, w1);
     }
   }
 }
@@ -498,6 +498,7 @@ struct Q4Attention {
   const int32_t* lengths;
   uint16_t* out;
   uint32_t ldq, heads, kv_heads, tiles;
+  uint32_t share;   // query heads per key / value head
   int32_t length_offset;
   uint32_t blocks;  // groups of query heads per key / value head
   float* parts;     // split over more CTAs than a cluster holds: each leaves its partial result here
@@ -512,8 +513,10 @@ __global__ void __launch_bounds__(32 * WARPS) decode_attention_q4_kernel(Q4Atten
   constexpr uint32_t CP = q4_columns(RP), TP = q4_tiles_at_once(G, RP);
   const uint32_t warp = warp_id(), lane = lane_id(), g = lane >> 2, t = lane & 3u;
   const uint32_t chunks = gridDim.x, chunk = blockIdx.x, s = blockIdx.z;
-  const uint32_t kvh = blockIdx.y / p.blocks, share = p.heads / p.kv_heads;
-  const uint32_t first = (blockIdx.y % p.blocks) * RP;  // of the key / value head's query heads
+  // (Integer divisions by numbers only known at launch cost about 25 instructions each: none where there is nothing to
+  // divide.)
+  const uint32_t share = RP == 1 ? 1 : p.share, kvh = p.blocks == 1 ? blockIdx.y : blockIdx.y / p.blocks;
+  const uint32_t first = (blockIdx.y - kvh * p.blocks) * RP;  // of the key / value head's query heads
   const uint32_t queries = min(uint32_t(RP), share - first);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarrierOffset) + warp * kRing;
   uint8_t* ring = smem + warp * L::kWarpRing;
@@ -530,7 +533,7 @@ __global__ void __launch_bounds__(32 * WARPS) decode_attention_q4_kernel(Q4Atten
   const uint32_t capacity = p.tiles * kQ4Tile;
   const uint32_t len = want <= 0 ? 0u : want < int64_t(capacity) ? uint32_t(want) : capacity;
   // The CTA's tiles [t_begin, t_end), a run of them for each warp.
-  const uint32_t used = (len + kQ4Tile - 1) / kQ4Tile, per = (used + chunks - 1) / chunks;
+  const uint32_t used = (len + kQ4Tile - 1) / kQ4Tile, per = chunks == 1 ? used : (used + chunks - 1) / chunks;
   const uint32_t t_begin = min(used, chunk * per), t_end = min(used, t_begin + per);
   const uint32_t share_w = (t_end - t_begin + WARPS - 1) / WARPS;
   const uint32_t w_begin = min(t_end, t_begin + warp * share_w), w_end = min(t_end, w_begin + share_w);
@@ -547,39 +550,53 @@ __global__ void __launch_bounds__(32 * WARPS) decode_attention_q4_kernel(Q4Atten
       if (i < pieces) fetch(i, i);
   }
 
-  // The query fragments: lane (g, t) holds dimensions 16 t .. 16 t + 15 of each group of its column's query.
+  // The query fragments: lane (g, t) holds dimensions 16 t .. 16 t + 15 of each group of its column's query, the row scaled
+  // by a power of two to a greatest magnitude below 2.
   uint32_t qf[G][8];
-  float qs[G][2];
+  float qs[G][2], unit[2];
+  {
+    float x[G][16], greatest = 0.f;
 #pragma unroll
-  for (int i = 0; i < G; ++i) {
-    float sum = 0.f;
-    uint4 a = make_uint4(0, 0, 0, 0), b = a;
-    if (g % CP < queries) {
-      const uint4* q4 = reinterpret_cast<const uint4*>(
-          p.q + size_t(s) * p.ldq + size_t(kvh * share + first + g % CP) * kWidth + i * 64 + t * 16);
-      a = q4[0];
-      b = q4[1];
+    for (int i = 0; i < G; ++i) {
+      uint4 a = make_uint4(0, 0, 0, 0), b = a;
+      if (g % CP < queries) {
+        const uint4* q4 = reinterpret_cast<const uint4*>(
+            p.q + size_t(s) * p.ldq + size_t(kvh * share + first + g % CP) * kWidth + i * 64 + t * 16);
+        a = q4[0];
+        b = q4[1];
+      }
+      float lo[8], hi[8];
+      unpack8(a, lo);
+      unpack8(b, hi);
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        x[i][d] = lo[d];
+        x[i][8 + d] = hi[d];
+        greatest = fmax3(greatest, fabsf(lo[d]), fabsf(hi[d]));
+      }
     }
-    // key_pair of a word, 4 n up, gives dimensions n and n + 4 of a word's eight.
-    qf[i][0] = __byte_perm(a.x, a.z, 0x5410);
-    qf[i][1] = __byte_perm(a.x, a.z, 0x7632);
-    qf[i][2] = __byte_perm(a.y, a.w, 0x5410);
-    qf[i][3] = __byte_perm(a.y, a.w, 0x7632);
-    qf[i][4] = __byte_perm(b.x, b.z, 0x5410);
-    qf[i][5] = __byte_perm(b.x, b.z, 0x7632);
-    qf[i][6] = __byte_perm(b.y, b.w, 0x5410);
-    qf[i][7] = __byte_perm(b.y, b.w, 0x7632);
-    float f[8];
-    unpack8(a, f);
+    greatest = fmaxf(greatest, __shfl_xor_sync(0xFFFFFFFFu, greatest, 1));
+    greatest = fmaxf(greatest, __shfl_xor_sync(0xFFFFFFFFu, greatest, 2));
+    const uint32_t exponent = min(max(__float_as_uint(greatest) >> 23, 1u), 253u);
+    const float down = __uint_as_float((254u - exponent) << 23), up = kDecodeLog2e * __uint_as_float(exponent << 23);
+    unit[0] = __shfl_sync(0xFFFFFFFFu, up, 8 * t);  // of the lane's own columns, 2 t and 2 t + 1
+    unit[1] = __shfl_sync(0xFFFFFFFFu, up, 8 * t + 4);
 #pragma unroll
-    for (int d = 0; d < 8; ++d) sum += f[d];
-    unpack8(b, f);
+    for (int i = 0; i < G; ++i) {
+      float sum = 0.f;
 #pragma unroll
-    for (int d = 0; d < 8; ++d) sum += f[d];
-    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
-    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
-    qs[i][0] = __shfl_sync(0xFFFFFFFFu, sum, 8 * t);      // the lane's own columns, 2 t and 2 t + 1
-    qs[i][1] = __shfl_sync(0xFFFFFFFFu, sum, 8 * t + 4);
+      for (int n = 0; n < 8; ++n) {
+        // pair0 and pair1 of a word and of its swapped form give dimensions n and n + 4 of a word's eight
+        const int d = n / 4 * 8 + n % 4;
+        const __half2 h = __floats2half2_rn(x[i][d] * down, x[i][d + 4] * down);
+        qf[i][n] = *reinterpret_cast<const uint32_t*>(&h);
+        sum += __low2float(h) + __high2float(h);
+      }
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+      qs[i][0] = __shfl_sync(0xFFFFFFFFu, sum, 8 * t);
+      qs[i][1] = __shfl_sync(0xFFFFFFFFu, sum, 8 * t + 4);
+    }
   }
 
   Q4State<G> st;
@@ -593,8 +610,7 @@ __global__ void __launch_bounds__(32 * WARPS) decode_attention_q4_kernel(Q4Atten
 #pragma unroll
       for (int c = 0; c < 4; ++c) st.acc[i][n][c] = 0.f;
   }
-  const Q4Constants kc{in_register(0x000F000Fu), in_register(0x43004300u), in_register(0x00F000F0u),
-                       in_register(0x54005400u)};
+  const Q4Constants kc{in_register(0x00F000F0u), in_register(0x54005400u), in_register(16u)};
   uint32_t slot = 0, phase = 0, limit = pieces;
   bool ok = true;
   for (uint32_t piece = 0; piece < limit; ++piece) {
@@ -611,11 +627,11 @@ __global__ void __launch_bounds__(32 * WARPS) decode_attention_q4_kernel(Q4Atten
       if (left == kPieceTiles * kQ4Tile) {
 #pragma unroll
         for (uint32_t i = 0; i < kPieceTiles; i += TP)
-          q4_tiles<G, RP, true>(st, qf, qs, data + i * kTileBytes, TP * kQ4Tile, g, t, kc);
+          q4_tiles<G, RP, true>(st, qf, qs, unit, data + i * kTileBytes, TP * kQ4Tile, g, t, kc);
       } else {
 #pragma unroll 1
         for (uint32_t i = 0; i * kQ4Tile < left; i += TP)
-          q4_tiles<G, RP, false>(st, qf, qs, data + i * kTileBytes, left - i * kQ4Tile, g, t, kc);
+          q4_tiles<G, RP, false>(st, qf, qs, unit, data + i * kTileBytes, left - i * kQ4Tile, g, t, kc);
       }
       __syncwarp();
       if (lane == 0 && piece + kRing < pieces) fetch(piece + kRing, slot);
@@ -728,7 +744,7 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_q4_kernel(Q4Attent
   __shared__ float sums[kShares][kWidth];
   pdl_wait();
   pdl_launch_dependents();
-  const uint32_t share = p.heads / p.kv_heads, h = blockIdx.x, s = blockIdx.y;
+  const uint32_t share = p.share, h = blockIdx.x, s = blockIdx.y;
   const uint32_t kvh = h / share, block = h % share / rp, query = h % share % rp;
   const float* parts = p.parts + size_t((s * p.kv_heads + kvh) * p.blocks + block) * chunks * kPart;
   const bool has = threadIdx.x < chunks;
@@ -788,15 +804,16 @@ template <int G, int RP, int WARPS>
 tempo_status launch_attention_warps(const Q4Attention& base, uint32_t seqs, uint32_t chunks, cudaStream_t stream) {
   Q4Attention p = base;
   auto kernel = decode_attention_q4_kernel<G, RP, WARPS>;
-  tempo_status status = set_smem(reinterpret_cast<const void*>(kernel), Q4Smem<G, WARPS>::kBytes);
-  if (status != TEMPO_OK) return status;
   const bool cluster = chunks > 1 && p.parts == nullptr;
+  const tempo_status status = set_smem(reinterpret_cast<const void*>(kernel), Q4Smem<G, WARPS>::bytes(true));
+  if (status != TEMPO_OK) return status;
   if (cluster && chunks > 8) {
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute(non-portable cluster size)");
   }
   p.early = single_wave(uint64_t(p.kv_heads) * p.blocks * seqs * chunks, 16 / WARPS);
-  return launch(kernel, dim3(chunks, p.kv_heads * p.blocks, seqs), dim3(32 * WARPS), Q4Smem<G, WARPS>::kBytes, stream,
+  return launch(kernel, dim3(chunks, p.kv_heads * p.blocks, seqs), dim3(32 * WARPS),
+                Q4Smem<G, WARPS>::bytes(cluster), stream,
                 cluster ? chunks : 1, "decode_attention_q4_kernel", p);
 }
 
@@ -937,6 +954,7 @@ extern "C" tempo_status tempo_decode_attention_q4(const void* q, uint32_t ldq, c
   p.ldq = ldq;
   p.heads = heads;
   p.kv_heads = kv_heads;
+  p.share = share;
   p.tiles = capacity / kQ4Tile;
   p.length_offset = length_offset;
   p.blocks = (share + rp - 1) / rp;
