@@ -4,6 +4,10 @@ It allocates only that kernel's operands, so a profiler capture of it stays smal
 
     python -m tempo_compiler_b200.kernel_bench gemm --m 65536 --n 3072 --k 768 --epilogue gelu
     python -m tempo_compiler_b200.kernel_bench decode_attention --seqs 64 --capacity 1152
+    python -m tempo_compiler_b200.kernel_bench decode_attention_q4 --seqs 512 --capacity 1152
+    python -m tempo_compiler_b200.kernel_bench kv_store_q4 --rows 65536
+    python -m tempo_compiler_b200.kernel_bench token_logprobs --rows 512 --top 20
+    python -m tempo_compiler_b200.kernel_bench gemm_f32 --m 64 --n 50257
     python -m tempo_compiler_b200.kernel_bench prefill_attention --seqs 8 --tokens 1024
     python -m tempo_compiler_b200.kernel_bench layernorm --rows 65536
     python -m tempo_compiler_b200.kernel_bench block_gemm --depth 768 --columns 3072
@@ -45,7 +49,8 @@ def _time(fn, repeats: int, warmup: int) -> float:
 def main() -> int:
     parser = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     parser.add_argument("kernel", choices=["gemm", "decode_attention", "prefill_attention", "layernorm", "block_gemm",
-                                           "stream_read"])
+                                           "stream_read", "decode_attention_q4", "kv_store_q4", "token_logprobs",
+                                           "gemm_f32"])
     parser.add_argument("--gib", type=float, default=2.0, help="stream_read: GiB read per launch")
     parser.add_argument("--m", type=int, default=65536)
     parser.add_argument("--n", type=int, default=3072)
@@ -59,6 +64,9 @@ def main() -> int:
     parser.add_argument("--rows", type=int, default=65536)
     parser.add_argument("--depth", type=int, default=768)
     parser.add_argument("--columns", type=int, default=3072)
+    parser.add_argument("--top", type=int, default=0, help="token_logprobs: alternatives of a row")
+    parser.add_argument("--vocab", type=int, default=50257)
+    parser.add_argument("--logits", choices=["float32", "bfloat16"], default="float32")
     parser.add_argument("--repeats", type=int, default=10)
     parser.add_argument("--warmup", type=int, default=3)
     args = parser.parse_args()
@@ -103,6 +111,44 @@ def main() -> int:
         nbytes = args.seqs * 12 * length * 64 * 2 * 2 + args.seqs * 3 * 768 * 2 + args.seqs * 768 * 2
         result.update(seqs=args.seqs, capacity=args.capacity, length=length, ms=ms,
                       bytes=nbytes, gbs=nbytes / ms / 1e6)
+    elif args.kernel in ("decode_attention_q4", "kv_store_q4"):
+        attend = args.kernel == "decode_attention_q4"
+        length = args.capacity if args.length is None else args.length
+        seqs, tokens = (args.seqs, length) if attend else (-(-args.rows // args.tokens), args.tokens)
+        cache = ops.kv_cache_q4(seqs, 12, max(args.capacity, tokens), device=dev)
+        block = torch.randn((min(seqs * tokens, 65536), 3 * 768), device=dev).to(bf)
+        seq = torch.arange(seqs, dtype=torch.int32, device=dev).repeat_interleave(tokens)
+        pos = torch.arange(tokens, dtype=torch.int32, device=dev).repeat(seqs)
+        for r in range(0, seq.numel(), block.shape[0]):
+            part = slice(r, min(r + block.shape[0], seq.numel()))
+            ops.kv_store_q4(block[:part.stop - r], cache, seq[part], pos[part])
+        if attend:
+            qkv = (torch.randn((seqs, 3 * 768), device=dev) * 0.125).to(bf)
+            lengths = torch.full((seqs,), length, dtype=torch.int32, device=dev)
+            out = torch.empty((seqs, 768), device=dev, dtype=bf)
+            ms = _time(lambda: ops.decode_attention_q4(qkv, cache, lengths, out=out), args.repeats, args.warmup)
+            nbytes = seqs * 12 * length * 72 + seqs * 2 * 768 * 2
+            result.update(seqs=seqs, capacity=args.capacity, length=length)
+        else:
+            rows = block.shape[0]
+            ms = _time(lambda: ops.kv_store_q4(block, cache, seq[:rows], pos[:rows]), args.repeats, args.warmup)
+            nbytes = rows * 12 * (2 * 64 * 2 + 72)
+            result.update(rows=rows)
+        result.update(ms=ms, bytes=nbytes, gbs=nbytes / ms / 1e6)
+    elif args.kernel == "token_logprobs":
+        logits = torch.randn((args.rows, args.vocab), device=dev).to(getattr(torch, args.logits))
+        ids = torch.zeros(args.rows, dtype=torch.int32, device=dev)
+        ms = _time(lambda: ops.token_logprobs(logits, ids, top=args.top), args.repeats, args.warmup)
+        nbytes = logits.numel() * logits.element_size() + args.rows * (12 + 8 * args.top)
+        result.update(rows=args.rows, vocab=args.vocab, logits=args.logits, top=args.top, ms=ms, bytes=nbytes,
+                      gbs=nbytes / ms / 1e6)
+    elif args.kernel == "gemm_f32":
+        a = torch.randn((args.m, args.k), device=dev).to(bf)
+        w = (torch.randn((args.n, args.k), device=dev) * 0.05).to(bf)
+        out = ops.gemm_f32(a, w)
+        ms = _time(lambda: ops.gemm_f32(a, w, out=out), args.repeats, args.warmup)
+        result.update(m=args.m, n=args.n, k=args.k, ms=ms, tflops=2.0 * args.m * args.n * args.k / ms / 1e9,
+                      gbs=(2 * args.k * (args.m + args.n) + 4 * args.m * args.n) / ms / 1e6)
     elif args.kernel == "prefill_attention":
         rows = args.seqs * args.tokens
         qkv = torch.randn((rows, 3 * 768), device=dev).to(bf)

@@ -52,41 +52,40 @@ def _check(t: torch.Tensor, dtype: torch.dtype, name: str) -> None:
         raise ValueError(f"{name} must be contiguous")
 
 
-def _check_rows(t: torch.Tensor, dtype: torch.dtype, name: str) -> None:
-    """A matrix whose rows are contiguous, at any row stride."""
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor: the B200 kernels have no CPU path")
-    if t.dtype != dtype:
+def _operand(t: torch.Tensor, dtype: torch.dtype, name: str, device: int) -> None:
+    """A contiguous operand on the call's device (its number, as get_device gives it)."""
+    if t.dtype is dtype and t.get_device() == device and t.is_contiguous():
+        return
+    _check(t, dtype, name)
+    raise ValueError(f"{name} is on {t.device}, the call's first operand on cuda:{device}")
+
+
+def _matrix(t: torch.Tensor, dtype: torch.dtype, name: str, device: int | None = None) -> tuple[int, int, int, int]:
+    """(rows, columns, row stride, device) of a matrix whose rows are contiguous, at any row stride; a single row's own
+    stride means nothing. Without `device` the matrix is the call's first operand."""
+    if t.dtype is not dtype or not t.is_cuda:
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor: the B200 kernels have no CPU path")
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
     if t.dim() == 2:
         rows, width = t.shape
         step, unit = t.stride()
         if (unit == 1 or width == 1) and (step >= width or rows == 1):
-            return
+            on = t.get_device()
+            if device is not None and on != device:
+                raise ValueError(f"{name} is on {t.device}, the call's first operand on cuda:{device}")
+            return rows, width, step if rows != 1 else (width + 7) // 8 * 8, on
     raise ValueError(f"{name} must be a matrix of contiguous rows that do not overlap")
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    """Elements from row to row of a matrix that _check_rows accepts (a single row's own stride means nothing)."""
-    return t.stride(0) if t.shape[0] != 1 else (t.shape[1] + 7) // 8 * 8
-
-
-def _check_devices(first: torch.Tensor, **others: torch.Tensor | None) -> None:
-    device = first.get_device()
-    for name, t in others.items():
-        if t is not None and t.get_device() != device:
-            raise ValueError(f"{name} is on {t.device}, the call's first operand on {first.device}")
 
 
 _ENTRIES: dict[str, object] = {}
 
 
-def _launch_at(t: torch.Tensor, name: str, *args) -> None:
-    """_launch on the current stream of `t`'s device, which need not be the current device."""
+def _launch_at(device: int, name: str, *args) -> None:
+    """_launch on the current stream of `device`, which need not be the current device."""
     entry = _ENTRIES.get(name)
     if entry is None:
         entry = _ENTRIES[name] = getattr(_lib.load(), name)
-    device = t.get_device()
     if device == torch._C._cuda_getDevice():
         status = entry(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
@@ -123,19 +122,19 @@ def gemm_f32(a: torch.Tensor, w_t: torch.Tensor, *, out: torch.Tensor | None = N
     """out[M, N] = a[M, K] @ w_t[N, K]^T in FP32, the accumulators unrounded (an LM head's logits). `out` may have a
     row stride of its own, a multiple of 8; without it the rows are padded to one and the view of N columns returned."""
     _check(a, torch.bfloat16, "a")
-    _check(w_t, torch.bfloat16, "w_t")
+    device = a.get_device()
+    _operand(w_t, torch.bfloat16, "w_t", device)
     m, k = a.shape
     n = w_t.shape[0]
     if w_t.shape[1] != k:
         raise ValueError(f"inner dimensions differ: a {tuple(a.shape)}, w_t {tuple(w_t.shape)}")
     if out is None:
         out = a.new_empty((m, (n + 7) // 8 * 8), dtype=torch.float32)[:, :n]
-    _check_rows(out, torch.float32, "out")
-    if out.shape != (m, n):
+    out_rows, out_columns, stride, _ = _matrix(out, torch.float32, "out", device)
+    if out_rows != m or out_columns != n:
         raise ValueError(f"out must be {(m, n)}, got {tuple(out.shape)}")
-    _check_devices(a, w_t=w_t, out=out)
-    _launch_at(a, "tempo_gemm", a.data_ptr(), k, w_t.data_ptr(), k, None, None, n, out.data_ptr(), _row_stride(out), m,
-               n, k, _lib.GEMM_F32, None, None)
+    _launch_at(device, "tempo_gemm", a.data_ptr(), k, w_t.data_ptr(), k, None, None, n, out.data_ptr(), stride, m, n, k,
+               _lib.GEMM_F32, None, None)
     return out
 
 
@@ -371,9 +370,11 @@ def kv_cache_q4(seqs: int, kv_heads: int, capacity: int, head: int = 64, *,
     return torch.zeros((seqs, kv_heads, tiles, _lib.Q4_BLOCK_BYTES * head // 64), dtype=torch.uint8, device=device)
 
 
-def _q4_shape(cache: torch.Tensor) -> tuple[int, int, int, int]:
+def _q4_shape(cache: torch.Tensor, device: int) -> tuple[int, int, int, int]:
     """(seqs, kv_heads, head, capacity) of a 4-bit cache."""
-    _check(cache, torch.uint8, "cache")
+    _operand(cache, torch.uint8, "cache", device)
+    if device < 0:
+        raise ValueError("cache must be a CUDA tensor: the B200 kernels have no CPU path")
     if cache.dim() == 4:
         seqs, kv_heads, tiles, size = cache.shape
         if size == _lib.Q4_BLOCK_BYTES or size == 2 * _lib.Q4_BLOCK_BYTES:
@@ -382,9 +383,9 @@ def _q4_shape(cache: torch.Tensor) -> tuple[int, int, int, int]:
                      f"{tuple(cache.shape)}")
 
 
-def _check_places(rows: int, seq_of: torch.Tensor, pos_of: torch.Tensor) -> None:
-    _check(seq_of, torch.int32, "seq_of")
-    _check(pos_of, torch.int32, "pos_of")
+def _places(rows: int, seq_of: torch.Tensor, pos_of: torch.Tensor, device: int) -> None:
+    _operand(seq_of, torch.int32, "seq_of", device)
+    _operand(pos_of, torch.int32, "pos_of", device)
     if seq_of.numel() != rows or pos_of.numel() != rows:
         raise ValueError(f"{rows} rows need as many sequences and positions, got {seq_of.numel()} and {pos_of.numel()}")
 
@@ -393,15 +394,13 @@ def kv_store_q4(qkv: torch.Tensor, cache: torch.Tensor, seq_of: torch.Tensor, po
     """kv_store into a 4-bit cache: the key and value columns of row r of qkv ([rows, (heads + 2 kv_heads) * head],
     at any row stride that is a multiple of 8; no query columns are needed) quantised into sequence seq_of[r] at
     position pos_of[r]. Rows outside the cache are skipped; the others must name different places."""
-    seqs, kv_heads, head, capacity = _q4_shape(cache)
-    _check_rows(qkv, torch.bfloat16, "qkv")
-    rows, width = qkv.shape
+    rows, width, stride, device = _matrix(qkv, torch.bfloat16, "qkv")
+    seqs, kv_heads, head, capacity = _q4_shape(cache, device)
     heads = width // head - 2 * kv_heads
     if width % head or heads < 0:
         raise ValueError(f"qkv rows of {width} are not query, key and value heads of {head} ({kv_heads} key heads)")
-    _check_places(rows, seq_of, pos_of)
-    _check_devices(qkv, cache=cache, seq_of=seq_of, pos_of=pos_of)
-    _launch_at(qkv, "tempo_kv_store_q4", qkv.data_ptr(), _row_stride(qkv), cache.data_ptr(), seq_of.data_ptr(),
+    _places(rows, seq_of, pos_of, device)
+    _launch_at(device, "tempo_kv_store_q4", qkv.data_ptr(), stride, cache.data_ptr(), seq_of.data_ptr(),
                pos_of.data_ptr(), rows, seqs, heads, kv_heads, head, capacity)
 
 
@@ -409,17 +408,18 @@ def kv_load_q4(cache: torch.Tensor, seq_of: torch.Tensor, pos_of: torch.Tensor, 
                out: torch.Tensor | None = None) -> torch.Tensor:
     """The keys and values a 4-bit cache holds at the given places, [rows, 2 kv_heads * head] BF16 (kv_store_q4 takes
     them back). Places outside the cache give zeros."""
-    seqs, kv_heads, head, capacity = _q4_shape(cache)
-    rows = pos_of.numel()
-    _check_places(rows, seq_of, pos_of)
+    device = cache.get_device()
+    seqs, kv_heads, head, capacity = _q4_shape(cache, device)
+    rows, width = pos_of.numel(), 2 * kv_heads * head
+    _places(rows, seq_of, pos_of, device)
+    stride = width
     if out is None:
-        out = cache.new_empty((rows, 2 * kv_heads * head), dtype=torch.bfloat16)
+        out = cache.new_empty((rows, width), dtype=torch.bfloat16)
     else:
-        _check_rows(out, torch.bfloat16, "out")
-        if out.shape != (rows, 2 * kv_heads * head):
-            raise ValueError(f"out must be {(rows, 2 * kv_heads * head)}, got {tuple(out.shape)}")
-    _check_devices(cache, seq_of=seq_of, pos_of=pos_of, out=out)
-    _launch_at(cache, "tempo_kv_load_q4", cache.data_ptr(), out.data_ptr(), _row_stride(out), seq_of.data_ptr(),
+        out_rows, out_width, stride, _ = _matrix(out, torch.bfloat16, "out", device)
+        if out_rows != rows or out_width != width:
+            raise ValueError(f"out must be {(rows, width)}, got {tuple(out.shape)}")
+    _launch_at(device, "tempo_kv_load_q4", cache.data_ptr(), out.data_ptr(), stride, seq_of.data_ptr(),
                pos_of.data_ptr(), rows, seqs, kv_heads, head, capacity)
     return out
 
@@ -437,30 +437,26 @@ def decode_attention_q4(qkv: torch.Tensor, cache: torch.Tensor, lengths: torch.T
     """decode_attention over a 4-bit cache: the query columns of row s of qkv (scaled by 1/sqrt(head)) over the first
     lengths[s] + length_offset positions of sequence s; a sequence without positions gives zeros. The row holds query,
     key and value heads, unless `heads` says how many query heads it begins with."""
-    seqs, kv_heads, head, capacity = _q4_shape(cache)
-    _check_rows(qkv, torch.bfloat16, "qkv")
-    _check(lengths, torch.int32, "lengths")
-    width = qkv.shape[1]
+    rows, width, stride, device = _matrix(qkv, torch.bfloat16, "qkv")
+    seqs, kv_heads, head, capacity = _q4_shape(cache, device)
+    _operand(lengths, torch.int32, "lengths", device)
     if heads is None:
         heads = width // head - 2 * kv_heads
     if width % head or heads <= 0 or heads % kv_heads or heads * head > width:
         raise ValueError(f"qkv rows of {width} do not begin with {heads} query heads of {head}, a multiple of "
                          f"{kv_heads} key heads")
-    if qkv.shape[0] != seqs or lengths.numel() != seqs:
-        raise ValueError(f"{seqs} sequences need a query row and a length each, got {qkv.shape[0]} and "
-                         f"{lengths.numel()}")
+    if rows != seqs or lengths.numel() != seqs:
+        raise ValueError(f"{seqs} sequences need a query row and a length each, got {rows} and {lengths.numel()}")
     if out is None:
         out = qkv.new_empty((seqs, heads * head))
     else:
-        _check(out, torch.bfloat16, "out")
+        _operand(out, torch.bfloat16, "out", device)
         if out.shape != (seqs, heads * head):
             raise ValueError(f"out must be {(seqs, heads * head)}, got {tuple(out.shape)}")
-    _check_devices(qkv, cache=cache, lengths=lengths, out=out)
     size = decode_attention_q4_workspace_bytes(seqs, heads, kv_heads, head, capacity)
     workspace = qkv.new_empty(size, dtype=torch.uint8) if size else None
-    _launch_at(qkv, "tempo_decode_attention_q4", qkv.data_ptr(), _row_stride(qkv), cache.data_ptr(),
-               lengths.data_ptr(), length_offset, out.data_ptr(), seqs, heads, kv_heads, head, capacity,
-               _ptr(workspace), size)
+    _launch_at(device, "tempo_decode_attention_q4", qkv.data_ptr(), stride, cache.data_ptr(), lengths.data_ptr(),
+               length_offset, out.data_ptr(), seqs, heads, kv_heads, head, capacity, _ptr(workspace), size)
     return out
 
 
@@ -483,13 +479,12 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, *, top: int = 0, out
     (a padded row) scores 0; include/tempo_b200.h says what infinities and NaN give. With `slots` (int32, one a row)
     the tensors of `out` have a leading dimension, and row r's results go to its index slots[r] + slot_offset, or
     nowhere when that is outside: one captured call serves every step."""
-    bf16 = logits.dtype == torch.bfloat16
-    _check_rows(logits, torch.bfloat16 if bf16 else torch.float32, "logits")
-    _check(ids, torch.int32, "ids")
-    rows, vocab = logits.shape
+    bf16 = logits.dtype is torch.bfloat16
+    rows, vocab, stride, device = _matrix(logits, torch.bfloat16 if bf16 else torch.float32, "logits")
+    _operand(ids, torch.int32, "ids", device)
     if ids.numel() != rows:
         raise ValueError(f"{rows} rows need as many ids, got {ids.numel()}")
-    if not 0 <= top <= min(32, vocab):
+    if top and not 0 < top <= min(32, vocab):
         raise ValueError(f"top must be in [0, {min(32, vocab)}], got {top}")
     blocks = 0
     if out is None:
@@ -507,7 +502,7 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, *, top: int = 0, out
     else:
         lead = ()
         if slots is not None:
-            _check(slots, torch.int32, "slots")
+            _operand(slots, torch.int32, "slots", device)
             if slots.numel() != rows:
                 raise ValueError(f"{rows} rows need as many slots, got {slots.numel()}")
             blocks = out.logprob.shape[0]
@@ -520,15 +515,12 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, *, top: int = 0, out
                 continue
             if t is None:
                 raise ValueError(f"out.{name} is needed for {top} alternatives")
-            _check(t, dtype, f"out.{name}")
+            _operand(t, dtype, f"out.{name}", device)
             if t.shape != shape:
                 raise ValueError(f"out.{name} must be {shape}, got {tuple(t.shape)}")
-        _check_devices(logits, logprob=out.logprob, entropy=out.entropy, top_logprob=out.top_logprob,
-                       top_ids=out.top_ids, slots=slots)
-    _check_devices(logits, ids=ids)
-    _launch_at(logits, "tempo_token_logprobs", logits.data_ptr(), _row_stride(logits), int(bf16), ids.data_ptr(), rows,
-               vocab, top, out.logprob.data_ptr(), out.entropy.data_ptr(), _ptr(out.top_logprob), _ptr(out.top_ids),
-               _ptr(slots), slot_offset, blocks)
+    _launch_at(device, "tempo_token_logprobs", logits.data_ptr(), stride, int(bf16), ids.data_ptr(), rows, vocab, top,
+               out.logprob.data_ptr(), out.entropy.data_ptr(), _ptr(out.top_logprob), _ptr(out.top_ids), _ptr(slots),
+               slot_offset, blocks)
     return out
 
 

@@ -329,6 +329,40 @@ def test_store_and_attention_in_one_graph_on_another_stream() -> None:
         assert torch.equal(out, want) and torch.equal(cache, eager_cache)
 
 
+def test_two_graphs_of_split_calls_at_once() -> None:
+    """Two captured calls that go through a workspace each, replayed on two streams at the same time."""
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(19)
+    states = []
+    for k in range(2):
+        cache = ops.kv_cache_q4(1, 2, 9000)
+        _fill(cache, rng)
+        qkv = (_rows(rng, 1, 6, 64) * 0.2).reshape(1, -1)
+        lengths = _i32([8000 + k])
+        assert ops.decode_attention_q4_workspace_bytes(1, 6, 2, 64, cache.shape[2] * 16) > 0
+        want = ops.decode_attention_q4(qkv, cache, lengths, heads=6)
+        stream, out = torch.cuda.Stream(), torch.zeros_like(want)
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            ops.decode_attention_q4(qkv, cache, lengths, heads=6, out=out)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                for _ in range(4):
+                    ops.decode_attention_q4(qkv, cache, lengths, heads=6, out=out)
+        states.append((stream, graph, out, want, (qkv, cache, lengths)))
+    torch.cuda.synchronize()
+    for _, _, out, _, _ in states:
+        out.zero_()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for stream, graph, _, _, _ in states:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, _, out, want, _ in states:
+        assert torch.equal(out, want)
+
+
 def test_the_same_inputs_give_the_same_bits() -> None:
     from tempo_compiler_b200 import ops
     rng = np.random.default_rng(18)
@@ -339,3 +373,38 @@ def test_the_same_inputs_give_the_same_bits() -> None:
     first = ops.decode_attention_q4(qkv, cache, lengths, heads=8)
     for _ in range(5):
         assert torch.equal(ops.decode_attention_q4(qkv, cache, lengths, heads=8), first)
+
+
+def test_the_wrappers_refuse_what_does_not_fit() -> None:
+    from tempo_compiler_b200 import ops
+    cache = ops.kv_cache_q4(2, 3, 32)
+    qkv = torch.zeros((2, 9 * 64), dtype=torch.bfloat16, device="cuda")
+    two, three = _i32([0, 1]), _i32([0, 1, 2])
+    out = torch.zeros((2, 192), dtype=torch.bfloat16, device="cuda")
+    cases = [
+        (lambda: ops.kv_store_q4(qkv.float(), cache, two, two), "bfloat16"),
+        (lambda: ops.kv_store_q4(qkv[:, :500], cache, two, two), "heads of 64"),
+        (lambda: ops.kv_store_q4(qkv[:, :320], cache, two, two), "heads of 64"),
+        (lambda: ops.kv_store_q4(qkv, cache, three, two), "as many"),
+        (lambda: ops.kv_store_q4(qkv, cache, two.long(), two), "int32"),
+        (lambda: ops.kv_store_q4(qkv, cache.view(2, 3, 1, 2304)[..., :1000], two, two), "contiguous"),
+        (lambda: ops.kv_store_q4(qkv, cache.view(2, 3, -1), two, two), "kv_cache_q4"),
+        (lambda: ops.kv_store_q4(qkv.T.contiguous().T, cache, two, two), "contiguous rows"),
+        (lambda: ops.kv_store_q4(qkv[:1].expand(2, -1), cache, two, two), "overlap"),
+        (lambda: ops.kv_store_q4(qkv[:0], cache, two[:0], two[:0]), "rows 0"),
+        (lambda: ops.kv_store_q4(qkv.view(-1)[4:4 + 2 * 512].view(2, 512)[:, :384], cache, two, two), "aligned"),
+        (lambda: ops.kv_load_q4(cache, two, three), "as many"),
+        (lambda: ops.kv_load_q4(cache, two, two, out=out), "out must be"),
+        (lambda: ops.decode_attention_q4(qkv, cache, three), "a length each"),
+        (lambda: ops.decode_attention_q4(qkv[:1], cache, two), "a length each"),
+        (lambda: ops.decode_attention_q4(qkv, cache, two, heads=4), "multiple of"),
+        (lambda: ops.decode_attention_q4(qkv, cache, two, heads=12), "query heads"),
+        (lambda: ops.decode_attention_q4(qkv[:, :384], cache, two), "query heads"),
+        (lambda: ops.decode_attention_q4(qkv, cache, two, out=out[:, :128]), "contiguous"),
+        (lambda: ops.decode_attention_q4(qkv, cache, two, out=out[:1]), "out must be"),
+        (lambda: ops.decode_attention_q4(qkv, cache, two.cpu()), "CUDA"),
+        (lambda: ops.decode_attention_q4(qkv, cache.cpu(), two), "CUDA"),
+    ]
+    for call, words in cases:
+        with pytest.raises(ValueError, match=words):
+            call()

@@ -284,3 +284,36 @@ def test_head_and_scores_together() -> None:
     ops.gemm_argmax(hidden, table, part_val, part_idx)
     ops.argmax_finish(part_val, part_idx, picked)
     assert torch.equal(picked, scores.top_ids[:, 0])
+
+
+def test_the_wrappers_refuse_what_does_not_fit() -> None:
+    from tempo_compiler_b200 import ops
+    logits, ids = torch.zeros((3, 40), device="cuda"), _i32([0, 1, 2])
+    good = ops.token_logprobs(logits, ids, top=2)
+    wide = ops.TokenScores(*(t[None].repeat(2, *[1] * t.dim()) for t in good))
+    a, w = (torch.zeros((4, 64), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    cases = [
+        (lambda: ops.token_logprobs(logits.half(), ids), "float32"),
+        (lambda: ops.token_logprobs(logits, ids[:2]), "as many ids"),
+        (lambda: ops.token_logprobs(logits, ids.long()), "int32"),
+        (lambda: ops.token_logprobs(logits, ids, top=33), "top"),
+        (lambda: ops.token_logprobs(logits, ids, top=-1), "top"),
+        (lambda: ops.token_logprobs(logits[:, :5], ids, top=6), "top"),
+        (lambda: ops.token_logprobs(logits.T, ids), "contiguous rows|as many"),
+        (lambda: ops.token_logprobs(logits[:1].expand(3, -1), ids), "overlap"),
+        (lambda: ops.token_logprobs(logits[:0], ids[:0]), "rows 0"),
+        (lambda: ops.token_logprobs(logits, ids, top=3, out=good), "must be"),
+        (lambda: ops.token_logprobs(logits, ids, top=2, out=good._replace(top_ids=None)), "needed"),
+        (lambda: ops.token_logprobs(logits, ids, top=2, out=good._replace(entropy=good.entropy.double())), "float32"),
+        (lambda: ops.token_logprobs(logits, ids, slots=ids), "outputs"),
+        (lambda: ops.token_logprobs(logits, ids, top=2, out=good, slots=ids), "must be"),
+        (lambda: ops.token_logprobs(logits, ids, top=2, out=wide, slots=ids[:2]), "as many slots"),
+        (lambda: ops.gemm_f32(a, w.float()), "bfloat16"),
+        (lambda: ops.gemm_f32(a, w[:, :32].contiguous()), "inner"),
+        (lambda: ops.gemm_f32(a, w, out=torch.zeros((4, 5), device="cuda")), "out must be"),
+        (lambda: ops.gemm_f32(a, w, out=torch.zeros((4, 5), device="cuda")[:, :4]), "row stride"),
+        (lambda: ops.gemm_f32(a, w, out=torch.zeros((4, 12), device="cuda")[:, 1:5]), "aligned"),
+    ]
+    for call, words in cases:
+        with pytest.raises(ValueError, match=words):
+            call()
