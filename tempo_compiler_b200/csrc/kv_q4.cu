@@ -18,8 +18,8 @@ TEMPO_WATCHDOG_READER(watchdog_kv_q4)
 
 namespace {
 
-constexpr uint32_t kStoreThreads = 256;
-constexpr uint32_t kUnitLanes = 4;  // lanes that share one row of 64 dimensions, 16 each
+constexpr uint32_t kStoreThreads = 128;
+constexpr uint32_t kUnitLanes = 4;  // lanes that share a position's 64 dimensions of one key / value head, 16 each
 
 // Division by a number known at launch: n / d = (mulhi(n, mul) + n) >> shift for n < 2^31.
 struct Divisor {
@@ -39,37 +39,42 @@ struct Q4Rows {
   const int32_t* seq_of;
   const int32_t* pos_of;
   uint32_t ld, count, seqs, kv_heads, tiles;
-  Divisor per_row;      // units of a row: 2 * kv_heads * groups
+  Divisor per_row;      // units of a row: kv_heads * groups
   uint32_t units_a_row;
 };
 
-// A unit: a row's 64 dimensions (columns 64 `column` on of row `row`) and where they are kept. Eight consecutive units, a
-// warp's, are the same column of eight rows: of a prompt, 256 bytes of codes side by side.
+// A unit: the 64 dimensions of a row's key and of its value that one block holds (group `of` of the row's key groups: the
+// key's columns 64 `of` on, the value's 64 (units_a_row + of) on) and where they are kept. Eight consecutive units, a
+// warp's, are the same columns of eight rows: of a prompt, 256 bytes of codes side by side. (Key and value as two units
+// made the index arithmetic a third of the instructions: 116 us for 65536 rows of 12 heads stored and read back instead
+// of 102.)
 template <int G>
 struct Q4Unit {
-  uint32_t row, column, seq, pos, value;
+  uint32_t row, of, seq, pos;
   __device__ __forceinline__ Q4Unit(const Q4Rows& p, uint32_t unit) {
     const uint32_t eight = divide(unit >> 3, p.per_row);
-    column = (unit >> 3) - eight * p.units_a_row;
+    of = (unit >> 3) - eight * p.units_a_row;
     row = eight * 8 + (unit & 7u);
     seq = pos = 0;
     if (row < p.count) {
       seq = uint32_t(p.seq_of[row]);
       pos = uint32_t(p.pos_of[row]);
     }
-    value = column >= p.kv_heads * G ? 1u : 0u;
   }
   // The unit's block, or null when the place is outside the cache.
   __device__ __forceinline__ uint8_t* place(const Q4Rows& p) const {
-    const uint32_t of = column - value * p.kv_heads * G;
     if (seq >= p.seqs || pos >= p.tiles * kQ4Tile) return nullptr;
     return p.cache + q4_block(seq, of / G, pos, of % G, p.kv_heads, p.tiles, G);
   }
-  __device__ __forceinline__ uint2* codes(uint8_t* block) const {
-    return reinterpret_cast<uint2*>(block + value * kQ4Codes + pos % kQ4Tile * 32);
+  // Lane li's 16 dimensions of the key (0) or the value (1) in a row.
+  __device__ __forceinline__ uint4* columns(const Q4Rows& p, uint32_t value, uint32_t li) const {
+    return reinterpret_cast<uint4*>(p.rows + size_t(row) * p.ld + (value * p.units_a_row + of) * kQ4Group) + 2 * li;
   }
-  __device__ __forceinline__ uint32_t* meta(uint8_t* block) const {
-    return reinterpret_cast<uint32_t*>(block + 2 * kQ4Codes) + pos % kQ4Tile * 2 + value;
+  __device__ __forceinline__ uint2* codes(uint8_t* block, uint32_t value, uint32_t li) const {
+    return reinterpret_cast<uint2*>(block + value * kQ4Codes + pos % kQ4Tile * 32) + li;
+  }
+  __device__ __forceinline__ uint2* meta(uint8_t* block) const {
+    return reinterpret_cast<uint2*>(block + 2 * kQ4Codes) + pos % kQ4Tile;
   }
 };
 
@@ -98,8 +103,7 @@ __device__ __forceinline__ uint32_t pack_codes(float c0, float c1, float c2, flo
 // A row of values that are all equal has scale 0 and codes 0; one with a NaN, an infinity or a range that
 // passes FP32 has a scale that is not finite, and reads back as NaN. (A first form, eight lanes to a row with a 64-bit
 // index division, FP32 divisions and conversions, took 304 us for storing and reading 65536 rows of 12 heads.)
-__device__ __forceinline__ void store_unit(const uint4& a, const uint4& b, uint32_t mask, uint32_t li, uint2* codes,
-                                           uint32_t* meta) {
+__device__ __forceinline__ uint2 quantise(const uint4& a, const uint4& b, uint32_t mask, uint32_t& meta) {
   const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
   uint32_t most = w[0], least = w[0];
 #pragma unroll
@@ -137,12 +141,11 @@ __device__ __forceinline__ void store_unit(const uint4& a, const uint4& b, uint3
       c[i] = scale > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(x - low, scale)), 0.f), 15.f) : 0.f;
     }
   }
-  if (codes == nullptr) return;
+  meta = pack_bf16x2(scale, finite ? low : 0.f);
   uint2 word;
   word.x = __byte_perm(pack_codes(c[0], c[1], c[2], c[3]), pack_codes(c[4], c[5], c[6], c[7]), 0x5410);
   word.y = __byte_perm(pack_codes(c[8], c[9], c[10], c[11]), pack_codes(c[12], c[13], c[14], c[15]), 0x5410);
-  codes[li] = word;
-  if (li == 0) *meta = pack_bf16x2(scale, finite ? low : 0.f);
+  return word;
 }
 
 template <int G>
@@ -153,10 +156,16 @@ __global__ void __launch_bounds__(kStoreThreads) kv_store_q4_kernel(Q4Rows p) {
   const Q4Unit<G> unit(p, (blockIdx.x * kStoreThreads + threadIdx.x) / kUnitLanes);
   if (unit.row >= p.count) return;  // whole units leave together
   // The row is on its way before its place is known; a place outside the cache only keeps it from being stored.
-  const uint4* src = reinterpret_cast<const uint4*>(p.rows + size_t(unit.row) * p.ld + unit.column * kQ4Group) + 2 * li;
-  const uint4 a = src[0], b = src[1];
+  const uint4* key = unit.columns(p, 0, li);
+  const uint4* value = unit.columns(p, 1, li);
+  const uint4 k0 = key[0], k1 = key[1], v0 = value[0], v1 = value[1];
   uint8_t* block = unit.place(p);
-  store_unit(a, b, mask, li, block == nullptr ? nullptr : unit.codes(block), unit.meta(block));
+  uint2 meta;
+  const uint2 k = quantise(k0, k1, mask, meta.x), v = quantise(v0, v1, mask, meta.y);
+  if (block == nullptr) return;
+  *unit.codes(block, 0, li) = k;
+  *unit.codes(block, 1, li) = v;
+  if (li == 0) *unit.meta(block) = meta;
 }
 
 // The rows' keys and values back as BF16: code x scale + low in FP32, rounded once.
@@ -168,31 +177,35 @@ __global__ void __launch_bounds__(kStoreThreads) kv_load_q4_kernel(Q4Rows p) {
   const Q4Unit<G> unit(p, (blockIdx.x * kStoreThreads + threadIdx.x) / kUnitLanes);
   if (unit.row >= p.count) return;
   uint8_t* block = unit.place(p);
-  uint2 codes = make_uint2(0, 0);
-  uint32_t meta = 0;  // a place outside the cache: zeros
+  uint2 codes[2] = {make_uint2(0, 0), make_uint2(0, 0)}, meta = make_uint2(0, 0);  // a place outside the cache: zeros
   if (block != nullptr) {
-    codes = unit.codes(block)[li];
+    codes[0] = *unit.codes(block, 0, li);
+    codes[1] = *unit.codes(block, 1, li);
     meta = *unit.meta(block);
   }
-  const float s = bf16_lo(meta), l = bf16_hi(meta);
-  uint32_t out[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t word = (i < 4 ? codes.x : codes.y) >> (8 * (i % 4));
-    // a code under the exponent of 2^23 is the float 2^23 + code
-    const float c0 = __uint_as_float((word & 15u) | 0x4B000000u) - 8388608.f;
-    const float c1 = __uint_as_float(((word >> 4) & 15u) | 0x4B000000u) - 8388608.f;
-    out[i] = pack_bf16x2(fmaf(c0, s, l), fmaf(c1, s, l));
+  for (uint32_t value = 0; value < 2; ++value) {
+    const uint32_t words = value ? meta.y : meta.x;
+    const float s = bf16_lo(words), l = bf16_hi(words);
+    uint32_t out[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t word = (i < 4 ? codes[value].x : codes[value].y) >> (8 * (i % 4));
+      // a code under the exponent of 2^23 is the float 2^23 + code
+      const float c0 = __uint_as_float((word & 15u) | 0x4B000000u) - 8388608.f;
+      const float c1 = __uint_as_float(((word >> 4) & 15u) | 0x4B000000u) - 8388608.f;
+      out[i] = pack_bf16x2(fmaf(c0, s, l), fmaf(c1, s, l));
+    }
+    uint4* dst = unit.columns(p, value, li);
+    dst[0] = make_uint4(out[0], out[1], out[2], out[3]);
+    dst[1] = make_uint4(out[4], out[5], out[6], out[7]);
   }
-  uint4* dst = reinterpret_cast<uint4*>(p.rows + size_t(unit.row) * p.ld + unit.column * kQ4Group) + 2 * li;
-  dst[0] = make_uint4(out[0], out[1], out[2], out[3]);
-  dst[1] = make_uint4(out[4], out[5], out[6], out[7]);
 }
 
 // Launches `kernel` over `rows` rows, in as many calls as 31-bit thread numbers need.
 tempo_status launch_rows(void (*kernel)(Q4Rows), Q4Rows p, uint32_t rows, uint32_t groups, cudaStream_t stream,
                          const char* name) {
-  p.units_a_row = 2 * p.kv_heads * groups;
+  p.units_a_row = p.kv_heads * groups;
   p.per_row = divisor(p.units_a_row);
   const uint32_t most = 0x7FFFFF00u / (8 * kUnitLanes * p.units_a_row) * 8;
   for (uint32_t done = 0; done < rows;) {
