@@ -256,7 +256,7 @@ constexpr uint32_t kQ4Queries = 8;
 constexpr uint32_t kQ4Piece = 4 * kQ4Block;  // bytes of one bulk copy: four tiles of a 64-wide head, two of a 128-wide
 constexpr uint32_t kRing = 2;
 constexpr float kSlack = 6.f;
-constexpr float kNoScore = -1e30f;  // the reference before any position: e^(anything - it) of an absent one is 0
+constexpr float kNoScore = -3.4028235e38f;  // the reference before any position: no finite score is below it
 
 template <int G, int WARPS>
 struct Q4Smem {

@@ -244,6 +244,26 @@ def test_scores_that_rise_and_fall_along_the_keys() -> None:
     _check_attention(qkv, cache, [n, n], 1, got)
 
 
+@pytest.mark.parametrize("rising", [False, True])
+@pytest.mark.parametrize("n", [1, 16, 300, 9000])
+def test_scores_far_below_zero(n: int, rising: bool) -> None:
+    """Scores from -6e35 down: the least negative position takes all of the weight, and its value row is the output but
+    for the FP16 rounding of its weight, a few FP32 roundings of 64 + 15 steps, and the output's own."""
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(n)
+    cache = ops.kv_cache_q4(1, 1, n)
+    rows = _rows(rng, n, 2, 64).float()
+    factor = 1 + np.minimum(np.arange(n), 100).astype(np.float32) / 8
+    rows[:, 0] = -1e17 * torch.from_numpy(factor[::-1].copy() if rising else factor).cuda()[:, None]
+    rows = rows.to(torch.bfloat16).reshape(n, -1)
+    ops.kv_store_q4(rows, cache, _i32(np.zeros(n)), _i32(np.arange(n)))
+    qkv = torch.full((1, 64), 1e17, dtype=torch.bfloat16, device="cuda")
+    got = ops.decode_attention_q4(qkv, cache, _i32([n]), heads=1).double().cpu().numpy()[0]
+    codes, scale, low = _q4.quantise(rows[n - 1 if rising else 0, 64:].float().cpu().numpy())
+    want, wide = codes * scale + low, 15 * scale
+    assert (np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + (2.0 ** -11 + 2.0 ** -16) * wide).all()
+
+
 def test_a_nan_key_or_value_within_the_length_shows_in_its_own_head() -> None:
     from tempo_compiler_b200 import ops
     rng = np.random.default_rng(14)
