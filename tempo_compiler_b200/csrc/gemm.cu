@@ -75,7 +75,7 @@ struct RowMajorSmem {
   static constexpr uint32_t kABytes = 128 * kBK * 2;
   static constexpr uint32_t kBBytes = BN * kBK * 2;
   static constexpr uint32_t kStageBytes = kABytes + kBBytes;
-  // STAGED: one 32 x 32 staging tile (2 KB of BF16, 4 KB of FP32) per epilogue warp for TMA stores of the output.
+  // STAGED: one 2 KB staging tile per epilogue warp (32 x 32 BF16 or 32 x 16 FP32) for TMA stores of the output.
   static constexpr uint32_t kStagingOffset = STAGES * kStageBytes;
   static constexpr uint32_t kStagingTile = 2048u;
   static constexpr uint32_t kStagingBytes = STAGED ? 16u * kStagingTile : 0u;
@@ -134,7 +134,7 @@ __device__ __forceinline__ void store_f32(const CUtensorMap* map, const uint32_t
   }
 }
 
-// The FP32 columns n0 .. n - 1 of one row, fewer than a staging tile's 32, by plain stores: a TMA store clips at 16-byte
+// The FP32 columns n0 .. n - 1 of one row, fewer than 32, by plain stores: a TMA store clips at 16-byte
 // steps and would overwrite up to three columns behind the row, which may be the caller's.
 __device__ __forceinline__ void store_f32_tail(const RowMajorParams& p, const uint32_t (&r)[32], uint32_t row,
                                                uint32_t n0) {
@@ -1283,7 +1283,7 @@ struct PairSmem {
   static constexpr uint32_t kABytes = 128 * kBK * 2;
   static constexpr uint32_t kBBytes = 128 * kBK * 2;
   static constexpr uint32_t kStageBytes = kABytes + kBBytes;
-  // One 32 x 32 staging tile (2 KB of BF16, 4 KB of FP32) per epilogue warp for the output's TMA stores.
+  // One 2 KB staging tile per epilogue warp (32 x 32 BF16 or 32 x 16 FP32) for the output's TMA stores.
   static constexpr uint32_t kStagingOffset = STAGES * kStageBytes;
   static constexpr uint32_t kStagingTile = 2048u;
   static constexpr uint32_t kStagingBytes = (kRowEpiThreads / 32) * kStagingTile;
