@@ -312,8 +312,7 @@ tempo_status tempo_decode_attention_q4(const void* q, uint32_t ldq, const void* 
  * element): logprob[r] = log softmax(logits[r])[ids[r]] (0 where ids[r] is outside [0, vocab): a row without a token),
  * entropy[r] = -sum p ln p, and, with 0 < top <= 32 and top <= vocab, the `top` greatest logits in descending order, ties
  * to the lower index, as top_ids / top_logprob [rows][top]. A logit of -infinity has probability 0. A row of nothing but
- * -infinity scores -infinity with entropy 0; a NaN, or a logit above 2e38, makes its row's scores NaN, and NaN ranks
- * first. With slot_of (NULL for none), the outputs hold `slots` blocks of `rows` rows and row r's results go to block
+ * -infinity scores -infinity with entropy 0; a NaN or +infinity makes its row's scores NaN, and NaN ranks first. With slot_of (NULL for none), the outputs hold `slots` blocks of `rows` rows and row r's results go to block
  * slot_of[r] + slot_offset, or nowhere when there is no such block: a captured decode step writes each step's results
  * behind the last's. */
 tempo_status tempo_token_logprobs(const void* logits, uint64_t ld, uint32_t bf16, const int32_t* ids, uint32_t rows,

@@ -11,7 +11,7 @@
 // and so have no ties) and sorts them by counting. A row with more
 // ties at the bar than the lists hold, or with a NaN, is searched exactly, at a slower pace. Few rows are split over the
 // CTAs of a cluster, whose sums and sorted candidates the first one merges. (Collecting candidates on the way, against
-// a threshold that rose with the row, took 230 us for 8192 BF16 rows of 50257 instead of 160.)
+// a threshold that rose with the row, took 230 us for 8192 BF16 rows of 50257 instead of 163.)
 
 #include <cuda_runtime.h>
 
@@ -217,9 +217,10 @@ __device__ __noinline__ void thin(Candidates& c, uint32_t top) {
 
 // A part of the row: l = sum 2^(y - m) and t = sum (y - m) 2^(y - m) over its logits in bits, y = x log2 e. One fused
 // multiply-add gives y - m, rounded once; m is whatever reference the products were taken against, so its own rounding
-// cancels. Logits at or below kDeep (masks of -infinity or of the type's lowest value) weigh nothing beside others; a
-// row of nothing else has l = 0 and is summed on its own.
-constexpr float kDeep = -1e30f;
+// cancels. That rounding grows with the logit, though, and 2^(y - m) with it. So logits at or below kDeep (masks) count
+// for nothing: floats above it lie at least 64 above, beside which they weigh e^-64; and a row whose reference is
+// beyond kLarge, or that has nothing above kDeep (l = 0), is summed again in plain units (plain_sums).
+constexpr float kDeep = -0x1p30f, kLarge = 0x1p24f;
 struct Sums {
   float m, l, t;
 };
@@ -323,9 +324,10 @@ __device__ __forceinline__ float add(Sums& s, const uint32_t (&w)[N]) {
   return most;
 }
 
-// A row of logits at or below kDeep by one CTA, in the plain units of the logits: d = x - greatest. Sums of e^d and d e^d.
+// A row's sums by one CTA in the plain units of the logits: d = x - greatest, the sums of e^d and d e^d (NaN when the row
+// holds a NaN or +infinity).
 template <typename T>
-__device__ __noinline__ Sums deep_sums(const T* row, uint32_t vocab, Sums* scratch) {
+__device__ __noinline__ Sums plain_sums(const T* row, uint32_t vocab, Sums* scratch) {
   Sums s{-INFINITY, 0.f, 0.f};
   for (uint32_t i = threadIdx.x; i < vocab; i += kThreads) s.m = fmaxf(s.m, Logits<T>::one(row + i));
 #pragma unroll
@@ -336,7 +338,7 @@ __device__ __noinline__ Sums deep_sums(const T* row, uint32_t vocab, Sums* scrat
   for (uint32_t w = 0; w < kWarps; ++w) s.m = fmaxf(s.m, scratch[w].m);
   if (s.m == -INFINITY) return s;
   for (uint32_t i = threadIdx.x; i < vocab; i += kThreads) {
-    const float d = fmaxf(Logits<T>::one(row + i) - s.m, -1000.f), e = fast_exp2(d * kLog2e);
+    const float below = Logits<T>::one(row + i) - s.m, d = below < -1000.f ? -1000.f : below, e = fast_exp2(d * kLog2e);
     s.l += e;
     s.t = fmaf(d, e, s.t);
   }
@@ -557,15 +559,15 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_logprobs_kernel(L
     s = cta_sums;
   }
 
-  const bool deep = s.l == 0.f;
-  if (deep) s = deep_sums<T>(row, p.vocab, warp_sums);  // (uniform: every thread has the row's sums)
-  const bool empty = deep && s.l == 0.f;
-  const float log_l = logf(s.l), unit = deep ? 1.f : kLn2;
+  const bool plain = s.l == 0.f || fabsf(s.m) > kLarge;
+  if (plain) s = plain_sums<T>(row, p.vocab, warp_sums);  // (uniform: every thread has the row's sums)
+  const bool empty = plain && s.l == 0.f;
+  const float log_l = logf(s.l), unit = plain ? 1.f : kLn2;
   auto log_probability = [&](float x) {
     if (empty) return -INFINITY;
-    if (deep) return x - s.m - log_l;
-    // (a masked logit in bits would overflow)
-    return x <= kDeep ? x - fmaf(s.m, kLn2, log_l) : fmaf(fmaf(x, kLog2e, -s.m), kLn2, -log_l);
+    if (plain) return x - s.m - log_l;
+    // (a logit of the type's lowest value would overflow in bits)
+    return x < -1e30f ? x - fmaf(s.m, kLn2, log_l) : fmaf(fmaf(x, kLog2e, -s.m), kLn2, -log_l);
   };
   uint64_t to = r;
   if (p.slot_of != nullptr) {

@@ -158,6 +158,32 @@ def test_masked_logits(dtype) -> None:
         _check(logits, ids, top, ops.token_logprobs(logits, _i32(ids), top=top))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [3001, 50257])
+@pytest.mark.parametrize("size", [1e6, 1e9, 1e10, 1e12, 1e20, 1e29, 1.5e38])
+def test_logits_of_any_size(dtype, vocab: int, size: float) -> None:
+    """Masks of any large negative value among ordinary logits, rows of nothing else, and rows of large positive logits."""
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(int(math.log2(size)))
+    logits = _logits(rng, 8, vocab, dtype)
+    logits[0, torch.from_numpy(rng.random(vocab) < 0.97).cuda()] = -size
+    logits[1, :vocab // 2] = -size            # before the others
+    logits[2, vocab // 2:] = -size            # behind them
+    logits[3] = -size                         # uniform
+    logits[4] = -size
+    logits[4, 500] = -size * 0.75             # one token takes all
+    logits[5, 77] = size
+    logits[6] = size
+    logits[6, ::2] = -size
+    logits[7, ::3] = size
+    logits[7, 1::3] = -math.inf
+    ids = np.array([vocab - 1, 0, vocab - 1, 9, 500, 78, 1, 3])
+    for top in (0, 5, 32):
+        _check(logits, ids, top, ops.token_logprobs(logits, _i32(ids), top=top))
+    many = logits.repeat(40, 1)               # a CTA to a row
+    _check(many, np.tile(ids, 40), 5, ops.token_logprobs(many, _i32(np.tile(ids, 40)), top=5))
+
+
 def test_nan_and_infinity() -> None:
     from tempo_compiler_b200 import ops
     rng = np.random.default_rng(5)
