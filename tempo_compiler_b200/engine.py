@@ -534,7 +534,10 @@ class Engine:
                              f"{tuple(ids.shape)}")
         if not 0 <= alternatives <= min(32, self.shape.vocab):
             raise ValueError(f"alternatives must be in [0, {min(32, self.shape.vocab)}], got {alternatives}")
-        host = torch.from_numpy(np.ascontiguousarray(ids, dtype=np.int32))
+        if ids.dtype.kind not in "iu":
+            raise ValueError(f"token ids must be integers, got {ids.dtype}")
+        # (an id that 32 bits do not hold is outside the vocabulary like any other)
+        host = torch.from_numpy(ids.astype(np.int64).clip(-1, self.shape.vocab).astype(np.int32))
         self.prompt_ids.view(self.batch, self.prompt).copy_(host)
         targets = torch.full((self.batch, self.prompt), -1, dtype=torch.int32, device=self.device)
         targets[:, :-1] = self.prompt_ids.view(self.batch, self.prompt)[:, 1:]

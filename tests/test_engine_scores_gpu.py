@@ -171,6 +171,17 @@ def test_padding_scores_zero(model) -> None:
     np.testing.assert_array_equal(padded.logprob[0], full.logprob[0])
 
 
+def test_ids_that_32_bits_do_not_hold_are_padding(model) -> None:
+    engine = _engine(model, 2, 10, 10)
+    ids = _ids(2, 10).astype(np.int64)
+    ids[1, 6:] = -1
+    want = engine.score(ids)
+    for far in (2 ** 32 + 5, -2 ** 32 + 5, 2 ** 62):
+        ids[1, 6:] = far
+        for a, b in zip(engine.score(ids), want):
+            np.testing.assert_array_equal(a, b)
+
+
 def test_refusals(model) -> None:
     for kwargs, word in ((dict(kv_bits=8), "kv_bits"), (dict(alternatives=33), "alternatives"),
                          (dict(alternatives=-1), "alternatives"), (dict(kv_bits=4, persistent_decode=True), "persistent"),
@@ -185,3 +196,5 @@ def test_refusals(model) -> None:
         engine.score(_ids(2, 8), alternatives=40)
     with pytest.raises(RuntimeError, match="scores"):
         engine.scores()
+    with pytest.raises(ValueError, match="integers"):
+        engine.score(_ids(2, 8).astype(np.float32))
