@@ -744,15 +744,16 @@ __global__ void __launch_bounds__(32 * WARPS) decode_attention_q4_kernel(Q4Atten
 }
 
 // One CTA per (sequence, query head): the partial results of `chunks` CTAs, summed in a fixed order. kMergeThreads / 64 G
-// threads share a dimension, so a long row of partials is a few loads deep.
-constexpr uint32_t kMergeThreads = 512;
+// threads share a dimension, and each has kMergeBatch values on their way at once, the first of them while the references
+// are compared. (A loop that loaded the last few of them one after the other cost up to 2 us.)
+constexpr uint32_t kMergeThreads = 512, kMergeBatch = 8;
 static_assert(kQ4MaxSplits <= kMergeThreads, "a thread for each partial result");
 
 template <int G>
 __global__ void __launch_bounds__(kMergeThreads) decode_merge_q4_kernel(Q4Attention p, uint32_t chunks, uint32_t rp) {
   using L = Q4Smem<G, 4>;
   constexpr uint32_t kWidth = 64 * G, kShares = kMergeThreads / kWidth, kPart = L::kPart / 4;
-  __shared__ float factor[kQ4MaxSplits];
+  __shared__ float factor[(kQ4MaxSplits + kMergeBatch * kShares - 1) / (kMergeBatch * kShares) * (kMergeBatch * kShares)];
   __shared__ float warp_m[kMergeThreads / 32], warp_l[kMergeThreads / 32];
   __shared__ float sums[kShares][kWidth];
   pdl_wait();
@@ -760,6 +761,17 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_q4_kernel(Q4Attent
   const uint32_t share = p.share, h = blockIdx.x, s = blockIdx.y;
   const uint32_t kvh = h / share, block = h % share / rp, query = h % share % rp;
   const float* parts = p.parts + size_t((s * p.kv_heads + kvh) * p.blocks + block) * chunks * kPart;
+  const uint32_t at = threadIdx.x % kWidth, part = threadIdx.x / kWidth;
+  const float* values = parts + query * L::kStride + at;
+  float v[kMergeBatch];
+  auto load = [&](uint32_t from) {
+#pragma unroll
+    for (uint32_t i = 0; i < kMergeBatch; ++i) {
+      const uint32_t c = from + part + i * kShares;
+      v[i] = c < chunks ? values[c * kPart] : 0.f;
+    }
+  };
+  load(0);
   const bool has = threadIdx.x < chunks;
   const float m = has ? parts[threadIdx.x * kPart + L::kReferences + query] : kNoScore;
   const float part_l = has ? parts[threadIdx.x * kPart + L::kSums + query] : 0.f;
@@ -771,14 +783,15 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_q4_kernel(Q4Attent
 #pragma unroll
   for (uint32_t w = 0; w < kMergeThreads / 32; ++w) most = fmaxf(most, warp_m[w]);
   const float f = fast_exp2(m - most), l_warp = warp_sum(part_l * f);
-  if (has) factor[threadIdx.x] = f;
+  if (threadIdx.x < sizeof(factor) / 4) factor[threadIdx.x] = has ? f : 0.f;
   if (lane_id() == 0) warp_l[warp_id()] = l_warp;
   __syncthreads();
-  const uint32_t at = threadIdx.x % kWidth, part = threadIdx.x / kWidth;
-  const float* values = parts + query * L::kStride + at;
   float a = 0.f;
-#pragma unroll 8
-  for (uint32_t c = part; c < chunks; c += kShares) a = fmaf(values[c * kPart], factor[c], a);
+  for (uint32_t from = 0; from < chunks; from += kMergeBatch * kShares) {
+    if (from > 0) load(from);
+#pragma unroll
+    for (uint32_t i = 0; i < kMergeBatch; ++i) a = fmaf(v[i], factor[from + part + i * kShares], a);
+  }
   sums[part][at] = a;
   __syncthreads();
   if (threadIdx.x >= kWidth) return;
