@@ -250,7 +250,6 @@ tempo_status launch_rows(void (*kernel)(Q4Rows), Q4Rows p, uint32_t rows, uint32
 // and merge through distributed shared memory, or, when a pair needs more of them, through a workspace and a second kernel.
 // ---------------------------------------------------------------------------------------------------------------
 
-constexpr uint32_t kQ4MaxChunks = 16;    // CTAs of a cluster
 constexpr uint32_t kQ4MaxSplits = 160;   // CTAs that share a pair through the workspace
 constexpr uint32_t kQ4Queries = 8;
 constexpr uint32_t kQ4Piece = 4 * kQ4Block;  // bytes of one bulk copy: four tiles of a 64-wide head, two of a 128-wide
@@ -807,23 +806,30 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_q4_kernel(Q4Attent
 
 // How the positions of a pair (a sequence's key / value head and block of query heads) are shared out: CTAs of `warps`
 // warps, `chunks` of them to a pair, merged through a cluster's shared memory or, with `parts`, through the workspace.
-//
-// The kernel wants about 20 warps an SM, each with four tiles or more. Measured on a B200 (us; w warps, c CTAs, p through
-// the workspace): 12 pairs of 72 tiles w4c4 4.8, w8c1 5.7; 192 pairs of 72 w4c1 7.6, w4c4 8.6; 768 of 72 w4c1 17.4, w8c1 18.8,
-// w4c2 20.0; 96 of 256 w4c8 11.5, w4c4 12.9; 16 of 4096 (128-wide) w4c48p 43.0, w8c16 50.0, w4c16 60.5. From 20 pairs an SM
-// on a CTA's fixed cost (a few microseconds of latency) weighs more than its width: 6144 of 72 w2c1 91, w4c1 97, w4c2 128.
 struct Q4Split {
   uint32_t warps, chunks;
   bool parts;
 };
-Q4Split q4_split(uint64_t pairs, uint32_t tiles) {
-  const uint64_t sms = uint64_t(sm_count()), wanted = std::min<uint64_t>(20 * sms / pairs, tiles / 4);  // warps of a pair
-  if (wanted > 8 * kQ4MaxChunks) return Q4Split{4, uint32_t(std::min<uint64_t>(wanted / 4, kQ4MaxSplits)), true};
-  uint32_t warps = 4;  // the nearest power of two
-  while (2ull * warps * warps <= wanted * wanted) warps *= 2;
-  if (warps == 4) return Q4Split{pairs >= 20 * sms ? 2u : 4u, 1, false};
-  if (warps == 8) return Q4Split{8, 1, false};
-  return warps / 4 <= kQ4MaxChunks ? Q4Split{4, warps / 4, false} : Q4Split{8, kQ4MaxChunks, false};
+
+// CTAs of four warps that fit an SM: 128 registers a thread for heads of 128, else 80, or 96 for two and four queries.
+uint32_t q4_resident(uint32_t head, uint32_t rp) { return head == 128 ? 4 : rp == 2 || rp == 4 ? 5 : 6; }
+
+// Twice as many CTAs as fit the GPU (lengths differ, and a second round fills what the short ones leave), as long as each
+// has 12 tiles, and more where there are many pairs, whose CTAs hide one another's latency. Measured on a B200 over 456
+// grids of 1 to 768 pairs of 12 to 4096 tiles, at full and at ragged lengths, against every split of up to 148 CTAs: 3.5 %
+// behind the best one on average, 28 % at worst (clusters of up to 16 CTAs chosen by warps alone: 8.3 % and 90 %). us (w
+// warps, c CTAs, p through the workspace): 768 pairs of 72 w4c1 17.4, w8c1 18.8, w4c2 20.0; 96 of 256 w4c8 12.8, w4c1 16.4,
+// w8c16 28.5; 32 of 512 (128-wide) w4c16p 16.0, w4c8 18.8, w8c16 24.4; 16 of 4096 w4c64p 36.2, w4c16 47.1; 6144 of 72 w2c1
+// 91, w4c1 97 (a CTA's latency weighs more than its width there).
+Q4Split q4_split(uint64_t pairs, uint32_t tiles, uint32_t head, uint32_t rp) {
+  const uint64_t sms = uint64_t(sm_count());
+  const uint64_t chunks = std::min(2 * q4_resident(head, rp) * sms / pairs, tiles * sms / (12 * sms + 32 * pairs));
+  if (chunks < 3) return Q4Split{pairs >= 20 * sms ? 2u : pairs <= 3 * sms && tiles >= 16 ? 8u : 4u, 1, false};
+  if (chunks <= 12) return Q4Split{4, chunks < 6 ? 4u : 8u, false};
+  // whole pieces to each warp
+  const uint32_t most = uint32_t(std::min<uint64_t>(chunks, kQ4MaxSplits));
+  const uint32_t per = ((tiles + most - 1) / most + 15) / 16 * 16;
+  return Q4Split{4, (tiles + per - 1) / per, true};
 }
 
 template <int G, int RP, int WARPS>
@@ -833,10 +839,6 @@ tempo_status launch_attention_warps(const Q4Attention& base, uint32_t seqs, uint
   const bool cluster = chunks > 1 && p.parts == nullptr;
   const tempo_status status = set_smem(reinterpret_cast<const void*>(kernel), Q4Smem<G, WARPS>::bytes(true));
   if (status != TEMPO_OK) return status;
-  if (cluster && chunks > 8) {
-    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute(non-portable cluster size)");
-  }
   p.early = single_wave(uint64_t(p.kv_heads) * p.blocks * seqs * chunks, 16 / WARPS);
   return launch(kernel, dim3(chunks, p.kv_heads * p.blocks, seqs), dim3(32 * WARPS),
                 Q4Smem<G, WARPS>::bytes(cluster), stream,
@@ -864,7 +866,7 @@ uint32_t q4_queries(uint32_t head, uint32_t share) {
 uint64_t q4_workspace(uint32_t seqs, uint32_t heads, uint32_t kv_heads, uint32_t head, uint32_t capacity) {
   const uint32_t share = heads / kv_heads, rp = q4_queries(head, share);
   const uint64_t pairs = uint64_t(seqs) * kv_heads * ((share + rp - 1) / rp);
-  const Q4Split split = q4_split(pairs, capacity / kQ4Tile);
+  const Q4Split split = q4_split(pairs, capacity / kQ4Tile, head, rp);
   return split.parts ? pairs * split.chunks * (head == 64 ? Q4Smem<1, 4>::kPart : Q4Smem<2, 4>::kPart) : 0;
 }
 
@@ -984,7 +986,7 @@ extern "C" tempo_status tempo_decode_attention_q4(const void* q, uint32_t ldq, c
   p.tiles = capacity / kQ4Tile;
   p.length_offset = length_offset;
   p.blocks = (share + rp - 1) / rp;
-  const Q4Split split = q4_split(uint64_t(seqs) * kv_heads * p.blocks, p.tiles);
+  const Q4Split split = q4_split(uint64_t(seqs) * kv_heads * p.blocks, p.tiles, head, rp);
   float* parts = static_cast<float*>(workspace);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (head == 128) {
