@@ -234,7 +234,9 @@ tempo_status launch_rows(void (*kernel)(Q4Rows), Q4Rows p, uint32_t rows, uint32
 //   sum_j p_j v_j = sum_j w_j (64 + code_j) - 64 sum_j w_j + sum_j p_j low_j,   w_j = p_j scale_j.
 // What bounds the kernel is the logic pipe: a code pair costs one logic operation to mask and one to move, of which those
 // to the left are multiplications by 16 and run beside them (shifts for all of them, the keys as BF16 integers 128 +
-// code, took 91 us for 512 sequences of 12 heads and 1152 positions instead of 89.6).
+// code, took 91 us for 512 sequences of 12 heads and 1152 positions instead of 89.6; moves to the right as the high half
+// of a product, in place of the byte swaps, 104 instead of 85). The values come through the transposing matrix load,
+// which puts the same dimensions of two positions side by side (85 us; byte permutations for it took 89).
 // The eight columns of the B operand (m16n8k16) are query heads of one key / value head times tiles:
 // grouped heads read the cache once, and with few heads one softmax serves several tiles (the first tensor-core form, one tile
 // and eight columns of queries whether they existed or not, issued 309 instructions a tile and was bound by the ALU pipe).
@@ -260,15 +262,14 @@ constexpr float kNoScore = -3.4028235e38f;  // the reference before any position
 template <int G, int WARPS>
 struct Q4Smem {
   static constexpr uint32_t kWarpRing = kRing * kQ4Piece;
-  // A partial result of eight queries: 64 G values each (dimension 64 i + 8 g + n at 64 i + 8 n + g, eight words more to
+  // A partial result of eight queries: 64 G values each (dimension 64 i + 4 g + n at 64 i + 8 n + g, eight words more to
   // the next query: the lanes of a fragment store into different banks), then the references, then the sums.
   static constexpr uint32_t kStride = 64 * G + 8;
   static constexpr uint32_t kReferences = kQ4Queries * kStride, kSums = kReferences + kQ4Queries;
   static constexpr uint32_t kPart = (kSums + kQ4Queries) * 4;
   static constexpr uint32_t kBarrierOffset = WARPS * kWarpRing;
   static constexpr uint32_t kMergeOffset = kBarrierOffset + WARPS * kRing * 8;
-  // The CTA's own partial result, which only a cluster needs: without it six CTAs of four warps fit an SM, not five.
-  static constexpr uint32_t bytes(bool cluster) { return kMergeOffset + (cluster ? kPart : 0); }
+  static constexpr uint32_t kBytes = kMergeOffset + kPart;  // the CTA's own partial result last, for its cluster
   static_assert(kPart <= kWarpRing && kPart % 16 == 0, "a warp's partial result fits its ring");
 };
 
@@ -301,6 +302,13 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
+// Four 8 x 8 matrices of 16-bit words, transposed: lane l gives the address of row l % 8 of matrix l / 8.
+__device__ __forceinline__ void load_transposed(uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d, uint32_t row) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(a), "=r"(b), "=r"(c), "=r"(d)
+               : "r"(row));
+}
+
 __device__ __forceinline__ float fast_log2(float x) {
   float y;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -331,7 +339,7 @@ __device__ __forceinline__ uint32_t pair1(const Q4Constants& k, uint32_t w) { re
 __device__ __forceinline__ uint32_t swap_bytes(uint32_t w) { return __byte_perm(w, 0, 0x2301); }
 
 // One warp's running state. The MMA fragments put columns 2 t and 2 t + 1 (t = lane % 4) on a lane; with g = lane / 4,
-// acc[i][n] holds dimensions 64 i + 8 g + n ([0], [1]) and 64 i + 8 g + 4 + n ([2], [3]) of the two columns.
+// acc[i][n] holds dimensions 64 i + 4 g + n ([0], [1]) and 32 more ([2], [3]) of the two columns.
 template <int G>
 struct Q4State {
   float acc[G][4][4];
@@ -357,9 +365,11 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
   constexpr uint32_t kTileBytes = G * kQ4Block, CP = q4_columns(RP), TP = q4_tiles_at_once(G, RP);
   constexpr bool kTwo = RP > 1;  // a single query takes the even columns only
   // Row r of the score MMA is position pi(r) (r < 8) or 8 + pi(r - 8) of a tile, pi = 0 2 1 3 6 4 7 5: the key words of
-  // eight lane groups, and the value words of the even and of the odd rows, then fall into different banks.
+  // eight lane groups then fall into different banks.
   const uint32_t pg = g & 1u ? (g >> 1) + 2 : (g < 4 ? g >> 1 : (g >> 1) + 4);
-  const uint32_t pe = t < 2 ? t : t + 4, po = t + 2;  // pi(2 t), pi(2 t + 1)
+  // Lane l's row of the transposing value load: position pi(l % 8), or 8 + that, and 32 dimensions.
+  const uint32_t l8 = lane_id() & 7u, pl = l8 & 1u ? (l8 >> 1) + 2 : (l8 < 4 ? l8 >> 1 : (l8 >> 1) + 4);
+  const uint32_t value_rows = smem_u32(tiles) + kQ4Codes + (pl + (lane_id() >> 4) * 8) * 32 + (lane_id() >> 3 & 1u) * 16;
   const uint32_t mine = 2 * t / CP;                   // the tile of this lane's two columns (none when >= TP)
   float d[G][4];
 #pragma unroll
@@ -474,17 +484,12 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
     if (!FULL && j * kQ4Tile >= left) break;
 #pragma unroll
     for (int i = 0; i < G; ++i) {
-      const uint8_t* words = tiles + j * kTileBytes + i * kQ4Block + kQ4Codes + g * 4;
-      const uint32_t va = *reinterpret_cast<const uint32_t*>(words + pe * 32);
-      const uint32_t vb = *reinterpret_cast<const uint32_t*>(words + po * 32);
-      const uint32_t vc = *reinterpret_cast<const uint32_t*>(words + (pe + 8) * 32);
-      const uint32_t vd = *reinterpret_cast<const uint32_t*>(words + (po + 8) * 32);
       const uint32_t w0 = TP == 1 || g / CP == j ? b0[i] : 0u, w1 = TP == 1 || g / CP == j ? b1[i] : 0u;
-      // The same dimension of two positions side by side: dimensions 8 g + 0, 1 in e, + 2, 3 in f, + 4, 5 in o, + 6, 7 in r.
-      const uint32_t e0 = __byte_perm(va, vb, 0x5410), f0 = __byte_perm(va, vb, 0x4501);
-      const uint32_t o0 = __byte_perm(va, vb, 0x7632), r0 = __byte_perm(va, vb, 0x6723);
-      const uint32_t e1 = __byte_perm(vc, vd, 0x5410), f1 = __byte_perm(vc, vd, 0x4501);
-      const uint32_t o1 = __byte_perm(vc, vd, 0x7632), r1 = __byte_perm(vc, vd, 0x6723);
+      // The same dimensions of two positions side by side: 4 g .. 4 g + 3 in the first word of each pair, 32 more in the
+      // second; codes 0 and 1, and 2 and 3 of each half with its bytes swapped.
+      uint32_t e0, o0, e1, o1;
+      load_transposed(e0, o0, e1, o1, value_rows + j * kTileBytes + i * kQ4Block);
+      const uint32_t f0 = swap_bytes(e0), r0 = swap_bytes(o0), f1 = swap_bytes(e1), r1 = swap_bytes(o1);
       mma_f16(st.acc[i][0], pair0(kc, e0), pair0(kc, o0), pair0(kc, e1), pair0(kc, o1), w0, w1);
       mma_f16(st.acc[i][1], pair1(kc, e0), pair1(kc, o0), pair1(kc, e1), pair1(kc, o1), w0, w1);
       mma_f16(st.acc[i][2], pair0(kc, f0), pair0(kc, r0), pair0(kc, f1), pair0(kc, r1), w0, w1);
@@ -502,7 +507,7 @@ __device__ __forceinline__ float ld_cluster(const float* local, uint32_t rank) {
 }
 
 // The dimension of word `at` of a query's values in a partial result.
-__device__ __forceinline__ uint32_t q4_dimension(uint32_t at) { return (at & ~63u) | (at & 7u) << 3 | (at >> 3 & 7u); }
+__device__ __forceinline__ uint32_t q4_dimension(uint32_t at) { return (at & ~31u) | (at & 7u) << 2 | (at >> 3 & 3u); }
 
 struct Q4Attention {
   const uint16_t* q;
@@ -517,8 +522,14 @@ struct Q4Attention {
   uint32_t early;   // the grid is resident at once: the next kernel may start at entry
 };
 
+// CTAs of `warps` warps that an SM is to hold: 128 registers a thread for heads of 128, 96 (80 for eight warps, of which two
+// CTAs would be too few) for 64. Fewer warps with more registers, and more with fewer, are slower: 512 sequences of 12 heads
+// and 1152 positions 80.9 us at 20 warps an SM, 83 at 16 and at 24; 64 query heads of 8 78.6, 78.4 and 82.4; 8 heads of 128
+// 112.5 at 16, 119.4 at 12, 122 at 20.
+constexpr uint32_t q4_resident(int head, int warps) { return head == 128 ? 16 / warps : warps == 8 ? 3 : 20 / warps; }
+
 template <int G, int RP, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS) decode_attention_q4_kernel(Q4Attention p) {
+__global__ void __launch_bounds__(32 * WARPS, q4_resident(64 * G, WARPS)) decode_attention_q4_kernel(Q4Attention p) {
   using L = Q4Smem<G, WARPS>;
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr uint32_t kWidth = 64 * G, kTileBytes = G * kQ4Block, kPieceTiles = kQ4Piece / kTileBytes;
@@ -811,19 +822,16 @@ struct Q4Split {
   bool parts;
 };
 
-// CTAs of four warps that fit an SM: 128 registers a thread for heads of 128, else 80, or 96 for two and four queries.
-uint32_t q4_resident(uint32_t head, uint32_t rp) { return head == 128 ? 4 : rp == 2 || rp == 4 ? 5 : 6; }
-
 // Twice as many CTAs as fit the GPU (lengths differ, and a second round fills what the short ones leave), as long as each
 // has 12 tiles, and more where there are many pairs, whose CTAs hide one another's latency. Measured on a B200 over 456
-// grids of 1 to 768 pairs of 12 to 4096 tiles, at full and at ragged lengths, against every split of up to 148 CTAs: 3.5 %
-// behind the best one on average, 28 % at worst (clusters of up to 16 CTAs chosen by warps alone: 8.3 % and 90 %). us (w
-// warps, c CTAs, p through the workspace): 768 pairs of 72 w4c1 17.4, w8c1 18.8, w4c2 20.0; 96 of 256 w4c8 12.8, w4c1 16.4,
-// w8c16 28.5; 32 of 512 (128-wide) w4c16p 16.0, w4c8 18.8, w8c16 24.4; 16 of 4096 w4c64p 36.2, w4c16 47.1; 6144 of 72 w2c1
-// 91, w4c1 97 (a CTA's latency weighs more than its width there).
-Q4Split q4_split(uint64_t pairs, uint32_t tiles, uint32_t head, uint32_t rp) {
+// grids of 1 to 768 pairs of 12 to 4096 tiles, at full and at ragged lengths, against every split of up to 148 CTAs: 3 %
+// behind the best one on average, 26 % at worst. us (w warps, c CTAs, p through the workspace): 768 pairs of 72 w4c1 16.4,
+// w8c1 17.9, w4c2 19.6; 192 of 72 w8c1 8.9, w4c2 9.6, w4c4 11.0; 96 of 256 w4c8 12.3, w4c1 15.0; 32 of 512 (128-wide) w4c18p
+// 15.4, w4c8 17.2, w4c37p 18.0; 16 of 4096 w4c64p 36.9, w4c16p 45.4, w4c8 72; 6144 of 72 w2c1 81, w4c1 89 (a CTA's latency
+// weighs more than its width there).
+Q4Split q4_split(uint64_t pairs, uint32_t tiles, uint32_t head) {
   const uint64_t sms = uint64_t(sm_count());
-  const uint64_t chunks = std::min(2 * q4_resident(head, rp) * sms / pairs, tiles * sms / (12 * sms + 32 * pairs));
+  const uint64_t chunks = std::min(2 * q4_resident(head, 4) * sms / pairs, tiles * sms / (12 * sms + 32 * pairs));
   if (chunks < 3) return Q4Split{pairs >= 20 * sms ? 2u : pairs <= 3 * sms && tiles >= 16 ? 8u : 4u, 1, false};
   if (chunks <= 12) return Q4Split{4, chunks < 6 ? 4u : 8u, false};
   // whole pieces to each warp
@@ -837,12 +845,11 @@ tempo_status launch_attention_warps(const Q4Attention& base, uint32_t seqs, uint
   Q4Attention p = base;
   auto kernel = decode_attention_q4_kernel<G, RP, WARPS>;
   const bool cluster = chunks > 1 && p.parts == nullptr;
-  const tempo_status status = set_smem(reinterpret_cast<const void*>(kernel), Q4Smem<G, WARPS>::bytes(true));
+  const tempo_status status = set_smem(reinterpret_cast<const void*>(kernel), Q4Smem<G, WARPS>::kBytes);
   if (status != TEMPO_OK) return status;
   p.early = single_wave(uint64_t(p.kv_heads) * p.blocks * seqs * chunks, 16 / WARPS);
   return launch(kernel, dim3(chunks, p.kv_heads * p.blocks, seqs), dim3(32 * WARPS),
-                Q4Smem<G, WARPS>::bytes(cluster), stream,
-                cluster ? chunks : 1, "decode_attention_q4_kernel", p);
+                Q4Smem<G, WARPS>::kBytes, stream, cluster ? chunks : 1, "decode_attention_q4_kernel", p);
 }
 
 template <int G, int RP>
@@ -866,7 +873,7 @@ uint32_t q4_queries(uint32_t head, uint32_t share) {
 uint64_t q4_workspace(uint32_t seqs, uint32_t heads, uint32_t kv_heads, uint32_t head, uint32_t capacity) {
   const uint32_t share = heads / kv_heads, rp = q4_queries(head, share);
   const uint64_t pairs = uint64_t(seqs) * kv_heads * ((share + rp - 1) / rp);
-  const Q4Split split = q4_split(pairs, capacity / kQ4Tile, head, rp);
+  const Q4Split split = q4_split(pairs, capacity / kQ4Tile, head);
   return split.parts ? pairs * split.chunks * (head == 64 ? Q4Smem<1, 4>::kPart : Q4Smem<2, 4>::kPart) : 0;
 }
 
@@ -986,7 +993,7 @@ extern "C" tempo_status tempo_decode_attention_q4(const void* q, uint32_t ldq, c
   p.tiles = capacity / kQ4Tile;
   p.length_offset = length_offset;
   p.blocks = (share + rp - 1) / rp;
-  const Q4Split split = q4_split(uint64_t(seqs) * kv_heads * p.blocks, p.tiles, head, rp);
+  const Q4Split split = q4_split(uint64_t(seqs) * kv_heads * p.blocks, p.tiles, head);
   float* parts = static_cast<float*>(workspace);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (head == 128) {
