@@ -20,17 +20,7 @@ namespace {
 
 constexpr uint32_t kStoreThreads = 128;
 constexpr uint32_t kUnitLanes = 4;  // lanes that share a position's 64 dimensions of one key / value head, 16 each
-
-// Division by a number known at launch: n / d = (mulhi(n, mul) + n) >> shift for n < 2^31.
-struct Divisor {
-  uint32_t mul, shift;
-};
-Divisor divisor(uint32_t d) {
-  uint32_t shift = 0;
-  while ((uint64_t(1) << shift) < d) ++shift;
-  return Divisor{uint32_t(((uint64_t(1) << 32) * ((uint64_t(1) << shift) - d)) / d + 1), shift};
-}
-__device__ __forceinline__ uint32_t divide(uint32_t n, Divisor d) { return (__umulhi(n, d.mul) + n) >> d.shift; }
+constexpr uint32_t kStoreRows = kStoreThreads / kUnitLanes;
 
 // Rows of keys and values (bf16, `ld` elements apart) and their places in a cache.
 struct Q4Rows {
@@ -39,22 +29,19 @@ struct Q4Rows {
   const int32_t* seq_of;
   const int32_t* pos_of;
   uint32_t ld, count, seqs, kv_heads, tiles;
-  Divisor per_row;      // units of a row: kv_heads * groups
-  uint32_t units_a_row;
 };
 
 // A unit: the 64 dimensions of a row's key and of its value that one block holds (group `of` of the row's key groups: the
-// key's columns 64 `of` on, the value's 64 (units_a_row + of) on) and where they are kept. Eight consecutive units, a
-// warp's, are the same columns of eight rows: of a prompt, 256 bytes of codes side by side. (Key and value as two units
-// made the index arithmetic a third of the instructions: 116 us for 65536 rows of 12 heads stored and read back instead
-// of 102.)
+// key's columns 64 `of` on, the value's as far behind all keys) and where they are kept. A warp takes the same columns of
+// eight rows: of a prompt, 256 bytes of codes side by side. (Key and value as two units made the index arithmetic a third of
+// the instructions: 116 us for 65536 rows of 12 heads stored and read back instead of 102; with units counted in one grid
+// dimension and divided out again 98 instead of 95.)
 template <int G>
 struct Q4Unit {
   uint32_t row, of, seq, pos;
-  __device__ __forceinline__ Q4Unit(const Q4Rows& p, uint32_t unit) {
-    const uint32_t eight = divide(unit >> 3, p.per_row);
-    of = (unit >> 3) - eight * p.units_a_row;
-    row = eight * 8 + (unit & 7u);
+  __device__ __forceinline__ explicit Q4Unit(const Q4Rows& p) {
+    of = blockIdx.x;
+    row = blockIdx.y * kStoreRows + threadIdx.x / kUnitLanes;
     seq = pos = 0;
     if (row < p.count) {
       seq = uint32_t(p.seq_of[row]);
@@ -68,7 +55,7 @@ struct Q4Unit {
   }
   // Lane li's 16 dimensions of the key (0) or the value (1) in a row.
   __device__ __forceinline__ uint4* columns(const Q4Rows& p, uint32_t value, uint32_t li) const {
-    return reinterpret_cast<uint4*>(p.rows + size_t(row) * p.ld + (value * p.units_a_row + of) * kQ4Group) + 2 * li;
+    return reinterpret_cast<uint4*>(p.rows + size_t(row) * p.ld + (value * gridDim.x + of) * kQ4Group) + 2 * li;
   }
   __device__ __forceinline__ uint2* codes(uint8_t* block, uint32_t value, uint32_t li) const {
     return reinterpret_cast<uint2*>(block + value * kQ4Codes + pos % kQ4Tile * 32) + li;
@@ -89,10 +76,12 @@ __device__ __forceinline__ uint32_t min_nan_bf16x2(uint32_t a, uint32_t b) {
   return d;
 }
 
-// Four codes (integers 0 .. 15 as floats) as a 16-bit field: c0 + 16 c1 + 256 c2 + 4096 c3 is exact in FP32, and adding
-// 2^23 leaves it in the low bits.
-__device__ __forceinline__ uint32_t pack_codes(float c0, float c1, float c2, float c3) {
-  return __float_as_uint(fmaf(4096.f, c3, fmaf(256.f, c2, fmaf(16.f, c1, c0))) + 8388608.f);
+// Eight codes as a word, the first in its lowest bits, from the floats 1.5 2^23 + code: these hold the code in their lowest
+// four bits and nothing in the eighteen above.
+__device__ __forceinline__ uint32_t pack_codes(const uint32_t* c) {
+  const uint32_t b01 = __byte_perm(c[1] * 16 + c[0], c[3] * 16 + c[2], 0x0040);
+  const uint32_t b23 = __byte_perm(c[5] * 16 + c[4], c[7] * 16 + c[6], 0x0040);
+  return __byte_perm(b01, b23, 0x5410);
 }
 
 // Storing is bound by the bytes it moves as long as the arithmetic stays near ten instructions a value. The least and
@@ -122,7 +111,7 @@ __device__ __forceinline__ uint2 quantise(const uint4& a, const uint4& b, uint32
   const float high = bf16_lo(most), low = bf16_lo(least);
   const bool finite = fabsf(high) < INFINITY && fabsf(low) < INFINITY;  // false for a NaN too
   const float scale = finite ? round_bf16(__fdiv_rn(high - low, 15.f)) : __int_as_float(0x7FC00000);
-  float c[16];
+  uint32_t c[16];
   if (scale >= 0x1p-90f && scale <= 0x1p100f) {
     const float r = __frcp_rn(scale);
     const uint64_t r2 = f2_splat(r), s2 = f2_splat(-scale), low2 = f2_splat(-low), round2 = f2_splat(12582912.f);
@@ -132,33 +121,59 @@ __device__ __forceinline__ uint2 quantise(const uint4& a, const uint4& b, uint32
       const uint64_t q = f2_mul(d, r2);
       const uint64_t exact = f2_fma(f2_fma(q, s2, d), r2, q);
       // in 0 .. 15: the scale's rounding moves a quotient by at most 15 / 256
-      f2_unpack(f2_add(f2_add(exact, round2), f2_splat(-12582912.f)), c[2 * i], c[2 * i + 1]);
+      float c0, c1;
+      f2_unpack(f2_add(exact, round2), c0, c1);
+      c[2 * i] = __float_as_uint(c0);
+      c[2 * i + 1] = __float_as_uint(c1);
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const float x = i % 2 ? bf16_hi(w[i / 2]) : bf16_lo(w[i / 2]);
-      c[i] = scale > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(x - low, scale)), 0.f), 15.f) : 0.f;
+      const float code = scale > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(x - low, scale)), 0.f), 15.f) : 0.f;
+      c[i] = __float_as_uint(code + 12582912.f);
     }
   }
   meta = pack_bf16x2(scale, finite ? low : 0.f);
-  uint2 word;
-  word.x = __byte_perm(pack_codes(c[0], c[1], c[2], c[3]), pack_codes(c[4], c[5], c[6], c[7]), 0x5410);
-  word.y = __byte_perm(pack_codes(c[8], c[9], c[10], c[11]), pack_codes(c[12], c[13], c[14], c[15]), 0x5410);
-  return word;
+  return make_uint2(pack_codes(c), pack_codes(c + 8));
 }
 
-template <int G>
+// 16 dimensions of a row, 32 bytes: one access where rows begin on 32 bytes (WIDE: reading back 65536 rows 46.5 us), else two
+// of 16, each of half a sector (49.8).
+template <bool WIDE>
+__device__ __forceinline__ void load_columns(const uint4* p, uint4& a, uint4& b) {
+  if constexpr (WIDE) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+                 : "l"(p));
+  } else {
+    a = p[0];
+    b = p[1];
+  }
+}
+template <bool WIDE>
+__device__ __forceinline__ void store_columns(uint4* p, const uint4& a, const uint4& b) {
+  if constexpr (WIDE) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z),
+                 "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+                 : "memory");
+  } else {
+    p[0] = a;
+    p[1] = b;
+  }
+}
+
+template <int G, bool WIDE>
 __global__ void __launch_bounds__(kStoreThreads) kv_store_q4_kernel(Q4Rows p) {
   pdl_wait();
   pdl_launch_dependents();
   const uint32_t li = threadIdx.x % kUnitLanes, mask = 0xFu << (threadIdx.x & 28u);
-  const Q4Unit<G> unit(p, (blockIdx.x * kStoreThreads + threadIdx.x) / kUnitLanes);
+  const Q4Unit<G> unit(p);
   if (unit.row >= p.count) return;  // whole units leave together
   // The row is on its way before its place is known; a place outside the cache only keeps it from being stored.
-  const uint4* key = unit.columns(p, 0, li);
-  const uint4* value = unit.columns(p, 1, li);
-  const uint4 k0 = key[0], k1 = key[1], v0 = value[0], v1 = value[1];
+  uint4 k0, k1, v0, v1;
+  load_columns<WIDE>(unit.columns(p, 0, li), k0, k1);
+  load_columns<WIDE>(unit.columns(p, 1, li), v0, v1);
   uint8_t* block = unit.place(p);
   uint2 meta;
   const uint2 k = quantise(k0, k1, mask, meta.x), v = quantise(v0, v1, mask, meta.y);
@@ -169,12 +184,12 @@ __global__ void __launch_bounds__(kStoreThreads) kv_store_q4_kernel(Q4Rows p) {
 }
 
 // The rows' keys and values back as BF16: code x scale + low in FP32, rounded once.
-template <int G>
+template <int G, bool WIDE>
 __global__ void __launch_bounds__(kStoreThreads) kv_load_q4_kernel(Q4Rows p) {
   pdl_wait();
   pdl_launch_dependents();
   const uint32_t li = threadIdx.x % kUnitLanes;
-  const Q4Unit<G> unit(p, (blockIdx.x * kStoreThreads + threadIdx.x) / kUnitLanes);
+  const Q4Unit<G> unit(p);
   if (unit.row >= p.count) return;
   uint8_t* block = unit.place(p);
   uint2 codes[2] = {make_uint2(0, 0), make_uint2(0, 0)}, meta = make_uint2(0, 0);  // a place outside the cache: zeros
@@ -196,29 +211,26 @@ __global__ void __launch_bounds__(kStoreThreads) kv_load_q4_kernel(Q4Rows p) {
       const float c1 = __uint_as_float(((word >> 4) & 15u) | 0x4B000000u) - 8388608.f;
       out[i] = pack_bf16x2(fmaf(c0, s, l), fmaf(c1, s, l));
     }
-    uint4* dst = unit.columns(p, value, li);
-    dst[0] = make_uint4(out[0], out[1], out[2], out[3]);
-    dst[1] = make_uint4(out[4], out[5], out[6], out[7]);
+    store_columns<WIDE>(unit.columns(p, value, li), make_uint4(out[0], out[1], out[2], out[3]),
+                        make_uint4(out[4], out[5], out[6], out[7]));
   }
 }
 
-// Launches `kernel` over `rows` rows, in as many calls as 31-bit thread numbers need.
+// Rows that all begin on 32 bytes.
+bool wide_rows(const Q4Rows& p) { return reinterpret_cast<uintptr_t>(p.rows) % 32 == 0 && p.ld % 16 == 0; }
+
+// Launches `kernel` over `rows` rows, in as many calls as the grid's 16-bit dimension needs.
 tempo_status launch_rows(void (*kernel)(Q4Rows), Q4Rows p, uint32_t rows, uint32_t groups, cudaStream_t stream,
                          const char* name) {
-  p.units_a_row = p.kv_heads * groups;
-  p.per_row = divisor(p.units_a_row);
-  const uint32_t most = 0x7FFFFF00u / (8 * kUnitLanes * p.units_a_row) * 8;
   for (uint32_t done = 0; done < rows;) {
-    const uint32_t count = rows - done < most ? rows - done : most;
-    p.count = count;
-    const uint32_t threads = (count + 7) / 8 * 8 * p.units_a_row * kUnitLanes;
-    const tempo_status status = launch(kernel, dim3((threads - 1) / kStoreThreads + 1), dim3(kStoreThreads), 0, stream, 1,
-                                       name, p);
+    p.count = std::min(rows - done, 65535 * kStoreRows);
+    const tempo_status status = launch(kernel, dim3(p.kv_heads * groups, (p.count - 1) / kStoreRows + 1),
+                                       dim3(kStoreThreads), 0, stream, 1, name, p);
     if (status != TEMPO_OK) return status;
-    p.rows += size_t(count) * p.ld;
-    p.seq_of += count;
-    p.pos_of += count;
-    done += count;
+    p.rows += size_t(p.count) * p.ld;
+    p.seq_of += p.count;
+    p.pos_of += p.count;
+    done += p.count;
   }
   return TEMPO_OK;
 }
@@ -920,8 +932,9 @@ extern "C" tempo_status tempo_kv_store_q4(const void* qkv, uint32_t ldq, void* c
   p.seqs = seqs;
   p.kv_heads = kv_heads;
   p.tiles = capacity / kQ4Tile;
-  return launch_rows(head == 64 ? kv_store_q4_kernel<1> : kv_store_q4_kernel<2>, p, rows, head / kQ4Group,
-                     static_cast<cudaStream_t>(stream), "kv_store_q4_kernel");
+  auto kernel = wide_rows(p) ? (head == 64 ? kv_store_q4_kernel<1, true> : kv_store_q4_kernel<2, true>)
+                             : (head == 64 ? kv_store_q4_kernel<1, false> : kv_store_q4_kernel<2, false>);
+  return launch_rows(kernel, p, rows, head / kQ4Group, static_cast<cudaStream_t>(stream), "kv_store_q4_kernel");
 }
 
 extern "C" tempo_status tempo_kv_load_q4(const void* cache, void* kv, uint32_t ldo, const int32_t* seq_of,
@@ -945,8 +958,9 @@ extern "C" tempo_status tempo_kv_load_q4(const void* cache, void* kv, uint32_t l
   p.seqs = seqs;
   p.kv_heads = kv_heads;
   p.tiles = capacity / kQ4Tile;
-  return launch_rows(head == 64 ? kv_load_q4_kernel<1> : kv_load_q4_kernel<2>, p, rows, head / kQ4Group,
-                     static_cast<cudaStream_t>(stream), "kv_load_q4_kernel");
+  auto kernel = wide_rows(p) ? (head == 64 ? kv_load_q4_kernel<1, true> : kv_load_q4_kernel<2, true>)
+                             : (head == 64 ? kv_load_q4_kernel<1, false> : kv_load_q4_kernel<2, false>);
+  return launch_rows(kernel, p, rows, head / kQ4Group, static_cast<cudaStream_t>(stream), "kv_load_q4_kernel");
 }
 
 extern "C" tempo_status tempo_decode_attention_q4_workspace(uint32_t seqs, uint32_t heads, uint32_t kv_heads,
