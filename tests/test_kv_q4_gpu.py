@@ -153,6 +153,29 @@ def test_rows_at_a_stride_and_offset() -> None:
     _check_attention(wide[:1, 64:7 * 64], cache, lengths, 2, got)
 
 
+@pytest.mark.parametrize("head", [64, 128])
+@pytest.mark.parametrize("offset,pad", [(0, 0), (8, 0), (0, 8), (8, 8), (16, 16)])
+def test_rows_on_16_and_on_32_bytes(head: int, offset: int, pad: int) -> None:
+    """Rows that begin on 32 bytes go by wider accesses than others; both store and read back alike, and nothing between
+    the rows is written."""
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(21)
+    rows, width = 71, 2 * 3 * head
+    stride = width + pad
+    flat = torch.zeros(rows * stride + 32, dtype=torch.bfloat16, device="cuda")
+    qkv = flat[offset:offset + rows * stride].view(rows, stride)[:, :width]
+    qkv.copy_(_rows(rng, rows, 6, head).reshape(rows, -1))
+    cache = ops.kv_cache_q4(2, 3, 64, head)
+    seq, pos = _i32(np.arange(rows) % 2), _i32(np.arange(rows) // 2)
+    ops.kv_store_q4(qkv, cache, seq, pos)
+    back = torch.full_like(flat, 7.0)
+    out = back[offset:offset + rows * stride].view(rows, stride)[:, :width]
+    ops.kv_load_q4(cache, seq, pos, out=out)
+    np.testing.assert_array_equal(out.float().cpu().numpy(), _expected(qkv, 3, head))
+    assert int((back == 7.0).sum()) >= back.numel() - rows * width and (back[:offset] == 7.0).all()
+    assert (back[offset + rows * stride - pad:] == 7.0).all()
+
+
 # ---- attention --------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("heads,kv_heads,head", [(12, 12, 64), (1, 1, 64), (8, 2, 64), (9, 1, 64), (40, 2, 64),
