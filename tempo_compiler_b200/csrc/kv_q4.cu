@@ -834,8 +834,8 @@ struct Q4Split {
   bool parts;
 };
 
-// Twice as many CTAs as fit the GPU (lengths differ, and a second round fills what the short ones leave), as long as each
-// has 12 tiles, and more where there are many pairs, whose CTAs hide one another's latency. Measured on a B200 over 456
+// Up to twice as many CTAs as fit the GPU (lengths differ, and a second round fills what the short ones leave), as long as
+// each has 12 tiles, and more where there are many pairs, whose CTAs hide one another's latency. Measured on a B200 over 456
 // grids of 1 to 768 pairs of 12 to 4096 tiles, at full and at ragged lengths, against every split of up to 148 CTAs: 3 %
 // behind the best one on average, 26 % at worst. us (w warps, c CTAs, p through the workspace): 768 pairs of 72 w4c1 16.4,
 // w8c1 17.9, w4c2 19.6; 192 of 72 w8c1 8.9, w4c2 9.6, w4c4 11.0; 96 of 256 w4c8 12.3, w4c1 15.0; 32 of 512 (128-wide) w4c18p
@@ -846,10 +846,21 @@ Q4Split q4_split(uint64_t pairs, uint32_t tiles, uint32_t head) {
   const uint64_t chunks = std::min(2 * q4_resident(head, 4) * sms / pairs, tiles * sms / (12 * sms + 32 * pairs));
   if (chunks < 3) return Q4Split{pairs >= 20 * sms ? 2u : pairs <= 3 * sms && tiles >= 16 ? 8u : 4u, 1, false};
   if (chunks <= 12) return Q4Split{4, chunks < 6 ? 4u : 8u, false};
-  // whole pieces to each warp
-  const uint32_t most = uint32_t(std::min<uint64_t>(chunks, kQ4MaxSplits));
-  const uint32_t per = ((tiles + most - 1) / most + 15) / 16 * 16;
-  return Q4Split{4, (tiles + per - 1) / per, true};
+  // As many as fit at once, or twice that, whichever has its rounds of CTAs done first: whole pieces to each warp, and a
+  // CTA's fixed cost about that of 12 tiles.
+  const uint64_t slots = q4_resident(head, 4) * sms;
+  uint64_t least = UINT64_MAX;
+  uint32_t best = 0;
+  for (uint32_t rounds = 1; rounds <= 2; ++rounds) {
+    const uint32_t most = uint32_t(std::min<uint64_t>({chunks, kQ4MaxSplits, rounds * slots / pairs}));
+    const uint32_t per = ((tiles + most - 1) / most + 15) / 16 * 16, count = (tiles + per - 1) / per;
+    const uint64_t cost = (pairs * count + slots - 1) / slots * (per + 12);
+    if (cost < least) {
+      least = cost;
+      best = count;
+    }
+  }
+  return Q4Split{4, best, true};
 }
 
 template <int G, int RP, int WARPS>
