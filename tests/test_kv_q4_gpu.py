@@ -406,6 +406,38 @@ def test_two_graphs_of_split_calls_at_once() -> None:
         assert torch.equal(out, want)
 
 
+def test_one_graph_of_every_split() -> None:
+    """Calls of one CTA a pair, of clusters and of the workspace in one captured graph beside an eager stream of others."""
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(23)
+    calls = []
+    for seqs, heads, kv_heads, head, n in ((3, 12, 12, 64, 384), (1, 12, 12, 64, 1152), (2, 8, 2, 128, 2100),
+                                           (1, 4, 1, 64, 9000), (300, 12, 12, 64, 40)):
+        cache = ops.kv_cache_q4(seqs, kv_heads, n, head)
+        _fill(cache, rng)
+        qkv = (_rows(rng, seqs, heads, head) * (1.5 / head ** 0.5)).reshape(seqs, -1)
+        lengths = rng.integers(0, n + 1, seqs)
+        want = ops.decode_attention_q4(qkv, cache, _i32(lengths), heads=heads)
+        _check_attention(qkv, cache, lengths, heads, want)
+        calls.append((qkv, cache, _i32(lengths), heads, torch.zeros_like(want), want))
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        for qkv, cache, lengths, heads, out, _ in calls:
+            ops.decode_attention_q4(qkv, cache, lengths, heads=heads, out=out)
+    for _ in range(4):
+        for call in calls:
+            call[4].zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        eager = [ops.decode_attention_q4(qkv, cache, lengths, heads=heads) for qkv, cache, lengths, heads, _, _ in calls]
+        torch.cuda.synchronize()
+        for (_, _, _, _, out, want), other in zip(calls, eager):
+            assert torch.equal(out, want) and torch.equal(other, want)
+
+
 def test_the_same_inputs_give_the_same_bits() -> None:
     from tempo_compiler_b200 import ops
     rng = np.random.default_rng(18)
