@@ -297,7 +297,7 @@ tempo_status tempo_kv_load_q4(const void* cache, void* kv, uint32_t ldo, const i
  * first heads * head columns, already scaled by 1/sqrt(head)) over the first lengths[s] + length_offset positions
  * (clamped to [0, capacity]); query head h reads key / value head h / (heads / kv_heads). A sequence of no positions is
  * written as zeros. Keys and values of more than 2^100 (1.3e30) in size may overflow on the way and give NaN, as may
- * scores that FP32 does not hold. out: [seqs, heads * head] BF16. Few sequences of a long capacity are split over more
+ * scores that FP32 does not hold, and where all values are below 2^-110 (8e-34) they lose bits. out: [seqs, heads * head] BF16. Few sequences of a long capacity are split over more
  * CTAs than a cluster holds; their partial results then go through `workspace` (tempo_decode_attention_q4_workspace
  * bytes, 16-byte aligned, of any content; NULL when that is 0), which no other call may use until this one has
  * finished. */

@@ -259,25 +259,29 @@ tempo_status launch_rows(void (*kernel)(Q4Rows), Q4Rows p, uint32_t rows, uint32
 // relative to a running reference that bounds w and p low alike; everything else, the sums included, is FP32.
 //
 // A CTA of four warps takes a run of tiles of one (sequence, key / value head, eight query heads); each warp streams its
-// own pieces (one bulk copy each, kRing in flight) and keeps an online softmax whose reference moves only when a score
-// passes it by 2^kSlack. Warps merge through shared memory; with `chunks` > 1 the CTAs of a cluster split the positions
+// own pieces (one bulk copy each, kRing in flight) and keeps an online softmax whose reference moves only when a weight
+// passes it kSlack times. Warps merge through shared memory; with `chunks` > 1 the CTAs of a cluster split the positions
 // and merge through distributed shared memory, or, when a pair needs more of them, through a workspace and a second kernel.
 // ---------------------------------------------------------------------------------------------------------------
 
+constexpr uint32_t kQ4MaxChunks = 8;     // CTAs of a cluster
 constexpr uint32_t kQ4MaxSplits = 160;   // CTAs that share a pair through the workspace
 constexpr uint32_t kQ4Queries = 8;
 constexpr uint32_t kQ4Piece = 4 * kQ4Block;  // bytes of one bulk copy: four tiles of a 64-wide head, two of a 128-wide
 constexpr uint32_t kRing = 2;
-constexpr float kSlack = 6.f;
-constexpr float kNoScore = -3.4028235e38f;  // the reference before any position: no finite score is below it
+constexpr float kSlack = 64.f;
+constexpr float kNoScore = -3.4028235e38f;  // the reference before any position: no finite score is below it,
+constexpr float kNoSize = -128.f;           // and no value's size
 
 template <int G, int WARPS>
 struct Q4Smem {
   static constexpr uint32_t kWarpRing = kRing * kQ4Piece;
   // A partial result of eight queries: 64 G values each (dimension 64 i + 4 g + n at 64 i + 8 n + g, eight words more to
-  // the next query: the lanes of a fragment store into different banks), then the references, then the sums.
+  // the next query: the lanes of a fragment store into different banks), then the references' scores and sizes, then the
+  // sums.
   static constexpr uint32_t kStride = 64 * G + 8;
-  static constexpr uint32_t kReferences = kQ4Queries * kStride, kSums = kReferences + kQ4Queries;
+  static constexpr uint32_t kReferences = kQ4Queries * kStride, kSizes = kReferences + kQ4Queries;
+  static constexpr uint32_t kSums = kSizes + kQ4Queries;
   static constexpr uint32_t kPart = (kSums + kQ4Queries) * 4;
   static constexpr uint32_t kBarrierOffset = WARPS * kWarpRing;
   static constexpr uint32_t kMergeOffset = kBarrierOffset + WARPS * kRing * 8;
@@ -355,7 +359,8 @@ __device__ __forceinline__ uint32_t swap_bytes(uint32_t w) { return __byte_perm(
 template <int G>
 struct Q4State {
   float acc[G][4][4];
-  float m[2], l[2];          // the reference (log2 of p times the value's size) and this lane's sum of p
+  float m[2], mg[2];         // the reference, log2 of p times the value's size, as a score and what lies above it
+  float l[2];                // this lane's sum of p
   float w[G][2], low[G][2];  // this lane's sums of w (as rounded) and of p low
 };
 
@@ -428,30 +433,50 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
     size0 = fmax3(size0, bf16_lo(meta0.y), 0.0625f * fabsf(bf16_hi(meta0.y)));
     size1 = fmax3(size1, bf16_lo(meta1.y), 0.0625f * fabsf(bf16_hi(meta1.y)));
   }
-  s0 = in0 ? s0 * unit[0] : -INFINITY;
-  s1 = in0 ? s1 * unit[1] : -INFINITY;
-  s2 = in1 ? s2 * unit[0] : -INFINITY;
-  s3 = in1 ? s3 * unit[1] : -INFINITY;
+  // (not joined with the differences below: a product that is rounded here and not there is off by its own rounding)
+  s0 = in0 ? __fmul_rn(s0, unit[0]) : -INFINITY;
+  s1 = in0 ? __fmul_rn(s1, unit[1]) : -INFINITY;
+  s2 = in1 ? __fmul_rn(s2, unit[0]) : -INFINITY;
+  s3 = in1 ? __fmul_rn(s3, unit[1]) : -INFINITY;
   // The reference follows log2(p size), size the value row's scale or a sixteenth of its low: w and p low stay small
-  // whatever the values' size, and a position of small values needs a larger p to move it.
-  const float g0 = fast_log2(fminf(size0, 0x1p100f)), g1 = fast_log2(fminf(size1, 0x1p100f));
-  float x0 = fmaxf(s0 + g0, s2 + g1), x1 = kTwo ? fmaxf(s1 + g0, s3 + g1) : 0.f;
-  if (__any_sync(0xFFFFFFFFu, x0 > st.m[0] + kSlack || (kTwo && x1 > st.m[1] + kSlack))) {
+  // whatever the values' size, and a position of small values needs a larger p to move it. It is kept as a score and a size
+  // (p = 2^(score - m - mg)): beside a score of 2^30 their sum would round the size away. It moves when p size passes
+  // kSlack, which NaN and infinity do too.
+  float p0 = fast_exp2(s0 - st.m[0] - st.mg[0]), p2 = fast_exp2(s2 - st.m[0] - st.mg[0]);
+  float p1 = kTwo ? fast_exp2(s1 - st.m[1] - st.mg[1]) : 0.f, p3 = kTwo ? fast_exp2(s3 - st.m[1] - st.mg[1]) : 0.f;
+  const bool far0 = !(fmaf(p0, size0, p2 * size1) <= kSlack), far1 = kTwo && !(fmaf(p1, size0, p3 * size1) <= kSlack);
+  if (__any_sync(0xFFFFFFFFu, far0 || far1)) {
+    const float g0 = fast_log2(fminf(size0, 0x1p100f)), g1 = fast_log2(fminf(size1, 0x1p100f));
+    float m0 = fmax3(s0, s2, st.m[0]), m1 = kTwo ? fmax3(s1, s3, st.m[1]) : 0.f;
+#pragma unroll
+    for (int o = 4; o <= 16; o <<= 1) {
+      m0 = fmaxf(m0, __shfl_xor_sync(0xFFFFFFFFu, m0, o));
+      if (kTwo) m1 = fmaxf(m1, __shfl_xor_sync(0xFFFFFFFFu, m1, o));
+    }
+    float x0 = fmaxf(s0 - m0 + g0, s2 - m0 + g1), x1 = kTwo ? fmaxf(s1 - m1 + g0, s3 - m1 + g1) : 0.f;
 #pragma unroll
     for (int o = 4; o <= 16; o <<= 1) {
       x0 = fmaxf(x0, __shfl_xor_sync(0xFFFFFFFFu, x0, o));
       if (kTwo) x1 = fmaxf(x1, __shfl_xor_sync(0xFFFFFFFFu, x1, o));
     }
-    x0 = fmaxf(x0, st.m[0]);
-    const float c0 = fast_exp2(st.m[0] - x0);
-    st.m[0] = x0;
+    const float was0 = st.m[0] - m0 + st.mg[0];
+    x0 = fmaxf(x0, was0);
+    const float c0 = fast_exp2(was0 - x0);
+    st.m[0] = m0;
+    st.mg[0] = x0;
     st.l[0] *= c0;
+    p0 = fast_exp2(s0 - m0 - x0);
+    p2 = fast_exp2(s2 - m0 - x0);
     float c1 = 0.f;
     if (kTwo) {
-      x1 = fmaxf(x1, st.m[1]);
-      c1 = fast_exp2(st.m[1] - x1);
-      st.m[1] = x1;
+      const float was1 = st.m[1] - m1 + st.mg[1];
+      x1 = fmaxf(x1, was1);
+      c1 = fast_exp2(was1 - x1);
+      st.m[1] = m1;
+      st.mg[1] = x1;
       st.l[1] *= c1;
+      p1 = fast_exp2(s1 - m1 - x1);
+      p3 = fast_exp2(s3 - m1 - x1);
     }
 #pragma unroll
     for (int i = 0; i < G; ++i) {
@@ -472,8 +497,6 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
       }
     }
   }
-  const float p0 = fast_exp2(s0 - st.m[0]), p2 = fast_exp2(s2 - st.m[0]);
-  const float p1 = kTwo ? fast_exp2(s1 - st.m[1]) : 0.f, p3 = kTwo ? fast_exp2(s3 - st.m[1]) : 0.f;
   st.l[0] += p0 + p2;
   if (kTwo) st.l[1] += p1 + p3;
   uint32_t b0[G], b1[G];
@@ -520,6 +543,33 @@ __device__ __forceinline__ float ld_cluster(const float* local, uint32_t rank) {
 
 // The dimension of word `at` of a query's values in a partial result.
 __device__ __forceinline__ uint32_t q4_dimension(uint32_t at) { return (at & ~31u) | (at & 7u) << 2 | (at >> 3 & 3u); }
+
+// Word `at` (of query `query`) of up to MOST partial results, of which there are `count`, brought to one reference; word(c, i)
+// reads word i of partial result c.
+struct Merged {
+  float m, mg, l, a;
+};
+template <typename L, uint32_t MOST, typename Word>
+__device__ __forceinline__ Merged merge_parts(uint32_t count, uint32_t query, uint32_t at, Word word) {
+  float m[MOST], mg[MOST];
+  Merged r{kNoScore, -INFINITY, 0.f, 0.f};
+#pragma unroll
+  for (uint32_t c = 0; c < MOST; ++c) {
+    m[c] = c < count ? word(c, L::kReferences + query) : kNoScore;
+    mg[c] = c < count ? word(c, L::kSizes + query) : kNoSize;
+    r.m = fmaxf(r.m, m[c]);
+  }
+#pragma unroll
+  for (uint32_t c = 0; c < MOST; ++c) r.mg = fmaxf(r.mg, m[c] - r.m + mg[c]);
+#pragma unroll
+  for (uint32_t c = 0; c < MOST; ++c) {
+    if (c >= count) break;
+    const float f = fast_exp2(m[c] - r.m + mg[c] - r.mg);
+    r.l = fmaf(word(c, L::kSums + query), f, r.l);
+    r.a = fmaf(word(c, at), f, r.a);
+  }
+  return r;
+}
 
 struct Q4Attention {
   const uint16_t* q;
@@ -636,6 +686,7 @@ __global__ void __launch_bounds__(32 * WARPS, q4_resident(64 * G, WARPS)) decode
 
   Q4State<G> st;
   st.m[0] = st.m[1] = kNoScore;
+  st.mg[0] = st.mg[1] = kNoSize;
   st.l[0] = st.l[1] = 0.f;
 #pragma unroll
   for (int i = 0; i < G; ++i) {
@@ -687,7 +738,11 @@ __global__ void __launch_bounds__(32 * WARPS, q4_resident(64 * G, WARPS)) decode
     float m = st.m[c];
 #pragma unroll
     for (int o = CP / 2; o < 4; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    const float f = fast_exp2(st.m[c] - m);
+    const float own = st.m[c] - m + st.mg[c];
+    float mg = own;
+#pragma unroll
+    for (int o = CP / 2; o < 4; o <<= 1) mg = fmaxf(mg, __shfl_xor_sync(0xFFFFFFFFu, mg, o));
+    const float f = fast_exp2(own - mg);
     float l = st.l[c] * f;
 #pragma unroll
     for (int o = CP / 2; o < 32; o <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
@@ -714,6 +769,7 @@ __global__ void __launch_bounds__(32 * WARPS, q4_resident(64 * G, WARPS)) decode
     }
     if (g == 0 && writes) {
       part[L::kReferences + query] = m;
+      part[L::kSizes + query] = mg;
       part[L::kSums + query] = l;
     }
   }
@@ -726,24 +782,16 @@ __global__ void __launch_bounds__(32 * WARPS, q4_resident(64 * G, WARPS)) decode
   uint16_t* out = p.out + (size_t(s) * p.heads + kvh * share + first) * kWidth;
   for (uint32_t i = threadIdx.x; i < queries * kWidth; i += 32 * WARPS) {
     const uint32_t query = i / kWidth, at = query * L::kStride + i % kWidth;
-    float m = kNoScore, l = 0.f, a = 0.f;
-#pragma unroll
-    for (uint32_t w = 0; w < WARPS; ++w)
-      m = fmaxf(m, reinterpret_cast<const float*>(smem + w * L::kWarpRing)[L::kReferences + query]);
-#pragma unroll
-    for (uint32_t w = 0; w < WARPS; ++w) {
-      const float* other = reinterpret_cast<const float*>(smem + w * L::kWarpRing);
-      const float f = fast_exp2(other[L::kReferences + query] - m);
-      l = fmaf(other[L::kSums + query], f, l);
-      a = fmaf(other[at], f, a);
-    }
+    const Merged r = merge_parts<L, WARPS>(
+        WARPS, query, at, [&](uint32_t w, uint32_t i) { return reinterpret_cast<const float*>(smem + w * L::kWarpRing)[i]; });
     if (whole) {
-      out[query * kWidth + q4_dimension(i % kWidth)] = float_to_bf16(len == 0 ? 0.f : a / l);
+      out[query * kWidth + q4_dimension(i % kWidth)] = float_to_bf16(len == 0 ? 0.f : r.a / r.l);
     } else {
-      merge[at] = a;
+      merge[at] = r.a;
       if (i % kWidth == 0) {
-        merge[L::kReferences + query] = m;
-        merge[L::kSums + query] = l;
+        merge[L::kReferences + query] = r.m;
+        merge[L::kSizes + query] = r.mg;
+        merge[L::kSums + query] = r.l;
       }
     }
   }
@@ -752,14 +800,9 @@ __global__ void __launch_bounds__(32 * WARPS, q4_resident(64 * G, WARPS)) decode
   // Each CTA finishes its share of the outputs, reading every CTA's partial result.
   for (uint32_t i = chunk * 32 * WARPS + threadIdx.x; i < queries * kWidth; i += chunks * 32 * WARPS) {
     const uint32_t query = i / kWidth, at = query * L::kStride + i % kWidth;
-    float m = kNoScore, l = 0.f, a = 0.f;
-    for (uint32_t c = 0; c < chunks; ++c) m = fmaxf(m, ld_cluster(merge + L::kReferences + query, c));
-    for (uint32_t c = 0; c < chunks; ++c) {
-      const float f = fast_exp2(ld_cluster(merge + L::kReferences + query, c) - m);
-      l = fmaf(ld_cluster(merge + L::kSums + query, c), f, l);
-      a = fmaf(ld_cluster(merge + at, c), f, a);
-    }
-    out[query * kWidth + q4_dimension(i % kWidth)] = float_to_bf16(len == 0 ? 0.f : a / l);
+    const Merged r = merge_parts<L, kQ4MaxChunks>(chunks, query, at,
+                                                  [&](uint32_t c, uint32_t i) { return ld_cluster(merge + i, c); });
+    out[query * kWidth + q4_dimension(i % kWidth)] = float_to_bf16(len == 0 ? 0.f : r.a / r.l);
   }
   // No CTA leaves while another may still read its shared memory.
   asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
@@ -776,7 +819,7 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_q4_kernel(Q4Attent
   using L = Q4Smem<G, 4>;
   constexpr uint32_t kWidth = 64 * G, kShares = kMergeThreads / kWidth, kPart = L::kPart / 4;
   __shared__ float factor[(kQ4MaxSplits + kMergeBatch * kShares - 1) / (kMergeBatch * kShares) * (kMergeBatch * kShares)];
-  __shared__ float warp_m[kMergeThreads / 32], warp_l[kMergeThreads / 32];
+  __shared__ float warp_m[kMergeThreads / 32], warp_mg[kMergeThreads / 32], warp_l[kMergeThreads / 32];
   __shared__ float sums[kShares][kWidth];
   pdl_wait();
   pdl_launch_dependents();
@@ -796,15 +839,19 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_q4_kernel(Q4Attent
   load(0);
   const bool has = threadIdx.x < chunks;
   const float m = has ? parts[threadIdx.x * kPart + L::kReferences + query] : kNoScore;
+  const float mg = has ? parts[threadIdx.x * kPart + L::kSizes + query] : kNoSize;
   const float part_l = has ? parts[threadIdx.x * kPart + L::kSums + query] : 0.f;
-  float most = m;
+  auto greatest = [&](float x, float* of_warps) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
-  if (lane_id() == 0) warp_m[warp_id()] = most;
-  __syncthreads();
+    for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, o));
+    if (lane_id() == 0) of_warps[warp_id()] = x;
+    __syncthreads();
 #pragma unroll
-  for (uint32_t w = 0; w < kMergeThreads / 32; ++w) most = fmaxf(most, warp_m[w]);
-  const float f = fast_exp2(m - most), l_warp = warp_sum(part_l * f);
+    for (uint32_t w = 0; w < (kQ4MaxSplits + 31) / 32; ++w) x = fmaxf(x, of_warps[w]);  // (the others have none)
+    return x;
+  };
+  const float above = m - greatest(m, warp_m) + mg;
+  const float f = fast_exp2(above - greatest(above, warp_mg)), l_warp = warp_sum(part_l * f);
   if (threadIdx.x < sizeof(factor) / 4) factor[threadIdx.x] = has ? f : 0.f;
   if (lane_id() == 0) warp_l[warp_id()] = l_warp;
   __syncthreads();

@@ -4,6 +4,8 @@ tests/test_q4_refusals_cpu.py."""
 
 from __future__ import annotations
 
+import math
+
 import numpy as np
 import pytest
 
@@ -285,6 +287,31 @@ def test_scores_far_below_zero(n: int, rising: bool) -> None:
     codes, scale, low = _q4.quantise(rows[n - 1 if rising else 0, 64:].float().cpu().numpy())
     want, wide = codes * scale + low, 15 * scale
     assert (np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + (2.0 ** -11 + 2.0 ** -16) * wide).all()
+
+
+@pytest.mark.parametrize("head,n", [(64, 40), (64, 1152), (128, 9000)])
+@pytest.mark.parametrize("score", [1e8, -1e8, 1e11, -1e11, 1e30, -1e30])
+@pytest.mark.parametrize("v_size", [1e-25, 1.0, 1e6, 1e25])
+def test_scores_and_values_of_any_size(head: int, n: int, score: float, v_size: float) -> None:
+    """Beside scores of 2^27 and more the values' size counts for nothing in FP32: the position with the greatest score still
+    gives its value row, as above."""
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(n)
+    cache = ops.kv_cache_q4(1, 1, n, head)
+    rows = _rows(rng, n, 2, head).float()
+    factor = 1 + np.minimum(np.arange(n), 100).astype(np.float32) / 8
+    size = math.sqrt(abs(score) / head)
+    rows[:, 0] = math.copysign(size, score) * torch.from_numpy(factor[::-1].copy() if score > 0 else factor).cuda()[:, None]
+    rows[:, 1] *= v_size
+    rows = rows.to(torch.bfloat16).reshape(n, -1)
+    ops.kv_store_q4(rows, cache, _i32(np.zeros(n)), _i32(np.arange(n)))
+    # the greatest score is position 0's, shared by as many as the factor's clamp gives it to
+    best = int((rows[:, 0] == rows[0, 0]).sum())
+    qkv = torch.full((1, 3 * head), size, dtype=torch.bfloat16, device="cuda")
+    got = ops.decode_attention_q4(qkv, cache, _i32([n]), heads=3).double().cpu().numpy().reshape(3, -1, 64)
+    codes, scale, low = _q4.quantise(rows[:best, head:].float().cpu().numpy().reshape(best, -1, 64))
+    want, wide = (codes * scale + low).mean(0), 15 * scale.max(0)
+    assert (np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + (2.0 ** -11 + 2.0 ** -16 + best * 2.0 ** -23) * wide).all()
 
 
 def test_a_nan_key_or_value_within_the_length_shows_in_its_own_head() -> None:
