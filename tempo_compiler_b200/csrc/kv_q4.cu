@@ -584,14 +584,15 @@ struct Q4Attention {
   uint32_t early;   // the grid is resident at once: the next kernel may start at entry
 };
 
-// CTAs of `warps` warps that an SM is to hold: 128 registers a thread for heads of 128, 96 (80 for eight warps, of which two
-// CTAs would be too few) for 64. Fewer warps with more registers, and more with fewer, are slower: 512 sequences of 12 heads
-// and 1152 positions 80.9 us at 20 warps an SM, 83 at 16 and at 24; 64 query heads of 8 78.6, 78.4 and 82.4; 8 heads of 128
-// 112.5 at 16, 119.4 at 12, 122 at 20.
-constexpr uint32_t q4_resident(int head, int warps) { return head == 128 ? 16 / warps : warps == 8 ? 3 : 20 / warps; }
+// CTAs of `warps` warps that an SM is to hold: 128 registers a thread for heads of 128, 96 for 64. Fewer warps with more
+// registers, and more with fewer, are slower: 512 sequences of 12 heads and 1152 positions 80.9 us at 20 warps an SM, 83 at 16
+// and at 24; 64 query heads of 8 78.6, 78.4 and 82.4; 8 heads of 128 112.5 at 16, 119.4 at 12, 122 at 20. CTAs of eight warps
+// come in two kinds, two to an SM as long as that holds the grid (192 pairs of 60 tiles 6.8 us against 7.7, 256 grouped pairs
+// of 72 9.0 against 11.5), else three (384 pairs of 72 10.6 against 11.5).
+constexpr uint32_t q4_resident(int head, int warps) { return head == 128 ? 16 / warps : warps == 8 ? 2 : 20 / warps; }
 
-template <int G, int RP, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS, q4_resident(64 * G, WARPS)) decode_attention_q4_kernel(Q4Attention p) {
+template <int G, int RP, int WARPS, int RESIDENT>
+__global__ void __launch_bounds__(32 * WARPS, RESIDENT) decode_attention_q4_kernel(Q4Attention p) {
   using L = Q4Smem<G, WARPS>;
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr uint32_t kWidth = 64 * G, kTileBytes = G * kQ4Block, kPieceTiles = kQ4Piece / kTileBytes;
@@ -910,10 +911,10 @@ Q4Split q4_split(uint64_t pairs, uint32_t tiles, uint32_t head) {
   return Q4Split{4, best, true};
 }
 
-template <int G, int RP, int WARPS>
+template <int G, int RP, int WARPS, int RESIDENT = q4_resident(64 * G, WARPS)>
 tempo_status launch_attention_warps(const Q4Attention& base, uint32_t seqs, uint32_t chunks, cudaStream_t stream) {
   Q4Attention p = base;
-  auto kernel = decode_attention_q4_kernel<G, RP, WARPS>;
+  auto kernel = decode_attention_q4_kernel<G, RP, WARPS, RESIDENT>;
   const bool cluster = chunks > 1 && p.parts == nullptr;
   const tempo_status status = set_smem(reinterpret_cast<const void*>(kernel), Q4Smem<G, WARPS>::kBytes);
   if (status != TEMPO_OK) return status;
@@ -928,7 +929,12 @@ tempo_status launch_attention(const Q4Attention& base, uint32_t seqs, const Q4Sp
   Q4Attention p = base;
   p.parts = split.parts ? workspace : nullptr;
   if (split.warps == 2) return launch_attention_warps<G, RP, 2>(p, seqs, split.chunks, stream);
-  if (split.warps == 8) return launch_attention_warps<G, RP, 8>(p, seqs, split.chunks, stream);
+  if (split.warps == 8) {
+    const uint64_t pairs = uint64_t(p.kv_heads) * p.blocks * seqs;
+    if (G == 1 && pairs > q4_resident(64, 8) * uint64_t(sm_count()))
+      return launch_attention_warps<G, RP, 8, G == 1 ? 3 : 2>(p, seqs, split.chunks, stream);
+    return launch_attention_warps<G, RP, 8>(p, seqs, split.chunks, stream);
+  }
   tempo_status status = launch_attention_warps<G, RP, 4>(p, seqs, split.chunks, stream);
   if (status != TEMPO_OK || !split.parts) return status;
   return launch(decode_merge_q4_kernel<G>, dim3(p.heads, seqs), dim3(kMergeThreads), 0, stream, 1, "decode_merge_q4_kernel", p,

@@ -219,6 +219,23 @@ def test_attention_over_grids_of_every_shape(seqs: int, heads: int, kv_heads: in
     _check_attention(qkv, cache, lengths, heads, got)
 
 
+@pytest.mark.parametrize("heads,kv_heads,head", [(12, 12, 64), (24, 12, 64), (48, 12, 64), (64, 8, 64), (12, 12, 128),
+                                                 (32, 8, 128), (64, 8, 128)])
+@pytest.mark.parametrize("seqs,length", [(3, 300), (20, 420), (30, 400), (45, 260), (260, 33), (2, 2000), (1, 6000)])
+def test_attention_over_every_split(seqs: int, length: int, heads: int, kv_heads: int, head: int) -> None:
+    """CTAs of two, four and eight warps, clusters and the workspace, for one to eight queries a key head."""
+    from tempo_compiler_b200 import ops
+    rng = np.random.default_rng(seqs)
+    cache = ops.kv_cache_q4(seqs, kv_heads, length, head)
+    _fill(cache, rng)
+    lengths = rng.integers(1, length + 1, seqs)
+    qkv = (_rows(rng, seqs, heads, head) * (1.5 / head ** 0.5)).reshape(seqs, -1)
+    got = ops.decode_attention_q4(qkv, cache, _i32(lengths), heads=heads)
+    some = np.unique(np.concatenate([[0, seqs - 1], rng.integers(0, seqs, 3)]))
+    index = torch.from_numpy(some).cuda()
+    _check_attention(qkv[index], cache[index], lengths[some], heads, got[index])
+
+
 def test_attention_reads_nothing_past_the_length() -> None:
     """NaN rows and a later, far greater key behind the last position change nothing."""
     from tempo_compiler_b200 import ops
