@@ -11,7 +11,7 @@
 // and so have no ties) and sorts them by counting. A row with more
 // ties at the bar than the lists hold, or with a NaN, is searched exactly, at a slower pace. Few rows are split over the
 // CTAs of a cluster, whose sums and sorted candidates the first one merges. (Collecting candidates on the way, against
-// a threshold that rose with the row, took 230 us for 8192 BF16 rows of 50257 instead of 163.)
+// a threshold that rose with the row, took 230 us for 8192 BF16 rows of 50257 when this took 163.)
 
 #include <cuda_runtime.h>
 
@@ -23,7 +23,9 @@ namespace {
 
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kWarps = kThreads / 32;
-constexpr uint32_t kVectors = 4;                    // 16-byte words of one thread and chunk
+// 16-byte words of one thread and chunk: as many as 64 registers hold (four CTAs an SM). 8192 BF16 rows with one alternative
+// take 160 us with five words, 163 with four, 172 with three, 175 with six, which spill.
+constexpr uint32_t kVectors = 5;
 constexpr uint32_t kChunk = kThreads * kVectors;    // a chunk, in 16-byte words
 constexpr uint32_t kLanes = 4;                      // of a group whose greatest keys give a threshold
 constexpr uint32_t kGroups = kThreads / kLanes;
@@ -357,7 +359,7 @@ __device__ __noinline__ Sums plain_sums(const T* row, uint32_t vocab, Sums* scra
 
 // A cluster of `chunks` CTAs per row, each taking a contiguous share of its 16-byte words. TOP: alternatives wanted.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_logprobs_kernel(LogprobParams p) {
+__global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(LogprobParams p) {
   using V = Logits<T>;
   constexpr uint32_t kN = 4 * V::kPerWord;  // logits of a 16-byte word
   extern __shared__ __align__(16) uint8_t raw[];
@@ -423,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) token_logprobs_kernel(L
     most = fmaxf(most, add<T>(s, w));
     if (TOP && ++in_cell == stride) close();
   }
-  // The words behind the whole chunks, a quarter chunk at a time, as far as the warp has any.
+  // The words behind the whole chunks, one of each thread at a time, as far as the warp has any.
 #pragma unroll
   for (uint32_t v = 0; v < kVectors; ++v) {
     const uint32_t at = begin + full * kChunk + v * kThreads + threadIdx.x;
