@@ -327,18 +327,27 @@ __device__ __forceinline__ float add(Sums& s, const uint32_t (&w)[N]) {
 }
 
 // A row's sums by one CTA in the plain units of the logits: d = x - greatest, the sums of e^d and d e^d (NaN when the row
-// holds a NaN or +infinity).
+// holds a NaN or +infinity; 0 when it holds nothing but -infinity). The greatest ignores NaN, so a row of NaN and -infinity
+// alone is told apart by looking for one.
 template <typename T>
 __device__ __noinline__ Sums plain_sums(const T* row, uint32_t vocab, Sums* scratch) {
   Sums s{-INFINITY, 0.f, 0.f};
-  for (uint32_t i = threadIdx.x; i < vocab; i += kThreads) s.m = fmaxf(s.m, Logits<T>::one(row + i));
+  bool nan = false;
+  for (uint32_t i = threadIdx.x; i < vocab; i += kThreads) {
+    const float x = Logits<T>::one(row + i);
+    nan = nan || x != x;
+    s.m = fmaxf(s.m, x);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s.m = fmaxf(s.m, __shfl_xor_sync(0xFFFFFFFFu, s.m, o));
   __syncthreads();
   if (lane_id() == 0) scratch[warp_id()].m = s.m;
-  __syncthreads();
+  nan = __syncthreads_or(nan);
   for (uint32_t w = 0; w < kWarps; ++w) s.m = fmaxf(s.m, scratch[w].m);
-  if (s.m == -INFINITY) return s;
+  if (s.m == -INFINITY) {
+    if (nan) s.l = s.t = __int_as_float(0x7FC00000);
+    return s;
+  }
   for (uint32_t i = threadIdx.x; i < vocab; i += kThreads) {
     const float below = Logits<T>::one(row + i) - s.m, d = below < -1000.f ? -1000.f : below, e = fast_exp2(d * kLog2e);
     s.l += e;
