@@ -256,11 +256,11 @@ tempo_status launch_rows(void (*kernel)(Q4Rows), Q4Rows p, uint32_t rows, uint32
 // weights of the other columns are zeroed before tile j's values are multiplied.
 // A query row is scaled by a power of two to at most 2, where FP16 holds its BF16 values but for what lies 2^-14 below its
 // greatest, and there to 2^-25; w is rounded to FP16 (2^-11 of each weight; an eighth of the output's own BF16 rounding),
-// relative to a running reference that bounds w and p low alike; everything else, the sums included, is FP32.
+// in a running unit that bounds w and p low alike; everything else, the sums included, is FP32.
 //
 // A CTA of four warps takes a run of tiles of one (sequence, key / value head, eight query heads); each warp streams its
-// own pieces (one bulk copy each, kRing in flight) and keeps an online softmax whose reference moves only when a weight
-// passes it kSlack times. Warps merge through shared memory; with `chunks` > 1 the CTAs of a cluster split the positions
+// own pieces (one bulk copy each, kRing in flight) and keeps an online softmax whose reference and unit move only when a
+// weight passes them kSlack times. Warps merge through shared memory; with `chunks` > 1 the CTAs of a cluster split the positions
 // and merge through distributed shared memory, or, when a pair needs more of them, through a workspace and a second kernel.
 // ---------------------------------------------------------------------------------------------------------------
 
@@ -269,19 +269,22 @@ constexpr uint32_t kQ4MaxSplits = 160;   // CTAs that share a pair through the w
 constexpr uint32_t kQ4Queries = 8;
 constexpr uint32_t kQ4Piece = 4 * kQ4Block;  // bytes of one bulk copy: four tiles of a 64-wide head, two of a 128-wide
 constexpr uint32_t kRing = 2;
-constexpr float kSlack = 64.f;
 constexpr float kNoScore = -3.4028235e38f;  // the reference before any position: no finite score is below it,
-constexpr float kNoSize = -128.f;           // and no value's size
+constexpr int kNoUnit = -100;               // and no unit
+// p = 2^(score - reference + kLift): its smallest, 2^-126, is 2^-150 of the greatest, as small as FP32 without the lift.
+constexpr float kLift = 24.f;
+constexpr float kSlack = 64.f;              // what w may reach before the unit moves,
+constexpr float kSlackP = 0x1p31f;          // and p times this before the reference does
 
 template <int G, int WARPS>
 struct Q4Smem {
   static constexpr uint32_t kWarpRing = kRing * kQ4Piece;
   // A partial result of eight queries: 64 G values each (dimension 64 i + 4 g + n at 64 i + 8 n + g, eight words more to
-  // the next query: the lanes of a fragment store into different banks), then the references' scores and sizes, then the
-  // sums.
+  // the next query: the lanes of a fragment store into different banks), then the references, the units' exponents and
+  // the sums.
   static constexpr uint32_t kStride = 64 * G + 8;
-  static constexpr uint32_t kReferences = kQ4Queries * kStride, kSizes = kReferences + kQ4Queries;
-  static constexpr uint32_t kSums = kSizes + kQ4Queries;
+  static constexpr uint32_t kReferences = kQ4Queries * kStride, kUnits = kReferences + kQ4Queries;
+  static constexpr uint32_t kSums = kUnits + kQ4Queries;
   static constexpr uint32_t kPart = (kSums + kQ4Queries) * 4;
   static constexpr uint32_t kBarrierOffset = WARPS * kWarpRing;
   static constexpr uint32_t kMergeOffset = kBarrierOffset + WARPS * kRing * 8;
@@ -359,10 +362,25 @@ __device__ __forceinline__ uint32_t swap_bytes(uint32_t w) { return __byte_perm(
 template <int G>
 struct Q4State {
   float acc[G][4][4];
-  float m[2], mg[2];         // the reference, log2 of p times the value's size, as a score and what lies above it
+  float m[2];                // the reference, a score
+  float inv[2];              // 1 / the unit (a power of two) in which acc, w and low are counted
   float l[2];                // this lane's sum of p
   float w[G][2], low[G][2];  // this lane's sums of w (as rounded) and of p low
 };
+
+__device__ __forceinline__ int unit_exponent(float inv) { return 127 - int(__float_as_uint(inv) >> 23); }
+__device__ __forceinline__ float inverse_unit(int exponent) { return __uint_as_float(uint32_t(127 - exponent) << 23); }
+
+__device__ __forceinline__ float q4_weight(float score, float reference) { return fast_exp2(score - reference + kLift); }
+
+// Moves a unit to hold weights of 2^(x + kLift) and what it held, whose reference rises by -down: returns the factor that
+// brings that to the new unit, at most 1.
+__device__ __forceinline__ float q4_move(float& inv, float down, float x) {
+  const int was = unit_exponent(inv);
+  const int now = int(fminf(fmaxf(fmaxf(ceilf(x) + kLift, ceilf(down) + float(was)), float(kNoUnit)), 126.f));
+  inv = inverse_unit(now);
+  return fast_exp2(down + float(was - now));
+}
 
 // Columns of a tile: the RP query heads, or two (the odd one empty) for a single head, which leaves half of each lane's
 // softmax out.
@@ -438,13 +456,16 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
   s1 = in0 ? __fmul_rn(s1, unit[1]) : -INFINITY;
   s2 = in1 ? __fmul_rn(s2, unit[0]) : -INFINITY;
   s3 = in1 ? __fmul_rn(s3, unit[1]) : -INFINITY;
-  // The reference follows log2(p size), size the value row's scale or a sixteenth of its low: w and p low stay small
-  // whatever the values' size, and a position of small values needs a larger p to move it. It is kept as a score and a size
-  // (p = 2^(score - m - mg)): beside a score of 2^30 their sum would round the size away. It moves when p size passes
-  // kSlack, which NaN and infinity do too.
-  float p0 = fast_exp2(s0 - st.m[0] - st.mg[0]), p2 = fast_exp2(s2 - st.m[0] - st.mg[0]);
-  float p1 = kTwo ? fast_exp2(s1 - st.m[1] - st.mg[1]) : 0.f, p3 = kTwo ? fast_exp2(s3 - st.m[1] - st.mg[1]) : 0.f;
-  const bool far0 = !(fmaf(p0, size0, p2 * size1) <= kSlack), far1 = kTwo && !(fmaf(p1, size0, p3 * size1) <= kSlack);
+  // The reference is a score and follows the scores alone: the sum l of p = 2^(score - m + kLift) keeps every position's
+  // share, whatever the values. The weights w = p scale and p low are counted in a unit of their own, a power of two that
+  // follows p size, size the value row's scale or a sixteenth of its low, so they stay small whatever the values' size.
+  // Both move when w passes kSlack or p 2^(kLift + 7) (which NaN and infinity do too).
+  float p0 = q4_weight(s0, st.m[0]), p2 = q4_weight(s2, st.m[0]);
+  float p1 = kTwo ? q4_weight(s1, st.m[1]) : 0.f, p3 = kTwo ? q4_weight(s3, st.m[1]) : 0.f;
+  auto far = [&](float a, float b, float inv) {
+    return !(fmaf(a * inv, size0, fmaf(b * inv, size1, (a + b) * (kSlack / kSlackP))) <= kSlack);
+  };
+  const bool far0 = far(p0, p2, st.inv[0]), far1 = kTwo && far(p1, p3, st.inv[1]);
   if (__any_sync(0xFFFFFFFFu, far0 || far1)) {
     const float g0 = fast_log2(fminf(size0, 0x1p100f)), g1 = fast_log2(fminf(size1, 0x1p100f));
     float m0 = fmax3(s0, s2, st.m[0]), m1 = kTwo ? fmax3(s1, s3, st.m[1]) : 0.f;
@@ -459,24 +480,18 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
       x0 = fmaxf(x0, __shfl_xor_sync(0xFFFFFFFFu, x0, o));
       if (kTwo) x1 = fmaxf(x1, __shfl_xor_sync(0xFFFFFFFFu, x1, o));
     }
-    const float was0 = st.m[0] - m0 + st.mg[0];
-    x0 = fmaxf(x0, was0);
-    const float c0 = fast_exp2(was0 - x0);
+    const float c0 = q4_move(st.inv[0], st.m[0] - m0, x0), l0 = fast_exp2(st.m[0] - m0);
     st.m[0] = m0;
-    st.mg[0] = x0;
-    st.l[0] *= c0;
-    p0 = fast_exp2(s0 - m0 - x0);
-    p2 = fast_exp2(s2 - m0 - x0);
+    st.l[0] *= l0;
+    p0 = q4_weight(s0, m0);
+    p2 = q4_weight(s2, m0);
     float c1 = 0.f;
     if (kTwo) {
-      const float was1 = st.m[1] - m1 + st.mg[1];
-      x1 = fmaxf(x1, was1);
-      c1 = fast_exp2(was1 - x1);
+      c1 = q4_move(st.inv[1], st.m[1] - m1, x1);
+      st.l[1] *= fast_exp2(st.m[1] - m1);
       st.m[1] = m1;
-      st.mg[1] = x1;
-      st.l[1] *= c1;
-      p1 = fast_exp2(s1 - m1 - x1);
-      p3 = fast_exp2(s3 - m1 - x1);
+      p1 = q4_weight(s1, m1);
+      p3 = q4_weight(s3, m1);
     }
 #pragma unroll
     for (int i = 0; i < G; ++i) {
@@ -499,6 +514,10 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
   }
   st.l[0] += p0 + p2;
   if (kTwo) st.l[1] += p1 + p3;
+  p0 *= st.inv[0];
+  p2 *= st.inv[0];
+  p1 *= st.inv[1];
+  p3 *= st.inv[1];
   uint32_t b0[G], b1[G];
 #pragma unroll
   for (int i = 0; i < G; ++i) {
@@ -544,29 +563,29 @@ __device__ __forceinline__ float ld_cluster(const float* local, uint32_t rank) {
 // The dimension of word `at` of a query's values in a partial result.
 __device__ __forceinline__ uint32_t q4_dimension(uint32_t at) { return (at & ~31u) | (at & 7u) << 2 | (at >> 3 & 3u); }
 
-// Word `at` (of query `query`) of up to MOST partial results, of which there are `count`, brought to one reference; word(c, i)
-// reads word i of partial result c.
+// Word `at` (of query `query`) of up to MOST partial results, of which there are `count`, brought to one reference and one
+// unit; word(c, i) reads word i of partial result c.
 struct Merged {
-  float m, mg, l, a;
+  float m, e, l, a;  // the reference, the unit's exponent, the sum and the value
+  __device__ __forceinline__ float average() const { return a / l * fast_exp2(e); }
 };
 template <typename L, uint32_t MOST, typename Word>
 __device__ __forceinline__ Merged merge_parts(uint32_t count, uint32_t query, uint32_t at, Word word) {
-  float m[MOST], mg[MOST];
+  float m[MOST], e[MOST];
   Merged r{kNoScore, -INFINITY, 0.f, 0.f};
 #pragma unroll
   for (uint32_t c = 0; c < MOST; ++c) {
     m[c] = c < count ? word(c, L::kReferences + query) : kNoScore;
-    mg[c] = c < count ? word(c, L::kSizes + query) : kNoSize;
+    e[c] = c < count ? word(c, L::kUnits + query) : float(kNoUnit);
     r.m = fmaxf(r.m, m[c]);
   }
 #pragma unroll
-  for (uint32_t c = 0; c < MOST; ++c) r.mg = fmaxf(r.mg, m[c] - r.m + mg[c]);
+  for (uint32_t c = 0; c < MOST; ++c) r.e = fmaxf(r.e, m[c] - r.m + e[c]);
 #pragma unroll
   for (uint32_t c = 0; c < MOST; ++c) {
     if (c >= count) break;
-    const float f = fast_exp2(m[c] - r.m + mg[c] - r.mg);
-    r.l = fmaf(word(c, L::kSums + query), f, r.l);
-    r.a = fmaf(word(c, at), f, r.a);
+    r.l = fmaf(word(c, L::kSums + query), fast_exp2(m[c] - r.m), r.l);
+    r.a = fmaf(word(c, at), fast_exp2(m[c] - r.m + e[c] - r.e), r.a);
   }
   return r;
 }
@@ -687,7 +706,7 @@ __global__ void __launch_bounds__(32 * WARPS, RESIDENT) decode_attention_q4_kern
 
   Q4State<G> st;
   st.m[0] = st.m[1] = kNoScore;
-  st.mg[0] = st.mg[1] = kNoSize;
+  st.inv[0] = st.inv[1] = inverse_unit(kNoUnit);
   st.l[0] = st.l[1] = 0.f;
 #pragma unroll
   for (int i = 0; i < G; ++i) {
@@ -730,7 +749,7 @@ __global__ void __launch_bounds__(32 * WARPS, RESIDENT) decode_attention_q4_kern
   }
   if (!p.early) pdl_launch_dependents();
 
-  // The warp's partial result, (values at the reference, reference, sum) of each query, into its own ring: the columns of
+  // The warp's partial result, (values in the unit, reference, unit, sum) of each query, into its own ring: the columns of
   // one query (CP / 2 lanes apart) and the lanes' sums come together first.
   __syncwarp();
   float* part = reinterpret_cast<float*>(ring);
@@ -739,12 +758,12 @@ __global__ void __launch_bounds__(32 * WARPS, RESIDENT) decode_attention_q4_kern
     float m = st.m[c];
 #pragma unroll
     for (int o = CP / 2; o < 4; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    const float own = st.m[c] - m + st.mg[c];
-    float mg = own;
+    const float own = st.m[c] - m + float(unit_exponent(st.inv[c]));
+    float e = own;
 #pragma unroll
-    for (int o = CP / 2; o < 4; o <<= 1) mg = fmaxf(mg, __shfl_xor_sync(0xFFFFFFFFu, mg, o));
-    const float f = fast_exp2(own - mg);
-    float l = st.l[c] * f;
+    for (int o = CP / 2; o < 4; o <<= 1) e = fmaxf(e, __shfl_xor_sync(0xFFFFFFFFu, e, o));
+    const float f = fast_exp2(own - e);
+    float l = st.l[c] * fast_exp2(st.m[c] - m);
 #pragma unroll
     for (int o = CP / 2; o < 32; o <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
     const uint32_t query = 2 * t % CP + c;
@@ -770,7 +789,7 @@ __global__ void __launch_bounds__(32 * WARPS, RESIDENT) decode_attention_q4_kern
     }
     if (g == 0 && writes) {
       part[L::kReferences + query] = m;
-      part[L::kSizes + query] = mg;
+      part[L::kUnits + query] = e;
       part[L::kSums + query] = l;
     }
   }
@@ -786,12 +805,12 @@ __global__ void __launch_bounds__(32 * WARPS, RESIDENT) decode_attention_q4_kern
     const Merged r = merge_parts<L, WARPS>(
         WARPS, query, at, [&](uint32_t w, uint32_t i) { return reinterpret_cast<const float*>(smem + w * L::kWarpRing)[i]; });
     if (whole) {
-      out[query * kWidth + q4_dimension(i % kWidth)] = float_to_bf16(len == 0 ? 0.f : r.a / r.l);
+      out[query * kWidth + q4_dimension(i % kWidth)] = float_to_bf16(len == 0 ? 0.f : r.average());
     } else {
       merge[at] = r.a;
       if (i % kWidth == 0) {
         merge[L::kReferences + query] = r.m;
-        merge[L::kSizes + query] = r.mg;
+        merge[L::kUnits + query] = r.e;
         merge[L::kSums + query] = r.l;
       }
     }
@@ -803,7 +822,7 @@ __global__ void __launch_bounds__(32 * WARPS, RESIDENT) decode_attention_q4_kern
     const uint32_t query = i / kWidth, at = query * L::kStride + i % kWidth;
     const Merged r = merge_parts<L, kQ4MaxChunks>(chunks, query, at,
                                                   [&](uint32_t c, uint32_t i) { return ld_cluster(merge + i, c); });
-    out[query * kWidth + q4_dimension(i % kWidth)] = float_to_bf16(len == 0 ? 0.f : r.a / r.l);
+    out[query * kWidth + q4_dimension(i % kWidth)] = float_to_bf16(len == 0 ? 0.f : r.average());
   }
   // No CTA leaves while another may still read its shared memory.
   asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
@@ -820,7 +839,7 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_q4_kernel(Q4Attent
   using L = Q4Smem<G, 4>;
   constexpr uint32_t kWidth = 64 * G, kShares = kMergeThreads / kWidth, kPart = L::kPart / 4;
   __shared__ float factor[(kQ4MaxSplits + kMergeBatch * kShares - 1) / (kMergeBatch * kShares) * (kMergeBatch * kShares)];
-  __shared__ float warp_m[kMergeThreads / 32], warp_mg[kMergeThreads / 32], warp_l[kMergeThreads / 32];
+  __shared__ float warp_m[kMergeThreads / 32], warp_e[kMergeThreads / 32], warp_l[kMergeThreads / 32];
   __shared__ float sums[kShares][kWidth];
   pdl_wait();
   pdl_launch_dependents();
@@ -840,7 +859,7 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_q4_kernel(Q4Attent
   load(0);
   const bool has = threadIdx.x < chunks;
   const float m = has ? parts[threadIdx.x * kPart + L::kReferences + query] : kNoScore;
-  const float mg = has ? parts[threadIdx.x * kPart + L::kSizes + query] : kNoSize;
+  const float e = has ? parts[threadIdx.x * kPart + L::kUnits + query] : float(kNoUnit);
   const float part_l = has ? parts[threadIdx.x * kPart + L::kSums + query] : 0.f;
   auto greatest = [&](float x, float* of_warps) {
 #pragma unroll
@@ -851,9 +870,9 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_q4_kernel(Q4Attent
     for (uint32_t w = 0; w < (kQ4MaxSplits + 31) / 32; ++w) x = fmaxf(x, of_warps[w]);  // (the others have none)
     return x;
   };
-  const float above = m - greatest(m, warp_m) + mg;
-  const float f = fast_exp2(above - greatest(above, warp_mg)), l_warp = warp_sum(part_l * f);
-  if (threadIdx.x < sizeof(factor) / 4) factor[threadIdx.x] = has ? f : 0.f;
+  const float below = m - greatest(m, warp_m), l_warp = warp_sum(part_l * fast_exp2(below));
+  const float unit = greatest(below + e, warp_e);
+  if (threadIdx.x < sizeof(factor) / 4) factor[threadIdx.x] = has ? fast_exp2(below + e - unit) : 0.f;
   if (lane_id() == 0) warp_l[warp_id()] = l_warp;
   __syncthreads();
   float a = 0.f;
@@ -872,7 +891,7 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_q4_kernel(Q4Attent
 #pragma unroll
   for (uint32_t i = 0; i < kShares; ++i) a += sums[i][at];
   const bool empty = int64_t(p.lengths[s]) + p.length_offset <= 0;
-  p.out[(size_t(s) * p.heads + h) * kWidth + q4_dimension(at)] = float_to_bf16(empty ? 0.f : a / l);
+  p.out[(size_t(s) * p.heads + h) * kWidth + q4_dimension(at)] = float_to_bf16(empty ? 0.f : Merged{0.f, unit, l, a}.average());
 }
 
 // How the positions of a pair (a sequence's key / value head and block of query heads) are shared out: CTAs of `warps`
