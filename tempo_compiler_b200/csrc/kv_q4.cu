@@ -280,11 +280,11 @@ template <int G, int WARPS>
 struct Q4Smem {
   static constexpr uint32_t kWarpRing = kRing * kQ4Piece;
   // A partial result of eight queries: 64 G values each (dimension 64 i + 4 g + n at 64 i + 8 n + g, eight words more to
-  // the next query: the lanes of a fragment store into different banks), then the references, the units' exponents and
-  // the sums.
+  // the next query: the lanes of a fragment store into different banks), then the references, the units' exponents
+  // (eight of each group) and the sums.
   static constexpr uint32_t kStride = 64 * G + 8;
   static constexpr uint32_t kReferences = kQ4Queries * kStride, kUnits = kReferences + kQ4Queries;
-  static constexpr uint32_t kSums = kUnits + kQ4Queries;
+  static constexpr uint32_t kSums = kUnits + G * kQ4Queries;
   static constexpr uint32_t kPart = (kSums + kQ4Queries) * 4;
   static constexpr uint32_t kBarrierOffset = WARPS * kWarpRing;
   static constexpr uint32_t kMergeOffset = kBarrierOffset + WARPS * kRing * 8;
@@ -363,7 +363,7 @@ template <int G>
 struct Q4State {
   float acc[G][4][4];
   float m[2];                // the reference, a score
-  float inv[2];              // 1 / the unit (a power of two) in which acc, w and low are counted
+  float inv[G][2];           // 1 / the unit (a power of two) in which a group's acc, w and low are counted
   float l[2];                // this lane's sum of p
   float w[G][2], low[G][2];  // this lane's sums of w (as rounded) and of p low
 };
@@ -432,7 +432,7 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
   const bool in1 = (TP == 4 || mine < TP) && (FULL || mine * kQ4Tile + pg + 8 < left);
   const uint8_t* own = tiles + (TP == 4 || mine < TP ? mine : 0u) * kTileBytes + 2 * kQ4Codes;
   float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;  // scores (log2): rows g and g + 8, columns 2 t and 2 t + 1
-  float size0 = 0x1p-100f, size1 = 0x1p-100f;
+  float size0[G], size1[G];
   uint32_t vm0[G], vm1[G];
 #pragma unroll
   for (int i = 0; i < G; ++i) {
@@ -448,8 +448,8 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
     if (kTwo) s3 = fmaf(ks1, d[i][3], fmaf(kl1, qs[i][1], s3));
     vm0[i] = meta0.y;
     vm1[i] = meta1.y;
-    size0 = fmax3(size0, bf16_lo(meta0.y), 0.0625f * fabsf(bf16_hi(meta0.y)));
-    size1 = fmax3(size1, bf16_lo(meta1.y), 0.0625f * fabsf(bf16_hi(meta1.y)));
+    size0[i] = fmax3(0x1p-100f, bf16_lo(meta0.y), 0.0625f * fabsf(bf16_hi(meta0.y)));
+    size1[i] = fmax3(0x1p-100f, bf16_lo(meta1.y), 0.0625f * fabsf(bf16_hi(meta1.y)));
   }
   // (not joined with the differences below: a product that is rounded here and not there is off by its own rounding)
   s0 = in0 ? __fmul_rn(s0, unit[0]) : -INFINITY;
@@ -457,44 +457,37 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
   s2 = in1 ? __fmul_rn(s2, unit[0]) : -INFINITY;
   s3 = in1 ? __fmul_rn(s3, unit[1]) : -INFINITY;
   // The reference is a score and follows the scores alone: the sum l of p = 2^(score - m + kLift) keeps every position's
-  // share, whatever the values. The weights w = p scale and p low are counted in a unit of their own, a power of two that
-  // follows p size, size the value row's scale or a sixteenth of its low, so they stay small whatever the values' size.
-  // Both move when w passes kSlack or p 2^(kLift + 7) (which NaN and infinity do too).
+  // share, whatever the values. A group's weights w = p scale and p low are counted in a unit of their own, a power of two
+  // that follows p size, size the value row's scale or a sixteenth of its low, so they stay small whatever the values' size
+  // and the halves of a head of 128 keep their bits beside one another. Reference and units move when w passes kSlack
+  // or p 2^(kLift + 7) (which NaN and infinity do too).
   float p0 = q4_weight(s0, st.m[0]), p2 = q4_weight(s2, st.m[0]);
   float p1 = kTwo ? q4_weight(s1, st.m[1]) : 0.f, p3 = kTwo ? q4_weight(s3, st.m[1]) : 0.f;
-  auto far = [&](float a, float b, float inv) {
-    return !(fmaf(a * inv, size0, fmaf(b * inv, size1, (a + b) * (kSlack / kSlackP))) <= kSlack);
+  auto far = [&](float a, float b, int c) {
+    float sum = (a + b) * (kSlack / kSlackP);
+#pragma unroll
+    for (int i = 0; i < G; ++i) sum = fmaf(a * st.inv[i][c], size0[i], fmaf(b * st.inv[i][c], size1[i], sum));
+    return !(sum <= kSlack);
   };
-  const bool far0 = far(p0, p2, st.inv[0]), far1 = kTwo && far(p1, p3, st.inv[1]);
+  const bool far0 = far(p0, p2, 0), far1 = kTwo && far(p1, p3, 1);
   if (__any_sync(0xFFFFFFFFu, far0 || far1)) {
-    const float g0 = fast_log2(fminf(size0, 0x1p100f)), g1 = fast_log2(fminf(size1, 0x1p100f));
     float m0 = fmax3(s0, s2, st.m[0]), m1 = kTwo ? fmax3(s1, s3, st.m[1]) : 0.f;
 #pragma unroll
     for (int o = 4; o <= 16; o <<= 1) {
       m0 = fmaxf(m0, __shfl_xor_sync(0xFFFFFFFFu, m0, o));
       if (kTwo) m1 = fmaxf(m1, __shfl_xor_sync(0xFFFFFFFFu, m1, o));
     }
-    float x0 = fmaxf(s0 - m0 + g0, s2 - m0 + g1), x1 = kTwo ? fmaxf(s1 - m1 + g0, s3 - m1 + g1) : 0.f;
-#pragma unroll
-    for (int o = 4; o <= 16; o <<= 1) {
-      x0 = fmaxf(x0, __shfl_xor_sync(0xFFFFFFFFu, x0, o));
-      if (kTwo) x1 = fmaxf(x1, __shfl_xor_sync(0xFFFFFFFFu, x1, o));
-    }
-    const float c0 = q4_move(st.inv[0], st.m[0] - m0, x0), l0 = fast_exp2(st.m[0] - m0);
-    st.m[0] = m0;
-    st.l[0] *= l0;
-    p0 = q4_weight(s0, m0);
-    p2 = q4_weight(s2, m0);
-    float c1 = 0.f;
-    if (kTwo) {
-      c1 = q4_move(st.inv[1], st.m[1] - m1, x1);
-      st.l[1] *= fast_exp2(st.m[1] - m1);
-      st.m[1] = m1;
-      p1 = q4_weight(s1, m1);
-      p3 = q4_weight(s3, m1);
-    }
+    const float down0 = st.m[0] - m0, down1 = kTwo ? st.m[1] - m1 : 0.f;
 #pragma unroll
     for (int i = 0; i < G; ++i) {
+      const float g0 = fast_log2(fminf(size0[i], 0x1p100f)), g1 = fast_log2(fminf(size1[i], 0x1p100f));
+      float x0 = fmaxf(s0 - m0 + g0, s2 - m0 + g1), x1 = kTwo ? fmaxf(s1 - m1 + g0, s3 - m1 + g1) : 0.f;
+#pragma unroll
+      for (int o = 4; o <= 16; o <<= 1) {
+        x0 = fmaxf(x0, __shfl_xor_sync(0xFFFFFFFFu, x0, o));
+        if (kTwo) x1 = fmaxf(x1, __shfl_xor_sync(0xFFFFFFFFu, x1, o));
+      }
+      const float c0 = q4_move(st.inv[i][0], down0, x0), c1 = kTwo ? q4_move(st.inv[i][1], down1, x1) : 0.f;
       st.w[i][0] *= c0;
       st.low[i][0] *= c0;
       if (kTwo) {
@@ -511,24 +504,32 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
         }
       }
     }
+    st.m[0] = m0;
+    st.l[0] *= fast_exp2(down0);
+    p0 = q4_weight(s0, m0);
+    p2 = q4_weight(s2, m0);
+    if (kTwo) {
+      st.m[1] = m1;
+      st.l[1] *= fast_exp2(down1);
+      p1 = q4_weight(s1, m1);
+      p3 = q4_weight(s3, m1);
+    }
   }
   st.l[0] += p0 + p2;
   if (kTwo) st.l[1] += p1 + p3;
-  p0 *= st.inv[0];
-  p2 *= st.inv[0];
-  p1 *= st.inv[1];
-  p3 *= st.inv[1];
   uint32_t b0[G], b1[G];
 #pragma unroll
   for (int i = 0; i < G; ++i) {
     const float vs0 = bf16_lo(vm0[i]), vs1 = bf16_lo(vm1[i]), vl0 = bf16_hi(vm0[i]), vl1 = bf16_hi(vm1[i]);
-    const __half2 h0 = __floats2half2_rn(p0 * vs0, kTwo ? p1 * vs0 : 0.f);
-    const __half2 h1 = __floats2half2_rn(p2 * vs1, kTwo ? p3 * vs1 : 0.f);
+    const float u0 = p0 * st.inv[i][0], u2 = p2 * st.inv[i][0];
+    const float u1 = kTwo ? p1 * st.inv[i][1] : 0.f, u3 = kTwo ? p3 * st.inv[i][1] : 0.f;
+    const __half2 h0 = __floats2half2_rn(u0 * vs0, kTwo ? u1 * vs0 : 0.f);
+    const __half2 h1 = __floats2half2_rn(u2 * vs1, kTwo ? u3 * vs1 : 0.f);
     st.w[i][0] += __low2float(h0) + __low2float(h1);
-    st.low[i][0] = fmaf(p0, vl0, fmaf(p2, vl1, st.low[i][0]));
+    st.low[i][0] = fmaf(u0, vl0, fmaf(u2, vl1, st.low[i][0]));
     if (kTwo) {
       st.w[i][1] += __high2float(h0) + __high2float(h1);
-      st.low[i][1] = fmaf(p1, vl0, fmaf(p3, vl1, st.low[i][1]));
+      st.low[i][1] = fmaf(u1, vl0, fmaf(u3, vl1, st.low[i][1]));
     }
     b0[i] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h0));
     b1[i] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h1));
@@ -563,20 +564,20 @@ __device__ __forceinline__ float ld_cluster(const float* local, uint32_t rank) {
 // The dimension of word `at` of a query's values in a partial result.
 __device__ __forceinline__ uint32_t q4_dimension(uint32_t at) { return (at & ~31u) | (at & 7u) << 2 | (at >> 3 & 3u); }
 
-// Word `at` (of query `query`) of up to MOST partial results, of which there are `count`, brought to one reference and one
-// unit; word(c, i) reads word i of partial result c.
+// Word `at` (of query `query`, in group `group`) of up to MOST partial results, of which there are `count`, brought to one
+// reference and one unit; word(c, i) reads word i of partial result c.
 struct Merged {
   float m, e, l, a;  // the reference, the unit's exponent, the sum and the value
   __device__ __forceinline__ float average() const { return a / l * fast_exp2(e); }
 };
 template <typename L, uint32_t MOST, typename Word>
-__device__ __forceinline__ Merged merge_parts(uint32_t count, uint32_t query, uint32_t at, Word word) {
+__device__ __forceinline__ Merged merge_parts(uint32_t count, uint32_t query, uint32_t group, uint32_t at, Word word) {
   float m[MOST], e[MOST];
   Merged r{kNoScore, -INFINITY, 0.f, 0.f};
 #pragma unroll
   for (uint32_t c = 0; c < MOST; ++c) {
     m[c] = c < count ? word(c, L::kReferences + query) : kNoScore;
-    e[c] = c < count ? word(c, L::kUnits + query) : float(kNoUnit);
+    e[c] = c < count ? word(c, L::kUnits + group * kQ4Queries + query) : float(kNoUnit);
     r.m = fmaxf(r.m, m[c]);
   }
 #pragma unroll
@@ -706,10 +707,10 @@ __global__ void __launch_bounds__(32 * WARPS, RESIDENT) decode_attention_q4_kern
 
   Q4State<G> st;
   st.m[0] = st.m[1] = kNoScore;
-  st.inv[0] = st.inv[1] = inverse_unit(kNoUnit);
   st.l[0] = st.l[1] = 0.f;
 #pragma unroll
   for (int i = 0; i < G; ++i) {
+    st.inv[i][0] = st.inv[i][1] = inverse_unit(kNoUnit);
     st.w[i][0] = st.w[i][1] = st.low[i][0] = st.low[i][1] = 0.f;
 #pragma unroll
     for (int n = 0; n < 4; ++n)
@@ -758,11 +759,6 @@ __global__ void __launch_bounds__(32 * WARPS, RESIDENT) decode_attention_q4_kern
     float m = st.m[c];
 #pragma unroll
     for (int o = CP / 2; o < 4; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    const float own = st.m[c] - m + float(unit_exponent(st.inv[c]));
-    float e = own;
-#pragma unroll
-    for (int o = CP / 2; o < 4; o <<= 1) e = fmaxf(e, __shfl_xor_sync(0xFFFFFFFFu, e, o));
-    const float f = fast_exp2(own - e);
     float l = st.l[c] * fast_exp2(st.m[c] - m);
 #pragma unroll
     for (int o = CP / 2; o < 32; o <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
@@ -770,6 +766,12 @@ __global__ void __launch_bounds__(32 * WARPS, RESIDENT) decode_attention_q4_kern
     const bool writes = 2 * t < CP && query < queries;
 #pragma unroll
     for (int i = 0; i < G; ++i) {
+      const float own = st.m[c] - m + float(unit_exponent(st.inv[i][c]));
+      float e = own;
+#pragma unroll
+      for (int o = CP / 2; o < 4; o <<= 1) e = fmaxf(e, __shfl_xor_sync(0xFFFFFFFFu, e, o));
+      const float f = fast_exp2(own - e);
+      if (g == 0 && writes) part[L::kUnits + i * kQ4Queries + query] = e;
       float rest = fmaf(-64.f, st.w[i][c], st.low[i][c]) * f;
 #pragma unroll
       for (int o = CP / 2; o < 32; o <<= 1) rest += __shfl_xor_sync(0xFFFFFFFFu, rest, o);
@@ -789,7 +791,6 @@ __global__ void __launch_bounds__(32 * WARPS, RESIDENT) decode_attention_q4_kern
     }
     if (g == 0 && writes) {
       part[L::kReferences + query] = m;
-      part[L::kUnits + query] = e;
       part[L::kSums + query] = l;
     }
   }
@@ -802,15 +803,16 @@ __global__ void __launch_bounds__(32 * WARPS, RESIDENT) decode_attention_q4_kern
   uint16_t* out = p.out + (size_t(s) * p.heads + kvh * share + first) * kWidth;
   for (uint32_t i = threadIdx.x; i < queries * kWidth; i += 32 * WARPS) {
     const uint32_t query = i / kWidth, at = query * L::kStride + i % kWidth;
+    const uint32_t group = i % kWidth / 64;
     const Merged r = merge_parts<L, WARPS>(
-        WARPS, query, at, [&](uint32_t w, uint32_t i) { return reinterpret_cast<const float*>(smem + w * L::kWarpRing)[i]; });
+        WARPS, query, group, at, [&](uint32_t w, uint32_t i) { return reinterpret_cast<const float*>(smem + w * L::kWarpRing)[i]; });
     if (whole) {
       out[query * kWidth + q4_dimension(i % kWidth)] = float_to_bf16(len == 0 ? 0.f : r.average());
     } else {
       merge[at] = r.a;
+      if (i % 64 == 0) merge[L::kUnits + group * kQ4Queries + query] = r.e;
       if (i % kWidth == 0) {
         merge[L::kReferences + query] = r.m;
-        merge[L::kUnits + query] = r.e;
         merge[L::kSums + query] = r.l;
       }
     }
@@ -820,7 +822,7 @@ __global__ void __launch_bounds__(32 * WARPS, RESIDENT) decode_attention_q4_kern
   // Each CTA finishes its share of the outputs, reading every CTA's partial result.
   for (uint32_t i = chunk * 32 * WARPS + threadIdx.x; i < queries * kWidth; i += chunks * 32 * WARPS) {
     const uint32_t query = i / kWidth, at = query * L::kStride + i % kWidth;
-    const Merged r = merge_parts<L, kQ4MaxChunks>(chunks, query, at,
+    const Merged r = merge_parts<L, kQ4MaxChunks>(chunks, query, i % kWidth / 64, at,
                                                   [&](uint32_t c, uint32_t i) { return ld_cluster(merge + i, c); });
     out[query * kWidth + q4_dimension(i % kWidth)] = float_to_bf16(len == 0 ? 0.f : r.average());
   }
@@ -838,8 +840,9 @@ template <int G>
 __global__ void __launch_bounds__(kMergeThreads) decode_merge_q4_kernel(Q4Attention p, uint32_t chunks, uint32_t rp) {
   using L = Q4Smem<G, 4>;
   constexpr uint32_t kWidth = 64 * G, kShares = kMergeThreads / kWidth, kPart = L::kPart / 4;
-  __shared__ float factor[(kQ4MaxSplits + kMergeBatch * kShares - 1) / (kMergeBatch * kShares) * (kMergeBatch * kShares)];
-  __shared__ float warp_m[kMergeThreads / 32], warp_e[kMergeThreads / 32], warp_l[kMergeThreads / 32];
+  constexpr uint32_t kFactors = (kQ4MaxSplits + kMergeBatch * kShares - 1) / (kMergeBatch * kShares) * (kMergeBatch * kShares);
+  __shared__ float factor[G][kFactors];
+  __shared__ float warp_m[kMergeThreads / 32], warp_e[G][kMergeThreads / 32], warp_l[kMergeThreads / 32];
   __shared__ float sums[kShares][kWidth];
   pdl_wait();
   pdl_launch_dependents();
@@ -859,7 +862,10 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_q4_kernel(Q4Attent
   load(0);
   const bool has = threadIdx.x < chunks;
   const float m = has ? parts[threadIdx.x * kPart + L::kReferences + query] : kNoScore;
-  const float e = has ? parts[threadIdx.x * kPart + L::kUnits + query] : float(kNoUnit);
+  float e[G], unit[G];
+#pragma unroll
+  for (int i = 0; i < G; ++i)
+    e[i] = has ? parts[threadIdx.x * kPart + L::kUnits + i * kQ4Queries + query] : float(kNoUnit);
   const float part_l = has ? parts[threadIdx.x * kPart + L::kSums + query] : 0.f;
   auto greatest = [&](float x, float* of_warps) {
 #pragma unroll
@@ -871,15 +877,18 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_q4_kernel(Q4Attent
     return x;
   };
   const float below = m - greatest(m, warp_m), l_warp = warp_sum(part_l * fast_exp2(below));
-  const float unit = greatest(below + e, warp_e);
-  if (threadIdx.x < sizeof(factor) / 4) factor[threadIdx.x] = has ? fast_exp2(below + e - unit) : 0.f;
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    unit[i] = greatest(below + e[i], warp_e[i]);
+    if (threadIdx.x < kFactors) factor[i][threadIdx.x] = has ? fast_exp2(below + e[i] - unit[i]) : 0.f;
+  }
   if (lane_id() == 0) warp_l[warp_id()] = l_warp;
   __syncthreads();
   float a = 0.f;
   for (uint32_t from = 0; from < chunks; from += kMergeBatch * kShares) {
     if (from > 0) load(from);
 #pragma unroll
-    for (uint32_t i = 0; i < kMergeBatch; ++i) a = fmaf(v[i], factor[from + part + i * kShares], a);
+    for (uint32_t i = 0; i < kMergeBatch; ++i) a = fmaf(v[i], factor[at / 64][from + part + i * kShares], a);
   }
   sums[part][at] = a;
   __syncthreads();
@@ -891,7 +900,7 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_q4_kernel(Q4Attent
 #pragma unroll
   for (uint32_t i = 0; i < kShares; ++i) a += sums[i][at];
   const bool empty = int64_t(p.lengths[s]) + p.length_offset <= 0;
-  p.out[(size_t(s) * p.heads + h) * kWidth + q4_dimension(at)] = float_to_bf16(empty ? 0.f : Merged{0.f, unit, l, a}.average());
+  p.out[(size_t(s) * p.heads + h) * kWidth + q4_dimension(at)] = float_to_bf16(empty ? 0.f : Merged{0.f, at < 64 ? unit[0] : unit[G - 1], l, a}.average());
 }
 
 // How the positions of a pair (a sequence's key / value head and block of query heads) are shared out: CTAs of `warps`

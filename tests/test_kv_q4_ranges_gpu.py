@@ -105,3 +105,17 @@ def test_runs_of_zero_values_beside_large_ones(head: int, n: int, copies: int, s
     q[0] = 0.0
     for heads in (1, 4):
         _check(q[:heads], held, _attend(q[:heads], cache, n, heads, copies))
+
+
+@pytest.mark.parametrize("n,copies", SPLITS)
+@pytest.mark.parametrize("ratio", [1e-3, 1e-5, 1e-7, 1e-10, 1e-20, 0.0])
+@pytest.mark.parametrize("smaller", [0, 1])
+def test_halves_of_a_value_row_of_different_size(n: int, copies: int, ratio: float, smaller: int) -> None:
+    """Each 64 of a head's 128 dimensions are as exact as they would be alone."""
+    rng = np.random.default_rng(n + copies)
+    keys, values = rng.standard_normal((2, n, 128))
+    values[:, 64 * smaller:64 * smaller + 64] *= ratio
+    cache, held = _cached(keys, values)
+    q = _bf16(rng.standard_normal((4, 128)) * 0.1)
+    for heads in (1, 4):
+        _check(q[:heads], held, _attend(q[:heads], cache, n, heads, copies))
