@@ -240,10 +240,12 @@ tempo_status launch_rows(void (*kernel)(Q4Rows), Q4Rows p, uint32_t rows, uint32
 //
 // At 72 bytes a position the cache streams past at more than 40 codes per clock and SM, which CUDA cores cannot
 // dequantise, multiply and add in FP32 (a first kernel that did so took 4 to 150 times the read time), so both products
-// run on mma.sync with the codes as the A operand: pairs of codes become the FP16 integers 64 + code by a logic operation,
-// and scale, low and the constants are applied to the products: with D = sum_d q_d (64 + code_d) and Q = sum_d q_d,
-//   q . k = scale D + (low - 64 scale) Q,
-//   sum_j p_j v_j = sum_j w_j (64 + code_j) - 64 sum_j w_j + sum_j p_j low_j,   w_j = p_j scale_j.
+// run on mma.sync with the codes as the A operand: masked where they stand in a 16-bit word, pairs of codes are the FP16
+// subnormals code 2^-20, and scale and low are applied to the products: with D = sum_d q_d code_d and Q = sum_d q_d,
+//   q . k = scale D + low Q,
+//   sum_j p_j v_j = sum_j w_j code_j + sum_j p_j low_j,   w_j = p_j scale_j.
+// (As the integers 64 + code, with 64 sum_j w_j taken off again, a warp's sums over 2^18 positions were 2 % of the values' range
+// off: the tensor core's additions round towards zero, and 64 sum_j w_j did not round alike.)
 // What bounds the kernel is the logic pipe: a code pair costs one logic operation to mask and one to move, of which those
 // to the left are multiplications by 16 and run beside them (shifts for all of them, the keys as BF16 integers 128 +
 // code, took 91 us for 512 sequences of 12 heads and 1152 positions instead of 89.6; moves to the right as the high half
@@ -255,12 +257,12 @@ tempo_status launch_rows(void (*kernel)(Q4Rows), Q4Rows p, uint32_t rows, uint32
 // Every column holds its head's query; the scores of tile j are kept in the lanes whose columns are tile j's, and the
 // weights of the other columns are zeroed before tile j's values are multiplied.
 // A query row is scaled by a power of two to at most 2, where FP16 holds its BF16 values but for what lies 2^-14 below its
-// greatest, and there to 2^-25; w is rounded to FP16 (2^-11 of each weight; an eighth of the output's own BF16 rounding),
-// in a running unit that bounds w and p low alike; everything else, the sums included, is FP32.
+// greatest, and there to 2^-25; w is rounded to FP16 (2^-11 of each weight, an eighth of the output's own BF16 rounding,
+// and 2^-33 of the greatest), in a running unit that bounds w and p low alike; everything else, the sums included, is FP32.
 //
 // A CTA of four warps takes a run of tiles of one (sequence, key / value head, eight query heads); each warp streams its
 // own pieces (one bulk copy each, kRing in flight) and keeps an online softmax whose reference and unit move only when a
-// weight passes them kSlack times. Warps merge through shared memory; with `chunks` > 1 the CTAs of a cluster split the positions
+// weight passes them some hundred times. Warps merge through shared memory; with `chunks` > 1 the CTAs of a cluster split the positions
 // and merge through distributed shared memory, or, when a pair needs more of them, through a workspace and a second kernel.
 // ---------------------------------------------------------------------------------------------------------------
 
@@ -269,12 +271,17 @@ constexpr uint32_t kQ4MaxSplits = 160;   // CTAs that share a pair through the w
 constexpr uint32_t kQ4Queries = 8;
 constexpr uint32_t kQ4Piece = 4 * kQ4Block;  // bytes of one bulk copy: four tiles of a 64-wide head, two of a 128-wide
 constexpr uint32_t kRing = 2;
+constexpr float kCodeOne = 0x1p20f;  // what makes a code of the A operands' whole
 constexpr float kNoScore = -3.4028235e38f;  // the reference before any position: no finite score is below it,
 constexpr int kNoUnit = -100;               // and no unit
 // p = 2^(score - reference + kLift): its smallest, 2^-126, is 2^-150 of the greatest, as small as FP32 without the lift.
 constexpr float kLift = 24.f;
-constexpr float kSlack = 64.f;              // what w may reach before the unit moves,
-constexpr float kSlackP = 0x1p31f;          // and p times this before the reference does
+// A unit holds the greatest weight it is set for as 2^kTop, so that w = 2^-24, the least that FP16 holds, is 2^-32 of it: what
+// that rounds away is half of it a position at most, 2^-13 of the values' range over a million. (At kTop 0 such a tail of weights
+// near 2^-25 was lost from the values and not from the sum.)
+constexpr float kTop = 8.f;
+constexpr float kSlack = 0x1p15f;           // what w may reach before the unit moves (FP16 holds 65504),
+constexpr float kSlackP = 0x1p37f;          // and p before the reference does
 
 template <int G, int WARPS>
 struct Q4Smem {
@@ -334,26 +341,20 @@ __device__ __forceinline__ float fast_log2(float x) {
   return y;
 }
 
-// (a & b) | c in one instruction; b and c are constants that the caller keeps in registers.
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
-}
-// A constant the compiler keeps in a register: as an immediate, (x & mask) | magic took two instructions, not one.
+// A constant that the compiler does not know, and keeps in a register.
 __device__ __forceinline__ uint32_t in_register(uint32_t c) {
   asm volatile("" : "+r"(c));
   return c;
 }
 
 struct Q4Constants {
-  uint32_t mask, magic, sixteen;
+  uint32_t mask, sixteen;
 };
 
-// Two codes as the FP16 integers 64 + code: code 0 or 1 of each half of w (bits 0 .. 3 or 4 .. 7). The multiplier is not
+// Two codes as the FP16 subnormals code 2^-20: code 0 or 1 of each half of w (bits 0 .. 3 or 4 .. 7). The multiplier is not
 // known to be 16 when the kernel is compiled, so the product stays one, beside the logic pipe.
-__device__ __forceinline__ uint32_t pair0(const Q4Constants& k, uint32_t w) { return and_or(w * k.sixteen, k.mask, k.magic); }
-__device__ __forceinline__ uint32_t pair1(const Q4Constants& k, uint32_t w) { return and_or(w, k.mask, k.magic); }
+__device__ __forceinline__ uint32_t pair0(const Q4Constants& k, uint32_t w) { return w * k.sixteen & k.mask; }
+__device__ __forceinline__ uint32_t pair1(const Q4Constants& k, uint32_t w) { return w & k.mask; }
 // The bytes of each half swapped: codes 2 and 3 where 0 and 1 were.
 __device__ __forceinline__ uint32_t swap_bytes(uint32_t w) { return __byte_perm(w, 0, 0x2301); }
 
@@ -362,10 +363,10 @@ __device__ __forceinline__ uint32_t swap_bytes(uint32_t w) { return __byte_perm(
 template <int G>
 struct Q4State {
   float acc[G][4][4];
-  float m[2];                // the reference, a score
-  float inv[G][2];           // 1 / the unit (a power of two) in which a group's acc, w and low are counted
-  float l[2];                // this lane's sum of p
-  float w[G][2], low[G][2];  // this lane's sums of w (as rounded) and of p low
+  float m[2];       // the reference, a score
+  float inv[G][2];  // 1 / the unit (a power of two) in which a group's acc and low are counted
+  float l[2];       // this lane's sum of p
+  float low[G][2];  // this lane's sums of p low
 };
 
 __device__ __forceinline__ int unit_exponent(float inv) { return 127 - int(__float_as_uint(inv) >> 23); }
@@ -373,11 +374,11 @@ __device__ __forceinline__ float inverse_unit(int exponent) { return __uint_as_f
 
 __device__ __forceinline__ float q4_weight(float score, float reference) { return fast_exp2(score - reference + kLift); }
 
-// Moves a unit to hold weights of 2^(x + kLift) and what it held, whose reference rises by -down: returns the factor that
-// brings that to the new unit, at most 1.
+// Moves a unit to hold weights of 2^(x + kLift) as 2^kTop, and what it held, whose reference rises by -down: returns the factor
+// that brings that to the new unit, at most 1.
 __device__ __forceinline__ float q4_move(float& inv, float down, float x) {
   const int was = unit_exponent(inv);
-  const int now = int(fminf(fmaxf(fmaxf(ceilf(x) + kLift, ceilf(down) + float(was)), float(kNoUnit)), 126.f));
+  const int now = int(fminf(fmaxf(fmaxf(ceilf(x) + (kLift - kTop), ceilf(down) + float(was)), float(kNoUnit)), 126.f));
   inv = inverse_unit(now);
   return fast_exp2(down + float(was - now));
 }
@@ -440,8 +441,8 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
     uint2 meta1 = *reinterpret_cast<const uint2*>(own + i * kQ4Block + (pg + 8) * 8);
     if (!in0) meta0 = make_uint2(0, 0);  // what lies behind the last position may be anything
     if (!in1) meta1 = make_uint2(0, 0);
-    const float ks0 = bf16_lo(meta0.x), ks1 = bf16_lo(meta1.x);
-    const float kl0 = fmaf(-64.f, ks0, bf16_hi(meta0.x)), kl1 = fmaf(-64.f, ks1, bf16_hi(meta1.x));
+    const float ks0 = bf16_lo(meta0.x) * kCodeOne, ks1 = bf16_lo(meta1.x) * kCodeOne;
+    const float kl0 = bf16_hi(meta0.x), kl1 = bf16_hi(meta1.x);
     s0 = fmaf(ks0, d[i][0], fmaf(kl0, qs[i][0], s0));
     if (kTwo) s1 = fmaf(ks0, d[i][1], fmaf(kl0, qs[i][1], s1));
     s2 = fmaf(ks1, d[i][2], fmaf(kl1, qs[i][0], s2));
@@ -460,7 +461,7 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
   // share, whatever the values. A group's weights w = p scale and p low are counted in a unit of their own, a power of two
   // that follows p size, size the value row's scale or a sixteenth of its low, so they stay small whatever the values' size
   // and the halves of a head of 128 keep their bits beside one another. Reference and units move when w passes kSlack
-  // or p 2^(kLift + 7) (which NaN and infinity do too).
+  // or p kSlackP (which NaN and infinity do too).
   float p0 = q4_weight(s0, st.m[0]), p2 = q4_weight(s2, st.m[0]);
   float p1 = kTwo ? q4_weight(s1, st.m[1]) : 0.f, p3 = kTwo ? q4_weight(s3, st.m[1]) : 0.f;
   auto far = [&](float a, float b, int c) {
@@ -488,12 +489,8 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
         if (kTwo) x1 = fmaxf(x1, __shfl_xor_sync(0xFFFFFFFFu, x1, o));
       }
       const float c0 = q4_move(st.inv[i][0], down0, x0), c1 = kTwo ? q4_move(st.inv[i][1], down1, x1) : 0.f;
-      st.w[i][0] *= c0;
       st.low[i][0] *= c0;
-      if (kTwo) {
-        st.w[i][1] *= c1;
-        st.low[i][1] *= c1;
-      }
+      if (kTwo) st.low[i][1] *= c1;
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         st.acc[i][n][0] *= c0;
@@ -525,12 +522,8 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
     const float u1 = kTwo ? p1 * st.inv[i][1] : 0.f, u3 = kTwo ? p3 * st.inv[i][1] : 0.f;
     const __half2 h0 = __floats2half2_rn(u0 * vs0, kTwo ? u1 * vs0 : 0.f);
     const __half2 h1 = __floats2half2_rn(u2 * vs1, kTwo ? u3 * vs1 : 0.f);
-    st.w[i][0] += __low2float(h0) + __low2float(h1);
     st.low[i][0] = fmaf(u0, vl0, fmaf(u2, vl1, st.low[i][0]));
-    if (kTwo) {
-      st.w[i][1] += __high2float(h0) + __high2float(h1);
-      st.low[i][1] = fmaf(u1, vl0, fmaf(u3, vl1, st.low[i][1]));
-    }
+    if (kTwo) st.low[i][1] = fmaf(u1, vl0, fmaf(u3, vl1, st.low[i][1]));
     b0[i] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h0));
     b1[i] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h1));
   }
@@ -711,13 +704,13 @@ __global__ void __launch_bounds__(32 * WARPS, RESIDENT) decode_attention_q4_kern
 #pragma unroll
   for (int i = 0; i < G; ++i) {
     st.inv[i][0] = st.inv[i][1] = inverse_unit(kNoUnit);
-    st.w[i][0] = st.w[i][1] = st.low[i][0] = st.low[i][1] = 0.f;
+    st.low[i][0] = st.low[i][1] = 0.f;
 #pragma unroll
     for (int n = 0; n < 4; ++n)
 #pragma unroll
       for (int c = 0; c < 4; ++c) st.acc[i][n][c] = 0.f;
   }
-  const Q4Constants kc{in_register(0x00F000F0u), in_register(0x54005400u), in_register(16u)};
+  const Q4Constants kc{in_register(0x00F000F0u), in_register(16u)};
   uint32_t slot = 0, phase = 0, limit = pieces;
   bool ok = true;
   for (uint32_t piece = 0; piece < limit; ++piece) {
@@ -772,12 +765,12 @@ __global__ void __launch_bounds__(32 * WARPS, RESIDENT) decode_attention_q4_kern
       for (int o = CP / 2; o < 4; o <<= 1) e = fmaxf(e, __shfl_xor_sync(0xFFFFFFFFu, e, o));
       const float f = fast_exp2(own - e);
       if (g == 0 && writes) part[L::kUnits + i * kQ4Queries + query] = e;
-      float rest = fmaf(-64.f, st.w[i][c], st.low[i][c]) * f;
+      float rest = st.low[i][c] * f;
 #pragma unroll
       for (int o = CP / 2; o < 32; o <<= 1) rest += __shfl_xor_sync(0xFFFFFFFFu, rest, o);
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        float lo = st.acc[i][n][c] * f, hi = st.acc[i][n][2 + c] * f;
+        float lo = st.acc[i][n][c] * (f * kCodeOne), hi = st.acc[i][n][2 + c] * (f * kCodeOne);
 #pragma unroll
         for (int o = CP / 2; o < 4; o <<= 1) {
           lo += __shfl_xor_sync(0xFFFFFFFFu, lo, o);

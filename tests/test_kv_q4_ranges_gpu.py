@@ -119,3 +119,26 @@ def test_halves_of_a_value_row_of_different_size(n: int, copies: int, ratio: flo
     q = _bf16(rng.standard_normal((4, 128)) * 0.1)
     for heads in (1, 4):
         _check(q[:heads], held, _attend(q[:heads], cache, n, heads, copies))
+
+
+def test_a_long_tail_of_small_weights_counts() -> None:
+    """A million positions of weight 2^-25.5 beside a few of weight 1: together they are 0.5 % of the average."""
+    from tempo_compiler_b200 import ops
+    n, heads, run = 1 << 20, 4096, 1 << 18   # so many queries that each four warps read all of it, a run to a warp
+    first, other = np.zeros((2, 128), np.float32)
+    even = np.arange(64) % 2 == 0
+    first[64:], other[64:] = np.where(even, 0, 15), np.where(even, 15, 0)
+    other[:64] = -0.55078125                 # (BF16 holds it)
+    rows = _bf16(np.stack([first, other]))[(torch.arange(n, device="cuda") % run != 0).long()]
+    cache = ops.kv_cache_q4(1, 1, n)
+    ops.kv_store_q4(rows, cache, _i32(np.zeros(n)), torch.arange(n, dtype=torch.int32, device="cuda"))
+    q = torch.full((1, heads * 64), 0.5, dtype=torch.bfloat16, device="cuda")
+    got = ops.decode_attention_q4(q, cache, _i32([n]), heads=heads).double().cpu().numpy().reshape(heads, 64)
+    ones = n // run
+    tail = (n - ones) * np.exp(-0.55078125 * 32)
+    want = np.where(even, 15 * tail, 15 * ones) / (ones + tail)
+    # as above, with exact products: the output's rounding, 2^-11 of the tail's share and of the others' for the weights'
+    # (they move the average by what they move apart), a running sum of run / 32 weights a lane, of 2^-24 each
+    share = tail / (ones + tail)
+    bound = 2.0 ** -8 * want + 15 * (2 * 2.0 ** -11 * share + share * (run / 32 * 2.0 ** -24 + 2.0 ** -20) + 2.0 ** -20)
+    assert (np.abs(got - want) <= bound).all(), np.max(np.abs(got - want) / bound)
