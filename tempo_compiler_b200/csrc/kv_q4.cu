@@ -256,8 +256,8 @@ tempo_status launch_rows(void (*kernel)(Q4Rows), Q4Rows p, uint32_t rows, uint32
 // and eight columns of queries whether they existed or not, issued 309 instructions a tile and was bound by the ALU pipe).
 // Every column holds its head's query; the scores of tile j are kept in the lanes whose columns are tile j's, and the
 // weights of the other columns are zeroed before tile j's values are multiplied.
-// A query row is scaled by a power of two to at most 2, where FP16 holds its BF16 values but for what lies 2^-14 below its
-// greatest, and there to 2^-25; w is rounded to FP16 (2^-11 of each weight, an eighth of the output's own BF16 rounding,
+// Each 64 dimensions of a query row are scaled by a power of two to at most 2, where FP16 holds their BF16 values but for what
+// lies 2^-14 below the greatest of them, and there to 2^-25 (as FP32 sums with keys that share a scale would); w is rounded to FP16 (2^-11 of each weight, an eighth of the output's own BF16 rounding,
 // and 2^-33 of the greatest), in a running unit that bounds w and p low alike; everything else, the sums included, is FP32.
 //
 // A CTA of four warps takes a run of tiles of one (sequence, key / value head, eight query heads); each warp streams its
@@ -395,7 +395,7 @@ __host__ __device__ constexpr uint32_t q4_tiles_at_once(int g, int rp) {
 // else `left` do.
 template <int G, int RP, bool FULL>
 __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G][8], const float (&qs)[G][2],
-                                         const float (&unit)[2],
+                                         const float (&unit)[G][2],
                                          const uint8_t* tiles, uint32_t left, uint32_t g, uint32_t t,
                                          const Q4Constants& kc) {
   constexpr uint32_t kTileBytes = G * kQ4Block, CP = q4_columns(RP), TP = q4_tiles_at_once(G, RP);
@@ -443,20 +443,17 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
     if (!in1) meta1 = make_uint2(0, 0);
     const float ks0 = bf16_lo(meta0.x) * kCodeOne, ks1 = bf16_lo(meta1.x) * kCodeOne;
     const float kl0 = bf16_hi(meta0.x), kl1 = bf16_hi(meta1.x);
-    s0 = fmaf(ks0, d[i][0], fmaf(kl0, qs[i][0], s0));
-    if (kTwo) s1 = fmaf(ks0, d[i][1], fmaf(kl0, qs[i][1], s1));
-    s2 = fmaf(ks1, d[i][2], fmaf(kl1, qs[i][0], s2));
-    if (kTwo) s3 = fmaf(ks1, d[i][3], fmaf(kl1, qs[i][1], s3));
+    s0 = __fmaf_rn(fmaf(ks0, d[i][0], kl0 * qs[i][0]), unit[i][0], s0);
+    if (kTwo) s1 = __fmaf_rn(fmaf(ks0, d[i][1], kl0 * qs[i][1]), unit[i][1], s1);
+    s2 = __fmaf_rn(fmaf(ks1, d[i][2], kl1 * qs[i][0]), unit[i][0], s2);
+    if (kTwo) s3 = __fmaf_rn(fmaf(ks1, d[i][3], kl1 * qs[i][1]), unit[i][1], s3);
     vm0[i] = meta0.y;
     vm1[i] = meta1.y;
     size0[i] = fmax3(0x1p-100f, bf16_lo(meta0.y), 0.0625f * fabsf(bf16_hi(meta0.y)));
     size1[i] = fmax3(0x1p-100f, bf16_lo(meta1.y), 0.0625f * fabsf(bf16_hi(meta1.y)));
   }
-  // (not joined with the differences below: a product that is rounded here and not there is off by its own rounding)
-  s0 = in0 ? __fmul_rn(s0, unit[0]) : -INFINITY;
-  s1 = in0 ? __fmul_rn(s1, unit[1]) : -INFINITY;
-  s2 = in1 ? __fmul_rn(s2, unit[0]) : -INFINITY;
-  s3 = in1 ? __fmul_rn(s3, unit[1]) : -INFINITY;
+  if (!in0) s0 = s1 = -INFINITY;
+  if (!in1) s2 = s3 = -INFINITY;
   // The reference is a score and follows the scores alone: the sum l of p = 2^(score - m + kLift) keeps every position's
   // share, whatever the values. A group's weights w = p scale and p low are counted in a unit of their own, a power of two
   // that follows p size, size the value row's scale or a sixteenth of its low, so they stay small whatever the values' size
@@ -649,53 +646,47 @@ __global__ void __launch_bounds__(32 * WARPS, RESIDENT) decode_attention_q4_kern
       if (i < pieces) fetch(i, i);
   }
 
-  // The query fragments: lane (g, t) holds dimensions 16 t .. 16 t + 15 of each group of its column's query, the row scaled
+  // The query fragments: lane (g, t) holds dimensions 16 t .. 16 t + 15 of each group of its column's query, the group scaled
   // by a power of two to a greatest magnitude below 2.
   uint32_t qf[G][8];
-  float qs[G][2], unit[2];
-  {
-    float x[G][16], greatest = 0.f;
+  float qs[G][2], unit[G][2];
 #pragma unroll
-    for (int i = 0; i < G; ++i) {
-      uint4 a = make_uint4(0, 0, 0, 0), b = a;
-      if (g % CP < queries) {
-        const uint4* q4 = reinterpret_cast<const uint4*>(
-            p.q + size_t(s) * p.ldq + size_t(kvh * share + first + g % CP) * kWidth + i * 64 + t * 16);
-        a = q4[0];
-        b = q4[1];
-      }
-      float lo[8], hi[8];
-      unpack8(a, lo);
-      unpack8(b, hi);
+  for (int i = 0; i < G; ++i) {
+    uint4 a = make_uint4(0, 0, 0, 0), b = a;
+    if (g % CP < queries) {
+      const uint4* q4 = reinterpret_cast<const uint4*>(
+          p.q + size_t(s) * p.ldq + size_t(kvh * share + first + g % CP) * kWidth + i * 64 + t * 16);
+      a = q4[0];
+      b = q4[1];
+    }
+    float x[16], lo[8], hi[8], greatest = 0.f;
+    unpack8(a, lo);
+    unpack8(b, hi);
 #pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        x[i][d] = lo[d];
-        x[i][8 + d] = hi[d];
-        greatest = fmax3(greatest, fabsf(lo[d]), fabsf(hi[d]));
-      }
+    for (int d = 0; d < 8; ++d) {
+      x[d] = lo[d];
+      x[8 + d] = hi[d];
+      greatest = fmax3(greatest, fabsf(lo[d]), fabsf(hi[d]));
     }
     greatest = fmaxf(greatest, __shfl_xor_sync(0xFFFFFFFFu, greatest, 1));
     greatest = fmaxf(greatest, __shfl_xor_sync(0xFFFFFFFFu, greatest, 2));
     const uint32_t exponent = min(max(__float_as_uint(greatest) >> 23, 1u), 253u);
     const float down = __uint_as_float((254u - exponent) << 23), up = kDecodeLog2e * __uint_as_float(exponent << 23);
-    unit[0] = __shfl_sync(0xFFFFFFFFu, up, 8 * t);  // of the lane's own columns, 2 t and 2 t + 1
-    unit[1] = __shfl_sync(0xFFFFFFFFu, up, 8 * t + 4);
+    unit[i][0] = __shfl_sync(0xFFFFFFFFu, up, 8 * t);  // of the lane's own columns, 2 t and 2 t + 1
+    unit[i][1] = __shfl_sync(0xFFFFFFFFu, up, 8 * t + 4);
+    float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < G; ++i) {
-      float sum = 0.f;
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        // pair0 and pair1 of a word and of its swapped form give dimensions n and n + 4 of a word's eight
-        const int d = n / 4 * 8 + n % 4;
-        const __half2 h = __floats2half2_rn(x[i][d] * down, x[i][d + 4] * down);
-        qf[i][n] = *reinterpret_cast<const uint32_t*>(&h);
-        sum += __low2float(h) + __high2float(h);
-      }
-      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
-      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
-      qs[i][0] = __shfl_sync(0xFFFFFFFFu, sum, 8 * t);
-      qs[i][1] = __shfl_sync(0xFFFFFFFFu, sum, 8 * t + 4);
+    for (int n = 0; n < 8; ++n) {
+      // pair0 and pair1 of a word and of its swapped form give dimensions n and n + 4 of a word's eight
+      const int d = n / 4 * 8 + n % 4;
+      const __half2 h = __floats2half2_rn(x[d] * down, x[d + 4] * down);
+      qf[i][n] = *reinterpret_cast<const uint32_t*>(&h);
+      sum += __low2float(h) + __high2float(h);
     }
+    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
+    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+    qs[i][0] = __shfl_sync(0xFFFFFFFFu, sum, 8 * t);
+    qs[i][1] = __shfl_sync(0xFFFFFFFFu, sum, 8 * t + 4);
   }
 
   Q4State<G> st;

@@ -121,6 +121,25 @@ def test_halves_of_a_value_row_of_different_size(n: int, copies: int, ratio: flo
         _check(q[:heads], held, _attend(q[:heads], cache, n, heads, copies))
 
 
+@pytest.mark.parametrize("n,copies", SPLITS)
+@pytest.mark.parametrize("ratio", [1e-3, 1e-6, 1e-8, 1e-12, 1e-25])
+@pytest.mark.parametrize("smaller", [0, 1])
+def test_halves_of_a_query_of_different_size(n: int, copies: int, ratio: float, smaller: int) -> None:
+    """A half of the query that is far smaller than the other decides the scores all the same where its keys are as much
+    larger than the others'."""
+    rng = np.random.default_rng(n + copies)
+    keys, values = rng.standard_normal((2, n, 128))
+    small, large = slice(64 * smaller, 64 * smaller + 64), slice(64 - 64 * smaller, 128 - 64 * smaller)
+    keys[:, small] /= ratio
+    q = rng.standard_normal((4, 128)) * 0.2
+    q[:, small] *= ratio
+    keys[:, large] *= 0.25
+    cache, held = _cached(keys, values)
+    q = _bf16(q)
+    for heads in (1, 4):
+        _check(q[:heads], held, _attend(q[:heads], cache, n, heads, copies))
+
+
 def test_a_long_tail_of_small_weights_counts() -> None:
     """A million positions of weight 2^-25.5 beside a few of weight 1: together they are 0.5 % of the average."""
     from tempo_compiler_b200 import ops
