@@ -176,7 +176,9 @@ tempo_status tempo_block_copy(const void* source, void* destination, uint32_t ro
  * residual[M, ldr] (added after GELU), FP32 accumulate, BF16 out; tcgen05 + TMA. K % 8 == 0; lda, ldw % 8 == 0.
  * In TEMPO_GEMM_ARGMAX mode `out` is unused and `part_val`/`part_idx` receive [M][ceil(N/256)] partials.
  * In TEMPO_GEMM_F32 mode (alone, without bias and residual) `out` is FP32: the logits of an LM head, whose BF16
- * rounding would cost up to 2^-8 of their size in each log probability. */
+ * rounding would cost up to 2^-8 of their size in each log probability. There both operands may be what an earlier call
+ * in the stream writes; in the other modes w_t is read before earlier calls of this library have finished, so it must be a
+ * table that is complete before they start (a model's weights). */
 tempo_status tempo_gemm(const void* a, uint32_t lda, const void* w_t, uint32_t ldw, const void* bias,
                         const void* residual, uint32_t ldr, void* out, uint32_t ldo, uint32_t m, uint32_t n,
                         uint32_t k, uint32_t flags, float* part_val, int32_t* part_idx, void* stream);

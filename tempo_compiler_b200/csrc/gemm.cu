@@ -106,6 +106,13 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
                : "memory");
 }
 
+// Asks a tile into the L2.
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int32_t x, int32_t y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];"
+               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y)
+               : "memory");
+}
+
 // Sixteen of one thread's accumulators into the warp's FP32 staging tile (32 rows x 16 columns), as they are: row `lane` at
 // 64 bytes, its 16-byte words swizzled as the TMA 64-byte swizzle has them.
 __device__ __forceinline__ void stage_f32(const uint32_t (&r)[32], uint32_t half, uint8_t* staging, uint32_t lane) {
@@ -446,13 +453,17 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       for (int s = 0; s < STAGES; ++s) used[s] = false;
       bool ok = true;
       // The weights are not the previous kernel's output: the first tile's first ring of B tiles streams in before
-      // the wait.
+      // the wait. (FP32 outputs: the second operand may be any matrix, one that the call before wrote among them, so before the
+      // wait its tiles only come into the L2, where that call's writes reach them. 64 rows of an LM head 15.0 us, with
+      // nothing before the wait 15.7.)
       const uint32_t early = blockIdx.x < tiles ? (kblocks < uint32_t(STAGES) ? kblocks : uint32_t(STAGES)) : 0u;
-      if (early > 0) {
-        const int32_t n0 = int32_t((blockIdx.x % p.n_tiles) * BN);
-        for (uint32_t kb = 0; kb < early; ++kb) {
+      const int32_t first_n0 = int32_t((blockIdx.x % p.n_tiles) * BN);
+      for (uint32_t kb = 0; kb < early; ++kb) {
+        if constexpr (F32) {
+          tma_prefetch_2d(&tmap_b, int32_t(kb * kBK), first_n0);
+        } else {
           mbar_arrive_expect_tx(&full[kb], p.stage_tx);
-          tma_load_2d(smem + kb * L::kStageBytes + L::kABytes, &tmap_b, &full[kb], int32_t(kb * kBK), n0);
+          tma_load_2d(smem + kb * L::kStageBytes + L::kABytes, &tmap_b, &full[kb], int32_t(kb * kBK), first_n0);
           used[kb] = true;  // a copy is in flight on this stage from here on
           last_parity[kb] = 0;
         }
@@ -464,7 +475,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         const int32_t n0 = int32_t((t % p.n_tiles) * BN);
         for (uint32_t kb = 0; kb < kblocks; ++kb) {
           uint8_t* a_dst = smem + stage * L::kStageBytes;
-          if (!(first && kb < early)) {
+          if (F32 || !(first && kb < early)) {
             if (!mbar_wait(&empty[stage], phase ^ 1u, kWatchEmpty, abort_flag)) { ok = false; break; }
             mbar_arrive_expect_tx(&full[stage], p.stage_tx);
             tma_load_2d(a_dst + L::kABytes, &tmap_b, &full[stage], int32_t(kb * kBK), n0);

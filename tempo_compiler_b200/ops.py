@@ -98,7 +98,8 @@ def _launch_at(device: int, name: str, *args) -> None:
 
 def gemm(a: torch.Tensor, w_t: torch.Tensor, *, bias: torch.Tensor | None = None,
          residual: torch.Tensor | None = None, gelu: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
-    """out[M, N] = epilogue(a[M, K] @ w_t[N, K]^T): + bias, exact-erf GELU (of the BF16-rounded sum), + residual."""
+    """out[M, N] = epilogue(a[M, K] @ w_t[N, K]^T): + bias, exact-erf GELU (of the BF16-rounded sum), + residual. The
+    kernel reads w_t before earlier calls of this module have finished: w_t must not be what they write."""
     _check(a, torch.bfloat16, "a")
     _check(w_t, torch.bfloat16, "w_t")
     m, k = a.shape
@@ -120,7 +121,8 @@ def gemm(a: torch.Tensor, w_t: torch.Tensor, *, bias: torch.Tensor | None = None
 
 def gemm_f32(a: torch.Tensor, w_t: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """out[M, N] = a[M, K] @ w_t[N, K]^T in FP32, the accumulators unrounded (an LM head's logits). `out` may have a
-    row stride of its own, a multiple of 8; without it the rows are padded to one and the view of N columns returned."""
+    row stride of its own, a multiple of 8; without it the rows are padded to one and the view of N columns returned.
+    Both operands may be what an earlier call writes."""
     _check(a, torch.bfloat16, "a")
     device = a.get_device()
     _operand(w_t, torch.bfloat16, "w_t", device)
