@@ -78,6 +78,13 @@ def _matrix(t: torch.Tensor, dtype: torch.dtype, name: str, device: int | None =
     raise ValueError(f"{name} must be a matrix of contiguous rows that do not overlap")
 
 
+def _stride32(stride: int, name: str) -> int:
+    """A row stride that the entry point takes in 32 bits."""
+    if stride >> 32:
+        raise ValueError(f"{name} has a row stride of {stride} elements: 32 bits hold no more than {2 ** 32 - 1}")
+    return stride
+
+
 _ENTRIES: dict[str, object] = {}
 
 
@@ -135,8 +142,8 @@ def gemm_f32(a: torch.Tensor, w_t: torch.Tensor, *, out: torch.Tensor | None = N
     out_rows, out_columns, stride, _ = _matrix(out, torch.float32, "out", device)
     if out_rows != m or out_columns != n:
         raise ValueError(f"out must be {(m, n)}, got {tuple(out.shape)}")
-    _launch_at(device, "tempo_gemm", a.data_ptr(), k, w_t.data_ptr(), k, None, None, n, out.data_ptr(), stride, m, n, k,
-               _lib.GEMM_F32, None, None)
+    _launch_at(device, "tempo_gemm", a.data_ptr(), k, w_t.data_ptr(), k, None, None, n, out.data_ptr(),
+               _stride32(stride, "out"), m, n, k, _lib.GEMM_F32, None, None)
     return out
 
 
@@ -402,7 +409,7 @@ def kv_store_q4(qkv: torch.Tensor, cache: torch.Tensor, seq_of: torch.Tensor, po
     if width % head or heads < 0:
         raise ValueError(f"qkv rows of {width} are not query, key and value heads of {head} ({kv_heads} key heads)")
     _places(rows, seq_of, pos_of, device)
-    _launch_at(device, "tempo_kv_store_q4", qkv.data_ptr(), stride, cache.data_ptr(), seq_of.data_ptr(),
+    _launch_at(device, "tempo_kv_store_q4", qkv.data_ptr(), _stride32(stride, "qkv"), cache.data_ptr(), seq_of.data_ptr(),
                pos_of.data_ptr(), rows, seqs, heads, kv_heads, head, capacity)
 
 
@@ -421,7 +428,7 @@ def kv_load_q4(cache: torch.Tensor, seq_of: torch.Tensor, pos_of: torch.Tensor, 
         out_rows, out_width, stride, _ = _matrix(out, torch.bfloat16, "out", device)
         if out_rows != rows or out_width != width:
             raise ValueError(f"out must be {(rows, width)}, got {tuple(out.shape)}")
-    _launch_at(device, "tempo_kv_load_q4", cache.data_ptr(), out.data_ptr(), stride, seq_of.data_ptr(),
+    _launch_at(device, "tempo_kv_load_q4", cache.data_ptr(), out.data_ptr(), _stride32(stride, "out"), seq_of.data_ptr(),
                pos_of.data_ptr(), rows, seqs, kv_heads, head, capacity)
     return out
 
@@ -457,8 +464,8 @@ def decode_attention_q4(qkv: torch.Tensor, cache: torch.Tensor, lengths: torch.T
             raise ValueError(f"out must be {(seqs, heads * head)}, got {tuple(out.shape)}")
     size = decode_attention_q4_workspace_bytes(seqs, heads, kv_heads, head, capacity)
     workspace = qkv.new_empty(size, dtype=torch.uint8) if size else None
-    _launch_at(device, "tempo_decode_attention_q4", qkv.data_ptr(), stride, cache.data_ptr(), lengths.data_ptr(),
-               length_offset, out.data_ptr(), seqs, heads, kv_heads, head, capacity, _ptr(workspace), size)
+    _launch_at(device, "tempo_decode_attention_q4", qkv.data_ptr(), _stride32(stride, "qkv"), cache.data_ptr(),
+               lengths.data_ptr(), length_offset, out.data_ptr(), seqs, heads, kv_heads, head, capacity, _ptr(workspace), size)
     return out
 
 
