@@ -85,6 +85,13 @@ def _stride32(stride: int, name: str) -> int:
     return stride
 
 
+def _int32(value: int, name: str) -> int:
+    """An offset that the entry point takes in 32 bits."""
+    if not -2 ** 31 <= value < 2 ** 31:
+        raise ValueError(f"{name} must be in [-2^31, 2^31), got {value}")
+    return value
+
+
 _ENTRIES: dict[str, object] = {}
 
 
@@ -465,7 +472,8 @@ def decode_attention_q4(qkv: torch.Tensor, cache: torch.Tensor, lengths: torch.T
     size = decode_attention_q4_workspace_bytes(seqs, heads, kv_heads, head, capacity)
     workspace = qkv.new_empty(size, dtype=torch.uint8) if size else None
     _launch_at(device, "tempo_decode_attention_q4", qkv.data_ptr(), _stride32(stride, "qkv"), cache.data_ptr(),
-               lengths.data_ptr(), length_offset, out.data_ptr(), seqs, heads, kv_heads, head, capacity, _ptr(workspace), size)
+               lengths.data_ptr(), _int32(length_offset, "length_offset"), out.data_ptr(), seqs, heads, kv_heads, head,
+               capacity, _ptr(workspace), size)
     return out
 
 
@@ -529,7 +537,7 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, *, top: int = 0, out
                 raise ValueError(f"out.{name} must be {shape}, got {tuple(t.shape)}")
     _launch_at(device, "tempo_token_logprobs", logits.data_ptr(), stride, int(bf16), ids.data_ptr(), rows, vocab, top,
                out.logprob.data_ptr(), out.entropy.data_ptr(), _ptr(out.top_logprob), _ptr(out.top_ids), _ptr(slots),
-               slot_offset, blocks)
+               _int32(slot_offset, "slot_offset"), blocks)
     return out
 
 

@@ -1,5 +1,5 @@
-"""The torch wrappers of the 4-bit cache and the scores pass strides on in 32 bits: what 32 bits do not hold is refused,
-not cut off (no GPU: stand-ins have the attributes of tensors on one)."""
+"""The torch wrappers of the 4-bit cache and the scores pass strides and offsets on in 32 bits: what 32 bits do not hold is
+refused, not cut off (no GPU: stand-ins have the attributes of tensors on one)."""
 
 from __future__ import annotations
 
@@ -79,3 +79,19 @@ def test_row_strides_of_more_than_32_bits_are_refused(launched, stride: int) -> 
     ops.token_logprobs(_OnGpu(torch.float32, (2, 40), (stride, 1)), two, out=ops.TokenScores(
         _OnGpu(torch.float32, (2,)), _OnGpu(torch.float32, (2,))))
     assert launched.pop()[1][1] == stride
+
+
+@pytest.mark.parametrize("offset", [2 ** 31, 2 ** 32 + 5, -2 ** 31 - 1])
+def test_offsets_of_more_than_32_bits_are_refused(launched, offset: int) -> None:
+    from tempo_compiler_b200 import ops
+    cache, two = _OnGpu(torch.uint8, (2, 12, 3, 1152)), _i32(2)
+    with pytest.raises(ValueError, match="length_offset"):
+        ops.decode_attention_q4(_OnGpu(torch.bfloat16, (2, 2304)), cache, two, length_offset=offset)
+    out = ops.TokenScores(_OnGpu(torch.float32, (3, 2)), _OnGpu(torch.float32, (3, 2)))
+    with pytest.raises(ValueError, match="slot_offset"):
+        ops.token_logprobs(_OnGpu(torch.float32, (2, 40)), two, out=out, slots=two, slot_offset=offset)
+    assert not launched
+    for held in (2 ** 31 - 1, -2 ** 31):
+        ops.decode_attention_q4(_OnGpu(torch.bfloat16, (2, 2304)), cache, two, length_offset=held)
+        ops.token_logprobs(_OnGpu(torch.float32, (2, 40)), two, out=out, slots=two, slot_offset=held)
+    assert len(launched) == 4
