@@ -274,7 +274,8 @@ constexpr uint32_t kRing = 2;
 constexpr float kCodeOne = 0x1p20f;  // what makes a code of the A operands' whole
 constexpr float kNoScore = -3.4028235e38f;  // the reference before any position: no finite score is below it,
 constexpr int kNoUnit = -100;               // and no unit
-// p = 2^(score - reference + kLift): its smallest, 2^-126, is 2^-150 of the greatest, as small as FP32 without the lift.
+// The reference is set kLift below the greatest score, so the smallest p = 2^(score - reference), 2^-126, is 2^-150 of the
+// greatest, as small as FP32 goes. (Beside large scores their difference rounds to anything from 0 to 32, which is as good.)
 constexpr float kLift = 24.f;
 // A unit holds the greatest weight it is set for as 2^kTop, so that w = 2^-24, the least that FP16 holds, is 2^-32 of it: what
 // that rounds away is half of it a position at most, 2^-13 of the values' range over a million. (At kTop 0 such a tail of weights
@@ -372,13 +373,18 @@ struct Q4State {
 __device__ __forceinline__ int unit_exponent(float inv) { return 127 - int(__float_as_uint(inv) >> 23); }
 __device__ __forceinline__ float inverse_unit(int exponent) { return __uint_as_float(uint32_t(127 - exponent) << 23); }
 
-__device__ __forceinline__ float q4_weight(float score, float reference) { return fast_exp2(score - reference + kLift); }
+// A value row's size: its scale, or a sixteenth of its low where that is more.
+__device__ __forceinline__ float q4_size(uint32_t meta) {
+  return fmax3(0x1p-100f, bf16_lo(meta), 0.0625f * fabsf(bf16_hi(meta)));
+}
 
-// Moves a unit to hold weights of 2^(x + kLift) as 2^kTop, and what it held, whose reference rises by -down: returns the factor
+__device__ __forceinline__ float q4_weight(float score, float reference) { return fast_exp2(score - reference); }
+
+// Moves a unit to hold weights of 2^x as 2^kTop, and what it held, whose reference rises by -down: returns the factor
 // that brings that to the new unit, at most 1.
 __device__ __forceinline__ float q4_move(float& inv, float down, float x) {
   const int was = unit_exponent(inv);
-  const int now = int(fminf(fmaxf(fmaxf(ceilf(x) + (kLift - kTop), ceilf(down) + float(was)), float(kNoUnit)), 126.f));
+  const int now = int(fminf(fmaxf(fmaxf(ceilf(x) - kTop, ceilf(down) + float(was)), float(kNoUnit)), 126.f));
   inv = inverse_unit(now);
   return fast_exp2(down + float(was - now));
 }
@@ -433,7 +439,6 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
   const bool in1 = (TP == 4 || mine < TP) && (FULL || mine * kQ4Tile + pg + 8 < left);
   const uint8_t* own = tiles + (TP == 4 || mine < TP ? mine : 0u) * kTileBytes + 2 * kQ4Codes;
   float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;  // scores (log2): rows g and g + 8, columns 2 t and 2 t + 1
-  float size0[G], size1[G];
   uint32_t vm0[G], vm1[G];
 #pragma unroll
   for (int i = 0; i < G; ++i) {
@@ -449,36 +454,46 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
     if (kTwo) s3 = __fmaf_rn(fmaf(ks1, d[i][3], kl1 * qs[i][1]), unit[i][1], s3);
     vm0[i] = meta0.y;
     vm1[i] = meta1.y;
-    size0[i] = fmax3(0x1p-100f, bf16_lo(meta0.y), 0.0625f * fabsf(bf16_hi(meta0.y)));
-    size1[i] = fmax3(0x1p-100f, bf16_lo(meta1.y), 0.0625f * fabsf(bf16_hi(meta1.y)));
   }
   if (!in0) s0 = s1 = -INFINITY;
   if (!in1) s2 = s3 = -INFINITY;
-  // The reference is a score and follows the scores alone: the sum l of p = 2^(score - m + kLift) keeps every position's
-  // share, whatever the values. A group's weights w = p scale and p low are counted in a unit of their own, a power of two
-  // that follows p size, size the value row's scale or a sixteenth of its low, so they stay small whatever the values' size
-  // and the halves of a head of 128 keep their bits beside one another. Reference and units move when w passes kSlack
-  // or p kSlackP (which NaN and infinity do too).
+  // The reference follows the scores alone: the sum l of p = 2^(score - reference) keeps every position's share, whatever the
+  // values. A group's weights w = p scale and p low are counted in a unit of their own, a power of two that follows p size,
+  // size the value row's scale or a sixteenth of its low, so they stay small whatever the values' size and the halves of a
+  // head of 128 keep their bits beside one another. Reference and units move when w passes kSlack or p kSlackP (which NaN and
+  // infinity do too).
   float p0 = q4_weight(s0, st.m[0]), p2 = q4_weight(s2, st.m[0]);
   float p1 = kTwo ? q4_weight(s1, st.m[1]) : 0.f, p3 = kTwo ? q4_weight(s3, st.m[1]) : 0.f;
-  auto far = [&](float a, float b, int c) {
-    float sum = (a + b) * (kSlack / kSlackP);
+  float u0[G], u1[G], u2[G], u3[G], l0 = p0 + p2, l1 = p1 + p3;  // u: p in the groups' units
+  auto scale = [&]() {
 #pragma unroll
-    for (int i = 0; i < G; ++i) sum = fmaf(a * st.inv[i][c], size0[i], fmaf(b * st.inv[i][c], size1[i], sum));
-    return !(sum <= kSlack);
+    for (int i = 0; i < G; ++i) {
+      u0[i] = p0 * st.inv[i][0];
+      u2[i] = p2 * st.inv[i][0];
+      u1[i] = kTwo ? p1 * st.inv[i][1] : 0.f;
+      u3[i] = kTwo ? p3 * st.inv[i][1] : 0.f;
+    }
   };
-  const bool far0 = far(p0, p2, 0), far1 = kTwo && far(p1, p3, 1);
-  if (__any_sync(0xFFFFFFFFu, far0 || far1)) {
-    float m0 = fmax3(s0, s2, st.m[0]), m1 = kTwo ? fmax3(s1, s3, st.m[1]) : 0.f;
+  scale();
+  float far0 = l0 * (kSlack / kSlackP), far1 = l1 * (kSlack / kSlackP);
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    far0 = fmaf(u0[i], q4_size(vm0[i]), fmaf(u2[i], q4_size(vm1[i]), far0));
+    if (kTwo) far1 = fmaf(u1[i], q4_size(vm0[i]), fmaf(u3[i], q4_size(vm1[i]), far1));
+  }
+  if (__any_sync(0xFFFFFFFFu, !(far0 <= kSlack) || (kTwo && !(far1 <= kSlack)))) {
+    float m0 = fmaxf(s0, s2) - kLift, m1 = kTwo ? fmaxf(s1, s3) - kLift : 0.f;
 #pragma unroll
     for (int o = 4; o <= 16; o <<= 1) {
       m0 = fmaxf(m0, __shfl_xor_sync(0xFFFFFFFFu, m0, o));
       if (kTwo) m1 = fmaxf(m1, __shfl_xor_sync(0xFFFFFFFFu, m1, o));
     }
+    m0 = fmaxf(m0, st.m[0]);
+    if (kTwo) m1 = fmaxf(m1, st.m[1]);
     const float down0 = st.m[0] - m0, down1 = kTwo ? st.m[1] - m1 : 0.f;
 #pragma unroll
     for (int i = 0; i < G; ++i) {
-      const float g0 = fast_log2(fminf(size0[i], 0x1p100f)), g1 = fast_log2(fminf(size1[i], 0x1p100f));
+      const float g0 = fast_log2(fminf(q4_size(vm0[i]), 0x1p100f)), g1 = fast_log2(fminf(q4_size(vm1[i]), 0x1p100f));
       float x0 = fmaxf(s0 - m0 + g0, s2 - m0 + g1), x1 = kTwo ? fmaxf(s1 - m1 + g0, s3 - m1 + g1) : 0.f;
 #pragma unroll
       for (int o = 4; o <= 16; o <<= 1) {
@@ -508,19 +523,20 @@ __device__ __forceinline__ void q4_tiles(Q4State<G>& st, const uint32_t (&qf)[G]
       p1 = q4_weight(s1, m1);
       p3 = q4_weight(s3, m1);
     }
+    scale();
+    l0 = p0 + p2;
+    l1 = p1 + p3;
   }
-  st.l[0] += p0 + p2;
-  if (kTwo) st.l[1] += p1 + p3;
+  st.l[0] += l0;
+  if (kTwo) st.l[1] += l1;
   uint32_t b0[G], b1[G];
 #pragma unroll
   for (int i = 0; i < G; ++i) {
     const float vs0 = bf16_lo(vm0[i]), vs1 = bf16_lo(vm1[i]), vl0 = bf16_hi(vm0[i]), vl1 = bf16_hi(vm1[i]);
-    const float u0 = p0 * st.inv[i][0], u2 = p2 * st.inv[i][0];
-    const float u1 = kTwo ? p1 * st.inv[i][1] : 0.f, u3 = kTwo ? p3 * st.inv[i][1] : 0.f;
-    const __half2 h0 = __floats2half2_rn(u0 * vs0, kTwo ? u1 * vs0 : 0.f);
-    const __half2 h1 = __floats2half2_rn(u2 * vs1, kTwo ? u3 * vs1 : 0.f);
-    st.low[i][0] = fmaf(u0, vl0, fmaf(u2, vl1, st.low[i][0]));
-    if (kTwo) st.low[i][1] = fmaf(u1, vl0, fmaf(u3, vl1, st.low[i][1]));
+    const __half2 h0 = __floats2half2_rn(u0[i] * vs0, kTwo ? u1[i] * vs0 : 0.f);
+    const __half2 h1 = __floats2half2_rn(u2[i] * vs1, kTwo ? u3[i] * vs1 : 0.f);
+    st.low[i][0] = fmaf(u0[i], vl0, fmaf(u2[i], vl1, st.low[i][0]));
+    if (kTwo) st.low[i][1] = fmaf(u1[i], vl0, fmaf(u3[i], vl1, st.low[i][1]));
     b0[i] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h0));
     b1[i] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h1));
   }
@@ -826,7 +842,7 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_q4_kernel(Q4Attent
   constexpr uint32_t kWidth = 64 * G, kShares = kMergeThreads / kWidth, kPart = L::kPart / 4;
   constexpr uint32_t kFactors = (kQ4MaxSplits + kMergeBatch * kShares - 1) / (kMergeBatch * kShares) * (kMergeBatch * kShares);
   __shared__ float factor[G][kFactors];
-  __shared__ float warp_m[kMergeThreads / 32], warp_e[G][kMergeThreads / 32], warp_l[kMergeThreads / 32];
+  __shared__ float warp_greatest[1 + G][kMergeThreads / 32], warp_l[kMergeThreads / 32];
   __shared__ float sums[kShares][kWidth];
   pdl_wait();
   pdl_launch_dependents();
@@ -846,26 +862,36 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_q4_kernel(Q4Attent
   load(0);
   const bool has = threadIdx.x < chunks;
   const float m = has ? parts[threadIdx.x * kPart + L::kReferences + query] : kNoScore;
-  float e[G], unit[G];
+  float e[G];
 #pragma unroll
   for (int i = 0; i < G; ++i)
     e[i] = has ? parts[threadIdx.x * kPart + L::kUnits + i * kQ4Queries + query] : float(kNoUnit);
   const float part_l = has ? parts[threadIdx.x * kPart + L::kSums + query] : 0.f;
-  auto greatest = [&](float x, float* of_warps) {
+  float (*of_warps)[kMergeThreads / 32] = warp_greatest;
+  auto greatest = [&](auto& x) {  // of every thread, for each of x
+    constexpr int kCount = sizeof(x) / sizeof(float);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, o));
-    if (lane_id() == 0) of_warps[warp_id()] = x;
+    for (int i = 0; i < kCount; ++i) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) x[i] = fmaxf(x[i], __shfl_xor_sync(0xFFFFFFFFu, x[i], o));
+      if (lane_id() == 0) of_warps[i][warp_id()] = x[i];
+    }
     __syncthreads();
 #pragma unroll
-    for (uint32_t w = 0; w < (kQ4MaxSplits + 31) / 32; ++w) x = fmaxf(x, of_warps[w]);  // (the others have none)
-    return x;
-  };
-  const float below = m - greatest(m, warp_m), l_warp = warp_sum(part_l * fast_exp2(below));
+    for (int i = 0; i < kCount; ++i)
 #pragma unroll
-  for (int i = 0; i < G; ++i) {
-    unit[i] = greatest(below + e[i], warp_e[i]);
+      for (uint32_t w = 0; w < (kQ4MaxSplits + 31) / 32; ++w) x[i] = fmaxf(x[i], of_warps[i][w]);  // (the others have none)
+    of_warps += kCount;
+  };
+  float reference[1] = {m}, unit[G];
+  greatest(reference);
+  const float below = m - reference[0], l_warp = warp_sum(part_l * fast_exp2(below));
+#pragma unroll
+  for (int i = 0; i < G; ++i) unit[i] = below + e[i];
+  greatest(unit);
+#pragma unroll
+  for (int i = 0; i < G; ++i)
     if (threadIdx.x < kFactors) factor[i][threadIdx.x] = has ? fast_exp2(below + e[i] - unit[i]) : 0.f;
-  }
   if (lane_id() == 0) warp_l[warp_id()] = l_warp;
   __syncthreads();
   float a = 0.f;
