@@ -299,10 +299,11 @@ tempo_status tempo_kv_load_q4(const void* cache, void* kv, uint32_t ldo, const i
  * first heads * head columns, already scaled by 1/sqrt(head)) over the first lengths[s] + length_offset positions
  * (clamped to [0, capacity]); query head h reads key / value head h / (heads / kv_heads). A sequence of no positions is
  * written as zeros. Keys and values of more than 2^100 (1.3e30) in size may overflow on the way and give NaN, as may
- * scores that FP32 does not hold, and where all values are below 2^-110 (8e-34) they lose bits. out: [seqs, heads * head] BF16. Few sequences of a long capacity are split over more
- * CTAs than a cluster holds; their partial results then go through `workspace` (tempo_decode_attention_q4_workspace
- * bytes, 16-byte aligned, of any content; NULL when that is 0), which no other call may use until this one has
- * finished. */
+ * scores that FP32 does not hold, and where all values are below 2^-110 (8e-34) they lose bits; a position whose weight is
+ * below 2^-149 of the greatest counts for nothing. out: [seqs, heads * head] BF16. Few sequences of a long capacity are
+ * split over more CTAs than a cluster holds; their partial results then go through `workspace`
+ * (tempo_decode_attention_q4_workspace bytes, 16-byte aligned, of any content; NULL when that is 0), which no other call may
+ * use until this one has finished. */
 tempo_status tempo_decode_attention_q4_workspace(uint32_t seqs, uint32_t heads, uint32_t kv_heads, uint32_t head,
                                                  uint32_t capacity, uint64_t* bytes);
 tempo_status tempo_decode_attention_q4(const void* q, uint32_t ldq, const void* cache, const int32_t* lengths,
@@ -314,7 +315,8 @@ tempo_status tempo_decode_attention_q4(const void* q, uint32_t ldq, const void* 
  * element): logprob[r] = log softmax(logits[r])[ids[r]] (0 where ids[r] is outside [0, vocab): a row without a token),
  * entropy[r] = -sum p ln p, and, with 0 < top <= 32 and top <= vocab, the `top` greatest logits in descending order, ties
  * to the lower index, as top_ids / top_logprob [rows][top]. A logit of -infinity has probability 0. A row of nothing but
- * -infinity scores -infinity with entropy 0; a NaN or +infinity makes its row's scores NaN, and NaN ranks first. With slot_of (NULL for none), the outputs hold `slots` blocks of `rows` rows and row r's results go to block
+ * -infinity scores -infinity with entropy 0; a NaN or +infinity makes its row's scores NaN (a row of NaN alone too), and NaN
+ * ranks first. With slot_of (NULL for none), the outputs hold `slots` blocks of `rows` rows and row r's results go to block
  * slot_of[r] + slot_offset, or nowhere when there is no such block: a captured decode step writes each step's results
  * behind the last's. */
 tempo_status tempo_token_logprobs(const void* logits, uint64_t ld, uint32_t bf16, const int32_t* ids, uint32_t rows,

@@ -70,7 +70,7 @@ struct RowMajorParams {
   KvStore kv;  // QKV projection: key and value columns also stored into the caches
 };
 
-template <int BN, int STAGES, bool STAGED = false, bool F32 = false>
+template <int BN, int STAGES, bool STAGED = false>
 struct RowMajorSmem {
   static constexpr uint32_t kABytes = 128 * kBK * 2;
   static constexpr uint32_t kBBytes = BN * kBK * 2;
@@ -392,7 +392,7 @@ template <int BN, int STAGES, bool STAGED, bool LN, bool F32>
 __global__ void __launch_bounds__(kRowThreads, 1)
     gemm_rowmajor_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                          const __grid_constant__ CUtensorMap tmap_out, RowMajorParams p) {
-  using L = RowMajorSmem<BN, STAGES, STAGED, F32>;
+  using L = RowMajorSmem<BN, STAGES, STAGED>;
   static_assert(STAGED || !F32, "FP32 outputs are staged");
   static_assert(!STAGED || BN >= 128, "staged stores need 32-column chunks");
   extern __shared__ uint8_t smem_raw[];
@@ -833,7 +833,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <int BN, int STAGES, bool STAGED = false, bool LN = false, bool F32 = false>
 tempo_status launch_rowmajor(const void* a, uint32_t lda, const void* w_t, uint32_t ldw, const RowMajorParams& base,
                              cudaStream_t stream) {
-  using L = RowMajorSmem<BN, STAGES, STAGED, F32>;
+  using L = RowMajorSmem<BN, STAGES, STAGED>;
   CUtensorMap ta, tb;
   const uint64_t a_dims[2] = {base.k, base.m};
   const uint64_t a_strides[1] = {uint64_t(lda) * 2};
@@ -1289,7 +1289,7 @@ tempo_status launch_splitk(const void* a, uint32_t lda, const void* w_t, uint32_
 
 constexpr uint32_t kPairBN = 256;
 
-template <int STAGES, bool F32 = false>
+template <int STAGES>
 struct PairSmem {
   static constexpr uint32_t kABytes = 128 * kBK * 2;
   static constexpr uint32_t kBBytes = 128 * kBK * 2;
@@ -1354,7 +1354,7 @@ template <int STAGES, bool F32>
 __global__ void __launch_bounds__(kRowThreads, 1)
     gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                      const __grid_constant__ CUtensorMap tmap_out, RowMajorParams p) {
-  using L = PairSmem<STAGES, F32>;
+  using L = PairSmem<STAGES>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarrierOffset);
@@ -1537,7 +1537,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
 template <int STAGES, bool F32 = false>
 tempo_status launch_pair(const void* a, uint32_t lda, const void* w_t, uint32_t ldw, const RowMajorParams& base,
                          cudaStream_t stream) {
-  using L = PairSmem<STAGES, F32>;
+  using L = PairSmem<STAGES>;
   CUtensorMap ta, tb;
   const uint64_t a_dims[2] = {base.k, base.m};
   const uint64_t a_strides[1] = {uint64_t(lda) * 2};

@@ -250,20 +250,23 @@ tempo_status launch_rows(void (*kernel)(Q4Rows), Q4Rows p, uint32_t rows, uint32
 // to the left are multiplications by 16 and run beside them (shifts for all of them, the keys as BF16 integers 128 +
 // code, took 91 us for 512 sequences of 12 heads and 1152 positions instead of 89.6; moves to the right as the high half
 // of a product, in place of the byte swaps, 104 instead of 85). The values come through the transposing matrix load,
-// which puts the same dimensions of two positions side by side (85 us; byte permutations for it took 89).
+// which puts the same dimensions of two positions side by side (85 us; byte permutations for it took 89). It now takes 77.3 us,
+// 0.96 of the measured copy rate; two sequences of 32 query heads over 8 of 128 and 40001 to 65536 positions 35.7.
 // The eight columns of the B operand (m16n8k16) are query heads of one key / value head times tiles:
 // grouped heads read the cache once, and with few heads one softmax serves several tiles (the first tensor-core form, one tile
 // and eight columns of queries whether they existed or not, issued 309 instructions a tile and was bound by the ALU pipe).
 // Every column holds its head's query; the scores of tile j are kept in the lanes whose columns are tile j's, and the
 // weights of the other columns are zeroed before tile j's values are multiplied.
 // Each 64 dimensions of a query row are scaled by a power of two to at most 2, where FP16 holds their BF16 values but for what
-// lies 2^-14 below the greatest of them, and there to 2^-25 (as FP32 sums with keys that share a scale would); w is rounded to FP16 (2^-11 of each weight, an eighth of the output's own BF16 rounding,
-// and 2^-33 of the greatest), in a running unit that bounds w and p low alike; everything else, the sums included, is FP32.
+// lies 2^-14 below the greatest of them, and there to 2^-25 (as FP32 sums with keys that share a scale would); w is rounded to
+// FP16 (2^-11 of each weight, an eighth of the output's own BF16 rounding, and 2^-33 of the greatest), in a running unit that
+// bounds w and p low alike; everything else, the sums included, is FP32.
 //
-// A CTA of four warps takes a run of tiles of one (sequence, key / value head, eight query heads); each warp streams its
-// own pieces (one bulk copy each, kRing in flight) and keeps an online softmax whose reference and unit move only when a
-// weight passes them some hundred times. Warps merge through shared memory; with `chunks` > 1 the CTAs of a cluster split the positions
-// and merge through distributed shared memory, or, when a pair needs more of them, through a workspace and a second kernel.
+// A CTA of two, four or eight warps takes a run of tiles of one (sequence, key / value head, up to eight query heads); each
+// warp streams its own pieces (one bulk copy each, kRing in flight) and keeps an online softmax whose reference and units move
+// only when a weight passes them some hundred times. Warps merge through shared memory; with `chunks` > 1 the CTAs of a
+// cluster split the positions and merge through distributed shared memory, or, when a pair needs more of them, through a
+// workspace and a second kernel.
 // ---------------------------------------------------------------------------------------------------------------
 
 constexpr uint32_t kQ4MaxChunks = 8;     // CTAs of a cluster
@@ -611,10 +614,11 @@ struct Q4Attention {
 };
 
 // CTAs of `warps` warps that an SM is to hold: 128 registers a thread for heads of 128, 96 for 64. Fewer warps with more
-// registers, and more with fewer, are slower: 512 sequences of 12 heads and 1152 positions 80.9 us at 20 warps an SM, 83 at 16
-// and at 24; 64 query heads of 8 78.6, 78.4 and 82.4; 8 heads of 128 112.5 at 16, 119.4 at 12, 122 at 20. CTAs of eight warps
-// come in two kinds, two to an SM as long as that holds the grid (192 pairs of 60 tiles 6.8 us against 7.7, 256 grouped pairs
-// of 72 9.0 against 11.5), else three (384 pairs of 72 10.6 against 11.5).
+// registers, and more with fewer, are slower: 512 sequences of 64 query heads over 8 and 576 positions 47.4 us at 20 warps an
+// SM, 48.3 at 16, 49.2 at 24; 256 of 32 over 8 heads of 128 and 1152 positions 70.2 at 16, 74.8 at 12, 89.9 at 20. CTAs of eight
+// warps come in two kinds, two to an SM as long as that holds the grid (192 pairs of 60 tiles 6.8 us against 7.7, 256 grouped
+// pairs of 72 9.0 against 11.5, when this was set), else three (384 pairs of 72 10.6 against 11.5, heads of 64 only: those of
+// 128 do not fit three, and two rounds of two are still faster, 384 pairs of 72 20.3 us against 21.6 by CTAs of four warps).
 constexpr uint32_t q4_resident(int head, int warps) { return head == 128 ? 16 / warps : warps == 8 ? 2 : 20 / warps; }
 
 template <int G, int RP, int WARPS, int RESIDENT>
@@ -804,8 +808,9 @@ __global__ void __launch_bounds__(32 * WARPS, RESIDENT) decode_attention_q4_kern
   for (uint32_t i = threadIdx.x; i < queries * kWidth; i += 32 * WARPS) {
     const uint32_t query = i / kWidth, at = query * L::kStride + i % kWidth;
     const uint32_t group = i % kWidth / 64;
-    const Merged r = merge_parts<L, WARPS>(
-        WARPS, query, group, at, [&](uint32_t w, uint32_t i) { return reinterpret_cast<const float*>(smem + w * L::kWarpRing)[i]; });
+    const Merged r = merge_parts<L, WARPS>(WARPS, query, group, at, [&](uint32_t w, uint32_t i) {
+      return reinterpret_cast<const float*>(smem + w * L::kWarpRing)[i];
+    });
     if (whole) {
       out[query * kWidth + q4_dimension(i % kWidth)] = float_to_bf16(len == 0 ? 0.f : r.average());
     } else {
@@ -910,7 +915,8 @@ __global__ void __launch_bounds__(kMergeThreads) decode_merge_q4_kernel(Q4Attent
 #pragma unroll
   for (uint32_t i = 0; i < kShares; ++i) a += sums[i][at];
   const bool empty = int64_t(p.lengths[s]) + p.length_offset <= 0;
-  p.out[(size_t(s) * p.heads + h) * kWidth + q4_dimension(at)] = float_to_bf16(empty ? 0.f : Merged{0.f, at < 64 ? unit[0] : unit[G - 1], l, a}.average());
+  const Merged all{0.f, at < 64 ? unit[0] : unit[G - 1], l, a};
+  p.out[(size_t(s) * p.heads + h) * kWidth + q4_dimension(at)] = float_to_bf16(empty ? 0.f : all.average());
 }
 
 // How the positions of a pair (a sequence's key / value head and block of query heads) are shared out: CTAs of `warps`
@@ -921,12 +927,14 @@ struct Q4Split {
 };
 
 // Up to twice as many CTAs as fit the GPU (lengths differ, and a second round fills what the short ones leave), as long as
-// each has 12 tiles, and more where there are many pairs, whose CTAs hide one another's latency. Measured on a B200 over 456
-// grids of 1 to 768 pairs of 12 to 4096 tiles, at full and at ragged lengths, against every split of up to 148 CTAs: 3 %
-// behind the best one on average, 26 % at worst. us (w warps, c CTAs, p through the workspace): 768 pairs of 72 w4c1 16.4,
-// w8c1 17.9, w4c2 19.6; 192 of 72 w8c1 8.9, w4c2 9.6, w4c4 11.0; 96 of 256 w4c8 12.3, w4c1 15.0; 32 of 512 (128-wide) w4c18p
-// 15.4, w4c8 17.2, w4c37p 18.0; 16 of 4096 w4c64p 36.9, w4c16p 45.4, w4c8 72; 6144 of 72 w2c1 81, w4c1 89 (a CTA's latency
-// weighs more than its width there).
+// each has 12 tiles, and more where there are many pairs, whose CTAs hide one another's latency. Measured on a B200 over 726
+// grids of up to 768 pairs and four times as many, of 4 to 4096 tiles, at full and at ragged lengths, against CTAs of two, four
+// and eight warps, clusters of two to eight and up to 148 CTAs through the workspace: 3 % behind the best of these on average,
+// 39 % at worst (440 ragged pairs of 24 tiles of heads of 128, which two rounds of eight-warp CTAs serve in 12.5 us and one of
+// four-warp CTAs in 9.0). us (w warps, c CTAs, p through the workspace): 768 pairs of 72 w4c1 15.4, w8c1 17.4, w4c2 18.8; 192
+// of 72 w8c1 7.4, w4c1 8.8, w4c2 9.2, w4c4 10.5; 96 of 256 w4c8 12.3, w4c1 14.8; 16 of 1024 (128-wide) 15.5, w4c37p 16.4,
+// w4c16p 17.8, w4c8 21.9; 16 of 4096 (128-wide) w4c37p 36.9, w4c64p 39.0, w4c16p 48.3, w4c8 73. Four times 768 of 72: w2c1 45.5,
+// w4c1 48.3 (a CTA's latency weighs more than its width there).
 Q4Split q4_split(uint64_t pairs, uint32_t tiles, uint32_t head) {
   const uint64_t sms = uint64_t(sm_count());
   const uint64_t chunks = std::min(2 * q4_resident(head, 4) * sms / pairs, tiles * sms / (12 * sms + 32 * pairs));

@@ -125,7 +125,9 @@ class Engine:
             whose cached keys and values are rounded to 16 levels per row. Excludes persistent_decode.
         alternatives: with 0 or more, each generated token's scores are kept for ``scores()``, with that many (at most
             32) of the likeliest tokens; None (the default) keeps none. Needs one decode group and excludes
-            persistent_decode. The tokens are the same with and without.
+            persistent_decode. The tokens are the same with and without: they come from the argmax head, the scores from
+            the FP32 one, whose sums over at most 8 sequences run in another order, so at a tie to the last bits of FP32
+            the likeliest alternative may be another token than the one picked.
     """
 
     def __init__(self, layers: list[dict], shared: dict, *, batch: int, prompt: int, capacity: int,

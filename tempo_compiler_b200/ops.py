@@ -416,8 +416,8 @@ def kv_store_q4(qkv: torch.Tensor, cache: torch.Tensor, seq_of: torch.Tensor, po
     if width % head or heads < 0:
         raise ValueError(f"qkv rows of {width} are not query, key and value heads of {head} ({kv_heads} key heads)")
     _places(rows, seq_of, pos_of, device)
-    _launch_at(device, "tempo_kv_store_q4", qkv.data_ptr(), _stride32(stride, "qkv"), cache.data_ptr(), seq_of.data_ptr(),
-               pos_of.data_ptr(), rows, seqs, heads, kv_heads, head, capacity)
+    _launch_at(device, "tempo_kv_store_q4", qkv.data_ptr(), _stride32(stride, "qkv"), cache.data_ptr(),
+               seq_of.data_ptr(), pos_of.data_ptr(), rows, seqs, heads, kv_heads, head, capacity)
 
 
 def kv_load_q4(cache: torch.Tensor, seq_of: torch.Tensor, pos_of: torch.Tensor, *,
@@ -435,8 +435,8 @@ def kv_load_q4(cache: torch.Tensor, seq_of: torch.Tensor, pos_of: torch.Tensor, 
         out_rows, out_width, stride, _ = _matrix(out, torch.bfloat16, "out", device)
         if out_rows != rows or out_width != width:
             raise ValueError(f"out must be {(rows, width)}, got {tuple(out.shape)}")
-    _launch_at(device, "tempo_kv_load_q4", cache.data_ptr(), out.data_ptr(), _stride32(stride, "out"), seq_of.data_ptr(),
-               pos_of.data_ptr(), rows, seqs, kv_heads, head, capacity)
+    _launch_at(device, "tempo_kv_load_q4", cache.data_ptr(), out.data_ptr(), _stride32(stride, "out"),
+               seq_of.data_ptr(), pos_of.data_ptr(), rows, seqs, kv_heads, head, capacity)
     return out
 
 
