@@ -51,10 +51,10 @@ def _cached(keys: np.ndarray, values: np.ndarray):
 def _check(q: "torch.Tensor", held, got: "torch.Tensor") -> None:
     """The bound of an output of 64 dimensions with the values' widest range R = 15 scale and greatest |low| L in those 64
     dimensions. The output's own rounding is 2^-8 of it. Rounding each weight to FP16 moves the average by at most 2^-11
-    of R. A score is a sum over the groups of 64, each of scale (code + 64) and (low - 64 scale) against the query, in
-    FP32 and with the query's dimensions rounded at 2^-25 of the greatest of its group: it is off by at most
-    (66 2^-23) sum |q| (143 scale + |low|) over the groups, and twice that, times R, moves the average. The sums over the
-    positions are off by n 2^-23, and the exponentials and powers of two by 2^-20, of R + L."""
+    of R. A score is a sum over the groups of 64, each of scale x code and low against the query, in FP32 and with the
+    query's dimensions rounded at 2^-25 of the greatest of its group: it is off by at most (66 2^-23) sum |q| (15 scale +
+    |low|) over the groups, and twice that, times R, moves the average. The sums over the positions are off by n 2^-23,
+    and the exponentials and powers of two by 2^-20, of R + L."""
     (keys, k_scale, k_low), (values, v_scale, v_low) = held
     n, head = keys.shape
     q = q.double().cpu().numpy().reshape(-1, head)
@@ -64,7 +64,7 @@ def _check(q: "torch.Tensor", held, got: "torch.Tensor") -> None:
     p = np.exp(score - score.max(1, keepdims=True))
     p /= p.sum(1, keepdims=True)
     want = p @ values
-    spread = (np.abs(q).reshape(len(q), -1, 64).sum(2) @ (143 * k_scale + np.abs(k_low)).T).max(1)[:, None]
+    spread = (np.abs(q).reshape(len(q), -1, 64).sum(2) @ (15 * k_scale + np.abs(k_low)).T).max(1)[:, None]
     wide = np.repeat(15 * v_scale.max(0), 64)
     size = wide + np.repeat(np.abs(v_low).max(0), 64)
     bound = (2.0 ** -8 * np.abs(want) + wide * (2.0 ** -11 + 2 * 66 * 2.0 ** -23 * spread) +
